@@ -651,6 +651,114 @@ int    i4_dmoe_down_wait(const void* x, int x_dtype, const i4_dmoe_weights* weig
                          hipStream_t stream);
 
 /* ------------------------------------------------------------------------
+ * A long conversation's KV cache.  The reference attends every cached position of one
+ * session with a 16-bit cache (clock.py:164-172); these entries take several tokens of
+ * several sequences, bound what they attend, and keep the cache in 8 bits.  No
+ * counterpart in the reference beyond the attention itself.
+ *
+ * Shared by them: B sequences of T tokens; token t of sequence b is at position
+ * p = pos + t with pos = pos_dev[b] (int32 on the device) or, with pos_dev NULL, the
+ * host's pos for every sequence.  counts (int32 [B] on the device, nullable) says how many
+ * of the T tokens sequence b has (clamped to [0, T]): the others are padding, for which
+ * nothing is read or written.  A position outside the cache, which only a device position
+ * can give, writes nothing to it and NaN to the token's output row.  head_dim == 128; any
+ * n_heads that is a multiple of n_kv_heads, at most 1024; B T n_heads < 2^31. */
+
+/* A 16-bit cache: k and v [batch][n_kv_heads][max_len][head_dim] with strides in elements
+ * (the same for k and v; a row's head_dim values adjacent, every row 16-byte aligned), so
+ * a [max_len][n_kv_heads][head_dim] layout works as well.  max_len <= 2^20, and one head's
+ * rows within 2^31 bytes. */
+typedef struct i4_kvcache {
+  void*   k;
+  void*   v;
+  int64_t batch_stride, head_stride, row_stride;
+  int32_t batch, n_kv_heads, max_len, head_dim;
+  int32_t dtype;             /* I4_F16 / I4_BF16 */
+} i4_kvcache;
+
+/* A cache in 8 bits, in blocks of I4_KV8_BLOCK tokens with one scale for each block and
+ * head: value = element * scale.  Blocks are rounded once, when their last token arrives;
+ * the tokens of the unfinished block wait in the tail in 16 bits and are attended there.
+ * Value blocks are kept [head_dim][token], the operand order of the product with the
+ * softmax's weights.  Every array is dense and 16-byte aligned; blocks <= 2^14. */
+#define I4_KV8_BLOCK 64
+#define I4_KV8_INT8  0       /* element = RNE(x / scale), scale = max |x| / 127 */
+#define I4_KV8_E4M3  1       /* OCP e4m3fn, scale = max |x| / 448 */
+typedef struct i4_kv8cache {
+  void*   k;                 /* [batch][n_kv_heads][blocks][64][head_dim]  8 bits */
+  void*   v;                 /* [batch][n_kv_heads][blocks][head_dim][64]  8 bits */
+  float*  k_scale;           /* [batch][n_kv_heads][blocks]                 */
+  float*  v_scale;
+  void*   k_tail;            /* [batch][n_kv_heads][64][head_dim]  dtype     */
+  void*   v_tail;
+  int32_t batch, n_kv_heads, blocks, head_dim;
+  int32_t dtype;             /* of the tail, and of the tokens and queries: I4_F16 / I4_BF16 */
+  int32_t format;            /* I4_KV8_* */
+} i4_kv8cache;
+
+/* q/k RMSNorm over head_dim and the rotary embedding of the fused q|k|v rows, and the
+ * cache append: what lies between the q|k|v projection and the attention
+ * (Qwen3OmniMoeThinkerTextAttention.forward, modeling_qwen3_omni_moe.py:1473-1500 in
+ * transformers 5.15), for many tokens.
+ *   qkv    token t of sequence b at qkv + b batch_stride + t token_stride (elements),
+ *          [n_heads + 2 n_kv_heads][head_dim], 4-byte aligned rows, x_dtype == cache->dtype;
+ *   q_out  [B][T][n_heads][head_dim], dense: the rotated queries;
+ *   cache  row (first_row or p's own) + t of each kv head receives the token's rotated key
+ *          and its value.  first_row < 0: the row is the position; >= 0: token t goes to row
+ *          first_row + t (<= max_len), and positions reach to 2^24.
+ * inv_freq is a host array [head_dim / 2].  Computed in fp32 (the angle p inv_freq as a sum
+ * of two floats) and rounded once. */
+int    i4_rope_append(const void* qkv, int x_dtype, int T, int64_t batch_stride,
+                      int64_t token_stride, int n_heads, const void* q_norm_w,
+                      const void* k_norm_w, float eps, const float* inv_freq,
+                      const int32_t* pos_dev, int pos, int first_row, const int32_t* counts,
+                      void* q_out, const i4_kvcache* cache, hipStream_t stream);
+
+/* Attention of B x T queries over a 16-bit cache that holds their own keys and values too:
+ *   out[b][t][h] = sum_j softmax_j(scale q . k_j) v_j over the visible j,
+ * j <= p, and with window > 0 only j > p - window or j < sinks (the first tokens stay
+ * visible); query head h reads kv head h / (n_heads / n_kv_heads).  window == 0: no bound
+ * (sinks must be 0).  Keys and values that a query does not see do not reach its row, be
+ * they infinite or NaN.  q at q + b q_batch_stride + t q_token_stride + h q_head_stride
+ * (elements, 16-byte aligned rows), x_dtype == cache->dtype; out dense
+ * [B][T][n_heads][head_dim], rounded once from fp32.  Workspace:
+ * i4_attn_window_workspace_bytes with keys = pos + T, or max_len for a device position;
+ * no initial contents, 256-byte aligned; calls sharing one must not overlap. */
+int    i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
+                      int64_t q_token_stride, int64_t q_head_stride, int n_heads,
+                      const i4_kvcache* cache, const int32_t* pos_dev, int pos,
+                      const int32_t* counts, int window, int sinks, float scale, void* out,
+                      void* workspace, size_t workspace_bytes, hipStream_t stream);
+size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
+                                      int window, int sinks);
+
+/* T tokens of k and v (token t, head g of sequence b at k + b batch_stride +
+ * t token_stride + g head_stride, elements, 16-byte aligned rows; the same strides for v)
+ * into an 8-bit cache, behind the pos tokens that it holds: the blocks that they finish are
+ * rounded from the 16-bit tail and tokens, the rest goes to the tail.  A block whose
+ * largest magnitude is below 2^-100 is scaled as if it were 2^-100; one that holds an
+ * infinity or a NaN gets the scale NaN and reads as NaN.  Tokens must arrive in order: a
+ * pos inside a finished block finds its earlier tokens in the tail no more. */
+int    i4_kv8_append(const void* k, const void* v, int x_dtype, int T, int64_t batch_stride,
+                     int64_t token_stride, int64_t head_stride, const i4_kv8cache* cache,
+                     const int32_t* pos_dev, int pos, const int32_t* counts,
+                     hipStream_t stream);
+
+/* The values of every block, fp32 [batch][n_kv_heads][64 blocks][head_dim] each (the tail
+ * is not among them). */
+int    i4_kv8_values(const i4_kv8cache* cache, float* k_out, float* v_out, hipStream_t stream);
+
+/* i4_attn_window over an 8-bit cache that holds the queries' own tokens too (appended
+ * first): positions in finished blocks of the pos + count tokens are read in 8 bits, the
+ * unfinished block from the tail.  Workspace: i4_attn_window_workspace_bytes, keys =
+ * pos + T, or 64 blocks for a device position. */
+int    i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride,
+                   int64_t q_token_stride, int64_t q_head_stride, int n_heads,
+                   const i4_kv8cache* cache, const int32_t* pos_dev, int pos,
+                   const int32_t* counts, int window, int sinks, float scale, void* out,
+                   void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------------------
  * No counterpart in the reference.  For callers that cannot allocate device
  * memory (code under hipGraph capture, tight serving loops, harnesses that
  * forbid hipMalloc): i4_moe_forward with its workspace taken from a static

@@ -9,6 +9,8 @@ Drop-in replacements for thecodacus/qwen3-omni-duplex's quantized compute:
                             src/duplex/loader.py:31 (packed triplets from safetensors)
   ThinkerDecoder         <- the Thinker[0:24] decode step the clock path runs
                             (clock.py:164-172): attention with KV cache + MoE per layer
+  attn_window, attn_kv8  <- the same attention for prompt chunks and several sessions, under
+                            a sliding window, over a 16-bit or an 8-bit cache (kv.py)
   FusedMoE               <- src/duplex/streaming/fused_moe.py:40 (16-bit / int8
                             experts + gated shared expert: the Talker's block)
   fuse_moe_blocks        <- fused_moe.py:144
@@ -31,6 +33,7 @@ from .ops import (dequant, dequant_gemv, linear, moe_down_combine, moe_down_wait
                   thinker_layer_decode,
                   thinker_layer_fits, thinker_layer_c, thinker_decode_step, dmoe_forward,
                   dmoe_status, dmoe_down_wait, StackLayerX)
+from .kv import KV8Cache, attn_kv8, attn_window, kv8_append, rope_append
 from .weights import QWeight, repack_awq_to_ct, repack_tile
 
 lib = _lib.lib
@@ -50,4 +53,5 @@ __all__ = [
     "ThinkerAttention", "ThinkerDecoderLayer", "ThinkerDecoder", "rope_inv_freq",
     "FusedMoE", "fuse_moe_blocks", "quantize_q8", "dmoe_forward", "dmoe_status",
     "dmoe_down_wait", "StackLayerX",
+    "KV8Cache", "attn_kv8", "attn_window", "kv8_append", "rope_append",
 ]

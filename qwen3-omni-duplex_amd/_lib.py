@@ -75,6 +75,24 @@ class ThinkerLayerC(ctypes.Structure):
                 ("qkv", QWeightC), ("o", QWeightC), ("moe", MoeWeightsC)]
 
 
+class KVCacheC(ctypes.Structure):
+    """struct i4_kvcache"""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("batch_stride", c_int64),
+                ("head_stride", c_int64), ("row_stride", c_int64), ("batch", c_int32),
+                ("n_kv_heads", c_int32), ("max_len", c_int32), ("head_dim", c_int32),
+                ("dtype", c_int32)]
+
+
+class KV8CacheC(ctypes.Structure):
+    """struct i4_kv8cache"""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("k_tail", c_void_p), ("v_tail", c_void_p), ("batch", c_int32),
+                ("n_kv_heads", c_int32), ("blocks", c_int32), ("head_dim", c_int32),
+                ("dtype", c_int32), ("format", c_int32)]
+
+
 # name -> (restype, argtypes); every function declared in include/i4moe.h
 SIGNATURES = {
     "i4_abi_version": (c_int, []),
@@ -163,6 +181,20 @@ SIGNATURES = {
                                        c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
     "i4_thinker_decode_step_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int,
                                                           c_int, c_int, c_int]),
+    "i4_rope_append": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int, c_void_p,
+                               c_void_p, ctypes.c_float, c_void_p, c_void_p, c_int, c_int,
+                               c_void_p, c_void_p, POINTER(KVCacheC), c_void_p]),
+    "i4_attn_window": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
+                               POINTER(KVCacheC), c_void_p, c_int, c_void_p, c_int, c_int,
+                               ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "i4_attn_window_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int,
+                                                  c_int]),
+    "i4_kv8_append": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_int64, c_int64,
+                              POINTER(KV8CacheC), c_void_p, c_int, c_void_p, c_void_p]),
+    "i4_kv8_values": (c_int, [POINTER(KV8CacheC), c_void_p, c_void_p, c_void_p]),
+    "i4_attn_kv8": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
+                            POINTER(KV8CacheC), c_void_p, c_int, c_void_p, c_int, c_int,
+                            ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
     "i4_dmoe_forward": (c_int, [c_void_p, c_int, c_int, POINTER(DmoeWeightsC), c_int, c_int,
                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_size_t, c_void_p]),

@@ -1,0 +1,288 @@
+"""A long conversation's KV cache: rotary append, bounded attention, 8-bit blocks.
+
+    rope_append   q/k RMSNorm + rotary embedding of many tokens, k and v into the cache
+                  (Qwen3OmniMoeThinkerTextAttention.forward between the q|k|v projection and
+                  the attention, modeling_qwen3_omni_moe.py:1473-1500 in transformers 5.15)
+    attn_window   attention of many tokens over a 16-bit cache, under a sliding window whose
+                  first tokens stay visible, or over everything
+    KV8Cache      a cache in 8 bits with a scale for each block of 64 tokens and head
+    kv8_append    tokens into it
+    attn_kv8      attn_window over it
+
+The clock path attends every cached position of one session one token at a time
+(src/duplex/streaming/clock.py:164-172; ops.attn_decode); these take prompt chunks and
+several sessions, bound what a token attends, and halve the cache.
+
+Tokens: [T, ...] of one sequence or [B, T, ...] of B, token t of sequence b at position
+pos + t.  pos is an int (every sequence), or an int32 device tensor of B elements that the
+kernels read, so that a captured graph serves every position.  counts (int32 device tensor of
+B elements, optional) says how many of the T tokens each sequence has; the rest is padding,
+whose output rows are left as they are.  A device position outside the cache writes nothing
+to it and NaN to the token's output row; an int is refused.
+
+Every op enqueues on torch's current stream of the tensors' device and never synchronises.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .ops import Workspace
+
+KV8_BLOCK = 64
+_FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
+
+
+def _pos(pos: int | torch.Tensor, B: int, dev: torch.device) -> tuple[int | None, int]:
+    """(device pointer, host value) of the first position(s)."""
+    if isinstance(pos, torch.Tensor):
+        if (pos.device != dev or pos.dtype != torch.int32 or pos.numel() != B
+                or not pos.is_contiguous()):
+            raise RuntimeError(f"device positions are {B} contiguous int32 on the tensors' device")
+        return pos.data_ptr(), 0
+    return None, int(pos)
+
+
+def _counts(counts: torch.Tensor | None, B: int, dev: torch.device) -> int | None:
+    if counts is None:
+        return None
+    if (counts.device != dev or counts.dtype != torch.int32 or counts.numel() != B
+            or not counts.is_contiguous()):
+        raise RuntimeError(f"counts are {B} contiguous int32 on the tensors' device")
+    return counts.data_ptr()
+
+
+def _batched(x: torch.Tensor, dims: int, name: str) -> torch.Tensor:
+    """x with its batch dimension (one sequence may come without)."""
+    if x.dim() == dims - 1:
+        return x.unsqueeze(0)
+    if x.dim() != dims:
+        raise RuntimeError(f"{name} has {x.dim()} dimensions, expected {dims - 1} or {dims}")
+    return x
+
+
+def _cache_c(k: torch.Tensor, v: torch.Tensor) -> _lib.KVCacheC:
+    """struct i4_kvcache of [n_kv_heads, max_len, head_dim] or [B, n_kv_heads, max_len,
+    head_dim] caches (views with any strides above a dense last dimension)."""
+    k, v = _batched(k, 4, "k_cache"), _batched(v, 4, "v_cache")
+    if k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+        raise RuntimeError("k_cache and v_cache must agree in shape, strides and dtype")
+    if k.stride(3) != 1 and k.shape[3] != 1:
+        raise RuntimeError("the caches' last dimension must be contiguous")
+    B, n, rows, d = k.shape
+    return _lib.KVCacheC(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), B, n,
+                         rows, d, _lib.half_code(k.dtype))
+
+
+def _out(out: torch.Tensor | None, like: torch.Tensor, shape: tuple[int, ...],
+         padded: bool) -> torch.Tensor:
+    """The given output, checked, or a new one (zeros where padding will stay unwritten)."""
+    if out is None:
+        make = torch.zeros if padded else torch.empty
+        return make(shape, dtype=like.dtype, device=like.device)
+    if out.numel() != math.prod(shape) or tuple(out.shape[-len(shape) + 1:]) != shape[1:] \
+            or out.dtype != like.dtype or not out.is_contiguous():
+        raise RuntimeError(f"out must be a contiguous {shape} tensor of {like.dtype}")
+    return out
+
+
+def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torch.Tensor,
+                k_norm_w: torch.Tensor, eps: float, inv_freq: torch.Tensor,
+                pos: int | torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
+                first_row: int | None = None, counts: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """RMSNorm over head_dim and rotary embedding of the queries and keys in the fused
+    projection rows qkv [T, (n_heads + 2 n_kv_heads) * head_dim] (or [B, T, ...]); returns
+    the rotated queries [T, n_heads, head_dim] (or [B, T, ...]) and writes each token's
+    rotated key and its value to the caches ([n_kv_heads, max_len, head_dim] or [B, ...]):
+    at the row of its position, or at first_row + t when first_row is given.  inv_freq is the
+    host fp32 table [head_dim / 2].  fp32 inside, rounded once (i4_rope_append)."""
+    dev = _lib.require_device(qkv, q_norm_w, k_norm_w, k_cache, v_cache, counts, out)
+    x = _batched(qkv, 3, "qkv")
+    cc = _cache_c(k_cache, v_cache)
+    B, T, width = x.shape
+    hd = cc.head_dim
+    if q_norm_w.dtype != x.dtype or k_norm_w.dtype != x.dtype:
+        raise RuntimeError("the norm weights must have the activation dtype")
+    if q_norm_w.numel() != hd or k_norm_w.numel() != hd:
+        raise RuntimeError(f"the norm weights hold head_dim = {hd} values")
+    if cc.batch != B or cc.n_kv_heads != n_kv_heads or width != (n_heads + 2 * n_kv_heads) * hd:
+        raise RuntimeError("qkv / cache shapes do not match the head counts")
+    if inv_freq.numel() != hd // 2:
+        raise RuntimeError("inv_freq must hold head_dim / 2 values")
+    if x.stride(2) != 1:
+        x = x.contiguous()
+    if inv_freq.dtype != torch.float32 or inv_freq.device.type != "cpu" \
+            or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.detach().to("cpu", torch.float32).contiguous()
+    qw, kw = q_norm_w.contiguous(), k_norm_w.contiguous()
+    if first_row is not None and first_row < 0:
+        raise RuntimeError("first_row must not be negative")
+    shape = (B, T, n_heads, hd)
+    q = _out(out, x, shape if qkv.dim() == 3 else shape[1:], counts is not None)
+    pd, ph = _pos(pos, B, dev)
+    _lib.check(_lib.lib().i4_rope_append(
+        x.data_ptr(), _lib.half_code(x.dtype), T, x.stride(0), x.stride(1), n_heads,
+        qw.data_ptr(), kw.data_ptr(), float(eps), inv_freq.data_ptr(), pd, ph,
+        -1 if first_row is None else int(first_row), _counts(counts, B, dev), q.data_ptr(),
+        ctypes.byref(cc), _lib.stream(dev)))
+    return q
+
+
+def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
+            pos: int | torch.Tensor, window: int | None, sinks: int, scale: float | None,
+            counts: torch.Tensor | None, out: torch.Tensor | None,
+            workspace: Workspace | None) -> torch.Tensor:
+    """The call that attn_window and attn_kv8 share; keys: the positions of the cache."""
+    x = _batched(q, 4, "q")
+    B, T, nh, hd = x.shape
+    if B != cc.batch or hd != cc.head_dim:
+        raise RuntimeError(f"q {tuple(q.shape)} does not match the cache's batch {cc.batch} and "
+                           f"head_dim {cc.head_dim}")
+    if window is not None and window < 1:
+        raise RuntimeError("window must be at least 1 (None: no bound)")
+    if window is None and sinks:
+        raise RuntimeError("sinks are the first tokens outside a window: give the window too")
+    if x.stride(3) != 1:
+        x = x.contiguous()
+    y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd), counts is not None)
+    pd, ph = _pos(pos, B, dev)
+    w = 0 if window is None else min(int(window), 2**31 - 1)
+    lb = _lib.lib()
+    need = lb.i4_attn_window_workspace_bytes(B, T, nh, cc.n_kv_heads,
+                                             keys if pd else min(max(ph, 0) + T, keys), w, sinks)
+    ws = (workspace or Workspace()).get(need, dev) if need else None
+    _lib.check(entry(x.data_ptr(), _lib.half_code(x.dtype), T, x.stride(0), x.stride(1),
+                     x.stride(2), nh, ctypes.byref(cc), pd, ph, _counts(counts, B, dev), w,
+                     int(sinks), 1.0 / math.sqrt(hd) if scale is None else float(scale),
+                     y.data_ptr(), _lib.ptr(ws), need, _lib.stream(dev)))
+    return y
+
+
+def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                pos: int | torch.Tensor, *, window: int | None = None, sinks: int = 0,
+                scale: float | None = None, counts: torch.Tensor | None = None,
+                out: torch.Tensor | None = None,
+                workspace: Workspace | None = None) -> torch.Tensor:
+    """Attention of rotated queries q [T, n_heads, head_dim] (or [B, T, ...]) at positions
+    pos + t over caches [n_kv_heads, max_len, head_dim] (or [B, ...]) that hold the tokens up
+    to and including theirs (rope_append): softmax(scale q k^T) v over the positions j <= p
+    and, with a window, j > p - window or j < sinks.  scale defaults to head_dim ** -0.5.
+    fp32 inside, rounded once to the activation dtype (i4_attn_window)."""
+    dev = _lib.require_device(q, k_cache, v_cache, counts, out)
+    cc = _cache_c(k_cache, v_cache)
+    return _attend(_lib.lib().i4_attn_window, cc, cc.max_len, q, dev, pos, window, sinks, scale,
+                   counts, out, workspace)
+
+
+class KV8Cache:
+    """A KV cache in 8 bits with one fp32 scale for each block of 64 tokens and head:
+
+    k [B, n_kv_heads, blocks, 64, head_dim] and v [B, n_kv_heads, blocks, head_dim, 64]
+    (value blocks are kept transposed), int8 or float8_e4m3fn; k_scale, v_scale
+    [B, n_kv_heads, blocks] fp32; k_tail, v_tail [B, n_kv_heads, 64, head_dim] in 16 bits, the
+    tokens of the unfinished block.  The kernels write the tensors in place and the object
+    holds their addresses, so they cannot be replaced."""
+
+    __slots__ = ("_t", "_c")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor,
+                 v_scale: torch.Tensor, k_tail: torch.Tensor, v_tail: torch.Tensor):
+        _lib.require_device(k, v, k_scale, v_scale, k_tail, v_tail)
+        if k.dtype not in _FORMATS or v.dtype != k.dtype:
+            raise RuntimeError(f"k and v are int8 or float8_e4m3fn, got {k.dtype}, {v.dtype}")
+        if k.dim() != 5 or k.shape[3] != KV8_BLOCK:
+            raise RuntimeError("k is [B, n_kv_heads, blocks, 64, head_dim]")
+        B, n, blocks, _, hd = k.shape
+        want = {"v": (v, (B, n, blocks, hd, KV8_BLOCK)), "k_scale": (k_scale, (B, n, blocks)),
+                "v_scale": (v_scale, (B, n, blocks)), "k_tail": (k_tail, (B, n, KV8_BLOCK, hd)),
+                "v_tail": (v_tail, (B, n, KV8_BLOCK, hd)), "k": (k, tuple(k.shape))}
+        for name, (t, shape) in want.items():
+            if tuple(t.shape) != shape or not t.is_contiguous():
+                raise RuntimeError(f"{name} must be a contiguous {shape} tensor")
+        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+            raise RuntimeError("the scales are float32")
+        if k_tail.dtype != v_tail.dtype:
+            raise RuntimeError("k_tail and v_tail must have one dtype")
+        self._t = (k, v, k_scale, v_scale, k_tail, v_tail)
+        self._c = _lib.KV8CacheC(*(t.data_ptr() for t in self._t), B, n, blocks, hd,
+                                 _lib.half_code(k_tail.dtype), _FORMATS[k.dtype])
+
+    @classmethod
+    def empty(cls, n_kv_heads: int, max_len: int, head_dim: int = 128, *, batch: int = 1,
+              dtype: torch.dtype = torch.bfloat16, kind: torch.dtype = torch.int8,
+              device: torch.device | str = "cuda") -> "KV8Cache":
+        """A cache of zeros for max_len tokens (rounded up to whole blocks)."""
+        blocks = -(-max_len // KV8_BLOCK)
+        shape = (batch, n_kv_heads, blocks)
+        bits = [torch.zeros(*shape, *s, dtype=torch.int8, device=device).view(kind)
+                for s in ((KV8_BLOCK, head_dim), (head_dim, KV8_BLOCK))]
+        scales = [torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2)]
+        tails = [torch.zeros(batch, n_kv_heads, KV8_BLOCK, head_dim, dtype=dtype, device=device)
+                 for _ in range(2)]
+        return cls(*bits, *scales, *tails)
+
+    k = property(lambda self: self._t[0])
+    v = property(lambda self: self._t[1])
+    k_scale = property(lambda self: self._t[2])
+    v_scale = property(lambda self: self._t[3])
+    k_tail = property(lambda self: self._t[4])
+    v_tail = property(lambda self: self._t[5])
+
+    @property
+    def max_len(self) -> int:
+        return self._c.blocks * KV8_BLOCK
+
+    def reset(self) -> None:
+        """Empty the cache in place (a new conversation)."""
+        for t in self._t:
+            (t.view(torch.int8) if t.element_size() == 1 else t).zero_()
+
+    def values(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """What the finished blocks stand for: k and v [B, n_kv_heads, max_len, head_dim]
+        fp32 (i4_kv8_values; the tail's tokens are not among them)."""
+        c, dev = self._c, self._t[0].device
+        out = torch.empty(2, c.batch, c.n_kv_heads, self.max_len, c.head_dim, dtype=torch.float32,
+                          device=dev)
+        k, v = out.unbind(0)
+        _lib.check(_lib.lib().i4_kv8_values(ctypes.byref(c), k.data_ptr(), v.data_ptr(),
+                                            _lib.stream(dev)))
+        return k, v
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, pos: int | torch.Tensor, *,
+               counts: torch.Tensor | None = None) -> None:
+    """The rotated keys and the values of T tokens, k and v [T, n_kv_heads, head_dim] (or
+    [B, T, ...], any strides above a dense last dimension), into the cache behind the pos
+    tokens it holds (i4_kv8_append).  The blocks that they finish are rounded from 16 bits;
+    the rest goes to the tail.  Tokens arrive in order: pos is what the cache holds, or lies
+    in its unfinished block."""
+    c = cache._c
+    dev = _lib.require_device(k, v, cache._t[0], counts)
+    k, v = _batched(k, 4, "k"), _batched(v, 4, "v")
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise RuntimeError("k and v must agree in shape and dtype")
+    if k.stride() != v.stride() or k.stride(3) != 1:
+        k, v = k.contiguous(), v.contiguous()
+    B, T, n, hd = k.shape
+    if (B, n, hd) != (c.batch, c.n_kv_heads, c.head_dim):
+        raise RuntimeError(f"k {tuple(k.shape)} does not match the cache")
+    pd, ph = _pos(pos, B, dev)
+    _lib.check(_lib.lib().i4_kv8_append(k.data_ptr(), v.data_ptr(), _lib.half_code(k.dtype), T,
+                                        k.stride(0), k.stride(1), k.stride(2), ctypes.byref(c),
+                                        pd, ph, _counts(counts, B, dev), _lib.stream(dev)))
+
+
+def attn_kv8(q: torch.Tensor, cache: KV8Cache, pos: int | torch.Tensor, *,
+             window: int | None = None, sinks: int = 0, scale: float | None = None,
+             counts: torch.Tensor | None = None, out: torch.Tensor | None = None,
+             workspace: Workspace | None = None) -> torch.Tensor:
+    """attn_window over an 8-bit cache whose last tokens are the queries' own (kv8_append):
+    positions in the finished blocks of the pos + T (or counts) tokens are read in 8 bits, the
+    unfinished block from the tail (i4_attn_kv8)."""
+    dev = _lib.require_device(q, cache._t[0], counts, out)
+    return _attend(_lib.lib().i4_attn_kv8, cache._c, cache.max_len, q, dev, pos, window, sinks,
+                   scale, counts, out, workspace)

@@ -1,0 +1,166 @@
+"""What rope_append, attn_window, kv8_append and attn_kv8 refuse, on the host and before any
+launch (no compute call is made here), and the references of their GPU tests."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from tests import _kv_ref as ref
+
+P = 0x10000  # an aligned address that nothing reads
+NULL, SHAPE, DTYPE, ALIGN, WORKSPACE, STRIDE = -1, -2, -3, -4, -7, -9
+
+
+def cache(lb, **kw):
+    base = dict(k=P, v=P, batch_stride=4 * 256 * 128, head_stride=256 * 128, row_stride=128,
+                batch=2, n_kv_heads=4, max_len=256, head_dim=128, dtype=2)
+    return lb.KVCacheC(**{**base, **kw})
+
+
+def cache8(lb, **kw):
+    base = dict(k=P, v=P, k_scale=P, v_scale=P, k_tail=P, v_tail=P, batch=2, n_kv_heads=4,
+                blocks=4, head_dim=128, dtype=2, format=0)
+    return lb.KV8CacheC(**{**base, **kw})
+
+
+BAD_TOKENS = [
+    (dict(T=0), SHAPE), (dict(T=-3), SHAPE), (dict(pos=-1), SHAPE), (dict(pos=256), SHAPE),
+    (dict(pos=250, T=7), SHAPE), (dict(pos=2**31 - 1, T=2**20), SHAPE),
+    (dict(nh=6), SHAPE), (dict(nh=2), SHAPE), (dict(nh=2048), SHAPE), (dict(xt=0), DTYPE),
+    (dict(xt=1), DTYPE), (dict(pos_dev=P + 2), ALIGN), (dict(counts=P + 1), ALIGN),
+    (dict(pos_dev=P, T=2**20 + 1), SHAPE),
+]
+BAD_CACHE = [
+    (dict(k=None), NULL), (dict(v=None), NULL), (dict(k=P + 8), ALIGN), (dict(v=P + 2), ALIGN),
+    (dict(head_dim=64), SHAPE), (dict(batch=0), SHAPE), (dict(n_kv_heads=0), SHAPE),
+    (dict(max_len=0), SHAPE), (dict(max_len=2**20 + 1), SHAPE), (dict(row_stride=120), STRIDE),
+    (dict(row_stride=132), ALIGN), (dict(head_stride=64), STRIDE), (dict(batch_stride=0), STRIDE),
+    (dict(row_stride=2**30), STRIDE), (dict(dtype=0), DTYPE), (dict(dtype=7), DTYPE),
+]
+BAD_CACHE8 = [(dict([(n, None)]), NULL) for n in ("k", "v", "k_scale", "v_scale", "k_tail",
+                                                   "v_tail")] + [
+    (dict(k=P + 4), ALIGN), (dict(v_tail=P + 4), ALIGN), (dict(head_dim=64), SHAPE),
+    (dict(batch=0), SHAPE), (dict(n_kv_heads=0), SHAPE), (dict(blocks=0), SHAPE),
+    (dict(blocks=2**14 + 1), SHAPE), (dict(dtype=0), DTYPE), (dict(format=2), DTYPE),
+    (dict(format=-1), DTYPE)]
+
+
+def call_rope(lb, lib, c=None, **kw):
+    a = {**dict(qkv=P, xt=2, T=1, bs=16 * 128, ts=16 * 128, nh=8, qw=P, kw=P, pos_dev=None, pos=0,
+                first=-1, counts=None, out=P), **kw}
+    tab = (ctypes.c_float * 64)()
+    return lib.i4_rope_append(a["qkv"], a["xt"], a["T"], a["bs"], a["ts"], a["nh"], a["qw"],
+                              a["kw"], 1e-6, tab if a.get("tab", True) else None, a["pos_dev"],
+                              a["pos"], a["first"], a["counts"], a["out"],
+                              ctypes.byref(c or cache(lb)), None)
+
+
+def call_attn(lb, lib, c=None, eight=False, **kw):
+    a = {**dict(q=P, xt=2, T=1, bs=8 * 128, ts=8 * 128, hs=128, nh=8, pos_dev=None, pos=0,
+                counts=None, window=0, sinks=0, scale=0.1, out=P, ws=P, wsb=1 << 40), **kw}
+    fn = lib.i4_attn_kv8 if eight else lib.i4_attn_window
+    return fn(a["q"], a["xt"], a["T"], a["bs"], a["ts"], a["hs"], a["nh"],
+              ctypes.byref(c or (cache8(lb) if eight else cache(lb))), a["pos_dev"], a["pos"],
+              a["counts"], a["window"], a["sinks"], a["scale"], a["out"], a["ws"], a["wsb"], None)
+
+
+def call_append(lb, lib, c=None, **kw):
+    a = {**dict(k=P, v=P, xt=2, T=1, bs=512, ts=512, hs=128, pos_dev=None, pos=0, counts=None),
+         **kw}
+    return lib.i4_kv8_append(a["k"], a["v"], a["xt"], a["T"], a["bs"], a["ts"], a["hs"],
+                             ctypes.byref(c or cache8(lb)), a["pos_dev"], a["pos"], a["counts"],
+                             None)
+
+
+@pytest.fixture
+def lb(pkg):
+    from qwen3_omni_duplex_amd import _lib
+
+    return _lib
+
+
+@pytest.mark.parametrize("bad,code", BAD_TOKENS + [
+    (dict(qkv=None), NULL), (dict(qw=None), NULL), (dict(kw=None), NULL), (dict(out=None), NULL),
+    (dict(tab=False), NULL), (dict(first=256), SHAPE), (dict(first=250, T=7), SHAPE),
+    (dict(first=0, pos=2**24), SHAPE), (dict(T=2, ts=100), STRIDE), (dict(bs=100), STRIDE),
+    (dict(qkv=P + 2), ALIGN), (dict(bs=16 * 128 + 1), ALIGN), (dict(out=P + 8), ALIGN)])
+def test_rope_refuses(lb, pkg, bad, code):
+    assert call_rope(lb, pkg.lib(), **bad) == code
+
+
+@pytest.mark.parametrize("bad,code", BAD_CACHE)
+def test_cache_refused(lb, pkg, bad, code):
+    c = cache(lb, **bad)
+    assert call_rope(lb, pkg.lib(), c) == code
+    assert call_attn(lb, pkg.lib(), c) == code
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("bad,code", BAD_TOKENS + [
+    (dict(q=None), NULL), (dict(out=None), NULL), (dict(window=-1), SHAPE),
+    (dict(sinks=-1, window=4), SHAPE), (dict(sinks=4), SHAPE), (dict(scale=0.0), SHAPE),
+    (dict(scale=-1.0), SHAPE), (dict(scale=math.inf), SHAPE), (dict(scale=math.nan), SHAPE),
+    (dict(T=2, ts=64), STRIDE), (dict(hs=64), STRIDE), (dict(bs=64), STRIDE),
+    (dict(q=P + 8), ALIGN), (dict(out=P + 8), ALIGN), (dict(hs=132), ALIGN),
+    (dict(ts=8 * 128 + 4, T=2), ALIGN)])
+def test_attention_refuses(lb, pkg, eight, bad, code):
+    assert call_attn(lb, pkg.lib(), eight=eight, **bad) == code
+
+
+@pytest.mark.parametrize("bad,code", BAD_CACHE8)
+def test_cache8_refused(lb, pkg, bad, code):
+    c = cache8(lb, **bad)
+    assert call_append(lb, pkg.lib(), c) == code
+    assert call_attn(lb, pkg.lib(), c, eight=True) == code
+    assert pkg.lib().i4_kv8_values(ctypes.byref(c), P, P, None) == code
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(T=0), SHAPE), (dict(pos=-1), SHAPE), (dict(pos=250, T=7), SHAPE), (dict(k=None), NULL),
+    (dict(v=None), NULL), (dict(xt=1), DTYPE), (dict(k=P + 8), ALIGN), (dict(hs=132), ALIGN),
+    (dict(T=2, ts=64), STRIDE), (dict(bs=64), STRIDE), (dict(counts=P + 2), ALIGN)])
+def test_append_refuses(lb, pkg, bad, code):
+    assert call_append(lb, pkg.lib(), **bad) == code
+
+
+def test_values_refuses(lb, pkg):
+    c = cache8(lb)
+    assert pkg.lib().i4_kv8_values(ctypes.byref(c), None, P, None) == NULL
+    assert pkg.lib().i4_kv8_values(ctypes.byref(c), P, P + 4, None) == ALIGN
+
+
+def test_cpu_tensors_are_refused(pkg):
+    x = torch.zeros(1, 1, 8, 128, dtype=torch.bfloat16)
+    k = torch.zeros(1, 4, 64, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        pkg.attn_window(x, k, k, 0)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        pkg.KV8Cache.empty(4, 64, device="cpu")
+    with pytest.raises(RuntimeError, match="HIP device"):
+        pkg.rope_append(x.view(1, 1, -1), 4, 2, x, x, 1e-6, pkg.rope_inv_freq(128, 1e6), 0, k, k)
+
+
+def test_reference_quantisation():
+    """The reference's e4m3 grid rounding against torch's own, and int8 against hand values."""
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(64, 128, generator=g)
+    e, s = ref.quantise(x, torch.float8_e4m3fn)
+    assert s == pytest.approx(x.abs().max().item() / 448, rel=1e-6)
+    near = (x.double() / s).float().to(torch.float8_e4m3fn).double()
+    assert (e != near).float().mean() < 1e-3  # double rounding through fp32 aside
+    y = torch.tensor([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, 63.49]])
+    e, s = ref.quantise(y, torch.int8)
+    assert s == 1.0 and e.tolist() == [[127, 0, 2, 2, 0, -2, 63]]
+    e, s = ref.quantise(torch.tensor([[448.0, 17.0, 19.0, 0.5 * 2 ** -9, 1.5 * 2 ** -9]]),
+                        torch.float8_e4m3fn)
+    assert s == 1.0 and e.tolist() == [[448.0, 16.0, 20.0, 0.0, 2 * 2.0 ** -9]]
+    assert math.isnan(ref.quantise(torch.tensor([[1.0, math.inf]]), torch.int8)[1])
+
+
+def test_reference_visibility():
+    assert ref.see(5, 8, None, 0).tolist() == [True] * 6 + [False] * 2
+    assert ref.see(5, 8, 2, 1).nonzero()[:, 0].tolist() == [0, 4, 5]
+    assert ref.see(0, 3, 1, 9).nonzero()[:, 0].tolist() == [0]
