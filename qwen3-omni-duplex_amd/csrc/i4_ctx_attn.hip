@@ -3,7 +3,13 @@
 // first tokens stay visible.
 //   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q . k_j,
 // over the visible j in one pass, with a running maximum m and sum.
-#include "i4_kv.h"
+#include "i4_ctx.h"
+
+// the bounds and the workspace of a call
+struct i4_span {
+  int window, sinks;
+  void* workspace;
+};
 
 namespace i4 {
 
@@ -69,15 +75,36 @@ __global__ __launch_bounds__(256) void k_ctx_row(const uint16_t* __restrict__ q,
   *dst = (u32)Half<XT>::from_f32(a0 * inv) | ((u32)Half<XT>::from_f32(a1 * inv) << 16);
 }
 
-static int launch(const void* q, int xt, int fmt, int B, int T, int64_t qbs, int64_t qts,
-                  int64_t qhs, int nq, int nkv, const Cache16& c, const Cache8& c8,
-                  const Tokens& tk, const Bounds& w, float scale, void* out,
+// How a call is split: a rule on its sizes alone (no device value), so that the workspace
+// can be named before the call.
+static int ctx_splits(int B, int T, int nq, int nkv, int keys, int window, int sinks) {
+  const int R = T * (nq / nkv);
+  if (R > 32) return 1;
+  int64_t tiles = (keys + 63) / 64;
+  if (window) {
+    const int64_t most = ((int64_t)window + T + 126) / 64 + (sinks + 63) / 64;
+    if (most < tiles) tiles = most;
+  }
+  const int64_t want = (1024 + (int64_t)B * nkv - 1) / ((int64_t)B * nkv);
+  const int64_t most = (tiles + 3) / 4;  // a tile a wave
+  const int64_t s = want < most ? want : most;
+  return s < 1 ? 1 : (int)s;
+}
+
+static int launch(CtxArgs& a, int B, int xt, int fmt, int keys, const i4_span& w,
                   hipStream_t stream) {
-  const int64_t rows = (int64_t)B * T * nq;
+  a.S = ctx_splits(B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks);
+  if (a.S > 1) {
+    a.part = (float*)w.workspace;
+    a.ml = a.part + (int64_t)B * a.nkv * a.R * a.S * KHD;
+  }
+  if (a.R <= 32) return i4_launch_ctx_rows(a, B, xt, fmt, stream);
+  const int64_t rows = (int64_t)B * a.tk.T * a.nq;
   const dim3 grid((unsigned)((rows + 3) / 4));
+  const float scale = a.c2 * 0.69314718f;
   auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, stream>>>((const uint16_t*)q, qbs, qts, qhs, nq, nkv, c, c8, tk, w,
-                                   scale, (uint16_t*)out, rows);
+    kern<<<grid, 256, 0, stream>>>(a.q, a.qbs, a.qts, a.qhs, a.nq, a.nkv, a.c, a.c8, a.tk, a.w,
+                                   scale, a.out, rows);
   };
   if (xt == I4_F16) {
     if (fmt < 0) go(k_ctx_row<I4_F16, -1>);
@@ -97,7 +124,11 @@ extern "C" {
 
 size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                       int window, int sinks) {
-  return 0;
+  if (B < 1 || T < 1 || T > i4::KV_MAX_LEN || n_kv_heads < 1 || n_heads < n_kv_heads ||
+      n_heads > 1024 || n_heads % n_kv_heads || keys < 1 || window < 0 || sinks < 0)
+    return 0;
+  const int64_t S = i4::ctx_splits(B, T, n_heads, n_kv_heads, keys, window, sinks);
+  return S > 1 ? (size_t)((int64_t)B * T * n_heads * S * (i4::KHD + 2) * 4) : 0;
 }
 
 // the positions that a call may attend (a host position is checked after this)
@@ -130,6 +161,20 @@ static int query_check(const void* q, int x_dtype, int dtype, int B, int T, int6
   return I4_OK;
 }
 
+static i4::CtxArgs ctx_args(const void* q, int T, int64_t qbs, int64_t qts, int64_t qhs, int nq,
+                            int nkv, const int32_t* pos_dev, int pos, const int32_t* counts,
+                            int window, int sinks, float scale, void* out) {
+  i4::CtxArgs a{};
+  a.q = (const uint16_t*)q;
+  a.qbs = qbs, a.qts = qts, a.qhs = qhs;
+  a.out = (uint16_t*)out;
+  a.tk = i4::Tokens{pos_dev, counts, pos, T};
+  a.w = i4::Bounds{window ? window : INT32_MAX, sinks};
+  a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.R = T * (nq / nkv);
+  a.c2 = scale * 1.44269504f;
+  return a;
+}
+
 int i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    int64_t q_token_stride, int64_t q_head_stride, int n_heads,
                    const i4_kvcache* cache, const int32_t* pos_dev, int pos,
@@ -145,11 +190,12 @@ int i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    workspace, workspace_bytes,
                    i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks));
   if (rc) return rc;
-  const Cache16 c{(uint16_t*)cache->k, (uint16_t*)cache->v, cache->batch_stride,
-                  cache->head_stride, cache->row_stride, cache->max_len};
-  return launch(q, x_dtype, -1, B, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv,
-                c, Cache8{}, Tokens{pos_dev, counts, pos, T},
-                Bounds{window ? window : INT32_MAX, sinks}, scale, out, stream);
+  CtxArgs a = ctx_args(q, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
+                       pos, counts, window, sinks, scale, out);
+  a.c = Cache16{(uint16_t*)cache->k, (uint16_t*)cache->v, cache->batch_stride,
+                cache->head_stride, cache->row_stride, cache->max_len};
+  a.len = cache->max_len;
+  return launch(a, B, x_dtype, -1, keys, i4_span{window, sinks, workspace}, stream);
 }
 
 int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64_t q_token_stride,
@@ -167,11 +213,12 @@ int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64
                    workspace_bytes,
                    i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks));
   if (rc) return rc;
-  const Cache8 c8{(uint8_t*)cache->k, (uint8_t*)cache->v, cache->k_scale, cache->v_scale,
-                  (uint16_t*)cache->k_tail, (uint16_t*)cache->v_tail, cache->blocks};
-  return launch(q, x_dtype, cache->format, B, T, q_batch_stride, q_token_stride, q_head_stride,
-                n_heads, nkv, Cache16{}, c8, Tokens{pos_dev, counts, pos, T},
-                Bounds{window ? window : INT32_MAX, sinks}, scale, out, stream);
+  CtxArgs a = ctx_args(q, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
+                       pos, counts, window, sinks, scale, out);
+  a.c8 = Cache8{(uint8_t*)cache->k, (uint8_t*)cache->v, cache->k_scale, cache->v_scale,
+                (uint16_t*)cache->k_tail, (uint16_t*)cache->v_tail, cache->blocks};
+  a.len = len;
+  return launch(a, B, x_dtype, cache->format, keys, i4_span{window, sinks, workspace}, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,517 @@
+// Attention of few query rows (at most 32 per kv head: one token of up to 32 query heads per
+// kv head, or a few tokens) over a long cached context.  Bound by the bytes of the keys and
+// values, so those stream from memory straight into the matrix operands' registers: no LDS,
+// no transposition through it.
+//
+// A wave takes context tiles of its own with a softmax state of its own; the waves of a
+// workgroup and then the S splits of the context are merged at the end.
+//   S^T = K Q^T   (16 keys x 16 rows x 32 dims, v_mfma 16x16x32): lane (m = lane % 16, qd =
+//                 lane / 16) supplies key m's dims, and gets the scores of query row m with
+//                 keys 4 qd + i of the 16.  The keys of a tile are dealt to the 16-key groups
+//                 so that lane qd ends up with the scores of 8 (16-bit cache) or 16 (8-bit)
+//                 adjacent keys,
+//   O^T = V^T P^T (16 dims x 16 rows x 32 keys): which is the operand layout of P^T: the
+//                 weights never leave their lane.  V^T's lane (m, qd) needs dims of the same
+//                 keys: from a 16-bit cache a lane loads 16 bytes (dims 8 m .. 8 m + 7) of
+//                 each of its 8 keys and pairs them with v_perm; 8-bit value blocks are kept
+//                 [dim][token], so 16 bytes are a lane's 16 keys.
+// Product t of the eight covers dims 8 m + t; a lane's sums are dims 32 qd + 8 i + t.
+//
+// The weights enter the product as a sum of two 16-bit numbers (the matrix cores are idle
+// most of the time here), so their rounding does not add to the output's; sums are fp32.
+// The running maximum is only raised when a score exceeds it by 2^kLazy.
+#include "i4_ctx.h"
+
+namespace i4 {
+
+template <int NT> struct RowAcc {
+  f32x4 o[NT][8];
+  float m[NT], l[NT];  // l: this lane's keys alone
+};
+
+__device__ inline float max_qd(float v) {  // over the lanes of a row (qd)
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ inline float sum_qd(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// scores (in place) -> weights; c: scale log2(e) (times the keys' scale); key0: the lane's
+// first key, key0 + 4 k + i the others
+template <int NT, int NK>
+__device__ inline void weights(RowAcc<NT>& acc, f32x4 (&s)[NT][NK], float c, bool partial,
+                               int key0, const int (&p)[NT], const Bounds& w) {
+  bool raise = false;
+  float top[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = s[n][k][i] * c;
+        if (partial) x = sees(w, p[n], key0 + 4 * k + i) ? x : -__builtin_inff();
+        s[n][k][i] = x;
+        mx = fmaxf(mx, x);
+      }
+    top[n] = mx;
+    raise |= mx > acc.m[n] + kLazy;
+  }
+  if (__builtin_amdgcn_ballot_w64(raise)) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float m = fmaxf(acc.m[n], max_qd(top[n]));
+      const float f = m > acc.m[n] ? exp2f(acc.m[n] - m) : 1.f;
+      acc.m[n] = m;
+      acc.l[n] *= f;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) acc.o[n][t] *= f;
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    // a row that has seen nothing yet has m = -inf and scores -inf: weights 0
+    const float base = acc.m[n] == -__builtin_inff() ? 0.f : acc.m[n] - kLift;
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[n][k][i] = __builtin_amdgcn_exp2f(s[n][k][i] - base);
+        acc.l[n] += s[n][k][i];
+      }
+  }
+}
+
+// eight weights as two operands that sum to them
+template <int XT> __device__ inline void split8(f32x4 a, f32x4 b, u32x4& hi, u32x4& lo) {
+  hi = u32x4{pack2<XT>(a[0], a[1]), pack2<XT>(a[2], a[3]), pack2<XT>(b[0], b[1]),
+             pack2<XT>(b[2], b[3])};
+  lo = u32x4{pack2<XT>(a[0] - lo_f32<XT>(hi[0]), a[1] - hi_f32<XT>(hi[0])),
+             pack2<XT>(a[2] - lo_f32<XT>(hi[1]), a[3] - hi_f32<XT>(hi[1])),
+             pack2<XT>(b[0] - lo_f32<XT>(hi[2]), b[1] - hi_f32<XT>(hi[2])),
+             pack2<XT>(b[2] - lo_f32<XT>(hi[3]), b[3] - hi_f32<XT>(hi[3]))};
+}
+
+// 32 positions of a 16-bit cache (or of the tail)
+struct Half16 {
+  u32x4 k[2][4], v[8];
+};
+// kr, vr end behind the last row that any query sees: rows past it read as zeros
+__device__ inline void load_k16(Half16& h, rsrc_t kr, int row0, u32 stride, int m, int qd) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const u32 at = (u32)(row0 + 8 * (m >> 2) + 4 * t + (m & 3)) * stride + 16u * qd;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      h.k[t][c] = __builtin_amdgcn_raw_buffer_load_b128(kr, at + 64u * c, 0, 0);
+  }
+}
+__device__ inline void load_v16(Half16& h, rsrc_t vr, int row0, u32 stride, int m, int qd) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    h.v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, (u32)(row0 + 8 * qd + j) * stride + 16u * m,
+                                                   0, 0);
+}
+template <int XT, int NT>
+__device__ inline void scores16(const Half16& h, const u32x4 (&q)[NT][4], f32x4 (&s)[NT][2]) {
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      s[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[n][t] = mfma16<XT>(h.k[t][c], q[n][c], s[n][t]);
+    }
+}
+
+// Values that a row does not see must not reach it (0 times an infinity is NaN): before the
+// product of a tile that is not seen in full, the values of keys that no row sees are
+// cleared; where rows differ, infinities and NaN are taken out and added to the rows that
+// see them.
+template <int XT, int NT>
+__device__ inline void clean16(RowAcc<NT>& acc, Half16& h, rsrc_t vr, int row0, u32 stride,
+                               int key0, int m, int qd, int plo, int phi, const int (&p)[NT],
+                               const Bounds& w) {
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int key = key0 + 8 * qd + j;
+    // some row sees it: the last one by position, the first one by the window
+    const bool seen = key <= phi && (key > plo - w.window || key < w.sinks);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h.v[j][e] = seen ? h.v[j][e] : 0u;
+      bad |= not_finite<XT>(h.v[j][e]);
+    }
+  }
+  if (plo == phi || !__builtin_amdgcn_ballot_w64(bad)) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h.v[j][e] = finite_pair<XT>(h.v[j][e]);
+  for (int j = 0; j < 32; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // dims 32 qd + 8 i + t
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(
+          vr, (u32)(row0 + j) * stride + 64u * qd + 16u * i, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const bool see = sees(w, p[n], key0 + j);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = lo_f32<XT>(x[e]), b = hi_f32<XT>(x[e]);
+          if (see && !(fabsf(a) < __builtin_inff())) acc.o[n][2 * e][i] += a;
+          if (see && !(fabsf(b) < __builtin_inff())) acc.o[n][2 * e + 1][i] += b;
+        }
+      }
+    }
+  }
+}
+
+template <int XT, int NT>
+__device__ inline void values16(RowAcc<NT>& acc, const Half16& h, const f32x4 (&s)[NT][2]) {
+  u32x4 hi[NT], lo[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) split8<XT>(s[n][0], s[n][1], hi[n], lo[n]);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    u32x4 a, b;  // dims 8 m + 2 e and 8 m + 2 e + 1 of the lane's 8 keys
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a[j] = __builtin_amdgcn_perm(h.v[2 * j + 1][e], h.v[2 * j][e], 0x05040100u);
+      b[j] = __builtin_amdgcn_perm(h.v[2 * j + 1][e], h.v[2 * j][e], 0x07060302u);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      acc.o[n][2 * e] = mfma16<XT>(a, hi[n], acc.o[n][2 * e]);
+      acc.o[n][2 * e] = mfma16<XT>(a, lo[n], acc.o[n][2 * e]);
+      acc.o[n][2 * e + 1] = mfma16<XT>(b, hi[n], acc.o[n][2 * e + 1]);
+      acc.o[n][2 * e + 1] = mfma16<XT>(b, lo[n], acc.o[n][2 * e + 1]);
+    }
+  }
+}
+
+// 64 positions of an 8-bit cache: one block
+struct Block8 {
+  u32x4 k[4][2], v[8];
+  float ks, vs;
+};
+__device__ inline void load_k8(Block8& x, const Cache8& c, int64_t blk, int m, int qd) {
+  const uint8_t* k = c.k + blk * (KBLK * KHD) + (16 * (m >> 2) + (m & 3)) * KHD + 16 * qd;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) x.k[t][u] = ldg16(k + 4 * t * KHD + 64 * u);
+  x.ks = c.ks[blk];
+}
+__device__ inline void load_v8(Block8& x, const Cache8& c, int64_t blk, int m, int qd) {
+  const uint8_t* v = c.v + blk * (KBLK * KHD) + 8 * m * KBLK + 16 * qd;
+#pragma unroll
+  for (int t = 0; t < 8; ++t) x.v[t] = ldg16(v + t * KBLK);
+  x.vs = c.vs[blk];
+}
+template <int XT, int FMT, int NT>
+__device__ inline void scores8(const Block8& x, const u32x4 (&q)[NT][4], f32x4 (&s)[NT][4]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const u32x4 a = cvt8<FMT, XT>(x.k[t][u][0], x.k[t][u][1]);
+      const u32x4 b = cvt8<FMT, XT>(x.k[t][u][2], x.k[t][u][3]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n][t] = mfma16<XT>(a, q[n][2 * u], s[n][t]);
+        s[n][t] = mfma16<XT>(b, q[n][2 * u + 1], s[n][t]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // one key group's conversions at a time
+  }
+}
+// The weights take the values' scale; both enter the product as bf16, whose range holds any
+// scale.  A block with scale NaN is NaN for the rows that see one of its keys.
+template <int FMT, int NT>
+__device__ inline void values8(RowAcc<NT>& acc, const Block8& x, f32x4 (&s)[NT][4], bool partial,
+                               int key0, const int (&p)[NT], const Bounds& w) {
+  u32x4 hi[NT][2], lo[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s[n][k] *= x.vs;
+      if (partial)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][k][i] = sees(w, p[n], key0 + 4 * k + i) ? s[n][k][i] : 0.f;
+    }
+    split8<I4_BF16>(s[n][0], s[n][1], hi[n][0], lo[n][0]);
+    split8<I4_BF16>(s[n][2], s[n][3], hi[n][1], lo[n][1]);
+  }
+#pragma unroll
+  for (int t = 0; t < 8; ++t)
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const u32x4 a = cvt8<FMT, I4_BF16>(x.v[t][2 * g], x.v[t][2 * g + 1]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        acc.o[n][t] = mfma16<I4_BF16>(a, hi[n][g], acc.o[n][t]);
+        acc.o[n][t] = mfma16<I4_BF16>(a, lo[n][g], acc.o[n][t]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Workgroup (split, row tile of 16 NT rows, kv head of a sequence).
+template <int XT, int FMT, int NT>
+__global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(CtxArgs a) {
+  __shared__ __align__(16) float s_o[4][16][KHD + 4];
+  __shared__ float s_m[4][16], s_l[4][16];
+  const int tiles = (a.R + 16 * NT - 1) / (16 * NT);
+  const int split = blockIdx.x % a.S;
+  const int rt = blockIdx.x / a.S % tiles, hb = blockIdx.x / a.S / tiles;
+  const int b = hb / a.nkv, g = hb % a.nkv;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, qd = lane >> 4;
+  const CtxSeq sq = ctx_seq(a, b);
+  const int r0 = rt * 16 * NT;
+  const int tlo = r0 / a.G, thi = min((r0 + 16 * NT - 1) / a.G, sq.fit - 1);
+  const bool any = tlo <= thi;  // a row with something to attend
+  RowAcc<NT> acc;
+  int p[NT];  // this lane's rows' positions; -1 sees nothing
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int t = (r0 + 16 * n + m) / a.G;
+    p[n] = r0 + 16 * n + m < a.R && t < sq.fit ? sq.p0 + t : -1;
+    acc.m[n] = -__builtin_inff();
+    acc.l[n] = 0.f;
+#pragma unroll
+    for (int t8 = 0; t8 < 8; ++t8) acc.o[n][t8] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (any) {
+    const int plo = sq.p0 + tlo, phi = sq.p0 + thi;
+    u32x4 q[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = p[n] < 0 ? tlo * a.G : r0 + 16 * n + m;  // any row that exists
+      const uint16_t* row =
+          a.q + b * a.qbs + (r / a.G) * a.qts + (int64_t)(g * a.G + r % a.G) * a.qhs;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)  // dims as the keys' lanes hold them
+        q[n][c] = ldg16(row + (FMT < 0 ? 32 * c + 8 * qd : 64 * (c >> 1) + 16 * qd + 8 * (c & 1)));
+    }
+    const CtxTiles ct = ctx_tiles(a.w, plo, phi);
+    // this workgroup's tiles, dealt to its waves in turn
+    const int i0 = (int)((int64_t)ct.n * split / a.S);
+    const int i1 = (int)((int64_t)ct.n * (split + 1) / a.S);
+    if constexpr (FMT < 0) {
+      const u32 stride = (u32)a.c.rs * 2u, bytes = (u32)phi * stride + KHD * 2u;
+      const int64_t base = b * a.c.bs + g * a.c.hs;
+      const rsrc_t kr = rsrc(a.c.k + base, bytes), vr = rsrc(a.c.v + base, bytes);
+      Half16 h;
+      // halves of 32 positions: 2 i + (0, 1) of tile i
+      const int e = 2 * i1;
+      int x = 2 * i0 + wave;
+      auto pos0 = [&](int y) { return 64 * ct.at(y >> 1) + 32 * (y & 1); };
+      if (x < e) {
+        load_k16(h, kr, pos0(x), stride, m, qd);
+        load_v16(h, vr, pos0(x), stride, m, qd);
+      }
+      for (; x < e; x += 4) {
+        const int j0 = pos0(x);
+        const bool partial = !all_see(a.w, plo, phi, j0, 32);
+        f32x4 s[NT][2];
+        scores16<XT, NT>(h, q, s);
+        const int jn = pos0(min(x + 4, e - 1));
+        if (x + 4 < e) load_k16(h, kr, jn, stride, m, qd);
+        weights<NT, 2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
+        if (partial) clean16<XT, NT>(acc, h, vr, j0, stride, j0, m, qd, plo, phi, p, a.w);
+        values16<XT, NT>(acc, h, s);
+        if (x + 4 < e) load_v16(h, vr, jn, stride, m, qd);
+      }
+    } else {
+      const int end = sq.p0 + sq.fit, full = end / KBLK;  // finished blocks, then the tail
+      const int64_t hblk = ((int64_t)b * a.nkv + g) * a.c8.blocks;
+      Block8 x8;
+      // the tail's tile is the last one of the list if it is there at all
+      const bool tail = i1 == ct.n && i1 > i0 && ct.at(ct.n - 1) >= full;
+      const int e = i1 - (tail ? 1 : 0);
+      int x = i0 + wave;
+      if (x < e) {
+        load_k8(x8, a.c8, hblk + ct.at(x), m, qd);
+        load_v8(x8, a.c8, hblk + ct.at(x), m, qd);
+      }
+      for (; x < e; x += 4) {
+        const int j0 = 64 * ct.at(x);
+        const bool partial = !all_see(a.w, plo, phi, j0, 64);
+        f32x4 s[NT][4];
+        scores8<XT, FMT, NT>(x8, q, s);
+        const float c = a.c2 * x8.ks;
+        const int64_t nb = hblk + ct.at(min(x + 4, e - 1));
+        if (x + 4 < e) load_k8(x8, a.c8, nb, m, qd);
+        weights<NT, 4>(acc, s, c, partial, j0 + 16 * qd, p, a.w);
+        values8<FMT, NT>(acc, x8, s, partial, j0 + 16 * qd, p, a.w);
+        if (x + 4 < e) load_v8(x8, a.c8, nb, m, qd);
+      }
+      if (tail && wave >= 2) {  // its halves, by the two waves that have the least to do
+        const int j0 = full * KBLK + 32 * (wave - 2);
+        if (j0 <= phi) {
+          const u32 stride = KHD * 2u, bytes = (u32)(phi - full * KBLK + 1) * stride;
+          const int64_t base = ((int64_t)b * a.nkv + g) * (KBLK * KHD);
+          const rsrc_t kr = rsrc(a.c8.kt + base, bytes), vr = rsrc(a.c8.vt + base, bytes);
+          u32x4 qn[NT][4];  // dims in the 16-bit order
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int r = p[n] < 0 ? tlo * a.G : r0 + 16 * n + m;
+            const uint16_t* row =
+                a.q + b * a.qbs + (r / a.G) * a.qts + (int64_t)(g * a.G + r % a.G) * a.qhs;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) qn[n][c] = ldg16(row + 32 * c + 8 * qd);
+          }
+          Half16 h;
+          const int row0 = 32 * (wave - 2);
+          load_k16(h, kr, row0, stride, m, qd);
+          load_v16(h, vr, row0, stride, m, qd);
+          f32x4 s[NT][2];
+          scores16<XT, NT>(h, qn, s);
+          weights<NT, 2>(acc, s, a.c2, true, j0 + 8 * qd, p, a.w);
+          clean16<XT, NT>(acc, h, vr, row0, stride, j0, m, qd, plo, phi, p, a.w);
+          values16<XT, NT>(acc, h, s);
+        }
+      }
+    }
+  }
+  // merge the waves: thread t takes row t / 16, dims 8 (t % 16) .. + 7
+  const int row = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    if (n) __syncthreads();
+    const float l = sum_qd(acc.l[n]);
+    if (qd == 0) {
+      s_m[wave][m] = acc.m[n];
+      s_l[wave][m] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < 8; t += 4)
+        *(f32x4*)&s_o[wave][m][32 * qd + 8 * i + t] =
+            f32x4{acc.o[n][t][i], acc.o[n][t + 1][i], acc.o[n][t + 2][i], acc.o[n][t + 3][i]};
+    __syncthreads();
+    const int r = r0 + 16 * n + row, t = r / a.G;
+    if (r < a.R && t < sq.have) {
+      float M = -__builtin_inff(), L = 0.f, o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = 0.f;
+      for (int v = 0; v < 4; ++v) M = fmaxf(M, s_m[v][row]);
+      for (int v = 0; v < 4; ++v) {
+        if (s_m[v][row] == -__builtin_inff() && s_l[v][row] == 0.f) continue;
+        const float f = exp2f(s_m[v][row] - M);
+        L = fmaf(s_l[v][row], f, L);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(s_o[v][row][d0 + i], f, o[i]);
+      }
+      if (a.S > 1 && t < sq.fit) {
+        const int64_t at = ((int64_t)hb * a.R + r) * a.S + split;
+        if (d0 == 0) *(float2*)(a.ml + 2 * at) = float2{M, L};
+        if (L != 0.f) {  // an empty part is skipped by its sum
+          *(f32x4*)(a.part + at * KHD + d0) = f32x4{o[0], o[1], o[2], o[3]};
+          *(f32x4*)(a.part + at * KHD + d0 + 4) = f32x4{o[4], o[5], o[6], o[7]};
+        }
+      } else if (a.S == 1) {
+        const float inv = t < sq.fit ? 1.0f / L : __builtin_nanf("");
+        u32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = pack2<XT>(o[2 * i] * inv, o[2 * i + 1] * inv);
+        if (!(t < sq.fit)) y = u32x4{} + (u32)Half<XT>::QNAN * 0x10001u;
+        *(u32x4*)(a.out + ctx_out(a, b, g, r) + d0) = y;
+      }
+    }
+  }
+}
+
+// The splits of a row merged, one workgroup a row: thread t takes dims 4 (t % 32) .. + 3 of
+// every eighth split, so that a row's parts are all in flight at once.
+template <int XT> __global__ __launch_bounds__(256) void k_ctx_merge(CtxArgs a) {
+  __shared__ float s_f[kMaxSplits];
+  __shared__ __align__(16) float s_o[8][KHD];
+  __shared__ float s_l[4];
+  const int64_t at = blockIdx.x;  // (sequence, kv head, row)
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int64_t hb = at / a.R;
+  const int r = (int)(at % a.R), t = r / a.G, b = (int)(hb / a.nkv), g = (int)(hb % a.nkv);
+  const CtxSeq sq = ctx_seq(a, b);
+  if (t >= sq.have) return;
+  u32* y = (u32*)(a.out + ctx_out(a, b, g, r));
+  if (t >= sq.fit) {
+    if (tid < KHD / 2) y[tid] = (u32)Half<XT>::QNAN * 0x10001u;
+    return;
+  }
+  const float2* ml = (const float2*)a.ml + at * a.S;
+  float M = -__builtin_inff();
+  for (int s = lane; s < a.S; s += 64) M = fmaxf(M, ml[s].x);
+  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
+  float L = 0.f;
+  for (int s = tid; s < a.S; s += 256) {
+    const float2 v = ml[s];
+    const float f = v.y == 0.f ? 0.f : exp2f(v.x - M);  // 0: nothing seen there, no part written
+    s_f[s] = f;
+    L = fmaf(v.y, f, L);
+  }
+  L = group_sum<64>(L);
+  if (lane == 0) s_l[wave] = L;
+  __syncthreads();
+  L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+  const int part = tid >> 5, d = 4 * (tid & 31);
+  const float* src = a.part + at * a.S * KHD + d;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = part; s < a.S; s += 8) {
+    const f32x4 x = *(const f32x4*)(src + (int64_t)s * KHD);
+    const float f = s_f[s];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = f == 0.f ? o[i] : fmaf(x[i], f, o[i]);
+  }
+  *(f32x4*)&s_o[part][d] = o;
+  __syncthreads();
+  if (tid < KHD / 2) {
+    float u = 0.f, v = 0.f;
+    for (int i = 0; i < 8; ++i) {
+      u += s_o[i][2 * tid];
+      v += s_o[i][2 * tid + 1];
+    }
+    y[tid] = pack2<XT>(u / L, v / L);
+  }
+}
+
+template <int XT, int FMT> static void rows_go(const CtxArgs& a, int B, hipStream_t s) {
+  const int nt = a.R <= 16 ? 1 : 2;
+  const dim3 grid((unsigned)(a.S * B * a.nkv * ((a.R + 16 * nt - 1) / (16 * nt))));
+  if (nt == 1) k_ctx_rows<XT, FMT, 1><<<grid, 256, 0, s>>>(a);
+  else k_ctx_rows<XT, FMT, 2><<<grid, 256, 0, s>>>(a);
+}
+
+}  // namespace i4
+
+int i4_launch_ctx_merge(const i4::CtxArgs& a, int B, int xt, hipStream_t s) {
+  const dim3 grid((unsigned)(B * a.nkv * a.R));
+  if (xt == I4_F16) i4::k_ctx_merge<I4_F16><<<grid, 256, 0, s>>>(a);
+  else i4::k_ctx_merge<I4_BF16><<<grid, 256, 0, s>>>(a);
+  return hipGetLastError() == hipSuccess ? I4_OK : I4_ERR_LAUNCH;
+}
+
+int i4_launch_ctx_rows(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t s) {
+  using namespace i4;
+  if (xt == I4_F16) {
+    if (fmt < 0) rows_go<I4_F16, -1>(a, B, s);
+    else if (fmt == I4_KV8_INT8) rows_go<I4_F16, I4_KV8_INT8>(a, B, s);
+    else rows_go<I4_F16, I4_KV8_E4M3>(a, B, s);
+  } else {
+    if (fmt < 0) rows_go<I4_BF16, -1>(a, B, s);
+    else if (fmt == I4_KV8_INT8) rows_go<I4_BF16, I4_KV8_INT8>(a, B, s);
+    else rows_go<I4_BF16, I4_KV8_E4M3>(a, B, s);
+  }
+  if (hipGetLastError() != hipSuccess) return I4_ERR_LAUNCH;
+  return a.S > 1 ? i4_launch_ctx_merge(a, B, xt, s) : I4_OK;
+}
