@@ -11,6 +11,8 @@
 namespace i4 {
 
 static constexpr int kMaxSplits = 1024;  // of one context
+static constexpr int kFewRows = 32;      // of a kv head: k_ctx_rows up to here
+static constexpr int kTileRows = 128;    // of a workgroup of k_ctx_tile
 
 struct CtxArgs {
   const uint16_t* q;
@@ -22,6 +24,7 @@ struct CtxArgs {
   Bounds w;
   int32_t nq, nkv, G, R;  // R = T G rows of a kv head
   int32_t len;            // positions of the cache
+  int32_t tiles;          // row tiles of a kv head
   int32_t S;              // splits of the context
   float c2;               // scale log2(e): weights are powers of two
   float* part;            // [B nkv R][S][128] sums of e v, then
@@ -151,4 +154,5 @@ template <int XT> __device__ inline u32 finite_pair(u32 x) {
 
 // i4_ctx_rows.hip / i4_ctx_tile.hip; fmt: -1 (16-bit cache) or I4_KV8_*
 int i4_launch_ctx_merge(const i4::CtxArgs& a, int B, int xt, hipStream_t s);
+int i4_launch_ctx_tile(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t s);
 int i4_launch_ctx_rows(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t s);

@@ -13,80 +13,24 @@ struct i4_span {
 
 namespace i4 {
 
-// One wave per query row: lane l holds dims 2l and 2l + 1.
-template <int XT, int FMT>
-__global__ __launch_bounds__(256) void k_ctx_row(const uint16_t* __restrict__ q, int64_t qbs,
-                                                 int64_t qts, int64_t qhs, int nq, int nkv,
-                                                 Cache16 c, Cache8 c8, Tokens tk, Bounds w,
-                                                 float scale, uint16_t* __restrict__ out,
-                                                 int64_t n_rows) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // (b, t, head)
-  if (row >= n_rows) return;
-  const int lane = threadIdx.x & 63;
-  const int h = (int)(row % nq);
-  const int64_t bt = row / nq;
-  const int b = (int)(bt / tk.T), t = (int)(bt % tk.T), g = h / (nq / nkv);
-  const int n = count_of(tk, b);
-  if (t >= n) return;
-  u32* dst = (u32*)(out + row * KHD) + lane;
-  const int p0 = first_pos(tk, b);
-  const int len = FMT < 0 ? c.max_len : c8.blocks * KBLK;
-  if (p0 < 0 || p0 >= len || t >= len - p0) {
-    *dst = (u32)Half<XT>::QNAN * 0x10001u;
-    return;
-  }
-  const int p = p0 + t, end = p0 + min(n, len - p0), tail0 = end / KBLK * KBLK;
-  const u32 qr = *((const u32*)(q + b * qbs + t * qts + h * qhs) + lane);
-  const float q0 = Half<XT>::to_f32((uint16_t)qr) * scale;
-  const float q1 = Half<XT>::to_f32((uint16_t)(qr >> 16)) * scale;
-  const int64_t hb = (int64_t)b * nkv + g;
-  float m = -__builtin_inff(), l = 0.f, a0 = 0.f, a1 = 0.f;
-  const int lo = max(0, p - w.window + 1), s = min(w.sinks, lo);
-  for (int i = 0; i < s + (p + 1 - lo); ++i) {
-    const int j = i < s ? i : lo + i - s;
-    float k0, k1, v0, v1;
-    if (FMT < 0 || j >= tail0) {
-      const int64_t o = FMT < 0 ? b * c.bs + g * c.hs + (int64_t)j * c.rs
-                                : (hb * KBLK + j - tail0) * KHD;
-      const u32 kr = *((const u32*)((FMT < 0 ? c.k : c8.kt) + o) + lane);
-      const u32 vr = *((const u32*)((FMT < 0 ? c.v : c8.vt) + o) + lane);
-      k0 = Half<XT>::to_f32((uint16_t)kr), k1 = Half<XT>::to_f32((uint16_t)(kr >> 16));
-      v0 = Half<XT>::to_f32((uint16_t)vr), v1 = Half<XT>::to_f32((uint16_t)(vr >> 16));
-    } else {
-      constexpr int F = FMT < 0 ? 0 : FMT;
-      const int64_t blk = hb * c8.blocks + j / KBLK;
-      const uint8_t *kb = c8.k + blk * KBLK * KHD, *vb = c8.v + blk * KBLK * KHD;
-      const float ks = c8.ks[blk], vs = c8.vs[blk];
-      const int r = j % KBLK;
-      k0 = from_8bit<F>(kb[r * KHD + 2 * lane]) * ks;
-      k1 = from_8bit<F>(kb[r * KHD + 2 * lane + 1]) * ks;
-      v0 = from_8bit<F>(vb[2 * lane * KBLK + r]) * vs;
-      v1 = from_8bit<F>(vb[(2 * lane + 1) * KBLK + r]) * vs;
-    }
-    const float x = group_sum<64>(q0 * k0 + q1 * k1);
-    const float mn = fmaxf(m, x);
-    const float f = expf(m - mn), e = expf(x - mn);
-    l = l * f + e;
-    a0 = a0 * f + e * v0;
-    a1 = a1 * f + e * v1;
-    m = mn;
-  }
-  const float inv = 1.0f / l;
-  *dst = (u32)Half<XT>::from_f32(a0 * inv) | ((u32)Half<XT>::from_f32(a1 * inv) << 16);
-}
-
 // How a call is split: a rule on its sizes alone (no device value), so that the workspace
 // can be named before the call.
+static int ctx_tiles_of(int R) {
+  return R <= 16 ? 1 : R <= kFewRows ? (R + 31) / 32 : (R + kTileRows - 1) / kTileRows;
+}
 static int ctx_splits(int B, int T, int nq, int nkv, int keys, int window, int sinks) {
   const int R = T * (nq / nkv);
-  if (R > 32) return 1;
+  const bool few = R <= kFewRows;
+  // the context tiles of 64 that one row tile sees at most
+  const int64_t span = few ? T : (kTileRows + nq / nkv - 1) / (nq / nkv) + 1;
   int64_t tiles = (keys + 63) / 64;
   if (window) {
-    const int64_t most = ((int64_t)window + T + 126) / 64 + (sinks + 63) / 64;
+    const int64_t most = ((int64_t)window + span + 126) / 64 + (sinks + 63) / 64;
     if (most < tiles) tiles = most;
   }
-  const int64_t want = (1024 + (int64_t)B * nkv - 1) / ((int64_t)B * nkv);
-  const int64_t most = (tiles + 3) / 4;  // a tile a wave
+  const int64_t wgs = (int64_t)B * nkv * ctx_tiles_of(R);
+  const int64_t want = ((few ? 1024 : 512) + wgs - 1) / wgs;
+  const int64_t most = (tiles + 3) / 4;  // few: a tile a wave
   const int64_t s = want < most ? want : most;
   return s < 1 ? 1 : (int)s;
 }
@@ -98,24 +42,9 @@ static int launch(CtxArgs& a, int B, int xt, int fmt, int keys, const i4_span& w
     a.part = (float*)w.workspace;
     a.ml = a.part + (int64_t)B * a.nkv * a.R * a.S * KHD;
   }
-  if (a.R <= 32) return i4_launch_ctx_rows(a, B, xt, fmt, stream);
-  const int64_t rows = (int64_t)B * a.tk.T * a.nq;
-  const dim3 grid((unsigned)((rows + 3) / 4));
-  const float scale = a.c2 * 0.69314718f;
-  auto go = [&](auto kern) {
-    kern<<<grid, 256, 0, stream>>>(a.q, a.qbs, a.qts, a.qhs, a.nq, a.nkv, a.c, a.c8, a.tk, a.w,
-                                   scale, a.out, rows);
-  };
-  if (xt == I4_F16) {
-    if (fmt < 0) go(k_ctx_row<I4_F16, -1>);
-    else if (fmt == I4_KV8_INT8) go(k_ctx_row<I4_F16, I4_KV8_INT8>);
-    else go(k_ctx_row<I4_F16, I4_KV8_E4M3>);
-  } else {
-    if (fmt < 0) go(k_ctx_row<I4_BF16, -1>);
-    else if (fmt == I4_KV8_INT8) go(k_ctx_row<I4_BF16, I4_KV8_INT8>);
-    else go(k_ctx_row<I4_BF16, I4_KV8_E4M3>);
-  }
-  return hipGetLastError() == hipSuccess ? I4_OK : I4_ERR_LAUNCH;
+  a.tiles = ctx_tiles_of(a.R);
+  return a.R <= kFewRows ? i4_launch_ctx_rows(a, B, xt, fmt, stream)
+                         : i4_launch_ctx_tile(a, B, xt, fmt, stream);
 }
 
 }  // namespace i4

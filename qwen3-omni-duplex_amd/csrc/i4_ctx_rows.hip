@@ -269,9 +269,8 @@ template <int XT, int FMT, int NT>
 __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(CtxArgs a) {
   __shared__ __align__(16) float s_o[4][16][KHD + 4];
   __shared__ float s_m[4][16], s_l[4][16];
-  const int tiles = (a.R + 16 * NT - 1) / (16 * NT);
   const int split = blockIdx.x % a.S;
-  const int rt = blockIdx.x / a.S % tiles, hb = blockIdx.x / a.S / tiles;
+  const int rt = blockIdx.x / a.S % a.tiles, hb = blockIdx.x / a.S / a.tiles;
   const int b = hb / a.nkv, g = hb % a.nkv;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, qd = lane >> 4;
   const CtxSeq sq = ctx_seq(a, b);
@@ -487,7 +486,7 @@ template <int XT> __global__ __launch_bounds__(256) void k_ctx_merge(CtxArgs a) 
 
 template <int XT, int FMT> static void rows_go(const CtxArgs& a, int B, hipStream_t s) {
   const int nt = a.R <= 16 ? 1 : 2;
-  const dim3 grid((unsigned)(a.S * B * a.nkv * ((a.R + 16 * nt - 1) / (16 * nt))));
+  const dim3 grid((unsigned)(a.S * a.tiles * B * a.nkv));
   if (nt == 1) k_ctx_rows<XT, FMT, 1><<<grid, 256, 0, s>>>(a);
   else k_ctx_rows<XT, FMT, 2><<<grid, 256, 0, s>>>(a);
 }
