@@ -701,7 +701,8 @@ typedef struct i4_kv8cache {
  * (Qwen3OmniMoeThinkerTextAttention.forward, modeling_qwen3_omni_moe.py:1473-1500 in
  * transformers 5.15), for many tokens.
  *   qkv    token t of sequence b at qkv + b batch_stride + t token_stride (elements),
- *          [n_heads + 2 n_kv_heads][head_dim], 4-byte aligned rows, x_dtype == cache->dtype;
+ *          [n_heads + 2 n_kv_heads][head_dim], 16-byte aligned as the norm weights are,
+ *          x_dtype == cache->dtype;
  *   q_out  [B][T][n_heads][head_dim], dense: the rotated queries;
  *   cache  row (first_row or p's own) + t of each kv head receives the token's rotated key
  *          and its value.  first_row < 0: the row is the position; >= 0: token t goes to row

@@ -10,22 +10,34 @@ namespace i4 {
 
 // x / s as fp32 rounded to odd: a quotient that fp32 does not hold gets an odd last bit, so
 // rounding it to the element's few bits afterwards rounds as the exact quotient would (a
-// nearest fp32 quotient could land on a tie that the exact one misses).  The remainder of a
-// correctly rounded quotient is exact in one fma.
-__device__ inline float quotient_to_odd(float x, float s) {
-  const float t = x / s;
+// nearest fp32 quotient could land on a tie that the exact one misses).  inv = 1 / s rounded;
+// one Newton step makes the product the quotient to within its last bit, and then the
+// remainder of the next fma is exact and says on which side of it the quotient lies.
+__device__ inline float quotient_to_odd(float x, float s, float inv) {
+  float t = x * inv;
+  t = fmaf(fmaf(-t, s, x), inv, t);
   const float r = fmaf(-t, s, x);
   const u32 b = __builtin_bit_cast(u32, t);
-  if (r == 0.f || (b & 1)) return t;
-  // |exact| > |t| when the remainder has t's sign: the odd neighbour lies on that side
-  const bool away = (r > 0.f) == (t > 0.f);
-  return __builtin_bit_cast(float, away ? b + 1 : b - 1);
+  // an even last bit and a remainder: the odd neighbour on the remainder's side
+  const u32 odd = (r > 0.f) == (t > 0.f) ? b + 1 : b - 1;
+  return __builtin_bit_cast(float, r == 0.f || (b & 1) ? b : odd);
 }
-
-template <int FMT> __device__ inline uint8_t to_8bit(float x, float s) {
-  const float y = quotient_to_odd(x, s);
-  if constexpr (FMT == I4_KV8_INT8) return (uint8_t)(int8_t)(int)rintf(y);
-  else return (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y, y, 0, false);
+// four elements in a word
+template <int FMT> __device__ inline u32 pack_8bit(float a, float b, float c, float d) {
+  if constexpr (FMT == I4_KV8_INT8) {
+    const u32 lo = ((u32)(int)rintf(a) & 0xFFu) | (((u32)(int)rintf(b) & 0xFFu) << 8);
+    return lo | (((u32)(int)rintf(c) & 0xFFu) << 16) | ((u32)(int)rintf(d) << 24);
+  } else {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (u32)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+  }
+}
+template <int XT> __device__ inline void widen8(u32x4 x, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = Half<XT>::to_f32((uint16_t)x[i]);
+    f[2 * i + 1] = Half<XT>::to_f32((uint16_t)(x[i] >> 16));
+  }
 }
 
 // Workgroup (touched block i of the sequence, kv head, sequence; keys or values).  The
@@ -33,12 +45,17 @@ template <int FMT> __device__ inline uint8_t to_8bit(float x, float s) {
 // A finished block is scaled and written; an unfinished one's new tokens go to the tail.
 // The first block reads the tail that the last one overwrites, so the first block's
 // workgroup does the last, unfinished block too, behind its own.
+// Thread t holds dims 8 (t % 16) .. + 7 of tokens 4 (t / 16) .. + 3: whole rows in a wave's
+// loads; a key row's 8 bytes are stored as they are, four tokens of a value dim make a word,
+// which LDS brings into rows.  Bound by the divisions (about 10 instructions an element) for
+// prompts: 4001 tokens of four heads take 7 us.
 template <int XT, int FMT>
 __global__ __launch_bounds__(256) void k_kv8_append(const uint16_t* __restrict__ k,
                                                     const uint16_t* __restrict__ v, int64_t bs,
                                                     int64_t ts, int64_t hs, int nkv, Tokens tk,
                                                     Cache8 c) {
   __shared__ float s_max[4];
+  __shared__ __align__(16) u32 s_t[KHD][KBLK / 4 + 1];  // a dim's tokens, padded
   const bool val = blockIdx.y & 1;
   const int g = (blockIdx.y >> 1) % nkv, b = (blockIdx.y >> 1) / nkv;
   const int p0 = first_pos(tk, b), len = c.blocks * KBLK;
@@ -48,62 +65,115 @@ __global__ __launch_bounds__(256) void k_kv8_append(const uint16_t* __restrict__
   const int64_t hb = (int64_t)b * nkv + g;
   const uint16_t* src = (val ? v : k) + b * bs + g * hs;
   uint16_t* tail = (val ? c.vt : c.kt) + hb * KBLK * KHD;
-  const int i = blockIdx.x;
-  // thread t holds dims [32 (t & 3), +32) of token t >> 2
-  const int tok = threadIdx.x >> 2, d0 = 32 * (threadIdx.x & 3);
+  const int i = blockIdx.x, tid = threadIdx.x;
+  const int d0 = 8 * (tid & 15), tok = 4 * (tid >> 4);
   if (i < done) {
-    const int n0 = i * KBLK + tok - r;  // the call's token, or one of the tail's
-    const uint16_t* row = n0 >= 0 ? src + n0 * ts : tail + (int64_t)tok * KHD;
     u32x4 x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = ldg16(row + d0 + 8 * u);
-    float f[32], m = KV8_TINY;
+    for (int j = 0; j < 4; ++j) {
+      const int at = i * KBLK + tok + j - r;  // the call's token, or one of the tail's
+      x[j] = ldg16((at >= 0 ? src + at * ts : tail + (int64_t)(tok + j) * KHD) + d0);
+    }
+    float f[4][8], m = KV8_TINY;
     bool bad = false;  // an infinity or a NaN
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      f[e] = Half<XT>::to_f32((uint16_t)(x[e >> 3][(e >> 1) & 3] >> (16 * (e & 1))));
-      bad |= !(fabsf(f[e]) < __builtin_inff());
-      m = fmaxf(m, fabsf(f[e]));
+    for (int j = 0; j < 4; ++j) {
+      widen8<XT>(x[j], f[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        bad |= !(fabsf(f[j][e]) < __builtin_inff());
+        m = fmaxf(m, fabsf(f[j][e]));
+      }
     }
     if (bad) m = __builtin_inff();
     for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
+    if ((tid & 63) == 0) s_max[tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
     const bool finite = m < __builtin_inff();
     const float scale = finite ? m / (FMT == I4_KV8_INT8 ? 127.f : 448.f) : __builtin_nanf("");
+    const float inv = 1.0f / scale;
     const int64_t blk = hb * c.blocks + first + i;
     uint8_t* dst = (val ? c.v : c.k) + blk * KBLK * KHD;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      const uint8_t q = finite ? to_8bit<FMT>(f[e], scale) : 0;
-      if (val) dst[(d0 + e) * KBLK + tok] = q;
-      else dst[tok * KHD + d0 + e] = q;
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[j][e] = finite ? quotient_to_odd(f[j][e], scale, inv) : 0.f;
+    if (val) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        s_t[d0 + e][tid >> 4] = pack_8bit<FMT>(f[0][e], f[1][e], f[2][e], f[3][e]);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // 16 words a dim
+        const int w = 256 * j + tid;
+        ((u32*)dst)[w] = s_t[w >> 4][w & 15];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(u32x2*)(dst + (tok + j) * KHD + d0) =
+            u32x2{pack_8bit<FMT>(f[j][0], f[j][1], f[j][2], f[j][3]),
+                  pack_8bit<FMT>(f[j][4], f[j][5], f[j][6], f[j][7])};
     }
-    if (threadIdx.x == 0) (val ? c.vs : c.ks)[blk] = scale;
+    if (tid == 0) (val ? c.vs : c.ks)[blk] = scale;
     __syncthreads();  // the tail has been read
   }
   if (i == 0) {
-    const int n0 = done * KBLK + tok - r;
-    if (n0 >= 0 && n0 < n) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        *(u32x4*)(tail + (int64_t)tok * KHD + d0 + 8 * u) = ldg16(src + n0 * ts + d0 + 8 * u);
+    for (int j = 0; j < 4; ++j) {
+      const int at = done * KBLK + tok + j - r;
+      if (at >= 0 && at < n)
+        *(u32x4*)(tail + (int64_t)(tok + j) * KHD + d0) = ldg16(src + at * ts + d0);
     }
   }
 }
 
+// The blocks' values in fp32, 16 bytes a lane; value blocks turn through LDS, four dims of
+// four tokens at a time.
 template <int FMT>
 __global__ __launch_bounds__(256) void k_kv8_values(Cache8 c, float* __restrict__ ko,
                                                     float* __restrict__ vo) {
+  __shared__ u32 s_t[KHD][KBLK / 4 + 1];
   const int64_t blk = blockIdx.x;
-  const bool val = blockIdx.y;
-  const uint8_t* src = (val ? c.v : c.k) + blk * KBLK * KHD;
-  const float scale = (val ? c.vs : c.ks)[blk];
-  float* dst = (val ? vo : ko) + blk * KBLK * KHD;
-  for (int e = threadIdx.x; e < KBLK * KHD; e += 256) {
-    const int tok = e / KHD, d = e % KHD;
-    dst[e] = from_8bit<FMT>(src[val ? d * KBLK + tok : e]) * scale;
+  const int tid = threadIdx.x;
+  auto four = [](u32 w, float s) {
+    return f32x4{from_8bit<FMT>((uint8_t)w) * s, from_8bit<FMT>((uint8_t)(w >> 8)) * s,
+                 from_8bit<FMT>((uint8_t)(w >> 16)) * s, from_8bit<FMT>((uint8_t)(w >> 24)) * s};
+  };
+  if (blockIdx.y == 0) {
+    const u32* src = (const u32*)(c.k + blk * KBLK * KHD);
+    const float s = c.ks[blk];
+    f32x4* dst = (f32x4*)(ko + blk * KBLK * KHD);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dst[256 * j + tid] = four(src[256 * j + tid], s);
+    return;
+  }
+  const u32* src = (const u32*)(c.v + blk * KBLK * KHD);
+  const float s = c.vs[blk];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int w = 256 * j + tid;
+    s_t[w >> 4][w & 15] = src[w];
+  }
+  __syncthreads();
+  const int d = 4 * (tid & 31);
+  f32x4* dst = (f32x4*)(vo + blk * KBLK * KHD) + (tid & 31);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int q = (tid >> 5) + 8 * j;  // tokens 4 q .. + 3
+    const u32 w[4] = {s_t[d][q], s_t[d + 1][q], s_t[d + 2][q], s_t[d + 3][q]};
+    // bytes (dim, token) -> (token, dim)
+    const u32 a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);
+    const u32 b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    const u32 e = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const u32 f = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    const u32 y[4] = {__builtin_amdgcn_perm(b, a, 0x05040100u),
+                      __builtin_amdgcn_perm(b, a, 0x07060302u),
+                      __builtin_amdgcn_perm(f, e, 0x05040100u),
+                      __builtin_amdgcn_perm(f, e, 0x07060302u)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[(4 * q + i) * (KHD / 4)] = four(y[i], s);
   }
 }
 
