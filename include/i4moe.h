@@ -724,12 +724,17 @@ int    i4_rope_append(const void* qkv, int x_dtype, int T, int64_t batch_stride,
  * (elements, 16-byte aligned rows), x_dtype == cache->dtype; out dense
  * [B][T][n_heads][head_dim], rounded once from fp32.  Workspace:
  * i4_attn_window_workspace_bytes with keys = pos + T, or max_len for a device position;
- * no initial contents, 256-byte aligned; calls sharing one must not overlap. */
+ * no initial contents, 256-byte aligned; calls sharing one must not overlap.  counters
+ * (nullable): I4_CTX_COUNTERS int32, zero when they are allocated and left zero by every
+ * call, shared as the workspace is; with them the parts of a context that few query rows
+ * are split over are merged by the last workgroup of the launch instead of a second one. */
+#define I4_CTX_COUNTERS 1024
 int    i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                       int64_t q_token_stride, int64_t q_head_stride, int n_heads,
                       const i4_kvcache* cache, const int32_t* pos_dev, int pos,
                       const int32_t* counts, int window, int sinks, float scale, void* out,
-                      void* workspace, size_t workspace_bytes, hipStream_t stream);
+                      void* workspace, size_t workspace_bytes, int32_t* counters,
+                      hipStream_t stream);
 size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                       int window, int sinks);
 
@@ -757,7 +762,8 @@ int    i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    int64_t q_token_stride, int64_t q_head_stride, int n_heads,
                    const i4_kv8cache* cache, const int32_t* pos_dev, int pos,
                    const int32_t* counts, int window, int sinks, float scale, void* out,
-                   void* workspace, size_t workspace_bytes, hipStream_t stream);
+                   void* workspace, size_t workspace_bytes, int32_t* counters,
+                   hipStream_t stream);
 
 /* ------------------------------------------------------------------------
  * No counterpart in the reference.  For callers that cannot allocate device

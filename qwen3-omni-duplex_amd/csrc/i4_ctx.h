@@ -29,6 +29,7 @@ struct CtxArgs {
   float c2;               // scale log2(e): weights are powers of two
   float* part;            // [B nkv R][S][128] sums of e v, then
   float* ml;              // [B nkv R][S][2] maximum and sum
+  int32_t* counters;      // nullable: parts of a row tile that are done, 0 between calls
 };
 
 // The context tiles (64 positions) that rows at positions [plo, phi] see: ns tiles with the
@@ -69,6 +70,9 @@ __device__ inline int64_t ctx_out(const CtxArgs& a, int b, int g, int r) {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// by value: a bit_cast of a vector's element would read element 0
+__device__ inline float as_f32(u32 x) { return __builtin_bit_cast(float, x); }
 
 template <int XT> __device__ inline f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
   if constexpr (XT == I4_F16)

@@ -9,6 +9,7 @@
 struct i4_span {
   int window, sinks;
   void* workspace;
+  int32_t* counters;
 };
 
 namespace i4 {
@@ -43,6 +44,9 @@ static int launch(CtxArgs& a, int B, int xt, int fmt, int keys, const i4_span& w
     a.ml = a.part + (int64_t)B * a.nkv * a.R * a.S * KHD;
   }
   a.tiles = ctx_tiles_of(a.R);
+  a.counters = a.S > 1 && a.R <= kFewRows && (int64_t)B * a.nkv * a.tiles <= I4_CTX_COUNTERS
+                   ? w.counters
+                   : nullptr;
   return a.R <= kFewRows ? i4_launch_ctx_rows(a, B, xt, fmt, stream)
                          : i4_launch_ctx_tile(a, B, xt, fmt, stream);
 }
@@ -71,7 +75,7 @@ static int query_check(const void* q, int x_dtype, int dtype, int B, int T, int6
                        int64_t qts, int64_t qhs, int n_heads, int nkv, const int32_t* pos_dev,
                        int pos, const int32_t* counts, int limit, int window, int sinks,
                        float scale, const void* out, const void* workspace, size_t have,
-                       size_t need) {
+                       size_t need, const int32_t* counters) {
   if (!q || !out) return I4_ERR_NULL;
   if (x_dtype != dtype) return I4_ERR_DTYPE;
   const int rc = i4_check_tokens(B, T, n_heads, nkv, pos_dev, pos, counts, limit);
@@ -81,7 +85,8 @@ static int query_check(const void* q, int x_dtype, int dtype, int B, int T, int6
     return I4_ERR_SHAPE;
   if ((T > 1 && qts < i4::KHD) || (B > 1 && qbs < i4::KHD) || (n_heads > 1 && qhs < i4::KHD))
     return I4_ERR_STRIDE;
-  if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || (qbs & 7) || (qts & 7) || (qhs & 7))
+  if (((uintptr_t)counters & 3) || ((uintptr_t)q & 15) || ((uintptr_t)out & 15) || (qbs & 7) ||
+      (qts & 7) || (qhs & 7))
     return I4_ERR_ALIGN;
   if (need) {
     if (!workspace || have < need) return I4_ERR_WORKSPACE;
@@ -108,7 +113,8 @@ int i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    int64_t q_token_stride, int64_t q_head_stride, int n_heads,
                    const i4_kvcache* cache, const int32_t* pos_dev, int pos,
                    const int32_t* counts, int window, int sinks, float scale, void* out,
-                   void* workspace, size_t workspace_bytes, hipStream_t stream) {
+                   void* workspace, size_t workspace_bytes, int32_t* counters,
+                   hipStream_t stream) {
   using namespace i4;
   int rc = i4_check_kvcache(cache);
   if (rc) return rc;
@@ -117,21 +123,22 @@ int i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
   rc = query_check(q, x_dtype, cache->dtype, B, T, q_batch_stride, q_token_stride, q_head_stride,
                    n_heads, nkv, pos_dev, pos, counts, cache->max_len, window, sinks, scale, out,
                    workspace, workspace_bytes,
-                   i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks));
+                   i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
+                   counters);
   if (rc) return rc;
   CtxArgs a = ctx_args(q, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
                        pos, counts, window, sinks, scale, out);
   a.c = Cache16{(uint16_t*)cache->k, (uint16_t*)cache->v, cache->batch_stride,
                 cache->head_stride, cache->row_stride, cache->max_len};
   a.len = cache->max_len;
-  return launch(a, B, x_dtype, -1, keys, i4_span{window, sinks, workspace}, stream);
+  return launch(a, B, x_dtype, -1, keys, i4_span{window, sinks, workspace, counters}, stream);
 }
 
 int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64_t q_token_stride,
                 int64_t q_head_stride, int n_heads, const i4_kv8cache* cache,
                 const int32_t* pos_dev, int pos, const int32_t* counts, int window, int sinks,
                 float scale, void* out, void* workspace, size_t workspace_bytes,
-                hipStream_t stream) {
+                int32_t* counters, hipStream_t stream) {
   using namespace i4;
   int rc = i4_check_kv8cache(cache);
   if (rc) return rc;
@@ -140,14 +147,16 @@ int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64
   rc = query_check(q, x_dtype, cache->dtype, B, T, q_batch_stride, q_token_stride, q_head_stride,
                    n_heads, nkv, pos_dev, pos, counts, len, window, sinks, scale, out, workspace,
                    workspace_bytes,
-                   i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks));
+                   i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
+                   counters);
   if (rc) return rc;
   CtxArgs a = ctx_args(q, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
                        pos, counts, window, sinks, scale, out);
   a.c8 = Cache8{(uint8_t*)cache->k, (uint8_t*)cache->v, cache->k_scale, cache->v_scale,
                 (uint16_t*)cache->k_tail, (uint16_t*)cache->v_tail, cache->blocks};
   a.len = len;
-  return launch(a, B, x_dtype, cache->format, keys, i4_span{window, sinks, workspace}, stream);
+  return launch(a, B, x_dtype, cache->format, keys, i4_span{window, sinks, workspace, counters},
+                stream);
 }
 
 }  // extern "C"

@@ -264,11 +264,85 @@ __device__ inline void values8(RowAcc<NT>& acc, const Block8& x, f32x4 (&s)[NT][
     }
 }
 
+// Parts go past the caches of this XCD (sc1), as the workgroup that merges them may run on
+// another: stored through, counted when the stores are done, read from memory.
+__device__ inline void put_part(float* p, float a, float b) {
+  const uint64_t v = (uint64_t)__builtin_bit_cast(u32, a) | (uint64_t)__builtin_bit_cast(u32, b)
+                                                                 << 32;
+  __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Rows [r0, r1) of the row tile from their S parts, by the whole workgroup: four rows at a
+// time, a wave each; lane (x = lane / 32) takes dims 4 (lane % 32) .. + 3 of every second
+// part, eight parts in flight.
+template <int XT>
+__device__ inline void merge_tile(const CtxArgs& a, int b, int g, int hb, const CtxSeq& sq,
+                                  int r0, int r1) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int x = lane >> 5, d = 4 * (lane & 31);
+  for (int r = r0 + wave; r < r1; r += 4) {
+    const int t = r / a.G;
+    if (t >= sq.have) continue;
+    u32x2* y = (u32x2*)(a.out + ctx_out(a, b, g, r) + d);
+    if (t >= sq.fit) {
+      if (x == 0) *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
+      continue;
+    }
+    const int64_t at = ((int64_t)hb * a.R + r) * a.S;
+    const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * a.S);
+    const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * a.S);
+    float M = -__builtin_inff(), L = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 8;
+    for (int s0 = x; s0 < a.S; s0 += 2 * U) {
+      u32x2 v[U];
+      u32x4 w[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {  // reads past the parts are zeros: an empty part
+        v[i] = __builtin_amdgcn_raw_buffer_load_b64(ml, 8u * (s0 + 2 * i), 0, kCoherent);
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(part, 4u * (KHD * (s0 + 2 * i) + d), 0,
+                                                     kCoherent);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      float mb = M;
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        mb = fmaxf(mb, as_f32(v[i][1]) == 0.f
+                           ? mb : as_f32(v[i][0]));
+      const float f0 = M == mb ? 1.f : exp2f(M - mb);
+      L *= f0;
+      o *= f0;
+      M = mb;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const float l = as_f32(v[i][1]);
+        if (l == 0.f) continue;
+        const float f = exp2f(as_f32(v[i][0]) - M);
+        L = fmaf(l, f, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(as_f32(w[i][e]), f, o[e]);
+      }
+    }
+    // the two halves of the wave
+    const float M2 = __shfl_xor(M, 32), top = fmaxf(M, M2);
+    const float f = M == top ? 1.f : exp2f(M - top);
+    L *= f;
+    L += __shfl_xor(L, 32);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[e] *= f;
+      o[e] += __shfl_xor(o[e], 32);
+    }
+    if (x == 0) *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
+  }
+}
+
 // Workgroup (split, row tile of 16 NT rows, kv head of a sequence).
 template <int XT, int FMT, int NT>
 __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(CtxArgs a) {
   __shared__ __align__(16) float s_o[4][16][KHD + 4];
   __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ int s_last;
   const int split = blockIdx.x % a.S;
   const int rt = blockIdx.x / a.S % a.tiles, hb = blockIdx.x / a.S / a.tiles;
   const int b = hb / a.nkv, g = hb % a.nkv;
@@ -413,10 +487,10 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
       }
       if (a.S > 1 && t < sq.fit) {
         const int64_t at = ((int64_t)hb * a.R + r) * a.S + split;
-        if (d0 == 0) *(float2*)(a.ml + 2 * at) = float2{M, L};
+        if (d0 == 0) put_part(a.ml + 2 * at, M, L);
         if (L != 0.f) {  // an empty part is skipped by its sum
-          *(f32x4*)(a.part + at * KHD + d0) = f32x4{o[0], o[1], o[2], o[3]};
-          *(f32x4*)(a.part + at * KHD + d0 + 4) = f32x4{o[4], o[5], o[6], o[7]};
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) put_part(a.part + at * KHD + d0 + i, o[i], o[i + 1]);
         }
       } else if (a.S == 1) {
         const float inv = t < sq.fit ? 1.0f / L : __builtin_nanf("");
@@ -428,6 +502,18 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
       }
     }
   }
+  if (!a.counters) return;
+  // the last of the row tile's workgroups merges its parts; the count returns to 0
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's parts are stored
+  __syncthreads();
+  int32_t* count = a.counters + blockIdx.x / a.S;
+  if (threadIdx.x == 0)
+    s_last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.S - 1;
+  __syncthreads();
+  if (!s_last) return;
+  if (threadIdx.x == 0)
+    __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  merge_tile<XT>(a, b, g, hb, sq, r0, min(r0 + 16 * NT, a.R));
 }
 
 // The splits of a row merged, one workgroup a row: thread t takes dims 4 (t % 32) .. + 3 of
@@ -512,5 +598,5 @@ int i4_launch_ctx_rows(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t
     else rows_go<I4_BF16, I4_KV8_E4M3>(a, B, s);
   }
   if (hipGetLastError() != hipSuccess) return I4_ERR_LAUNCH;
-  return a.S > 1 ? i4_launch_ctx_merge(a, B, xt, s) : I4_OK;
+  return a.S > 1 && !a.counters ? i4_launch_ctx_merge(a, B, xt, s) : I4_OK;
 }

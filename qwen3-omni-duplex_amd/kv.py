@@ -25,7 +25,6 @@ Every op enqueues on torch's current stream of the tensors' device and never syn
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -36,45 +35,35 @@ KV8_BLOCK = 64
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
-def _pos(pos: int | torch.Tensor, B: int, dev: torch.device) -> tuple[int | None, int]:
-    """(device pointer, host value) of the first position(s)."""
-    if isinstance(pos, torch.Tensor):
-        if (pos.device != dev or pos.dtype != torch.int32 or pos.numel() != B
-                or not pos.is_contiguous()):
-            raise RuntimeError(f"device positions are {B} contiguous int32 on the tensors' device")
-        return pos.data_ptr(), 0
-    return None, int(pos)
-
-
-def _counts(counts: torch.Tensor | None, B: int, dev: torch.device) -> int | None:
-    if counts is None:
+def _int32(t: torch.Tensor | None, B: int, dev: torch.device, name: str) -> int | None:
+    """The address of B int32 on the device (None: not given)."""
+    if t is None:
         return None
-    if (counts.device != dev or counts.dtype != torch.int32 or counts.numel() != B
-            or not counts.is_contiguous()):
-        raise RuntimeError(f"counts are {B} contiguous int32 on the tensors' device")
-    return counts.data_ptr()
+    if t.dtype != torch.int32 or t.numel() != B or t.device != dev or not t.is_contiguous():
+        raise RuntimeError(f"{name} on the device: {B} contiguous int32 on the tensors' device")
+    return t.data_ptr()
 
 
 def _batched(x: torch.Tensor, dims: int, name: str) -> torch.Tensor:
     """x with its batch dimension (one sequence may come without)."""
+    if x.dim() == dims:
+        return x
     if x.dim() == dims - 1:
         return x.unsqueeze(0)
-    if x.dim() != dims:
-        raise RuntimeError(f"{name} has {x.dim()} dimensions, expected {dims - 1} or {dims}")
-    return x
+    raise RuntimeError(f"{name} has {x.dim()} dimensions, expected {dims - 1} or {dims}")
 
 
 def _cache_c(k: torch.Tensor, v: torch.Tensor) -> _lib.KVCacheC:
     """struct i4_kvcache of [n_kv_heads, max_len, head_dim] or [B, n_kv_heads, max_len,
     head_dim] caches (views with any strides above a dense last dimension)."""
     k, v = _batched(k, 4, "k_cache"), _batched(v, 4, "v_cache")
-    if k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+    shape, strides = k.shape, k.stride()
+    if shape != v.shape or k.dtype != v.dtype or strides != v.stride():
         raise RuntimeError("k_cache and v_cache must agree in shape, strides and dtype")
-    if k.stride(3) != 1 and k.shape[3] != 1:
+    if strides[3] != 1:
         raise RuntimeError("the caches' last dimension must be contiguous")
-    B, n, rows, d = k.shape
-    return _lib.KVCacheC(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), B, n,
-                         rows, d, _lib.half_code(k.dtype))
+    return _lib.KVCacheC(k.data_ptr(), v.data_ptr(), *strides[:3], *shape,
+                         _lib.half_code(k.dtype))
 
 
 def _out(out: torch.Tensor | None, like: torch.Tensor, shape: tuple[int, ...],
@@ -83,10 +72,32 @@ def _out(out: torch.Tensor | None, like: torch.Tensor, shape: tuple[int, ...],
     if out is None:
         make = torch.zeros if padded else torch.empty
         return make(shape, dtype=like.dtype, device=like.device)
-    if out.numel() != math.prod(shape) or tuple(out.shape[-len(shape) + 1:]) != shape[1:] \
-            or out.dtype != like.dtype or not out.is_contiguous():
+    if tuple(out.shape) != shape or out.dtype != like.dtype or not out.is_contiguous():
         raise RuntimeError(f"out must be a contiguous {shape} tensor of {like.dtype}")
     return out
+
+
+def _call(dev: torch.device, entry, *args) -> None:
+    """entry(*args, stream) with the tensors' device current: a launch on the default stream
+    goes to the current one."""
+    if torch.cuda.current_device() == dev.index:
+        rc = entry(*args, _lib.stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _lib.stream(dev))
+    if rc:
+        _lib.check(rc)
+
+
+_STREAM_WS: dict = {}
+
+
+def _kept_workspace(dev: torch.device) -> Workspace:
+    """The workspace of calls that bring none: one per stream, whose calls run in order; under
+    capture one of the call's own, which the graph then owns."""
+    if torch.cuda.is_current_stream_capturing():
+        return Workspace()
+    return _STREAM_WS.setdefault((dev.index, _lib.stream(dev)), Workspace())
 
 
 def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torch.Tensor,
@@ -105,6 +116,8 @@ def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torc
     cc = _cache_c(k_cache, v_cache)
     B, T, width = x.shape
     hd = cc.head_dim
+    if cc.dtype != _lib.half_code(x.dtype):
+        raise RuntimeError("the caches must have the activation dtype")
     if q_norm_w.dtype != x.dtype or k_norm_w.dtype != x.dtype:
         raise RuntimeError("the norm weights must have the activation dtype")
     if q_norm_w.numel() != hd or k_norm_w.numel() != hd:
@@ -118,17 +131,17 @@ def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torc
     if inv_freq.dtype != torch.float32 or inv_freq.device.type != "cpu" \
             or not inv_freq.is_contiguous():
         inv_freq = inv_freq.detach().to("cpu", torch.float32).contiguous()
-    qw, kw = q_norm_w.contiguous(), k_norm_w.contiguous()
+    q_norm_w, k_norm_w = q_norm_w.contiguous(), k_norm_w.contiguous()
     if first_row is not None and first_row < 0:
         raise RuntimeError("first_row must not be negative")
     shape = (B, T, n_heads, hd)
     q = _out(out, x, shape if qkv.dim() == 3 else shape[1:], counts is not None)
-    pd, ph = _pos(pos, B, dev)
-    _lib.check(_lib.lib().i4_rope_append(
-        x.data_ptr(), _lib.half_code(x.dtype), T, x.stride(0), x.stride(1), n_heads,
-        qw.data_ptr(), kw.data_ptr(), float(eps), inv_freq.data_ptr(), pd, ph,
-        -1 if first_row is None else int(first_row), _counts(counts, B, dev), q.data_ptr(),
-        ctypes.byref(cc), _lib.stream(dev)))
+    on_dev = isinstance(pos, torch.Tensor)
+    _call(dev, _lib.lib().i4_rope_append, x.data_ptr(), cc.dtype, T, x.stride(0), x.stride(1),
+          n_heads, q_norm_w.data_ptr(), k_norm_w.data_ptr(), eps, inv_freq.data_ptr(),
+          _int32(pos, B, dev, "pos") if on_dev else None, 0 if on_dev else int(pos),
+          -1 if first_row is None else int(first_row), _int32(counts, B, dev, "counts"),
+          q.data_ptr(), ctypes.byref(cc))
     return q
 
 
@@ -149,16 +162,18 @@ def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
     if x.stride(3) != 1:
         x = x.contiguous()
     y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd), counts is not None)
-    pd, ph = _pos(pos, B, dev)
+    on_dev = isinstance(pos, torch.Tensor)
+    pd, ph = (_int32(pos, B, dev, "pos"), 0) if on_dev else (None, int(pos))
     w = 0 if window is None else min(int(window), 2**31 - 1)
-    lb = _lib.lib()
-    need = lb.i4_attn_window_workspace_bytes(B, T, nh, cc.n_kv_heads,
-                                             keys if pd else min(max(ph, 0) + T, keys), w, sinks)
-    ws = (workspace or Workspace()).get(need, dev) if need else None
-    _lib.check(entry(x.data_ptr(), _lib.half_code(x.dtype), T, x.stride(0), x.stride(1),
-                     x.stride(2), nh, ctypes.byref(cc), pd, ph, _counts(counts, B, dev), w,
-                     int(sinks), 1.0 / math.sqrt(hd) if scale is None else float(scale),
-                     y.data_ptr(), _lib.ptr(ws), need, _lib.stream(dev)))
+    need = _lib.lib().i4_attn_window_workspace_bytes(
+        B, T, nh, cc.n_kv_heads, keys if on_dev else min(max(ph, 0) + T, keys), w, sinks)
+    ws = counters = None
+    if need:
+        kept = workspace or _kept_workspace(dev)
+        ws, counters = kept.get(need, dev).data_ptr(), _lib.ptr(kept.counters(dev))
+    _call(dev, entry, x.data_ptr(), _lib.half_code(x.dtype), T, *x.stride()[:3], nh,
+          ctypes.byref(cc), pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
+          hd ** -0.5 if scale is None else scale, y.data_ptr(), ws, need, counters)
     return y
 
 
@@ -248,8 +263,7 @@ class KV8Cache:
         out = torch.empty(2, c.batch, c.n_kv_heads, self.max_len, c.head_dim, dtype=torch.float32,
                           device=dev)
         k, v = out.unbind(0)
-        _lib.check(_lib.lib().i4_kv8_values(ctypes.byref(c), k.data_ptr(), v.data_ptr(),
-                                            _lib.stream(dev)))
+        _call(dev, _lib.lib().i4_kv8_values, ctypes.byref(c), k.data_ptr(), v.data_ptr())
         return k, v
 
 
@@ -270,10 +284,10 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, pos: int | tor
     B, T, n, hd = k.shape
     if (B, n, hd) != (c.batch, c.n_kv_heads, c.head_dim):
         raise RuntimeError(f"k {tuple(k.shape)} does not match the cache")
-    pd, ph = _pos(pos, B, dev)
-    _lib.check(_lib.lib().i4_kv8_append(k.data_ptr(), v.data_ptr(), _lib.half_code(k.dtype), T,
-                                        k.stride(0), k.stride(1), k.stride(2), ctypes.byref(c),
-                                        pd, ph, _counts(counts, B, dev), _lib.stream(dev)))
+    on_dev = isinstance(pos, torch.Tensor)
+    _call(dev, _lib.lib().i4_kv8_append, k.data_ptr(), v.data_ptr(), _lib.half_code(k.dtype), T,
+          *k.stride()[:3], ctypes.byref(c), _int32(pos, B, dev, "pos") if on_dev else None,
+          0 if on_dev else int(pos), _int32(counts, B, dev, "counts"))
 
 
 def attn_kv8(q: torch.Tensor, cache: KV8Cache, pos: int | torch.Tensor, *,

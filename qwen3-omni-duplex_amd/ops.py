@@ -293,6 +293,18 @@ class Workspace:
         self.buf: torch.Tensor | None = None
         self.kept: list[torch.Tensor] = []
         self._captured = False  # whether self.buf was handed out under capture
+        self._counters: torch.Tensor | None = None
+
+    def counters(self, device: torch.device) -> torch.Tensor | None:
+        """The 1024 int32 that the attention over a cached context counts a launch's finished
+        parts with: zeros when allocated, and left so by every call.  None under capture
+        unless they are there already (a fill would belong to the graph alone)."""
+        c = self._counters
+        if c is None or c.device != device:
+            if _capturing(device):
+                return None
+            c = self._counters = torch.zeros(1024, dtype=torch.int32, device=device)
+        return c
 
     def get(self, nbytes: int, device: torch.device, zeroed: bool = False) -> torch.Tensor:
         """At least nbytes; zeroed: a new buffer is allocated as zeros."""

@@ -60,11 +60,12 @@ def call_rope(lb, lib, c=None, **kw):
 
 def call_attn(lb, lib, c=None, eight=False, **kw):
     a = {**dict(q=P, xt=2, T=1, bs=8 * 128, ts=8 * 128, hs=128, nh=8, pos_dev=None, pos=0,
-                counts=None, window=0, sinks=0, scale=0.1, out=P, ws=P, wsb=1 << 40), **kw}
+                counts=None, window=0, sinks=0, scale=0.1, out=P, ws=P, wsb=1 << 40, counters=None), **kw}
     fn = lib.i4_attn_kv8 if eight else lib.i4_attn_window
     return fn(a["q"], a["xt"], a["T"], a["bs"], a["ts"], a["hs"], a["nh"],
               ctypes.byref(c or (cache8(lb) if eight else cache(lb))), a["pos_dev"], a["pos"],
-              a["counts"], a["window"], a["sinks"], a["scale"], a["out"], a["ws"], a["wsb"], None)
+              a["counts"], a["window"], a["sinks"], a["scale"], a["out"], a["ws"], a["wsb"],
+              a["counters"], None)
 
 
 def call_append(lb, lib, c=None, **kw):
@@ -105,9 +106,20 @@ def test_cache_refused(lb, pkg, bad, code):
     (dict(scale=-1.0), SHAPE), (dict(scale=math.inf), SHAPE), (dict(scale=math.nan), SHAPE),
     (dict(T=2, ts=64), STRIDE), (dict(hs=64), STRIDE), (dict(bs=64), STRIDE),
     (dict(q=P + 8), ALIGN), (dict(out=P + 8), ALIGN), (dict(hs=132), ALIGN),
-    (dict(ts=8 * 128 + 4, T=2), ALIGN)])
+    (dict(ts=8 * 128 + 4, T=2), ALIGN), (dict(counters=P + 2), ALIGN)])
 def test_attention_refuses(lb, pkg, eight, bad, code):
     assert call_attn(lb, pkg.lib(), eight=eight, **bad) == code
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("bad,code", [(dict(ws=None), WORKSPACE), (dict(wsb=1 << 10), WORKSPACE),
+                                      (dict(ws=P + 128), ALIGN)])
+def test_workspace_refused(lb, pkg, eight, bad, code):
+    c = cache8(lb, blocks=128) if eight else cache(lb, max_len=8192, head_stride=8192 * 128,
+                                                   batch_stride=4 * 8192 * 128)
+    need = pkg.lib().i4_attn_window_workspace_bytes(2, 1, 8, 4, 8001, 0, 0)
+    assert need > 1 << 10 and pkg.lib().i4_attn_window_workspace_bytes(2, 1, 8, 4, 64, 0, 0) == 0
+    assert call_attn(lb, pkg.lib(), c, eight=eight, pos=8000, **bad) == code
 
 
 @pytest.mark.parametrize("bad,code", BAD_CACHE8)
@@ -141,6 +153,60 @@ def test_cpu_tensors_are_refused(pkg):
         pkg.KV8Cache.empty(4, 64, device="cpu")
     with pytest.raises(RuntimeError, match="HIP device"):
         pkg.rope_append(x.view(1, 1, -1), 4, 2, x, x, 1e-6, pkg.rope_inv_freq(128, 1e6), 0, k, k)
+
+
+def test_python_refuses(pkg, monkeypatch):
+    """Argument checks that come before any address is taken, on CPU tensors."""
+    from qwen3_omni_duplex_amd import _lib, kv
+
+    monkeypatch.setattr(_lib, "require_device", lambda *ts: torch.device("cpu"))
+    q = torch.zeros(2, 3, 8, 128, dtype=torch.bfloat16)
+    k = torch.zeros(2, 4, 64, 128, dtype=torch.bfloat16)
+    cpu = torch.device("cpu")
+    for bad, match in (
+            (dict(window=0), "at least 1"), (dict(sinks=3), "window"),
+            (dict(out=torch.zeros(2, 3, 8, 64, dtype=torch.bfloat16)), "contiguous"),
+            (dict(out=torch.zeros(3, 2, 8, 128, dtype=torch.bfloat16)), "contiguous"),
+            (dict(out=torch.zeros(2, 3, 8, 128)), "contiguous")):
+        with pytest.raises(RuntimeError, match=match):
+            kv.attn_window(q, k, k, 0, **bad)
+    with pytest.raises(RuntimeError, match="batch"):
+        kv.attn_window(q[:1], k, k, 0)
+    with pytest.raises(RuntimeError, match="dimensions"):
+        kv.attn_window(q[0, 0], k, k, 0)
+    with pytest.raises(RuntimeError, match="strides"):
+        kv.attn_window(q, k, k.transpose(0, 1).contiguous().transpose(0, 1), 0)
+    with pytest.raises(RuntimeError, match="last dimension"):
+        kv.attn_window(q, k.mT, k.mT, 0)
+    for t in (torch.zeros(2), torch.zeros(1, dtype=torch.int32),
+              torch.zeros(4, dtype=torch.int32)[::2]):
+        with pytest.raises(RuntimeError, match="int32"):
+            kv._int32(t, 2, cpu, "pos")
+    w, inv = torch.zeros(128, dtype=torch.bfloat16), pkg.rope_inv_freq(128, 1e6)
+    x = torch.zeros(2, 3, 16 * 128, dtype=torch.bfloat16)
+    for args, kw, match in (
+            ((x, 8, 4, w[:64], w, 1e-6, inv, 0, k, k), {}, "head_dim"),
+            ((x, 8, 4, w.float(), w, 1e-6, inv, 0, k, k), {}, "dtype"),
+            ((x, 9, 4, w, w, 1e-6, inv, 0, k, k), {}, "head counts"),
+            ((x, 8, 4, w, w, 1e-6, inv[:32], 0, k, k), {}, "inv_freq"),
+            ((x, 8, 4, w, w, 1e-6, inv, 0, k.half(), k.half()), {}, "dtype"),
+            ((x, 8, 4, w, w, 1e-6, inv, 0, k, k), {"first_row": -1}, "first_row")):
+        with pytest.raises(RuntimeError, match=match):
+            kv.rope_append(*args, **kw)
+    c = pkg.KV8Cache.empty(4, 100, batch=2, device="cpu")
+    assert c.max_len == 128 and c.v.shape == (2, 4, 2, 128, 64)
+    kk = torch.zeros(2, 3, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="does not match"):
+        kv.kv8_append(kk[:, :, :2], kk[:, :, :2], c, 0)
+    with pytest.raises(RuntimeError, match="agree"):
+        kv.kv8_append(kk, kk.half(), c, 0)
+    t = list(c._t)
+    for i, bad, match in ((0, t[0].view(torch.uint8), "int8 or float8"), (0, t[0][:, :, 0], "k is"),
+                          (1, t[1].transpose(3, 4), "v must"), (2, t[2].double(), "float32"),
+                          (3, t[3][:1], "v_scale"), (4, t[4].half(), "one dtype"),
+                          (5, t[5][:, :, :32], "v_tail")):
+        with pytest.raises(RuntimeError, match=match):
+            pkg.KV8Cache(*(bad if j == i else y for j, y in enumerate(t)))
 
 
 def test_reference_quantisation():
