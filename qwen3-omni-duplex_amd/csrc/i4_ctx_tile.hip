@@ -33,43 +33,65 @@ struct TileAcc {
 __device__ inline u32x4 lds_b128(const lds_t* p) {
   return *(const __attribute__((address_space(3))) u32x4*)p;
 }
+__device__ inline void lds_put(lds_t* p, u32x4 x) {
+  *(__attribute__((address_space(3))) u32x4*)p = x;
+}
 // four rows of four dims each turned: lane i of 16 gets dim i of the rows
 __device__ inline u32x2v lds_tr(const lds_t* p) {
   return __builtin_bit_cast(u32x2v, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                         (__attribute__((address_space(3))) s16x4*)p));
 }
 
-// 64 rows of a 16-bit cache into LDS (K, then V), straight from memory: each wave instruction
-// brings 4 rows.  The loads are not waited for here.  row: of the cache, limited to last.
-struct Stage16 {
-  u32 k[4], v[4];  // this lane's byte offsets of the chunks within rows
-  int row[4];
-};
-__device__ inline Stage16 stage16_lane(int wave, int lane) {
-  Stage16 st;
+// 64 rows of a 16-bit cache into LDS (K, then V), straight from memory: a wave instruction
+// brings 4 rows, lane x the 16 bytes that belong at 16 x of its kilobyte.  The loads are not
+// waited for here: that is wait_loads(), before the barrier in front of their use.  They are
+// written out because the compiler waits for one of its own before the next LDS read of
+// whatever address, here for the tile after the one that is read.  m0 says where in LDS; no
+// register is written.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"  // m0 is reserved: nothing else holds it here
+__device__ inline void load_lds16(uint64_t base, u32 off, u32 lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(off), "s"(base), "s"(lds)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// every load of this wave (the builtin, so that the compiler knows its own to be there)
+__device__ inline void wait_loads() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// an address that is the same in all lanes
+__device__ inline uint64_t uniform(const void* p) {
+  const uint64_t x = (uint64_t)p;
+  return (uint64_t)(u32)__builtin_amdgcn_readfirstlane((int)x) |
+         (uint64_t)(u32)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
+// Row j0 + r of the cache, limited to last.
+__device__ inline void stage16(uint64_t k, uint64_t v, int j0, int last, u32 stride, u32 lds,
+                               int wave, int lane) {
+  const int r4 = lane >> 4, c = lane & 15;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = 16 * wave + 4 * i + (lane >> 4), c = lane & 15;
-    st.row[i] = r;
-    st.k[i] = 16u * (c ^ (r & 15));
-    st.v[i] = 16u * (c ^ ((r & 7) << 1));
-  }
-  return st;
-}
-__device__ inline void load_lds16(const void* base, u32 off, u32 lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) u32*)((const char*)base + off),
-     (__attribute__((address_space(3))) u32*)(uintptr_t)lds, 16, 0, 0);
-}
-__device__ inline void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ inline void stage16(const Stage16& st, const void* k, const void* v, int j0, int last,
-                               u32 stride, u32 lds, int wave) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const u32 row = (u32)min(j0 + st.row[i], last) * stride;
+    const int r = 16 * wave + 4 * i + r4;
+    const u32 row = (u32)min(j0 + r, last) * stride;
     const u32 dst = lds + 1024u * (4 * wave + i);
-    load_lds16(k, row + st.k[i], dst);
-    load_lds16(v, row + st.v[i], dst + TBYTES);
+    load_lds16(k, row + 16u * (c ^ (4 * i + r4)), dst);
+    load_lds16(v, row + 16u * (c ^ ((4 * (i & 1) + r4) << 1)), dst + TBYTES);
   }
+}
+
+// A fence for the scheduler: LDS reads are issued two products ahead of their use, which it
+// would undo to save registers (a wave then waits out LDS's latency at every product).
+#define I4_ORDER() __builtin_amdgcn_sched_barrier(0)
+
+// x as a value that nothing is known of: what the rare tiles compute from it stays with them
+// instead of being prepared in front of the loop, where it took registers from the others.
+__device__ inline int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 // scores of the tile's 64 keys
@@ -78,33 +100,36 @@ __device__ inline void tile_scores(const lds_t* k, const u32x4 (&q)[8], f32x16 (
                                    int h) {
   const lds_t* row = k + n * 256;
   const int x = (h ^ (n & 15)) * 16;
+  u32x4 a[3][2];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) a[c % 3][t] = lds_b128(row + t * 8192 + (x ^ (32 * c)));
+  };
+  load(0);
+  load(1);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
 #pragma unroll
-  for (int c = 0; c < 8; ++c)
+  for (int c = 0; c < 8; ++c) {
+    if (c < 6) load(c + 2);
+    I4_ORDER();
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      s[t] = mfma32<XT>(lds_b128(row + t * 8192 + (x ^ (32 * c))), q[c], s[t]);
+    for (int t = 0; t < 2; ++t) s[t] = mfma32<XT>(a[c % 3][t], q[c], s[t]);
+    I4_ORDER();
+  }
 }
 
-// scores -> weights in place; c: scale log2(e) (times the keys' scale); key0: the tile's first
-// position + 4 h, p: the row's position
-__device__ inline void tile_weights(TileAcc& acc, f32x16 (&s)[2], float c, bool partial, int key0,
-                                    int p, const Bounds& w) {
-  if (partial)
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (!sees(w, p, key0 + 32 * t + 8 * (i >> 2) + (i & 3))) s[t][i] = -__builtin_inff();
+// whether the maximum has to be raised for these scores, and raising it; c: scale log2(e)
+// (times the keys' scale), positive
+__device__ inline void tile_max(TileAcc& acc, const f32x16 (&s)[2], float c) {
   float mx = -__builtin_inff();
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-  mx *= c;  // c > 0
+  mx *= c;
   if (__builtin_amdgcn_ballot_w64(mx > acc.m + kLazy)) {
     const float m = fmaxf(acc.m, fmaxf(mx, __shfl_xor(mx, 32)));
     const float f = m > acc.m ? exp2f(acc.m - m) : 1.f;
@@ -113,14 +138,29 @@ __device__ inline void tile_weights(TileAcc& acc, f32x16 (&s)[2], float c, bool 
 #pragma unroll
     for (int t = 0; t < 4; ++t) acc.o[t] *= f;
   }
+}
+// scores -> weights times 2^lift in place; returns their sum
+__device__ inline float tile_weights(const TileAcc& acc, f32x16 (&s)[2], float c, float lift) {
   // a row that has seen nothing yet has m = -inf and scores -inf: weights 0
-  const float base = acc.m == -__builtin_inff() ? 0.f : acc.m - kLift;
+  const float base = acc.m == -__builtin_inff() ? lift : lift - acc.m;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, -base));
-      acc.l += s[t][i];
+      s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, base));
+      sum[i & 3] += s[t][i];
+    }
+  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+// v where the row does not see the key; key0: the tile's first position + 4 h
+__device__ inline void tile_mask(f32x16 (&s)[2], int key0, int p, const Bounds& w, float v) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (!sees(w, p, key0 + 32 * t + 8 * (i >> 2) + (i & 3))) s[t][i] = v;
+      if ((i & 3) == 3) I4_ORDER();  // few conditions at a time
     }
 }
 
@@ -142,53 +182,79 @@ template <int PT> __device__ inline u32x4 weights_lo(const f32x16 (&s)[2], int k
   return r;
 }
 
-// O^T += V^T P^T for a 16-bit tile.  CLEAN: a tile that some row does not see in full;
-// infinities and NaN are taken out of the product (0 times them is NaN) and added to the
-// rows that see them.
-template <int XT, bool CLEAN>
-__device__ __attribute__((always_inline)) inline void tile_values16(TileAcc& acc, const f32x16 (&s)[2], const lds_t* v, int lane,
-                                     int key0, int p, const Bounds& w) {
+// O^T += V^T P^T for a 16-bit tile
+template <int XT>
+__device__ inline void tile_values16(TileAcc& acc, const f32x16 (&s)[2], const lds_t* v,
+                                     int lane) {
   const int h = lane >> 5, gq = (lane >> 4) & 1, i16 = lane & 15;
   const lds_t* row = v + (4 * h + (i16 >> 2)) * 256 + (i16 & 1) * 8;
   const int x = ((2 * gq + ((i16 & 3) >> 1)) ^ ((4 * h + (i16 >> 2)) << 1)) * 16;
+  u32x4 a[3][2];  // two of a step's four products at a time
+  auto load = [&](int y) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const lds_t* at = row + (y >> 1) * 4096 + (x ^ (64 * (2 * (y & 1) + u)));
+      const u32x2v a0 = lds_tr(at), a1 = lds_tr(at + 2048);
+      a[y % 3][u] = u32x4{a0[0], a0[1], a1[0], a1[1]};
+    }
+  };
+  load(0);
+  load(1);
+  u32x4 b;
+#pragma unroll
+  for (int y = 0; y < 8; ++y) {
+    if (y < 6) load(y + 2);
+    if ((y & 1) == 0) b = weights_hi<XT>(s, y >> 1);
+    I4_ORDER();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = 2 * (y & 1) + u;
+      acc.o[t] = mfma32<XT>(a[y % 3][u], b, acc.o[t]);
+    }
+    I4_ORDER();
+  }
+}
+
+// Values that a row does not see must not reach it, and 0 times an infinity or a NaN would.
+// In a tile that some row does not see in full they are cleared in LDS (this thread's 64
+// bytes of it; returns whether there were any)
+template <int XT> __device__ inline bool clear_not_finite(lds_t* v, int tid) {
   bool bad = false;
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    const u32x4 b = weights_hi<XT>(s, ks);
+  for (int j = 0; j < 4; ++j) {
+    lds_t* at = v + 4096 * j + 16 * tid;
+    u32x4 x = lds_b128(at);
+    const bool here = not_finite<XT>(x[0]) || not_finite<XT>(x[1]) || not_finite<XT>(x[2]) ||
+                      not_finite<XT>(x[3]);
+    if (here) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const lds_t* at = row + ks * 4096 + (x ^ (64 * t));
-      const u32x2v a0 = lds_tr(at), a1 = lds_tr(at + 2048);
-      u32x4 a = {a0[0], a0[1], a1[0], a1[1]};
-      if constexpr (CLEAN) {
+      for (int e = 0; e < 4; ++e) x[e] = finite_pair<XT>(x[e]);
+      lds_put(at, x);
+    }
+    bad |= here;
+  }
+  return bad;
+}
+// and added to the rows that see them when all tiles are done: whatever they meet, they stay.
+// v: the rows of the tile at position j0, of which `rows` exist
+template <int XT>
+__device__ inline void add_not_finite(TileAcc& acc, const uint16_t* v, u32 stride, int rows,
+                                      int j0, int p, int h, const Bounds& w) {
+  for (int key = 0; key < rows; ++key) {
+    const bool see = sees(w, p, j0 + key);
+    const char* r = (const char*)v + (int64_t)key * stride + 8 * h;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          bad |= not_finite<XT>(a[e]);
-          a[e] = finite_pair<XT>(a[e]);
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // dims 32 t + 8 i + 4 h ..
+        const u32x2v y = *(const u32x2v*)(r + 64 * t + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float u = lo_f32<XT>(y[e]), z = hi_f32<XT>(y[e]);
+          if (see && !(fabsf(u) < __builtin_inff())) acc.o[t][4 * i + 2 * e] += u;
+          if (see && !(fabsf(z) < __builtin_inff())) acc.o[t][4 * i + 2 * e + 1] += z;
         }
       }
-      acc.o[t] = mfma32<XT>(a, b, acc.o[t]);
-    }
-  }
-  if constexpr (CLEAN) {
-    if (!__builtin_amdgcn_ballot_w64(bad)) return;
-    for (int key = 0; key < TKEYS; ++key) {
-      const bool see = sees(w, p, key0 + key);
-      const lds_t* r = v + key * 256;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {  // dims 32 t + 8 i + 4 h ..
-          const u32x2v y = *(const __attribute__((address_space(3))) u32x2v*)(
-              r + ((4 * t + i) ^ ((key & 7) << 1)) * 16 + 8 * h);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float u = lo_f32<XT>(y[e]), z = hi_f32<XT>(y[e]);
-            if (see && !(fabsf(u) < __builtin_inff())) acc.o[t][4 * i + 2 * e] += u;
-            if (see && !(fabsf(z) < __builtin_inff())) acc.o[t][4 * i + 2 * e + 1] += z;
-          }
-        }
-    }
   }
 }
 
@@ -198,17 +264,30 @@ template <bool TWO>
 __device__ inline void tile_values8(TileAcc& acc, const f32x16 (&s)[2], const lds_t* v, int n,
                                     int h) {
   const lds_t* row = v + n * 128;
+  u32x4 a[3][2];
+  auto load = [&](int y) {
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    const u32x4 b = weights_hi<I4_BF16>(s, ks);
-    u32x4 b2;
-    if constexpr (TWO) b2 = weights_lo<I4_BF16>(s, ks, b);
+    for (int u = 0; u < 2; ++u)
+      a[y % 3][u] = lds_b128(row + (2 * (y & 1) + u) * 4096 + ((((y & ~1) + h) ^ (n & 7)) * 16));
+  };
+  load(0);
+  load(1);
+  u32x4 b, b2;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const u32x4 a = lds_b128(row + t * 4096 + (((2 * ks + h) ^ (n & 7)) * 16));
-      acc.o[t] = mfma32<I4_BF16>(a, b, acc.o[t]);
-      if constexpr (TWO) acc.o[t] = mfma32<I4_BF16>(a, b2, acc.o[t]);
+  for (int y = 0; y < 8; ++y) {
+    if (y < 6) load(y + 2);
+    if ((y & 1) == 0) {
+      b = weights_hi<I4_BF16>(s, y >> 1);
+      if constexpr (TWO) b2 = weights_lo<I4_BF16>(s, y >> 1, b);
     }
+    I4_ORDER();
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int t = 2 * (y & 1) + u;
+      acc.o[t] = mfma32<I4_BF16>(a[y % 3][u], b, acc.o[t]);
+      if constexpr (TWO) acc.o[t] = mfma32<I4_BF16>(a[y % 3][u], b2, acc.o[t]);
+    }
+    I4_ORDER();
   }
 }
 
@@ -225,9 +304,6 @@ __device__ inline void load8(Stage8& st, const Cache8& c, int64_t blk, int tid) 
   st.v[1] = ldg16(v + 16);
   st.ks = c.ks[blk];
   st.vs = c.vs[blk];
-}
-__device__ inline void lds_put(lds_t* p, u32x4 x) {
-  *(__attribute__((address_space(3))) u32x4*)p = x;
 }
 template <int XT, int FMT> __device__ inline void store8(const Stage8& st, lds_t* buf, int tid) {
   const int key = tid >> 2, c0 = 4 * (tid & 3);  // 32 dims: chunks c0 .. c0 + 3
@@ -284,29 +360,40 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
     const int i0 = (int)((int64_t)ct.n * split / a.S);
     const int i1 = (int)((int64_t)ct.n * (split + 1) / a.S);
     lds_t* lds = (lds_t*)&s_tile[0][0];
-    const u32 lds0 = (u32)(uintptr_t)lds;
-    const Stage16 st = stage16_lane(wave, lane);
+    const u32 lds0 = __builtin_amdgcn_readfirstlane((u32)(uintptr_t)lds);
     f32x16 s[2];
-    auto attend16 = [&](const lds_t* buf, int j0) {
-      const bool partial = !all_see(a.w, plo, phi, j0, TKEYS);
+    bool bad = false;  // values that are not finite in a tile that not all rows see in full
+    auto whole = [&](int i) { return all_see(a.w, plo, phi, 64 * ct.at(i), TKEYS); };
+    auto attend16 = [&](lds_t* buf, int j0, bool edge) {
+      if (edge) bad |= __syncthreads_or(clear_not_finite<XT>(buf + TBYTES, tid));
       tile_scores<XT>(buf, q, s, n, h);
-      tile_weights(acc, s, a.c2, partial, j0 + 4 * h, p, a.w);
-      if (partial) tile_values16<XT, true>(acc, s, buf + TBYTES, lane, j0, p, a.w);
-      else tile_values16<XT, false>(acc, s, buf + TBYTES, lane, j0, p, a.w);
+      if (edge) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
+      tile_max(acc, s, a.c2);
+      acc.l += tile_weights(acc, s, a.c2, kLift);
+      tile_values16<XT>(acc, s, buf + TBYTES, lane);
     };
     if constexpr (FMT < 0) {
       const u32 stride = (u32)a.c.rs * 2u;
       const uint16_t* k = a.c.k + b * a.c.bs + g * a.c.hs;
       const uint16_t* v = a.c.v + b * a.c.bs + g * a.c.hs;
-      if (i0 < i1) stage16(st, k, v, 64 * ct.at(i0), phi, stride, lds0, wave);
+      const uint64_t ku = uniform(k), vu = uniform(v);
+      if (i0 < i1) stage16(ku, vu, 64 * ct.at(i0), phi, stride, lds0, wave, lane);
       for (int i = i0; i < i1; ++i) {
         const int cur = (i - i0) & 1;
         wait_loads();
         __syncthreads();  // the tile is here, and its other half is free
         if (i + 1 < i1)
-          stage16(st, k, v, 64 * ct.at(i + 1), phi, stride, lds0 + (cur ^ 1) * 2 * TBYTES, wave);
-        attend16(lds + cur * 2 * TBYTES, 64 * ct.at(i));
+          stage16(ku, vu, 64 * ct.at(i + 1), phi, stride, lds0 + (cur ^ 1) * 2 * TBYTES, wave,
+                  lane);
+        attend16(lds + cur * 2 * TBYTES, 64 * ct.at(i), !whole(i));
       }
+      if (bad)
+        for (int i = i0; i < i1; ++i) {
+          const int j0 = 64 * ct.at(i);
+          if (!whole(i))
+            add_not_finite<XT>(acc, (const uint16_t*)((const char*)v + (int64_t)j0 * stride),
+                               stride, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
+        }
     } else {
       const int end = sq.p0 + sq.fit, full = end / KBLK;  // finished blocks, then the tail
       const int64_t hblk = (int64_t)hb * a.c8.blocks;
@@ -324,28 +411,18 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
         const int cur = (i - i0) & 1, j0 = 64 * ct.at(i);
         __syncthreads();
         if (i + 1 < e) load8(s8, a.c8, hblk + ct.at(i + 1), tid);
-        const bool partial = !all_see(a.w, plo, phi, j0, TKEYS);
         const lds_t* buf = lds + cur * 2 * TBYTES;
-        tile_scores<XT>(buf, q, s, n, h);
-        if (ks != ks)  // a block that reads as NaN: so do its scores, where they are seen
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int x = 0; x < 16; ++x) s[u][x] = ks;
-        tile_weights(acc, s, ks != ks ? a.c2 : a.c2 * ks, partial, j0 + 4 * h, p, a.w);
-        // the weights take the values' scale; NaN (a block that reads as NaN) reaches the
-        // rows that see one of its keys
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int x = 0; x < 16; ++x) s[u][x] *= vs;
-        if (partial)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-              if (!sees(a.w, p, j0 + 4 * h + 32 * u + 8 * (x >> 2) + (x & 3))) s[u][x] = 0.f;
-        tile_values8<XT == I4_F16>(acc, s, buf + TBYTES, n, h);
+        if (ks + vs == ks + vs) {
+          tile_scores<XT>(buf, q, s, n, h);
+          if (!whole(i)) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
+          tile_max(acc, s, a.c2 * ks);
+          // the weights that enter the product take the values' scale, in the exponent; their
+          // sum gives it back
+          acc.l = fmaf(tile_weights(acc, s, a.c2 * ks, kLift + log2f(vs)), 1.0f / vs, acc.l);
+          tile_values8<XT == I4_F16>(acc, s, buf + TBYTES, n, h);
+        } else if (j0 <= p && (min(j0 + KBLK - 1, p) > p - a.w.window || j0 < a.w.sinks)) {
+          acc.l = __builtin_nanf("");  // a block that reads as NaN, for a row that sees a key
+        }
         if (i + 1 < e) {
           store8<XT, FMT>(s8, lds + (cur ^ 1) * 2 * TBYTES, tid);
           ks = s8.ks, vs = s8.vs;
@@ -353,11 +430,15 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       }
       if (tail) {
         const int64_t at = (int64_t)hb * (KBLK * KHD);
+        const int rows = phi - full * KBLK + 1;
         __syncthreads();
-        stage16(st, a.c8.kt + at, a.c8.vt + at, 0, phi - full * KBLK, KHD * 2u, lds0, wave);
+        stage16(uniform(a.c8.kt + at), uniform(a.c8.vt + at), 0, rows - 1, KHD * 2u, lds0, wave,
+                lane);
         wait_loads();
         __syncthreads();
-        attend16(lds, full * KBLK);
+        attend16(lds, full * KBLK, true);
+        if (bad)
+          add_not_finite<XT>(acc, a.c8.vt + at, KHD * 2u, rows, full * KBLK, p, h, a.w);
       }
     }
     if (mine) {
