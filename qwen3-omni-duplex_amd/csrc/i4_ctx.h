@@ -10,7 +10,6 @@
 
 namespace i4 {
 
-static constexpr int kMaxSplits = 1024;  // of one context
 static constexpr int kFewRows = 32;      // of a kv head: k_ctx_rows up to here
 static constexpr int kTileRows = 128;    // of a workgroup of k_ctx_tile
 

@@ -17,7 +17,7 @@ namespace i4 {
 // How a call is split: a rule on its sizes alone (no device value), so that the workspace
 // can be named before the call.
 static int ctx_tiles_of(int R) {
-  return R <= 16 ? 1 : R <= kFewRows ? (R + 31) / 32 : (R + kTileRows - 1) / kTileRows;
+  return R <= kFewRows ? 1 : (R + kTileRows - 1) / kTileRows;
 }
 static int ctx_splits(int B, int T, int nq, int nkv, int keys, int window, int sinks) {
   const int R = T * (nq / nkv);
@@ -30,10 +30,24 @@ static int ctx_splits(int B, int T, int nq, int nkv, int keys, int window, int s
     if (most < tiles) tiles = most;
   }
   const int64_t wgs = (int64_t)B * nkv * ctx_tiles_of(R);
-  const int64_t want = ((few ? 1024 : 512) + wgs - 1) / wgs;
-  const int64_t most = (tiles + 3) / 4;  // few: a tile a wave
-  const int64_t s = want < most ? want : most;
-  return s < 1 ? 1 : (int)s;
+  if (few) {
+    // as many workgroups as the chip holds at once, twice over, and a tile for each wave
+    const int64_t want = 1024 / wgs, most = (tiles + 3) / 4;
+    const int64_t s = want < most ? want : most;
+    return s < 1 ? 1 : (int)s;
+  }
+  // Two workgroups fit a CU: 512 take 2.1 us a tile together, 256 that have their CU to
+  // themselves 1.3 us.  Parts cost 1040 bytes a row, written and read, and a launch.
+  double best = 0;
+  int s = 1;
+  for (int c = 1; c <= 64 && (c == 1 || c <= tiles / 4); ++c) {
+    const int64_t w = wgs * c, rest = w % 512;
+    const double rounds = 2.1 * (double)(w / 512) + (rest == 0 ? 0 : rest <= 256 ? 1.3 : 2.1);
+    double t = rounds * (double)((tiles + c - 1) / c);
+    if (c > 1) t += 4 + (double)((int64_t)B * T * nq) * c * 1040 / 4e6;
+    if (c == 1 || t < best) best = t, s = c;
+  }
+  return s;
 }
 
 static int launch(CtxArgs& a, int B, int xt, int fmt, int keys, const i4_span& w,

@@ -516,58 +516,69 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
   merge_tile<XT>(a, b, g, hb, sq, r0, min(r0 + 16 * NT, a.R));
 }
 
-// The splits of a row merged, one workgroup a row: thread t takes dims 4 (t % 32) .. + 3 of
-// every eighth split, so that a row's parts are all in flight at once.
-template <int XT> __global__ __launch_bounds__(256) void k_ctx_merge(CtxArgs a) {
-  __shared__ float s_f[kMaxSplits];
+// The splits of rows merged: 32 P lanes a row, each dims 4 (t % 32) .. + 3 of every P-th
+// part.  P = 8 (a workgroup a row) keeps many parts in flight at once; few parts take P = 1,
+// eight rows a workgroup.
+template <int XT, int P> __global__ __launch_bounds__(256) void k_ctx_merge(CtxArgs a, int64_t n) {
   __shared__ __align__(16) float s_o[8][KHD];
-  __shared__ float s_l[4];
-  const int64_t at = blockIdx.x;  // (sequence, kv head, row)
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int64_t hb = at / a.R;
-  const int r = (int)(at % a.R), t = r / a.G, b = (int)(hb / a.nkv), g = (int)(hb % a.nkv);
+  __shared__ float s_m[8], s_l[8];
+  const int tid = threadIdx.x, grp = tid >> 5, part = grp % P, d = 4 * (tid & 31);
+  const int64_t at = (int64_t)blockIdx.x * (8 / P) + grp / P;  // (sequence, kv head, row)
+  const bool here = at < n;
+  const int64_t hb = here ? at / a.R : 0;
+  const int r = here ? (int)(at % a.R) : 0, t = r / a.G, b = (int)(hb / a.nkv);
   const CtxSeq sq = ctx_seq(a, b);
-  if (t >= sq.have) return;
-  u32* y = (u32*)(a.out + ctx_out(a, b, g, r));
-  if (t >= sq.fit) {
-    if (tid < KHD / 2) y[tid] = (u32)Half<XT>::QNAN * 0x10001u;
-    return;
-  }
-  const float2* ml = (const float2*)a.ml + at * a.S;
-  float M = -__builtin_inff();
-  for (int s = lane; s < a.S; s += 64) M = fmaxf(M, ml[s].x);
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
-  float L = 0.f;
-  for (int s = tid; s < a.S; s += 256) {
-    const float2 v = ml[s];
-    const float f = v.y == 0.f ? 0.f : exp2f(v.x - M);  // 0: nothing seen there, no part written
-    s_f[s] = f;
-    L = fmaf(v.y, f, L);
-  }
-  L = group_sum<64>(L);
-  if (lane == 0) s_l[wave] = L;
-  __syncthreads();
-  L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-  const int part = tid >> 5, d = 4 * (tid & 31);
-  const float* src = a.part + at * a.S * KHD + d;
+  float M = -__builtin_inff(), L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int s = part; s < a.S; s += 8) {
-    const f32x4 x = *(const f32x4*)(src + (int64_t)s * KHD);
-    const float f = s_f[s];
+  if (here && t < sq.fit) {
+    const float2* ml = (const float2*)a.ml + at * a.S;
+    const float* src = a.part + at * a.S * KHD + d;
+    constexpr int U = P == 1 ? 2 : 4;
+    for (int s0 = part; s0 < a.S; s0 += U * P) {
+      float2 v[U];
+      f32x4 x[U];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = f == 0.f ? o[i] : fmaf(x[i], f, o[i]);
-  }
-  *(f32x4*)&s_o[part][d] = o;
-  __syncthreads();
-  if (tid < KHD / 2) {
-    float u = 0.f, v = 0.f;
-    for (int i = 0; i < 8; ++i) {
-      u += s_o[i][2 * tid];
-      v += s_o[i][2 * tid + 1];
+      for (int u = 0; u < U; ++u) {
+        const int s = min(s0 + u * P, a.S - 1);
+        v[u] = ml[s];
+        x[u] = *(const f32x4*)(src + (int64_t)s * KHD);
+        if (s0 + u * P >= a.S) v[u].y = 0.f;
+      }
+      float mb = M;  // a sum of 0: nothing seen there, no part written
+#pragma unroll
+      for (int u = 0; u < U; ++u) mb = v[u].y == 0.f ? mb : fmaxf(mb, v[u].x);
+      const float f0 = M == mb ? 1.f : exp2f(M - mb);
+      L *= f0;
+      o *= f0;
+      M = mb;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (v[u].y == 0.f) continue;
+        const float f = exp2f(v[u].x - M);
+        L = fmaf(v[u].y, f, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[u][e], f, o[e]);
+      }
     }
-    y[tid] = pack2<XT>(u / L, v / L);
   }
+  if constexpr (P > 1) {
+    *(f32x4*)&s_o[grp][d] = o;
+    if (d == 0) s_m[grp] = M, s_l[grp] = L;
+    __syncthreads();
+    M = -__builtin_inff(), L = 0.f, o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < P; ++i) M = s_l[i] == 0.f ? M : fmaxf(M, s_m[i]);
+    for (int i = 0; i < P; ++i) {
+      if (s_l[i] == 0.f) continue;
+      const float f = exp2f(s_m[i] - M);
+      L = fmaf(s_l[i], f, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(s_o[i][d + e], f, o[e]);
+    }
+  }
+  if (!here || t >= sq.have || part != 0) return;
+  u32x2* y = (u32x2*)(a.out + ctx_out(a, b, (int)(hb % a.nkv), r) + d);
+  if (t >= sq.fit) *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
+  else *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
 }
 
 template <int XT, int FMT> static void rows_go(const CtxArgs& a, int B, hipStream_t s) {
@@ -580,9 +591,16 @@ template <int XT, int FMT> static void rows_go(const CtxArgs& a, int B, hipStrea
 }  // namespace i4
 
 int i4_launch_ctx_merge(const i4::CtxArgs& a, int B, int xt, hipStream_t s) {
-  const dim3 grid((unsigned)(B * a.nkv * a.R));
-  if (xt == I4_F16) i4::k_ctx_merge<I4_F16><<<grid, 256, 0, s>>>(a);
-  else i4::k_ctx_merge<I4_BF16><<<grid, 256, 0, s>>>(a);
+  const int64_t rows = (int64_t)B * a.nkv * a.R;
+  const bool few = a.S <= 16;
+  const dim3 grid((unsigned)(few ? (rows + 7) / 8 : rows));
+  if (xt == I4_F16) {
+    if (few) i4::k_ctx_merge<I4_F16, 1><<<grid, 256, 0, s>>>(a, rows);
+    else i4::k_ctx_merge<I4_F16, 8><<<grid, 256, 0, s>>>(a, rows);
+  } else {
+    if (few) i4::k_ctx_merge<I4_BF16, 1><<<grid, 256, 0, s>>>(a, rows);
+    else i4::k_ctx_merge<I4_BF16, 8><<<grid, 256, 0, s>>>(a, rows);
+  }
   return hipGetLastError() == hipSuccess ? I4_OK : I4_ERR_LAUNCH;
 }
 
