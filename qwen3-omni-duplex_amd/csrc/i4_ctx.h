@@ -11,6 +11,7 @@
 namespace i4 {
 
 static constexpr int kFewRows = 32;      // of a kv head: k_ctx_rows up to here
+static constexpr int kShared = I4_CTX_COUNTERS;  // kv heads whose contexts are shared out
 static constexpr int kTileRows = 128;    // of a workgroup of k_ctx_tile
 
 struct CtxArgs {
@@ -23,12 +24,14 @@ struct CtxArgs {
   Bounds w;
   int32_t nq, nkv, G, R;  // R = T G rows of a kv head
   int32_t len;            // positions of the cache
+  int32_t B;
   int32_t tiles;          // row tiles of a kv head
-  int32_t S;              // splits of the context
+  int32_t S;              // splits of the context (k_ctx_tile), or
+  int32_t wgs;            // workgroups that the contexts are shared out to (k_ctx_rows)
   float c2;               // scale log2(e): weights are powers of two
-  float* part;            // [B nkv R][S][128] sums of e v, then
-  float* ml;              // [B nkv R][S][2] maximum and sum
-  int32_t* counters;      // nullable: parts of a row tile that are done, 0 between calls
+  float* part;            // [B nkv R][S] or [wgs][rows], [128] sums of e v each, then
+  float* ml;              // [2] each: maximum and sum
+  int32_t* counters;      // nullable: parts of a kv head that are done, 0 between calls
 };
 
 // The context tiles (64 positions) that rows at positions [plo, phi] see: ns tiles with the
@@ -156,6 +159,5 @@ template <int XT> __device__ inline u32 finite_pair(u32 x) {
 }  // namespace i4
 
 // i4_ctx_rows.hip / i4_ctx_tile.hip; fmt: -1 (16-bit cache) or I4_KV8_*
-int i4_launch_ctx_merge(const i4::CtxArgs& a, int B, int xt, hipStream_t s);
-int i4_launch_ctx_tile(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t s);
-int i4_launch_ctx_rows(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t s);
+int i4_launch_ctx_tile(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s);
+int i4_launch_ctx_rows(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s);

@@ -16,10 +16,11 @@ namespace i4 {
 
 // How a call is split: a rule on its sizes alone (no device value), so that the workspace
 // can be named before the call.
-static int ctx_tiles_of(int R) {
-  return R <= kFewRows ? 1 : (R + kTileRows - 1) / kTileRows;
-}
-static int ctx_splits(int B, int T, int nq, int nkv, int keys, int window, int sinks) {
+struct CtxSplit {
+  int S, wgs;      // k_ctx_tile's splits; k_ctx_rows' workgroups
+  int64_t parts;   // rows that are written as parts
+};
+static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, int sinks) {
   const int R = T * (nq / nkv);
   const bool few = R <= kFewRows;
   // the context tiles of 64 that one row tile sees at most
@@ -29,40 +30,40 @@ static int ctx_splits(int B, int T, int nq, int nkv, int keys, int window, int s
     const int64_t most = ((int64_t)window + span + 126) / 64 + (sinks + 63) / 64;
     if (most < tiles) tiles = most;
   }
-  const int64_t wgs = (int64_t)B * nkv * ctx_tiles_of(R);
+  const int64_t heads = (int64_t)B * nkv;
   if (few) {
-    // as many workgroups as the chip holds at once, twice over, and a tile for each wave
-    const int64_t want = 1024 / wgs, most = (tiles + 3) / 4;
-    const int64_t s = want < most ? want : most;
-    return s < 1 ? 1 : (int)s;
+    // as many workgroups as the chip holds at once (two a CU), or two or four times that
+    // where the heads are too many to share that evenly; at least a tile for each wave
+    int64_t w = heads <= 128 ? 512 : heads <= 256 ? 1024 : 2048;
+    if (w > heads * ((tiles + 3) / 4)) w = heads * ((tiles + 3) / 4);
+    if (w <= heads || heads > kShared) w = heads;
+    return {1, (int)w, w > heads ? w * (R <= 16 ? 16 : 32) : 0};
   }
   // Two workgroups fit a CU: 512 take 2.1 us a tile together, 256 that have their CU to
   // themselves 1.3 us.  Parts cost 1040 bytes a row, written and read, and a launch.
+  const int64_t wgs = heads * ((R + kTileRows - 1) / kTileRows), rows = (int64_t)B * T * nq;
   double best = 0;
   int s = 1;
   for (int c = 1; c <= 64 && (c == 1 || c <= tiles / 4); ++c) {
     const int64_t w = wgs * c, rest = w % 512;
     const double rounds = 2.1 * (double)(w / 512) + (rest == 0 ? 0 : rest <= 256 ? 1.3 : 2.1);
     double t = rounds * (double)((tiles + c - 1) / c);
-    if (c > 1) t += 4 + (double)((int64_t)B * T * nq) * c * 1040 / 4e6;
+    if (c > 1) t += 4 + (double)rows * c * 1040 / 4e6;
     if (c == 1 || t < best) best = t, s = c;
   }
-  return s;
+  return {s, 0, s > 1 ? rows * s : 0};
 }
 
-static int launch(CtxArgs& a, int B, int xt, int fmt, int keys, const i4_span& w,
-                  hipStream_t stream) {
-  a.S = ctx_splits(B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks);
-  if (a.S > 1) {
-    a.part = (float*)w.workspace;
-    a.ml = a.part + (int64_t)B * a.nkv * a.R * a.S * KHD;
-  }
-  a.tiles = ctx_tiles_of(a.R);
-  a.counters = a.S > 1 && a.R <= kFewRows && (int64_t)B * a.nkv * a.tiles <= I4_CTX_COUNTERS
-                   ? w.counters
-                   : nullptr;
-  return a.R <= kFewRows ? i4_launch_ctx_rows(a, B, xt, fmt, stream)
-                         : i4_launch_ctx_tile(a, B, xt, fmt, stream);
+static int launch(CtxArgs& a, int xt, int fmt, int keys, const i4_span& w, hipStream_t stream) {
+  const CtxSplit sp = ctx_split(a.B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks);
+  a.S = sp.S;
+  a.wgs = sp.wgs;
+  a.part = (float*)w.workspace;
+  a.ml = a.part + sp.parts * KHD;
+  a.counters = w.counters;
+  a.tiles = (a.R + kTileRows - 1) / kTileRows;
+  return a.R <= kFewRows ? i4_launch_ctx_rows(a, xt, fmt, stream)
+                         : i4_launch_ctx_tile(a, xt, fmt, stream);
 }
 
 }  // namespace i4
@@ -74,8 +75,9 @@ size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads,
   if (B < 1 || T < 1 || T > i4::KV_MAX_LEN || n_kv_heads < 1 || n_heads < n_kv_heads ||
       n_heads > 1024 || n_heads % n_kv_heads || keys < 1 || window < 0 || sinks < 0)
     return 0;
-  const int64_t S = i4::ctx_splits(B, T, n_heads, n_kv_heads, keys, window, sinks);
-  return S > 1 ? (size_t)((int64_t)B * T * n_heads * S * (i4::KHD + 2) * 4) : 0;
+  if (n_kv_heads > 1024 || B > 65535) return 0;
+  return (size_t)i4::ctx_split(B, T, n_heads, n_kv_heads, keys, window, sinks).parts *
+         ((i4::KHD + 2) * 4);
 }
 
 // the positions that a call may attend (a host position is checked after this)
@@ -109,7 +111,7 @@ static int query_check(const void* q, int x_dtype, int dtype, int B, int T, int6
   return I4_OK;
 }
 
-static i4::CtxArgs ctx_args(const void* q, int T, int64_t qbs, int64_t qts, int64_t qhs, int nq,
+static i4::CtxArgs ctx_args(const void* q, int B, int T, int64_t qbs, int64_t qts, int64_t qhs, int nq,
                             int nkv, const int32_t* pos_dev, int pos, const int32_t* counts,
                             int window, int sinks, float scale, void* out) {
   i4::CtxArgs a{};
@@ -118,6 +120,7 @@ static i4::CtxArgs ctx_args(const void* q, int T, int64_t qbs, int64_t qts, int6
   a.out = (uint16_t*)out;
   a.tk = i4::Tokens{pos_dev, counts, pos, T};
   a.w = i4::Bounds{window ? window : INT32_MAX, sinks};
+  a.B = B;
   a.nq = nq, a.nkv = nkv, a.G = nq / nkv, a.R = T * (nq / nkv);
   a.c2 = scale * 1.44269504f;
   return a;
@@ -140,12 +143,12 @@ int i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
                    counters);
   if (rc) return rc;
-  CtxArgs a = ctx_args(q, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
+  CtxArgs a = ctx_args(q, B, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
                        pos, counts, window, sinks, scale, out);
   a.c = Cache16{(uint16_t*)cache->k, (uint16_t*)cache->v, cache->batch_stride,
                 cache->head_stride, cache->row_stride, cache->max_len};
   a.len = cache->max_len;
-  return launch(a, B, x_dtype, -1, keys, i4_span{window, sinks, workspace, counters}, stream);
+  return launch(a, x_dtype, -1, keys, i4_span{window, sinks, workspace, counters}, stream);
 }
 
 int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64_t q_token_stride,
@@ -164,12 +167,12 @@ int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64
                    i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
                    counters);
   if (rc) return rc;
-  CtxArgs a = ctx_args(q, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
+  CtxArgs a = ctx_args(q, B, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
                        pos, counts, window, sinks, scale, out);
   a.c8 = Cache8{(uint8_t*)cache->k, (uint8_t*)cache->v, cache->k_scale, cache->v_scale,
                 (uint16_t*)cache->k_tail, (uint16_t*)cache->v_tail, cache->blocks};
   a.len = len;
-  return launch(a, B, x_dtype, cache->format, keys, i4_span{window, sinks, workspace, counters},
+  return launch(a, x_dtype, cache->format, keys, i4_span{window, sinks, workspace, counters},
                 stream);
 }
 

@@ -272,36 +272,97 @@ __device__ inline void put_part(float* p, float a, float b) {
   __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// Rows [r0, r1) of the row tile from their S parts, by the whole workgroup: four rows at a
+// The contexts shared out: every workgroup gets up to q tiles of one kv head, and kv head
+// (b, g) as many workgroups, one behind the other, as its tiles need, with the smallest q
+// for which that is at most a.wgs in all.  Sequences of different ages then take the same
+// time; every workgroup works this out for itself from the positions.
+struct Share {
+  int b, g, first, n;  // kv head and its workgroups [first, first + n)
+};
+__device__ inline int seq_tiles(const CtxArgs& a, int b) {
+  const CtxSeq sq = ctx_seq(a, b);
+  return sq.fit > 0 ? ctx_tiles(a.w, sq.p0, sq.p0 + sq.fit - 1).n : 0;
+}
+__device__ inline int parts_of(int tiles, int q) { return max((tiles + q - 1) / q, 1); }
+// the share of workgroup `wg`, or with head >= 0 that of this kv head (b nkv + g); false: none
+__device__ inline bool find_share(const CtxArgs& a, int wg, int head, int* s_n, Share& sh) {
+  if (a.wgs == a.B * a.nkv) {  // a workgroup each
+    const int hb = head < 0 ? wg : head;
+    sh = Share{hb / a.nkv, hb % a.nkv, hb, 1};
+    return true;
+  }
+  const int lane = threadIdx.x & 63;
+  for (int b = threadIdx.x; b < a.B; b += 256) s_n[b] = seq_tiles(a, b);
+  __syncthreads();
+  // sums of whole numbers below 2^24, exact in fp32
+  auto total = [&](auto of) {
+    float n = 0.f;
+    for (int b = lane; b < a.B; b += 64) n += (float)of(s_n[b]);
+    return (int)group_sum<64>(n) * a.nkv;
+  };
+  auto fits = [&](int q) {
+    return total([&](int n) { return parts_of(n, q); }) <= a.wgs;
+  };
+  // at least 4: a tile a wave
+  int lo = max((total([](int n) { return n; }) + a.wgs - 1) / a.wgs, 4);
+  if (!fits(lo)) {
+    int hi = 0;  // the longest context: one workgroup each
+    for (int b = lane; b < a.B; b += 64) hi = max(hi, s_n[b]);
+    for (int o = 1; o < 64; o <<= 1) hi = max(hi, __shfl_xor(hi, o));
+    for (++lo; lo < hi;) {
+      const int q = (lo + hi) >> 1;
+      if (fits(q)) hi = q;
+      else lo = q + 1;
+    }
+  }
+  int before = 0;  // workgroups of the sequences before
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int n = b0 + lane < a.B ? parts_of(s_n[b0 + lane], lo) : 0;
+    const int end = before + a.nkv * wave_incl_scan(n);
+    const uint64_t hit = __ballot(head < 0 ? wg < end : b0 + lane == head / a.nkv);
+    if (hit) {
+      const int l = __ffsll((unsigned long long)hit) - 1;
+      const int parts = __shfl(n, l), start = __shfl(end, l) - a.nkv * parts;
+      if (parts == 0) return false;  // lanes past the last sequence
+      const int g = head < 0 ? (wg - start) / parts : head % a.nkv;
+      sh = Share{b0 + l, g, start + g * parts, parts};
+      return true;
+    }
+    before = __shfl(end, 63);
+  }
+  return false;
+}
+
+// The rows of a kv head from the parts of its workgroups, by one of them: four rows at a
 // time, a wave each; lane (x = lane / 32) takes dims 4 (lane % 32) .. + 3 of every second
 // part, eight parts in flight.
-template <int XT>
-__device__ inline void merge_tile(const CtxArgs& a, int b, int g, int hb, const CtxSeq& sq,
-                                  int r0, int r1) {
+template <int XT, int ROWS>
+__device__ inline void merge_share(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int x = lane >> 5, d = 4 * (lane & 31);
-  for (int r = r0 + wave; r < r1; r += 4) {
+  for (int r = wave; r < a.R; r += 4) {
     const int t = r / a.G;
     if (t >= sq.have) continue;
-    u32x2* y = (u32x2*)(a.out + ctx_out(a, b, g, r) + d);
+    u32x2* y = (u32x2*)(a.out + ctx_out(a, sh.b, sh.g, r) + d);
     if (t >= sq.fit) {
       if (x == 0) *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
       continue;
     }
-    const int64_t at = ((int64_t)hb * a.R + r) * a.S;
-    const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * a.S);
-    const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * a.S);
+    const int64_t at = (int64_t)sh.first * ROWS + r;
+    const u32 bytes = 8u * (ROWS * (sh.n - 1) + 1);  // up to the last part's row
+    const rsrc_t ml = rsrc(a.ml + 2 * at, bytes);
+    const rsrc_t part = rsrc(a.part + at * KHD, bytes / 8u * (4u * KHD));
     float M = -__builtin_inff(), L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     constexpr int U = 8;
-    for (int s0 = x; s0 < a.S; s0 += 2 * U) {
+    for (int s0 = x; s0 < sh.n; s0 += 2 * U) {
       u32x2 v[U];
       u32x4 w[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {  // reads past the parts are zeros: an empty part
-        v[i] = __builtin_amdgcn_raw_buffer_load_b64(ml, 8u * (s0 + 2 * i), 0, kCoherent);
-        w[i] = __builtin_amdgcn_raw_buffer_load_b128(part, 4u * (KHD * (s0 + 2 * i) + d), 0,
-                                                     kCoherent);
+        const u32 k = ROWS * (s0 + 2 * i);
+        v[i] = __builtin_amdgcn_raw_buffer_load_b64(ml, 8u * k, 0, kCoherent);
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(part, 4u * (KHD * k + d), 0, kCoherent);
       }
       __builtin_amdgcn_sched_barrier(0);
       float mb = M;
@@ -337,37 +398,37 @@ __device__ inline void merge_tile(const CtxArgs& a, int b, int g, int hb, const 
   }
 }
 
-// Workgroup (split, row tile of 16 NT rows, kv head of a sequence).
+// A workgroup takes its share of the context of one kv head, all of whose rows fit into 16 NT.
 template <int XT, int FMT, int NT>
 __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(CtxArgs a) {
   __shared__ __align__(16) float s_o[4][16][KHD + 4];
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ int s_last;
-  const int split = blockIdx.x % a.S;
-  const int rt = blockIdx.x / a.S % a.tiles, hb = blockIdx.x / a.S / a.tiles;
-  const int b = hb / a.nkv, g = hb % a.nkv;
+  Share sh;
+  if (!find_share(a, blockIdx.x, -1, (int*)&s_o[0][0][0], sh)) return;
+  const int b = __builtin_amdgcn_readfirstlane(sh.b), g = __builtin_amdgcn_readfirstlane(sh.g);
+  const int parts = __builtin_amdgcn_readfirstlane(sh.n);
+  const int split = __builtin_amdgcn_readfirstlane(blockIdx.x - sh.first);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, qd = lane >> 4;
   const CtxSeq sq = ctx_seq(a, b);
-  const int r0 = rt * 16 * NT;
-  const int tlo = r0 / a.G, thi = min((r0 + 16 * NT - 1) / a.G, sq.fit - 1);
-  const bool any = tlo <= thi;  // a row with something to attend
+  const int thi = min((a.R - 1) / a.G, sq.fit - 1);  // the last token with something to attend
   RowAcc<NT> acc;
   int p[NT];  // this lane's rows' positions; -1 sees nothing
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int t = (r0 + 16 * n + m) / a.G;
-    p[n] = r0 + 16 * n + m < a.R && t < sq.fit ? sq.p0 + t : -1;
+    const int t = (16 * n + m) / a.G;
+    p[n] = 16 * n + m < a.R && t < sq.fit ? sq.p0 + t : -1;
     acc.m[n] = -__builtin_inff();
     acc.l[n] = 0.f;
 #pragma unroll
     for (int t8 = 0; t8 < 8; ++t8) acc.o[n][t8] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (any) {
-    const int plo = sq.p0 + tlo, phi = sq.p0 + thi;
+  if (thi >= 0) {
+    const int plo = sq.p0, phi = sq.p0 + thi;
     u32x4 q[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = p[n] < 0 ? tlo * a.G : r0 + 16 * n + m;  // any row that exists
+      const int r = p[n] < 0 ? 0 : 16 * n + m;  // any row that exists
       const uint16_t* row =
           a.q + b * a.qbs + (r / a.G) * a.qts + (int64_t)(g * a.G + r % a.G) * a.qhs;
 #pragma unroll
@@ -376,8 +437,8 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
     }
     const CtxTiles ct = ctx_tiles(a.w, plo, phi);
     // this workgroup's tiles, dealt to its waves in turn
-    const int i0 = (int)((int64_t)ct.n * split / a.S);
-    const int i1 = (int)((int64_t)ct.n * (split + 1) / a.S);
+    const int i0 = (int)((int64_t)ct.n * split / parts);
+    const int i1 = (int)((int64_t)ct.n * (split + 1) / parts);
     if constexpr (FMT < 0) {
       const u32 stride = (u32)a.c.rs * 2u, bytes = (u32)phi * stride + KHD * 2u;
       const int64_t base = b * a.c.bs + g * a.c.hs;
@@ -436,7 +497,7 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
           u32x4 qn[NT][4];  // dims in the 16-bit order
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const int r = p[n] < 0 ? tlo * a.G : r0 + 16 * n + m;
+            const int r = p[n] < 0 ? 0 : 16 * n + m;
             const uint16_t* row =
                 a.q + b * a.qbs + (r / a.G) * a.qts + (int64_t)(g * a.G + r % a.G) * a.qhs;
 #pragma unroll
@@ -459,7 +520,7 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
   const int row = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (n) __syncthreads();
+    __syncthreads();  // s_o has been read
     const float l = sum_qd(acc.l[n]);
     if (qd == 0) {
       s_m[wave][m] = acc.m[n];
@@ -472,7 +533,7 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
         *(f32x4*)&s_o[wave][m][32 * qd + 8 * i + t] =
             f32x4{acc.o[n][t][i], acc.o[n][t + 1][i], acc.o[n][t + 2][i], acc.o[n][t + 3][i]};
     __syncthreads();
-    const int r = r0 + 16 * n + row, t = r / a.G;
+    const int r = 16 * n + row, t = r / a.G;
     if (r < a.R && t < sq.have) {
       float M = -__builtin_inff(), L = 0.f, o[8];
 #pragma unroll
@@ -485,14 +546,14 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = fmaf(s_o[v][row][d0 + i], f, o[i]);
       }
-      if (a.S > 1 && t < sq.fit) {
-        const int64_t at = ((int64_t)hb * a.R + r) * a.S + split;
+      if (parts > 1 && t < sq.fit) {
+        const int64_t at = (int64_t)blockIdx.x * (16 * NT) + r;
         if (d0 == 0) put_part(a.ml + 2 * at, M, L);
         if (L != 0.f) {  // an empty part is skipped by its sum
 #pragma unroll
           for (int i = 0; i < 8; i += 2) put_part(a.part + at * KHD + d0 + i, o[i], o[i + 1]);
         }
-      } else if (a.S == 1) {
+      } else if (parts == 1) {
         const float inv = t < sq.fit ? 1.0f / L : __builtin_nanf("");
         u32x4 y;
 #pragma unroll
@@ -502,119 +563,49 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
       }
     }
   }
-  if (!a.counters) return;
-  // the last of the row tile's workgroups merges its parts; the count returns to 0
+  if (parts == 1 || !a.counters) return;
+  // the last of the kv head's workgroups merges their parts; the count returns to 0
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's parts are stored
   __syncthreads();
-  int32_t* count = a.counters + blockIdx.x / a.S;
+  int32_t* count = a.counters + b * a.nkv + g;
   if (threadIdx.x == 0)
-    s_last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.S - 1;
+    s_last =
+        __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
   __syncthreads();
   if (!s_last) return;
   if (threadIdx.x == 0)
     __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  merge_tile<XT>(a, b, g, hb, sq, r0, min(r0 + 16 * NT, a.R));
+  merge_share<XT, 16 * NT>(a, sh, sq);
 }
 
-// The splits of rows merged: 32 P lanes a row, each dims 4 (t % 32) .. + 3 of every P-th
-// part.  P = 8 (a workgroup a row) keeps many parts in flight at once; few parts take P = 1,
-// eight rows a workgroup.
-template <int XT, int P> __global__ __launch_bounds__(256) void k_ctx_merge(CtxArgs a, int64_t n) {
-  __shared__ __align__(16) float s_o[8][KHD];
-  __shared__ float s_m[8], s_l[8];
-  const int tid = threadIdx.x, grp = tid >> 5, part = grp % P, d = 4 * (tid & 31);
-  const int64_t at = (int64_t)blockIdx.x * (8 / P) + grp / P;  // (sequence, kv head, row)
-  const bool here = at < n;
-  const int64_t hb = here ? at / a.R : 0;
-  const int r = here ? (int)(at % a.R) : 0, t = r / a.G, b = (int)(hb / a.nkv);
-  const CtxSeq sq = ctx_seq(a, b);
-  float M = -__builtin_inff(), L = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  if (here && t < sq.fit) {
-    const float2* ml = (const float2*)a.ml + at * a.S;
-    const float* src = a.part + at * a.S * KHD + d;
-    constexpr int U = P == 1 ? 2 : 4;
-    for (int s0 = part; s0 < a.S; s0 += U * P) {
-      float2 v[U];
-      f32x4 x[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int s = min(s0 + u * P, a.S - 1);
-        v[u] = ml[s];
-        x[u] = *(const f32x4*)(src + (int64_t)s * KHD);
-        if (s0 + u * P >= a.S) v[u].y = 0.f;
-      }
-      float mb = M;  // a sum of 0: nothing seen there, no part written
-#pragma unroll
-      for (int u = 0; u < U; ++u) mb = v[u].y == 0.f ? mb : fmaxf(mb, v[u].x);
-      const float f0 = M == mb ? 1.f : exp2f(M - mb);
-      L *= f0;
-      o *= f0;
-      M = mb;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (v[u].y == 0.f) continue;
-        const float f = exp2f(v[u].x - M);
-        L = fmaf(v[u].y, f, L);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[u][e], f, o[e]);
-      }
-    }
-  }
-  if constexpr (P > 1) {
-    *(f32x4*)&s_o[grp][d] = o;
-    if (d == 0) s_m[grp] = M, s_l[grp] = L;
-    __syncthreads();
-    M = -__builtin_inff(), L = 0.f, o = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < P; ++i) M = s_l[i] == 0.f ? M : fmaxf(M, s_m[i]);
-    for (int i = 0; i < P; ++i) {
-      if (s_l[i] == 0.f) continue;
-      const float f = exp2f(s_m[i] - M);
-      L = fmaf(s_l[i], f, L);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(s_o[i][d + e], f, o[e]);
-    }
-  }
-  if (!here || t >= sq.have || part != 0) return;
-  u32x2* y = (u32x2*)(a.out + ctx_out(a, b, (int)(hb % a.nkv), r) + d);
-  if (t >= sq.fit) *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
-  else *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
+// The same merge as a launch of its own, a workgroup for each kv head.
+template <int XT, int ROWS> __global__ __launch_bounds__(256) void k_ctx_rows_merge(CtxArgs a) {
+  __shared__ int s_n[kShared];
+  Share sh;
+  if (!find_share(a, 0, blockIdx.x, s_n, sh) || sh.n == 1) return;
+  merge_share<XT, ROWS>(a, sh, ctx_seq(a, sh.b));
 }
 
-template <int XT, int FMT> static void rows_go(const CtxArgs& a, int B, hipStream_t s) {
-  const int nt = a.R <= 16 ? 1 : 2;
-  const dim3 grid((unsigned)(a.S * a.tiles * B * a.nkv));
-  if (nt == 1) k_ctx_rows<XT, FMT, 1><<<grid, 256, 0, s>>>(a);
-  else k_ctx_rows<XT, FMT, 2><<<grid, 256, 0, s>>>(a);
+template <int XT, int FMT> static void rows_go(const CtxArgs& a, hipStream_t s) {
+  if (a.R <= 16) k_ctx_rows<XT, FMT, 1><<<a.wgs, 256, 0, s>>>(a);
+  else k_ctx_rows<XT, FMT, 2><<<a.wgs, 256, 0, s>>>(a);
+  if (a.wgs == a.B * a.nkv || a.counters) return;
+  if (a.R <= 16) k_ctx_rows_merge<XT, 16><<<a.B * a.nkv, 256, 0, s>>>(a);
+  else k_ctx_rows_merge<XT, 32><<<a.B * a.nkv, 256, 0, s>>>(a);
 }
 
 }  // namespace i4
 
-int i4_launch_ctx_merge(const i4::CtxArgs& a, int B, int xt, hipStream_t s) {
-  const int64_t rows = (int64_t)B * a.nkv * a.R;
-  const bool few = a.S <= 16;
-  const dim3 grid((unsigned)(few ? (rows + 7) / 8 : rows));
-  if (xt == I4_F16) {
-    if (few) i4::k_ctx_merge<I4_F16, 1><<<grid, 256, 0, s>>>(a, rows);
-    else i4::k_ctx_merge<I4_F16, 8><<<grid, 256, 0, s>>>(a, rows);
-  } else {
-    if (few) i4::k_ctx_merge<I4_BF16, 1><<<grid, 256, 0, s>>>(a, rows);
-    else i4::k_ctx_merge<I4_BF16, 8><<<grid, 256, 0, s>>>(a, rows);
-  }
-  return hipGetLastError() == hipSuccess ? I4_OK : I4_ERR_LAUNCH;
-}
-
-int i4_launch_ctx_rows(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t s) {
+int i4_launch_ctx_rows(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s) {
   using namespace i4;
   if (xt == I4_F16) {
-    if (fmt < 0) rows_go<I4_F16, -1>(a, B, s);
-    else if (fmt == I4_KV8_INT8) rows_go<I4_F16, I4_KV8_INT8>(a, B, s);
-    else rows_go<I4_F16, I4_KV8_E4M3>(a, B, s);
+    if (fmt < 0) rows_go<I4_F16, -1>(a, s);
+    else if (fmt == I4_KV8_INT8) rows_go<I4_F16, I4_KV8_INT8>(a, s);
+    else rows_go<I4_F16, I4_KV8_E4M3>(a, s);
   } else {
-    if (fmt < 0) rows_go<I4_BF16, -1>(a, B, s);
-    else if (fmt == I4_KV8_INT8) rows_go<I4_BF16, I4_KV8_INT8>(a, B, s);
-    else rows_go<I4_BF16, I4_KV8_E4M3>(a, B, s);
+    if (fmt < 0) rows_go<I4_BF16, -1>(a, s);
+    else if (fmt == I4_KV8_INT8) rows_go<I4_BF16, I4_KV8_INT8>(a, s);
+    else rows_go<I4_BF16, I4_KV8_E4M3>(a, s);
   }
-  if (hipGetLastError() != hipSuccess) return I4_ERR_LAUNCH;
-  return a.S > 1 && !a.counters ? i4_launch_ctx_merge(a, B, xt, s) : I4_OK;
+  return hipGetLastError() == hipSuccess ? I4_OK : I4_ERR_LAUNCH;
 }

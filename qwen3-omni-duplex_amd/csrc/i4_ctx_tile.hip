@@ -474,11 +474,90 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
   }
 }
 
+// The splits of rows merged: 32 P lanes a row, each dims 4 (t % 32) .. + 3 of every P-th
+// part.  P = 8 (a workgroup a row) keeps many parts in flight at once; few parts take P = 1,
+// eight rows a workgroup.
+template <int XT, int P> __global__ __launch_bounds__(256) void k_ctx_merge(CtxArgs a, int64_t n) {
+  __shared__ __align__(16) float s_o[8][KHD];
+  __shared__ float s_m[8], s_l[8];
+  const int tid = threadIdx.x, grp = tid >> 5, part = grp % P, d = 4 * (tid & 31);
+  const int64_t at = (int64_t)blockIdx.x * (8 / P) + grp / P;  // (sequence, kv head, row)
+  const bool here = at < n;
+  const int64_t hb = here ? at / a.R : 0;
+  const int r = here ? (int)(at % a.R) : 0, t = r / a.G, b = (int)(hb / a.nkv);
+  const CtxSeq sq = ctx_seq(a, b);
+  float M = -__builtin_inff(), L = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (here && t < sq.fit) {
+    const float2* ml = (const float2*)a.ml + at * a.S;
+    const float* src = a.part + at * a.S * KHD + d;
+    constexpr int U = P == 1 ? 2 : 4;
+    for (int s0 = part; s0 < a.S; s0 += U * P) {
+      float2 v[U];
+      f32x4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = min(s0 + u * P, a.S - 1);
+        v[u] = ml[s];
+        x[u] = *(const f32x4*)(src + (int64_t)s * KHD);
+        if (s0 + u * P >= a.S) v[u].y = 0.f;
+      }
+      float mb = M;  // a sum of 0: nothing seen there, no part written
+#pragma unroll
+      for (int u = 0; u < U; ++u) mb = v[u].y == 0.f ? mb : fmaxf(mb, v[u].x);
+      const float f0 = M == mb ? 1.f : exp2f(M - mb);
+      L *= f0;
+      o *= f0;
+      M = mb;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (v[u].y == 0.f) continue;
+        const float f = exp2f(v[u].x - M);
+        L = fmaf(v[u].y, f, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(x[u][e], f, o[e]);
+      }
+    }
+  }
+  if constexpr (P > 1) {
+    *(f32x4*)&s_o[grp][d] = o;
+    if (d == 0) s_m[grp] = M, s_l[grp] = L;
+    __syncthreads();
+    M = -__builtin_inff(), L = 0.f, o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < P; ++i) M = s_l[i] == 0.f ? M : fmaxf(M, s_m[i]);
+    for (int i = 0; i < P; ++i) {
+      if (s_l[i] == 0.f) continue;
+      const float f = exp2f(s_m[i] - M);
+      L = fmaf(s_l[i], f, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(s_o[i][d + e], f, o[e]);
+    }
+  }
+  if (!here || t >= sq.have || part != 0) return;
+  u32x2* y = (u32x2*)(a.out + ctx_out(a, b, (int)(hb % a.nkv), r) + d);
+  if (t >= sq.fit) *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
+  else *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
+}
+
 }  // namespace i4
 
-int i4_launch_ctx_tile(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t s) {
+static int launch_merge(const i4::CtxArgs& a, int xt, hipStream_t s) {
+  const int64_t rows = (int64_t)a.B * a.nkv * a.R;
+  const bool few = a.S <= 16;
+  const dim3 grid((unsigned)(few ? (rows + 7) / 8 : rows));
+  if (xt == I4_F16) {
+    if (few) i4::k_ctx_merge<I4_F16, 1><<<grid, 256, 0, s>>>(a, rows);
+    else i4::k_ctx_merge<I4_F16, 8><<<grid, 256, 0, s>>>(a, rows);
+  } else {
+    if (few) i4::k_ctx_merge<I4_BF16, 1><<<grid, 256, 0, s>>>(a, rows);
+    else i4::k_ctx_merge<I4_BF16, 8><<<grid, 256, 0, s>>>(a, rows);
+  }
+  return hipGetLastError() == hipSuccess ? I4_OK : I4_ERR_LAUNCH;
+}
+
+int i4_launch_ctx_tile(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s) {
   using namespace i4;
-  const dim3 grid((unsigned)(a.tiles * a.S * B * a.nkv));
+  const dim3 grid((unsigned)(a.tiles * a.S * a.B * a.nkv));
   auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a); };
   if (xt == I4_F16) {
     if (fmt < 0) go(k_ctx_tile<I4_F16, -1>);
@@ -490,5 +569,5 @@ int i4_launch_ctx_tile(const i4::CtxArgs& a, int B, int xt, int fmt, hipStream_t
     else go(k_ctx_tile<I4_BF16, I4_KV8_E4M3>);
   }
   if (hipGetLastError() != hipSuccess) return I4_ERR_LAUNCH;
-  return a.S > 1 ? i4_launch_ctx_merge(a, B, xt, s) : I4_OK;
+  return a.S > 1 ? launch_merge(a, xt, s) : I4_OK;
 }
