@@ -34,6 +34,13 @@ struct CtxArgs {
   int32_t* counters;      // nullable: parts of a kv head that are done, 0 between calls
 };
 
+// All of the arguments' cache lines asked for at once, at a kernel's start: the compiler
+// loads each group of them where it is used, and every such load is a trip to host memory.
+__device__ inline void touch(const CtxArgs& a) {
+  asm volatile("" ::"s"(a.q), "s"(a.out), "s"(a.c.v), "s"(a.c8.k), "s"(a.c8.vt), "s"(a.tk.counts),
+               "s"(a.nq), "s"(a.part), "s"(a.counters));
+}
+
 // The context tiles (64 positions) that rows at positions [plo, phi] see: ns tiles with the
 // first tokens, then those of the window from tile w0 on; n in all.
 struct CtxTiles {
@@ -65,8 +72,12 @@ __device__ inline CtxSeq ctx_seq(const CtxArgs& a, int b) {
   s.fit = s.p0 < 0 || s.p0 >= a.len ? 0 : min(s.have, a.len - s.p0);
   return s;
 }
+// where row r of a kv head, of token t, has its output
+__device__ inline int64_t ctx_out_of(const CtxArgs& a, int b, int g, int r, int t) {
+  return (((int64_t)b * a.tk.T + t) * a.nq + g * a.G + r - t * a.G) * KHD;
+}
 __device__ inline int64_t ctx_out(const CtxArgs& a, int b, int g, int r) {
-  return (((int64_t)b * a.tk.T + r / a.G) * a.nq + g * a.G + r % a.G) * KHD;
+  return ctx_out_of(a, b, g, r, r / a.G);
 }
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));

@@ -24,6 +24,16 @@
 
 namespace i4 {
 
+// A short call is mostly instruction fetch: the code of a launch comes from L2 at some 70
+// cycles a 64-byte line, so what runs once is kept small here (no integer division, rolled
+// loops).
+
+// n / d for 0 <= n < 2^22, d > 0: the reciprocal is off by 2^-23 of the quotient, less than
+// the half that is added
+__device__ inline int udiv(int n, int d) {
+  return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)d));
+}
+
 template <int NT> struct RowAcc {
   f32x4 o[NT][8];
   float m[NT], l[NT];  // l: this lane's keys alone
@@ -64,7 +74,7 @@ __device__ inline void weights(RowAcc<NT>& acc, f32x4 (&s)[NT][NK], float c, boo
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const float m = fmaxf(acc.m[n], max_qd(top[n]));
-      const float f = m > acc.m[n] ? exp2f(acc.m[n] - m) : 1.f;
+      const float f = m > acc.m[n] ? __builtin_amdgcn_exp2f(acc.m[n] - m) : 1.f;
       acc.m[n] = m;
       acc.l[n] *= f;
 #pragma unroll
@@ -142,12 +152,14 @@ __device__ inline void clean16(RowAcc<NT>& acc, Half16& h, rsrc_t vr, int row0, 
     // some row sees it: the last one by position, the first one by the window
     const bool seen = key <= phi && (key > plo - w.window || key < w.sinks);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      h.v[j][e] = seen ? h.v[j][e] : 0u;
-      bad |= not_finite<XT>(h.v[j][e]);
-    }
+    for (int e = 0; e < 4; ++e) h.v[j][e] = seen ? h.v[j][e] : 0u;
   }
-  if (plo == phi || !__builtin_amdgcn_ballot_w64(bad)) return;
+  if (plo == phi) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bad |= not_finite<XT>(h.v[j][e]);
+  if (!__builtin_amdgcn_ballot_w64(bad)) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -283,13 +295,21 @@ __device__ inline int seq_tiles(const CtxArgs& a, int b) {
   const CtxSeq sq = ctx_seq(a, b);
   return sq.fit > 0 ? ctx_tiles(a.w, sq.p0, sq.p0 + sq.fit - 1).n : 0;
 }
-__device__ inline int parts_of(int tiles, int q) { return max((tiles + q - 1) / q, 1); }
+__device__ inline int parts_of(int tiles, int q) { return max(udiv(tiles + q - 1, q), 1); }
 // the share of workgroup `wg`, or with head >= 0 that of this kv head (b nkv + g); false: none
 __device__ inline bool find_share(const CtxArgs& a, int wg, int head, int* s_n, Share& sh) {
   if (a.wgs == a.B * a.nkv) {  // a workgroup each
     const int hb = head < 0 ? wg : head;
-    sh = Share{hb / a.nkv, hb % a.nkv, hb, 1};
+    const int b = (int)((uint32_t)hb / (uint32_t)a.nkv);
+    sh = Share{b, hb - b * a.nkv, hb, 1};
     return true;
+  }
+  if (a.B == 1) {
+    const int n = seq_tiles(a, 0), most = udiv(a.wgs, a.nkv);  // workgroups for a kv head
+    const int parts = parts_of(n, max(parts_of(n, most), 4));
+    const int g = head < 0 ? udiv(wg, parts) : head;
+    sh = Share{0, g, g * parts, parts};
+    return g < a.nkv;
   }
   const int lane = threadIdx.x & 63;
   for (int b = threadIdx.x; b < a.B; b += 256) s_n[b] = seq_tiles(a, b);
@@ -333,69 +353,60 @@ __device__ inline bool find_share(const CtxArgs& a, int wg, int head, int* s_n, 
   return false;
 }
 
-// The rows of a kv head from the parts of its workgroups, by one of them: four rows at a
-// time, a wave each; lane (x = lane / 32) takes dims 4 (lane % 32) .. + 3 of every second
-// part, eight parts in flight.
+// The rows of a kv head from the parts of its workgroups, by one of them: a row to each half
+// of a wave, whose lanes take 4 dims, with 16 parts in flight (a round of loads past the caches takes
+// 1.2 us).
 template <int XT, int ROWS>
 __device__ inline void merge_share(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int x = lane >> 5, d = 4 * (lane & 31);
-  for (int r = wave; r < a.R; r += 4) {
-    const int t = r / a.G;
-    if (t >= sq.have) continue;
-    u32x2* y = (u32x2*)(a.out + ctx_out(a, sh.b, sh.g, r) + d);
-    if (t >= sq.fit) {
-      if (x == 0) *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
-      continue;
-    }
-    const int64_t at = (int64_t)sh.first * ROWS + r;
-    const u32 bytes = 8u * (ROWS * (sh.n - 1) + 1);  // up to the last part's row
-    const rsrc_t ml = rsrc(a.ml + 2 * at, bytes);
-    const rsrc_t part = rsrc(a.part + at * KHD, bytes / 8u * (4u * KHD));
+  const int d = 4 * (threadIdx.x & 31);
+  constexpr int U = 16;
+  const int64_t at = (int64_t)sh.first * ROWS;
+  const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * ROWS * sh.n);
+  const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * ROWS * sh.n);
+#pragma unroll 1
+  for (int r = threadIdx.x >> 5; r < a.R; r += 8) {
     float M = -__builtin_inff(), L = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    constexpr int U = 8;
-    for (int s0 = x; s0 < sh.n; s0 += 2 * U) {
+#pragma unroll 1
+    for (int s0 = 0; s0 < sh.n; s0 += U) {
       u32x2 v[U];
       u32x4 w[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {  // reads past the parts are zeros: an empty part
-        const u32 k = ROWS * (s0 + 2 * i);
-        v[i] = __builtin_amdgcn_raw_buffer_load_b64(ml, 8u * k, 0, kCoherent);
-        w[i] = __builtin_amdgcn_raw_buffer_load_b128(part, 4u * (KHD * k + d), 0, kCoherent);
+        const u32 row = ROWS * (s0 + i) + r;
+        v[i] = __builtin_amdgcn_raw_buffer_load_b64(ml, 8u * row, 0, kCoherent);
+        w[i] = __builtin_amdgcn_raw_buffer_load_b128(part, 4u * (KHD * row + d), 0, kCoherent);
       }
       __builtin_amdgcn_sched_barrier(0);
       float mb = M;
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        mb = fmaxf(mb, as_f32(v[i][1]) == 0.f
-                           ? mb : as_f32(v[i][0]));
-      const float f0 = M == mb ? 1.f : exp2f(M - mb);
+      for (int i = 0; i < U; ++i) mb = as_f32(v[i][1]) == 0.f ? mb : fmaxf(mb, as_f32(v[i][0]));
+      const float f0 = M == mb ? 1.f : __builtin_amdgcn_exp2f(M - mb);
       L *= f0;
       o *= f0;
       M = mb;
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const float l = as_f32(v[i][1]);
-        if (l == 0.f) continue;
-        const float f = exp2f(as_f32(v[i][0]) - M);
+        if (l == 0.f) continue;  // its sums were never written
+        const float f = __builtin_amdgcn_exp2f(as_f32(v[i][0]) - mb);
         L = fmaf(l, f, L);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = fmaf(as_f32(w[i][e]), f, o[e]);
       }
     }
-    // the two halves of the wave
-    const float M2 = __shfl_xor(M, 32), top = fmaxf(M, M2);
-    const float f = M == top ? 1.f : exp2f(M - top);
-    L *= f;
-    L += __shfl_xor(L, 32);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[e] *= f;
-      o[e] += __shfl_xor(o[e], 32);
-    }
-    if (x == 0) *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
+    const int t = udiv(r, a.G);
+    if (t >= sq.have) continue;
+    u32x2* y = (u32x2*)(a.out + ctx_out_of(a, sh.b, sh.g, r, t) + d);
+    const float inv = 1.0f / L;
+    *y = t < sq.fit ? u32x2{pack2<XT>(o[0] * inv, o[1] * inv), pack2<XT>(o[2] * inv, o[3] * inv)}
+                    : u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
   }
+}
+
+__device__ inline const uint16_t* query_row(const CtxArgs& a, int b, int g, int r) {
+  const int t = udiv(r, a.G);
+  return a.q + b * a.qbs + t * a.qts + (int64_t)(g * a.G + r - t * a.G) * a.qhs;
 }
 
 // A workgroup takes its share of the context of one kv head, all of whose rows fit into 16 NT.
@@ -404,6 +415,7 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
   __shared__ __align__(16) float s_o[4][16][KHD + 4];
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ int s_last;
+  touch(a);
   Share sh;
   if (!find_share(a, blockIdx.x, -1, (int*)&s_o[0][0][0], sh)) return;
   const int b = __builtin_amdgcn_readfirstlane(sh.b), g = __builtin_amdgcn_readfirstlane(sh.g);
@@ -411,12 +423,12 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
   const int split = __builtin_amdgcn_readfirstlane(blockIdx.x - sh.first);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, qd = lane >> 4;
   const CtxSeq sq = ctx_seq(a, b);
-  const int thi = min((a.R - 1) / a.G, sq.fit - 1);  // the last token with something to attend
+  const int thi = sq.fit - 1;  // the last token with something to attend
   RowAcc<NT> acc;
   int p[NT];  // this lane's rows' positions; -1 sees nothing
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int t = (16 * n + m) / a.G;
+    const int t = udiv(16 * n + m, a.G);
     p[n] = 16 * n + m < a.R && t < sq.fit ? sq.p0 + t : -1;
     acc.m[n] = -__builtin_inff();
     acc.l[n] = 0.f;
@@ -428,17 +440,15 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
     u32x4 q[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = p[n] < 0 ? 0 : 16 * n + m;  // any row that exists
-      const uint16_t* row =
-          a.q + b * a.qbs + (r / a.G) * a.qts + (int64_t)(g * a.G + r % a.G) * a.qhs;
+      const uint16_t* row = query_row(a, b, g, p[n] < 0 ? 0 : 16 * n + m);  // one that exists
 #pragma unroll
       for (int c = 0; c < 4; ++c)  // dims as the keys' lanes hold them
         q[n][c] = ldg16(row + (FMT < 0 ? 32 * c + 8 * qd : 64 * (c >> 1) + 16 * qd + 8 * (c & 1)));
     }
     const CtxTiles ct = ctx_tiles(a.w, plo, phi);
     // this workgroup's tiles, dealt to its waves in turn
-    const int i0 = (int)((int64_t)ct.n * split / parts);
-    const int i1 = (int)((int64_t)ct.n * (split + 1) / parts);
+    const int each = udiv(ct.n, parts), more = ct.n - each * parts;
+    const int i0 = split * each + min(split, more), i1 = i0 + each + (split < more ? 1 : 0);
     if constexpr (FMT < 0) {
       const u32 stride = (u32)a.c.rs * 2u, bytes = (u32)phi * stride + KHD * 2u;
       const int64_t base = b * a.c.bs + g * a.c.hs;
@@ -497,9 +507,7 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
           u32x4 qn[NT][4];  // dims in the 16-bit order
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const int r = p[n] < 0 ? 0 : 16 * n + m;
-            const uint16_t* row =
-                a.q + b * a.qbs + (r / a.G) * a.qts + (int64_t)(g * a.G + r % a.G) * a.qhs;
+            const uint16_t* row = query_row(a, b, g, p[n] < 0 ? 0 : 16 * n + m);
 #pragma unroll
             for (int c = 0; c < 4; ++c) qn[n][c] = ldg16(row + 32 * c + 8 * qd);
           }
@@ -533,15 +541,16 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
         *(f32x4*)&s_o[wave][m][32 * qd + 8 * i + t] =
             f32x4{acc.o[n][t][i], acc.o[n][t + 1][i], acc.o[n][t + 2][i], acc.o[n][t + 3][i]};
     __syncthreads();
-    const int r = 16 * n + row, t = r / a.G;
+    const int r = 16 * n + row, t = udiv(r, a.G);
     if (r < a.R && t < sq.have) {
       float M = -__builtin_inff(), L = 0.f, o[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = 0.f;
       for (int v = 0; v < 4; ++v) M = fmaxf(M, s_m[v][row]);
+#pragma unroll 1
       for (int v = 0; v < 4; ++v) {
         if (s_m[v][row] == -__builtin_inff() && s_l[v][row] == 0.f) continue;
-        const float f = exp2f(s_m[v][row] - M);
+        const float f = __builtin_amdgcn_exp2f(s_m[v][row] - M);
         L = fmaf(s_l[v][row], f, L);
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] = fmaf(s_o[v][row][d0 + i], f, o[i]);
@@ -559,7 +568,7 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = pack2<XT>(o[2 * i] * inv, o[2 * i + 1] * inv);
         if (!(t < sq.fit)) y = u32x4{} + (u32)Half<XT>::QNAN * 0x10001u;
-        *(u32x4*)(a.out + ctx_out(a, b, g, r) + d0) = y;
+        *(u32x4*)(a.out + ctx_out_of(a, b, g, r, t) + d0) = y;
       }
     }
   }
