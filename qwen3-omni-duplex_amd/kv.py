@@ -56,22 +56,26 @@ def _batched(x: torch.Tensor, dims: int, name: str) -> torch.Tensor:
 def _cache_c(k: torch.Tensor, v: torch.Tensor) -> _lib.KVCacheC:
     """struct i4_kvcache of [n_kv_heads, max_len, head_dim] or [B, n_kv_heads, max_len,
     head_dim] caches (views with any strides above a dense last dimension)."""
-    k, v = _batched(k, 4, "k_cache"), _batched(v, 4, "v_cache")
-    shape, strides = k.shape, k.stride()
-    if shape != v.shape or k.dtype != v.dtype or strides != v.stride():
+    if k.dim() != 4 or v.dim() != 4:
+        k, v = _batched(k, 4, "k_cache"), _batched(v, 4, "v_cache")
+    shape, strides, dtype = k.shape, k.stride(), k.dtype
+    if shape != v.shape or dtype != v.dtype or strides != v.stride():
         raise RuntimeError("k_cache and v_cache must agree in shape, strides and dtype")
     if strides[3] != 1:
         raise RuntimeError("the caches' last dimension must be contiguous")
-    return _lib.KVCacheC(k.data_ptr(), v.data_ptr(), *strides[:3], *shape,
-                         _lib.half_code(k.dtype))
+    return _lib.KVCacheC(k.data_ptr(), v.data_ptr(), strides[0], strides[1], strides[2], *shape,
+                         _lib.half_code(dtype))
 
 
 def _out(out: torch.Tensor | None, like: torch.Tensor, shape: tuple[int, ...],
          padded: bool) -> torch.Tensor:
     """The given output, checked, or a new one (zeros where padding will stay unwritten)."""
     if out is None:
-        make = torch.zeros if padded else torch.empty
-        return make(shape, dtype=like.dtype, device=like.device)
+        if padded:
+            return torch.zeros(shape, dtype=like.dtype, device=like.device)
+        if like.shape == shape and like.is_contiguous():
+            return torch.empty_like(like)  # 0.5 us less than spelling it out
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
     if tuple(out.shape) != shape or out.dtype != like.dtype or not out.is_contiguous():
         raise RuntimeError(f"out must be a contiguous {shape} tensor of {like.dtype}")
     return out
@@ -92,12 +96,21 @@ def _call(dev: torch.device, entry, *args) -> None:
 _STREAM_WS: dict = {}
 
 
-def _kept_workspace(dev: torch.device) -> Workspace:
-    """The workspace of calls that bring none: one per stream, whose calls run in order; under
-    capture one of the call's own, which the graph then owns."""
-    if torch.cuda.is_current_stream_capturing():
-        return Workspace()
-    return _STREAM_WS.setdefault((dev.index, _lib.stream(dev)), Workspace())
+def _scratch(workspace: Workspace | None, need: int,
+             dev: torch.device) -> tuple[int, int | None]:
+    """The addresses of `need` bytes and of the counters: of the caller's workspace, else of
+    one per stream, whose calls run in order; under capture one of the call's own, which the
+    graph then owns."""
+    if workspace is None:
+        if torch.cuda.is_current_stream_capturing():
+            workspace = Workspace()
+        else:
+            key = (dev.index, _lib.stream(dev))
+            workspace = _STREAM_WS.get(key) or _STREAM_WS.setdefault(key, Workspace())
+            buf, counters = workspace.buf, workspace._counters
+            if buf is not None and buf.numel() >= need and counters is not None:
+                return buf.data_ptr(), counters.data_ptr()
+    return workspace.get(need, dev).data_ptr(), _lib.ptr(workspace.counters(dev))
 
 
 def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torch.Tensor,
@@ -164,15 +177,13 @@ def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
     y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd), counts is not None)
     on_dev = isinstance(pos, torch.Tensor)
     pd, ph = (_int32(pos, B, dev, "pos"), 0) if on_dev else (None, int(pos))
-    w = 0 if window is None else min(int(window), 2**31 - 1)
+    w = 0 if window is None else min(window, 2**31 - 1)
     need = _lib.lib().i4_attn_window_workspace_bytes(
         B, T, nh, cc.n_kv_heads, keys if on_dev else min(max(ph, 0) + T, keys), w, sinks)
-    ws = counters = None
-    if need:
-        kept = workspace or _kept_workspace(dev)
-        ws, counters = kept.get(need, dev).data_ptr(), _lib.ptr(kept.counters(dev))
-    _call(dev, entry, x.data_ptr(), _lib.half_code(x.dtype), T, *x.stride()[:3], nh,
-          ctypes.byref(cc), pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
+    ws, counters = _scratch(workspace, need, dev) if need else (None, None)
+    s0, s1, s2, _ = x.stride()
+    _call(dev, entry, x.data_ptr(), _lib.half_code(x.dtype), T, s0, s1, s2, nh, ctypes.byref(cc),
+          pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
           hd ** -0.5 if scale is None else scale, y.data_ptr(), ws, need, counters)
     return y
 
