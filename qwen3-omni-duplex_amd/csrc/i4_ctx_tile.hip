@@ -164,24 +164,13 @@ __device__ inline void tile_mask(f32x16 (&s)[2], int key0, int p, const Bounds& 
     }
 }
 
-// the weights of 16 keys (step ks of the tile's four) as the product's operand, and what
-// their rounding left
-template <int PT> __device__ inline u32x4 weights_hi(const f32x16 (&s)[2], int ks) {
+// the weights of 16 keys (step ks of the tile's four) as the product's operand
+template <int PT> __device__ inline u32x4 weights16(const f32x16 (&s)[2], int ks) {
   const f32x16& x = s[ks >> 1];
   const int o = 8 * (ks & 1);
   return u32x4{pack2<PT>(x[o], x[o + 1]), pack2<PT>(x[o + 2], x[o + 3]),
                pack2<PT>(x[o + 4], x[o + 5]), pack2<PT>(x[o + 6], x[o + 7])};
 }
-template <int PT> __device__ inline u32x4 weights_lo(const f32x16 (&s)[2], int ks, u32x4 hi) {
-  const f32x16& x = s[ks >> 1];
-  const int o = 8 * (ks & 1);
-  u32x4 r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    r[i] = pack2<PT>(x[o + 2 * i] - lo_f32<PT>(hi[i]), x[o + 2 * i + 1] - hi_f32<PT>(hi[i]));
-  return r;
-}
-
 // O^T += V^T P^T for a 16-bit tile
 template <int XT>
 __device__ inline void tile_values16(TileAcc& acc, const f32x16 (&s)[2], const lds_t* v,
@@ -204,7 +193,7 @@ __device__ inline void tile_values16(TileAcc& acc, const f32x16 (&s)[2], const l
 #pragma unroll
   for (int y = 0; y < 8; ++y) {
     if (y < 6) load(y + 2);
-    if ((y & 1) == 0) b = weights_hi<XT>(s, y >> 1);
+    if ((y & 1) == 0) b = weights16<XT>(s, y >> 1);
     I4_ORDER();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -258,9 +247,8 @@ __device__ inline void add_not_finite(TileAcc& acc, const uint16_t* v, u32 strid
   }
 }
 
-// O^T += V^T P^T for an 8-bit block, in bf16, whose range holds any scale.  TWO: the weights
-// as a sum of two (queries in fp16 have three bits more than one bf16 weight)
-template <bool TWO>
+// O^T += V^T P^T for an 8-bit block
+template <int XT>
 __device__ inline void tile_values8(TileAcc& acc, const f32x16 (&s)[2], const lds_t* v, int n,
                                     int h) {
   const lds_t* row = v + n * 128;
@@ -272,20 +260,16 @@ __device__ inline void tile_values8(TileAcc& acc, const f32x16 (&s)[2], const ld
   };
   load(0);
   load(1);
-  u32x4 b, b2;
+  u32x4 b;
 #pragma unroll
   for (int y = 0; y < 8; ++y) {
     if (y < 6) load(y + 2);
-    if ((y & 1) == 0) {
-      b = weights_hi<I4_BF16>(s, y >> 1);
-      if constexpr (TWO) b2 = weights_lo<I4_BF16>(s, y >> 1, b);
-    }
+    if ((y & 1) == 0) b = weights16<XT>(s, y >> 1);
     I4_ORDER();
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int t = 2 * (y & 1) + u;
-      acc.o[t] = mfma32<I4_BF16>(a[y % 3][u], b, acc.o[t]);
-      if constexpr (TWO) acc.o[t] = mfma32<I4_BF16>(a[y % 3][u], b2, acc.o[t]);
+      acc.o[t] = mfma32<XT>(a[y % 3][u], b, acc.o[t]);
     }
     I4_ORDER();
   }
@@ -320,8 +304,8 @@ template <int XT, int FMT> __device__ inline void store8(const Stage8& st, lds_t
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int c = 4 * (tid & 1) + 2 * i;
-    lds_put(v + ((c ^ (d & 7)) * 16), cvt8<FMT, I4_BF16>(st.v[i][0], st.v[i][2]));
-    lds_put(v + (((c + 1) ^ (d & 7)) * 16), cvt8<FMT, I4_BF16>(st.v[i][1], st.v[i][3]));
+    lds_put(v + ((c ^ (d & 7)) * 16), cvt8<FMT, XT>(st.v[i][0], st.v[i][2]));
+    lds_put(v + (((c + 1) ^ (d & 7)) * 16), cvt8<FMT, XT>(st.v[i][1], st.v[i][3]));
   }
 }
 
@@ -402,6 +386,18 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       const int e = i1 - (tail ? 1 : 0);
       Stage8 s8;
       float ks = 0.f, vs = 0.f;
+      // The weights that enter the product take the values' scale, in the exponent; their sum
+      // gives it back.  In fp16, whose range does not hold any scale, the scale is taken in
+      // units of a power of two near it, and the sums so far follow when the unit changes.
+      // It stays above 2^-30 of the largest one there was: what a block of so much smaller
+      // values adds is lost only to rows that met larger ones (and their sums would overflow).
+      float unit = 1.f, top = 0.f;
+      auto set_unit = [&](float u) {
+        const float f = unit / u;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc.o[t] *= f;
+        unit = u;
+      };
       if (i0 < e) {
         load8(s8, a.c8, hblk + ct.at(i0), tid);
         store8<XT, FMT>(s8, lds, tid);
@@ -416,10 +412,19 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
           tile_scores<XT>(buf, q, s, n, h);
           if (!whole(i)) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
           tile_max(acc, s, a.c2 * ks);
-          // the weights that enter the product take the values' scale, in the exponent; their
-          // sum gives it back
-          acc.l = fmaf(tile_weights(acc, s, a.c2 * ks, kLift + log2f(vs)), 1.0f / vs, acc.l);
-          tile_values8<XT == I4_F16>(acc, s, buf + TBYTES, n, h);
+          float r = vs;
+          if constexpr (XT == I4_F16) {
+            if (!(vs <= unit && vs > 0.125f * unit)) {
+              // the power of two above vs
+              const float near = as_f32((__builtin_bit_cast(u32, vs) & 0x7F800000u) + 0x00800000u);
+              top = fmaxf(top, near);
+              const float u = fmaxf(near, 0x1p-30f * top);
+              if (u != unit) set_unit(u);
+            }
+            r = vs / unit;
+          }
+          acc.l = fmaf(tile_weights(acc, s, a.c2 * ks, kLift + log2f(r)), 1.0f / r, acc.l);
+          tile_values8<XT>(acc, s, buf + TBYTES, n, h);
         } else if (j0 <= p && (min(j0 + KBLK - 1, p) > p - a.w.window || j0 < a.w.sinks)) {
           acc.l = __builtin_nanf("");  // a block that reads as NaN, for a row that sees a key
         }
@@ -428,6 +433,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
           ks = s8.ks, vs = s8.vs;
         }
       }
+      if (XT == I4_F16 && unit != 1.f) set_unit(1.f);
       if (tail) {
         const int64_t at = (int64_t)hb * (KBLK * KHD);
         const int rows = phi - full * KBLK + 1;

@@ -404,6 +404,28 @@ def test_attn_kv8_matches_64_bits(pkg, dev, dtype, kind, B, T, nh, nkv, pos, win
         check(pkg.attn_kv8(q[0], cache, pos, window=window, sinks=sinks)[None], want, tol)
 
 
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,nh", [(1, 4), (6, 4), (130, 2)])
+def test_attn_kv8_block_scales(pkg, dev, dtype, kind, T, nh):
+    """Value blocks of very different magnitudes, zeros among them, up and down."""
+    total = 64 * 14 + T
+    kv = rand(dev, 2, 1, total, 1, HD, seed=4, dtype=torch.float32)
+    steps = [0, 6, -9, -9, 3, 14, None, 0, -4, 10, None, 2, -14, 5, 0, 0, 1]
+    for i, p in enumerate(steps):
+        kv[1, :, 64 * i:64 * i + 64] *= 0.0 if p is None else 2.0 ** p
+    kv = kv.to(dtype)
+    cache = pkg.KV8Cache.empty(1, total, dtype=dtype, kind=kind, device=dev)
+    want8 = ref.Cache8(1, 1, cache.max_len // 64, kind, dtype)
+    pkg.kv8_append(kv[0], kv[1], cache, 0)
+    want8.append(kv, [0], [total])
+    q = rand(dev, 1, T, nh, HD, seed=8, dtype=dtype)
+    k, v = want8.rows([total])
+    for window, sinks in ((None, 0), (70, 0), (200, 65)):
+        want, tol = ref.attention(q, k, v, [total - T], [T], window, sinks)
+        check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("T,nh", [(1, 8), (2, 8), (5, 24), (120, 8)])
 def test_attn_kv8_padding_outside_and_bad_blocks(pkg, dev, kind, T, nh):
