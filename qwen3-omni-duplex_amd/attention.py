@@ -14,13 +14,16 @@ heads), and q/k norm, rotary embedding, KV-cache append and GQA attention in
 i4_attn_decode_qkv_o.  The KV cache is preallocated
 ([n_kv_heads, max_len, head_dim] per layer, the activation dtype) instead of
 transformers' growing DynamicCache.
+
+Prompts and chunks of several tokens, a bounded context (window, sinks) and an 8-bit cache
+(kv_dtype) run launch by launch instead, on rope_append and attn_window / attn_kv8 (kv.py).
 """
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
 
-from . import _lib, ops
+from . import _lib, kv, ops
 from .linear import PackedLinear, PackedQKV
 from .moe import FusedPackedMoE
 
@@ -32,13 +35,23 @@ def rope_inv_freq(head_dim: int, theta: float) -> torch.Tensor:
 
 
 class ThinkerAttention(nn.Module):
-    """One decode token of the attention half of a Thinker layer, residual included."""
+    """The attention half of a Thinker layer, residual included: one decode token, or the
+    several tokens of a prompt or chunk.
+
+    window: a token attends the last `window` positions (its own among them) and the first
+    `sinks` ones; None: every position.  kv_dtype torch.int8 or torch.float8_e4m3fn: the cache
+    is a KV8Cache (self.kv8) instead of the 16-bit k_cache / v_cache, and tokens arrive in
+    order."""
 
     def __init__(self, qkv: PackedQKV, o_proj: PackedLinear, q_norm_w: torch.Tensor,
                  k_norm_w: torch.Tensor, input_norm_w: torch.Tensor, n_heads: int,
                  n_kv_heads: int, head_dim: int = 128, eps: float = 1e-6,
-                 rope_theta: float = 1_000_000.0, max_len: int = 4096):
+                 rope_theta: float = 1_000_000.0, max_len: int = 4096,
+                 window: int | None = None, sinks: int = 0,
+                 kv_dtype: torch.dtype | None = None):
         super().__init__()
+        if window is not None and window < 1 or sinks < 0 or (window is None and sinks):
+            raise ValueError("window must be at least 1, and sinks need a window")
         if qkv.lin.w.layout != "ct":
             raise ValueError("the q|k|v weight must be in the CT layout: the input norm runs "
                              "inside its GEMV (build PackedQKV with repack=True)")
@@ -52,12 +65,16 @@ class ThinkerAttention(nn.Module):
         self.register_buffer("k_norm_w", k_norm_w.to(dt).contiguous(), persistent=False)
         self.register_buffer("input_norm_w", input_norm_w.contiguous(), persistent=False)
         self.inv_freq = rope_inv_freq(head_dim, rope_theta)  # host table
-        shape = (n_kv_heads, max_len, head_dim)
         dev = input_norm_w.device
+        self.window, self.sinks = window, int(sinks)
+        self.kv8 = None if kv_dtype is None else kv.KV8Cache.empty(
+            n_kv_heads, max_len, head_dim, dtype=dt, kind=kv_dtype, device=dev)
+        shape = (n_kv_heads, max_len if kv_dtype is None else 0, head_dim)
         self.register_buffer("_k_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
         self.register_buffer("_v_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
         self.max_len = int(max_len)
         self.workspace = ops.Workspace()
+        self.context_workspace = ops.Workspace()  # of _attend: its counters stay with it
 
     # The caches are written in place by the kernels and their addresses are held by the
     # decoder's layer structs, so they cannot be replaced: fill them in place
@@ -74,21 +91,38 @@ class ThinkerAttention(nn.Module):
         """Empty the KV cache in place (a new conversation)."""
         self._k_cache.zero_()
         self._v_cache.zero_()
+        if self.kv8 is not None:
+            self.kv8.reset()
+
+    def _apply(self, fn, *args, **kwargs):
+        super()._apply(fn, *args, **kwargs)
+        dev = self.input_norm_w.device
+        if self.kv8 is not None and self.kv8.k.device != dev:
+            self.kv8 = kv.KV8Cache(*(t.to(dev) for t in self.kv8.tensors))
+        return self
+
+    def whole_context(self) -> bool:
+        """Whether tokens attend a 16-bit cache without a bound, as the decode entries do."""
+        return self.window is None and self.kv8 is None
 
     def __setattr__(self, name, value):
         super().__setattr__(name, value)
         ops.weights_changed()
 
     def forward(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
-        """h [1, H] (one token at cache position pos) -> h + o_proj(attn(norm(h))).
+        """h [T, H] (T tokens at cache positions pos, pos + 1, ...) -> h + o_proj(attn(norm(h))).
 
         pos is an int, or an int32 device tensor of one element that the kernels read (a
         decode step captured in a hipGraph then serves every token; a position outside the
         cache gives NaN and leaves the cache untouched)."""
-        if h.numel() != h.shape[-1]:
-            raise ValueError("ThinkerAttention decodes one token")
-        if not isinstance(pos, torch.Tensor) and not 0 <= pos < self.max_len:
-            raise ValueError(f"position {pos} outside the cache (max_len {self.max_len})")
+        T = h.numel() // h.shape[-1]
+        if T < 1:
+            raise ValueError("no token")
+        if not isinstance(pos, torch.Tensor) and not 0 <= pos <= self.max_len - T:
+            raise ValueError(f"positions {pos} to {pos + T - 1} outside the cache "
+                             f"(max_len {self.max_len})")
+        if T > 1 or not self.whole_context():
+            return self._attend(h, pos)
         if self.o_proj.w.layout == "ct":
             # input_layernorm + q|k|v inside the attention chunk launch, then the head
             # merge and o_proj (+ the residual) in one more
@@ -105,8 +139,32 @@ class ThinkerAttention(nn.Module):
         return ops.linear(a.view(1, -1), self.o_proj.w, bias=h.reshape(-1)).view(h.shape)
 
 
+    def _attend(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
+        """Several tokens, a bounded context or an 8-bit cache, launch by launch."""
+        H, n, hd = h.shape[-1], self.n_kv_heads, self.head_dim
+        x = h.reshape(-1, H)
+        qkv = self.qkv.lin(ops.rmsnorm(x, self.input_norm_w, self.eps))
+        eight = self.kv8 is not None
+        if eight:  # the tokens' keys and values on their way to the 8-bit blocks
+            k, v = torch.empty(2, n, x.shape[0], hd, dtype=h.dtype, device=h.device).unbind(0)
+        else:
+            k, v = self.k_cache, self.v_cache
+        q = kv.rope_append(qkv, self.n_heads, n, self.q_norm_w, self.k_norm_w, self.eps,
+                           self.inv_freq, pos, k, v, first_row=0 if eight else None)
+        bounds = {"window": self.window, "sinks": self.sinks, "workspace": self.context_workspace}
+        if eight:
+            kv.kv8_append(k.transpose(0, 1), v.transpose(0, 1), self.kv8, pos)
+            a = kv.attn_kv8(q, self.kv8, pos, **bounds)
+        else:
+            a = kv.attn_window(q, k, v, pos, **bounds)
+        a = a.view(x.shape[0], -1)
+        if x.shape[0] == 1:  # the residual enters the o_proj launch as its bias
+            return ops.linear(a, self.o_proj.w, bias=x.reshape(-1)).view(h.shape)
+        return self.o_proj(a).add_(x).view(h.shape)
+
+
 class ThinkerDecoderLayer(nn.Module):
-    """Qwen3OmniMoeThinkerTextDecoderLayer.forward for one decode token."""
+    """Qwen3OmniMoeThinkerTextDecoderLayer.forward for one decode token, or several tokens."""
 
     def __init__(self, attn: ThinkerAttention, moe: FusedPackedMoE):
         super().__init__()
@@ -121,7 +179,7 @@ class ThinkerDecoderLayer(nn.Module):
         a, m = self.attn, self.moe
         if self._fused is None:
             self._fused = bool(
-                a.qkv.lin.w.layout == "ct" and a.o_proj.w.layout == "ct"
+                a.whole_context() and a.qkv.lin.w.layout == "ct" and a.o_proj.w.layout == "ct"
                 and m.gate_up.layout == "ct" and m.router_w is not None
                 and ops.thinker_layer_fits(a.n_heads, a.n_kv_heads, a.head_dim, a.max_len,
                                            m.hidden, m.down.K, m.gate_up.E, m.top_k))
@@ -146,8 +204,9 @@ class ThinkerDecoderLayer(nn.Module):
 
 
 class ThinkerDecoder(nn.Module):
-    """Thinker[0:n] decode: step(h, pos) runs every layer on one token and returns the
-    hidden state after the last layer (the clock path's layer-24 tap, clock.py:168)."""
+    """Thinker[0:n] decode: step(h, pos) runs every layer on one token, or on the several
+    tokens of a prompt, and returns the hidden state after the last layer (the clock path's
+    layer-24 tap, clock.py:168)."""
 
     def __init__(self, layers: list[ThinkerDecoderLayer]):
         super().__init__()

@@ -88,8 +88,8 @@ __device__ inline void stage16(uint64_t k, uint64_t v, int j0, int last, u32 str
 // 5000-token one over 8 bits.
 //
 // Tried and slower: the next tile's scores computed between this tile's exponentials within
-// a wave (321 us against 293: two of the 256 registers' worth of scores cost the operands
-// that are read ahead), and the weights' sum as dot products of the packed weights (312).
+// a wave (11 % more cycles: a second set of scores leaves fewer operands read ahead).  The
+// weights' sum as dot products of the packed weights: no difference.
 
 // A fence for the scheduler: LDS reads are issued two products ahead of their use, which it
 // would undo to save registers (a wave then waits out LDS's latency at every product).

@@ -251,6 +251,11 @@ class KV8Cache:
                  for _ in range(2)]
         return cls(*bits, *scales, *tails)
 
+    @property
+    def tensors(self) -> tuple[torch.Tensor, ...]:
+        """k, v, k_scale, v_scale, k_tail, v_tail: what the constructor takes."""
+        return self._t
+
     k = property(lambda self: self._t[0])
     v = property(lambda self: self._t[1])
     k_scale = property(lambda self: self._t[2])

@@ -224,8 +224,10 @@ def rope_theta(tc: dict) -> float:
 
 
 def load_thinker_layer(ckpt: Checkpoint, layer: int, device="cuda", dtype=torch.bfloat16,
-                       max_len: int = 4096, layouts: str = "both") -> ThinkerDecoderLayer:
-    """One Thinker decoder layer for decode: attention (input_layernorm, q|k|v in one
+                       max_len: int = 4096, layouts: str = "both",
+                       **context) -> ThinkerDecoderLayer:
+    """One Thinker decoder layer for decode (context: ThinkerAttention's window, sinks and
+    kv_dtype): attention (input_layernorm, q|k|v in one
     launch, q_norm / k_norm, rotary, KV cache of max_len positions, o_proj) and the MoE
     block with its post_attention_layernorm (clock.py:45-103 loads the same tensors)."""
     tc = ckpt.text_config()
@@ -238,13 +240,15 @@ def load_thinker_layer(ckpt: Checkpoint, layer: int, device="cuda", dtype=torch.
         ckpt.tensor(f"{base}.self_attn.q_norm.weight").to(device, dtype),
         ckpt.tensor(f"{base}.self_attn.k_norm.weight").to(device, dtype),
         ckpt.tensor(f"{base}.input_layernorm.weight").to(device, dtype),
-        nh, nkv, hd, float(tc.get("rms_norm_eps", 1e-6)), rope_theta(tc), max_len)
+        nh, nkv, hd, float(tc.get("rms_norm_eps", 1e-6)), rope_theta(tc), max_len, **context)
     return ThinkerDecoderLayer(attn, load_moe_layer(ckpt, layer, device, dtype, layouts))
 
 
 def load_thinker_decoder(root: str | Path, n_layers: int = 24, device="cuda",
-                         dtype=torch.bfloat16, max_len: int = 4096) -> ThinkerDecoder:
-    """Thinker[0:n_layers] for one-token decode steps (the clock path's prefix)."""
+                         dtype=torch.bfloat16, max_len: int = 4096,
+                         **context) -> ThinkerDecoder:
+    """Thinker[0:n_layers] for decode steps and prompts (the clock path's prefix); context:
+    ThinkerAttention's window, sinks and kv_dtype."""
     ckpt = Checkpoint(root)
-    return ThinkerDecoder([load_thinker_layer(ckpt, layer, device, dtype, max_len)
+    return ThinkerDecoder([load_thinker_layer(ckpt, layer, device, dtype, max_len, **context)
                            for layer in range(n_layers)])
