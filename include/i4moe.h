@@ -744,7 +744,8 @@ size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads,
  * rounded from the 16-bit tail and tokens, the rest goes to the tail.  A block whose
  * largest magnitude is below 2^-100 is scaled as if it were 2^-100; one that holds an
  * infinity or a NaN gets the scale NaN and reads as NaN.  Tokens must arrive in order: a
- * pos inside a finished block finds its earlier tokens in the tail no more. */
+ * pos inside a finished block finds its earlier tokens in the tail no more.
+ * batch n_kv_heads <= 32767. */
 int    i4_kv8_append(const void* k, const void* v, int x_dtype, int T, int64_t batch_stride,
                      int64_t token_stride, int64_t head_stride, const i4_kv8cache* cache,
                      const int32_t* pos_dev, int pos, const int32_t* counts,

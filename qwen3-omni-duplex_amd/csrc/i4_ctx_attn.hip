@@ -27,7 +27,7 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
   const int64_t span = few ? T : (kTileRows + nq / nkv - 1) / (nq / nkv) + 1;
   int64_t tiles = (keys + 63) / 64;
   if (window) {
-    const int64_t most = ((int64_t)window + span + 126) / 64 + (sinks + 63) / 64;
+    const int64_t most = ((int64_t)window + span + 126) / 64 + ((int64_t)sinks + 63) / 64;
     if (most < tiles) tiles = most;
   }
   const int64_t heads = (int64_t)B * nkv;

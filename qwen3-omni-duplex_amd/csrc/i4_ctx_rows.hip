@@ -358,8 +358,8 @@ __device__ inline bool find_share(const CtxArgs& a, int wg, int head, int* s_n, 
 }
 
 // The rows of a kv head from the parts of its workgroups, by one of them: a row to each half
-// of a wave, whose lanes take 4 dims, with 16 parts in flight (a round of loads past the caches takes
-// 1.2 us).
+// of a wave, whose lanes take 4 dims, with 16 parts in flight (a round of loads past the
+// caches takes 1.2 us).
 template <int XT, int ROWS>
 __device__ inline void merge_share(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
   const int d = 4 * (threadIdx.x & 31);

@@ -44,6 +44,13 @@ def _int32(t: torch.Tensor | None, B: int, dev: torch.device, name: str) -> int 
     return t.data_ptr()
 
 
+def _host_pos(pos: int, T: int, limit: int) -> int:
+    """A host position whose T tokens fit below limit (ctypes would wrap a larger int)."""
+    if not 0 <= pos <= limit - T:
+        raise RuntimeError(f"positions {pos} to {pos + T - 1} outside [0, {limit})")
+    return int(pos)
+
+
 def _batched(x: torch.Tensor, dims: int, name: str) -> torch.Tensor:
     """x with its batch dimension (one sequence may come without)."""
     if x.dim() == dims:
@@ -145,14 +152,16 @@ def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torc
             or not inv_freq.is_contiguous():
         inv_freq = inv_freq.detach().to("cpu", torch.float32).contiguous()
     q_norm_w, k_norm_w = q_norm_w.contiguous(), k_norm_w.contiguous()
-    if first_row is not None and first_row < 0:
-        raise RuntimeError("first_row must not be negative")
+    if first_row is not None:
+        if not 0 <= first_row <= cc.max_len - T:
+            raise RuntimeError(f"first_row {first_row}: {T} rows do not fit the cache")
     shape = (B, T, n_heads, hd)
     q = _out(out, x, shape if qkv.dim() == 3 else shape[1:], counts is not None)
     on_dev = isinstance(pos, torch.Tensor)
     _call(dev, _lib.lib().i4_rope_append, x.data_ptr(), cc.dtype, T, x.stride(0), x.stride(1),
           n_heads, q_norm_w.data_ptr(), k_norm_w.data_ptr(), eps, inv_freq.data_ptr(),
-          _int32(pos, B, dev, "pos") if on_dev else None, 0 if on_dev else int(pos),
+          _int32(pos, B, dev, "pos") if on_dev else None,
+          0 if on_dev else _host_pos(pos, T, cc.max_len if first_row is None else 1 << 24),
           -1 if first_row is None else int(first_row), _int32(counts, B, dev, "counts"),
           q.data_ptr(), ctypes.byref(cc))
     return q
@@ -170,16 +179,17 @@ def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
                            f"head_dim {cc.head_dim}")
     if window is not None and window < 1:
         raise RuntimeError("window must be at least 1 (None: no bound)")
+    sinks = min(sinks, 2**31 - 1)
     if window is None and sinks:
         raise RuntimeError("sinks are the first tokens outside a window: give the window too")
     if x.stride(3) != 1:
         x = x.contiguous()
     y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd), counts is not None)
     on_dev = isinstance(pos, torch.Tensor)
-    pd, ph = (_int32(pos, B, dev, "pos"), 0) if on_dev else (None, int(pos))
+    pd, ph = (_int32(pos, B, dev, "pos"), 0) if on_dev else (None, _host_pos(pos, T, keys))
     w = 0 if window is None else min(window, 2**31 - 1)
     need = _lib.lib().i4_attn_window_workspace_bytes(
-        B, T, nh, cc.n_kv_heads, keys if on_dev else min(max(ph, 0) + T, keys), w, sinks)
+        B, T, nh, cc.n_kv_heads, keys if on_dev else ph + T, w, sinks)
     ws, counters = _scratch(workspace, need, dev) if need else (None, None)
     s0, s1, s2, _ = x.stride()
     _call(dev, entry, x.data_ptr(), _lib.half_code(x.dtype), T, s0, s1, s2, nh, ctypes.byref(cc),
@@ -303,7 +313,7 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, cache: KV8Cache, pos: int | tor
     on_dev = isinstance(pos, torch.Tensor)
     _call(dev, _lib.lib().i4_kv8_append, k.data_ptr(), v.data_ptr(), _lib.half_code(k.dtype), T,
           *k.stride()[:3], ctypes.byref(c), _int32(pos, B, dev, "pos") if on_dev else None,
-          0 if on_dev else int(pos), _int32(counts, B, dev, "counts"))
+          0 if on_dev else _host_pos(pos, T, cache.max_len), _int32(counts, B, dev, "counts"))
 
 
 def attn_kv8(q: torch.Tensor, cache: KV8Cache, pos: int | torch.Tensor, *,

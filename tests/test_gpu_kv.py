@@ -160,6 +160,60 @@ def test_attn_window_matches_64_bits(pkg, dev, dtype, B, T, nh, nkv, pos, window
         check(one[None], want, tol)
 
 
+@pytest.mark.parametrize("B,nh,nkv,T", [
+    (70, 4, 1, 1),     # more sequences than a wave has lanes
+    (150, 16, 2, 2),   # more kv heads than share 512 workgroups
+    (300, 3, 1, 1), (600, 2, 2, 1),  # 1200 kv heads: a workgroup each
+    (1, 32, 4, 4), (2, 31, 1, 1), (1, 33, 1, 1)])  # 32, 31 and 33 rows
+@pytest.mark.parametrize("eight", [False, True])
+def test_many_sequences_of_different_ages(pkg, dev, eight, B, nh, nkv, T):
+    g = torch.Generator().manual_seed(B)
+    first = (torch.rand(B, generator=g) ** 3 * 900).int().tolist()
+    counts = [T - (b % 7 == 3) for b in range(B)]
+    rows = 900 + T
+    q, k, v = case(dev, B, T, nh, nkv, rows, torch.bfloat16, seed=B)
+    keep = [0, 1, B // 3, B // 2, B - 1] + sorted(range(B), key=lambda b: -first[b])[:3]
+    keep = sorted({b for b in keep if b < B})
+    sub = lambda x: torch.stack([x[b] for b in keep])  # noqa: E731
+    pos, cnt = [first[b] for b in keep], [counts[b] for b in keep]
+    if eight:
+        cache = pkg.KV8Cache.empty(nkv, rows, batch=B, device=dev)
+        pkg.kv8_append(k.transpose(1, 2), v.transpose(1, 2), cache, 0,
+                       counts=i32(dev, [p + c for p, c in zip(first, counts)]))
+        got = pkg.attn_kv8(q, cache, i32(dev, first), counts=i32(dev, counts))
+        kk, vv = cache.values()
+        end = [p + c for p, c in zip(pos, cnt)]
+        kk, vv = sub(kk).cpu(), sub(vv).cpu()
+        for i, (b, e) in enumerate(zip(keep, end)):
+            kk[i, :, e // 64 * 64:e] = cache.k_tail[b, :, :e % 64].float().cpu()
+            vv[i, :, e // 64 * 64:e] = cache.v_tail[b, :, :e % 64].float().cpu()
+    else:
+        got = pkg.attn_window(q, k, v, i32(dev, first), counts=i32(dev, counts))
+        kk, vv = sub(k), sub(v)
+    want, tol = ref.attention(sub(q), kk, vv, pos, cnt, None, 0)
+    check(sub(got), want, tol)
+
+
+@pytest.mark.parametrize("T,nh", [(3, 4), (20, 8)])
+def test_masked_infinities_in_the_tail(pkg, dev, T, nh):
+    """Tokens of the unfinished block with NaN and infinities reach the later rows alone."""
+    pos = 64 * 3 + 5
+    kv = rand(dev, 2, 1, pos + T, 1, HD, seed=6)
+    bad = pos + T - 2
+    kv[0, 0, bad, 0, 3] = math.nan
+    kv[1, 0, bad, 0, 9] = math.inf
+    cache = pkg.KV8Cache.empty(1, pos + T, device=dev)
+    want8 = ref.Cache8(1, 1, cache.max_len // 64, torch.int8, torch.bfloat16)
+    pkg.kv8_append(kv[0], kv[1], cache, 0)
+    want8.append(kv, [0], [pos + T])
+    q = rand(dev, 1, T, nh, HD, seed=8)
+    got = pkg.attn_kv8(q, cache, pos)
+    k, v = want8.rows([pos + T])
+    want, tol = ref.attention(q, k, v, [pos], [T - 2], None, 0)
+    check(got[:, :T - 2], want[:, :T - 2], tol[:, :T - 2])
+    assert torch.isnan(got[:, T - 2:]).all()
+
+
 @pytest.mark.parametrize("T", [1, 4, 40, 150])
 def test_attn_window_strides(pkg, dev, T):
     """[max_len, n_kv_heads, head_dim] caches and q as a view of the fused rows."""
@@ -500,6 +554,39 @@ def test_positions_of_a_captured_graph(pkg, dev):
         assert same(a, wa) and same(b, wb), p
         assert same(taped[0], eager[0]) and same(taped[2].k_tail, eager[2].k_tail)
     assert same(taped[2].k, eager[2].k) and same(taped[2].v_scale, eager[2].v_scale)
+
+
+@pytest.mark.parametrize("T", [2, 60])
+def test_chunks_of_a_captured_graph(pkg, dev, T):
+    """A chunk's attention over both caches, split along the context, captured without a
+    workspace and replayed over positions and counts."""
+    nh, nkv, rows = 16, 2, 4000
+    q, k, v = case(dev, 1, T, nh, nkv, rows, torch.bfloat16, seed=T)
+    c8 = pkg.KV8Cache.empty(nkv, rows, device=dev)
+    pkg.kv8_append(k.transpose(1, 2), v.transpose(1, 2), c8, 0)
+    pos, counts = i32(dev, [0]), i32(dev, [T])
+
+    def step():
+        return (pkg.attn_window(q, k, v, pos, window=3000, sinks=4, counts=counts),
+                pkg.attn_kv8(q, c8, pos, counts=counts))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = step()
+    # whole blocks, so that the appended tail is never asked for
+    for p, n in ((0, T), (3904 - T, T), (64 - T, T), (1920 - T + 1, T - 1), (3840 - T, T)):
+        pos.fill_(p)
+        counts.fill_(n)
+        graph.replay()
+        wa, wb = step()
+        torch.cuda.synchronize()
+        # the graph's own zeros are of its capture: rows behind the count stay
+        assert same(a[:, :n], wa[:, :n]) and same(b[:, :n], wb[:, :n]), (p, n)
 
 
 @pytest.mark.parametrize("T", [1, 3, 100])

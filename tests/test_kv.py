@@ -122,6 +122,19 @@ def test_workspace_refused(lb, pkg, eight, bad, code):
     assert call_attn(lb, pkg.lib(), c, eight=eight, pos=8000, **bad) == code
 
 
+def test_workspace_sizes(pkg):
+    """No size overflows, and a bound never asks for more than none."""
+    size = pkg.lib().i4_attn_window_workspace_bytes
+    big = 2**31 - 1
+    for T, nh, nkv in ((1, 32, 4), (4, 32, 4), (5, 32, 4), (300, 8, 8)):
+        most = size(2, T, nh, nkv, 1 << 20, 0, 0)
+        assert 0 < most < 1 << 31
+        for window, sinks in ((1, 0), (100, big), (big, big), (big, 0), (5000, 64)):
+            assert 0 <= size(2, T, nh, nkv, 1 << 20, window, sinks) <= 2 * most
+    assert size(0, 1, 8, 4, 64, 0, 0) == size(1, 0, 8, 4, 64, 0, 0) == 0
+    assert size(1, 1, 9, 4, 64, 0, 0) == size(1, 1, 8, 0, 64, 0, 0) == 0
+
+
 @pytest.mark.parametrize("bad,code", BAD_CACHE8)
 def test_cache8_refused(lb, pkg, bad, code):
     c = cache8(lb, **bad)
@@ -170,6 +183,9 @@ def test_python_refuses(pkg, monkeypatch):
             (dict(out=torch.zeros(2, 3, 8, 128)), "contiguous")):
         with pytest.raises(RuntimeError, match=match):
             kv.attn_window(q, k, k, 0, **bad)
+    for pos in (-1, 62, 2**31, 2**32, 2**40 + 3):  # 3 tokens, 64 rows
+        with pytest.raises(RuntimeError, match="outside"):
+            kv.attn_window(q, k, k, pos)
     with pytest.raises(RuntimeError, match="batch"):
         kv.attn_window(q[:1], k, k, 0)
     with pytest.raises(RuntimeError, match="dimensions"):
@@ -190,7 +206,11 @@ def test_python_refuses(pkg, monkeypatch):
             ((x, 9, 4, w, w, 1e-6, inv, 0, k, k), {}, "head counts"),
             ((x, 8, 4, w, w, 1e-6, inv[:32], 0, k, k), {}, "inv_freq"),
             ((x, 8, 4, w, w, 1e-6, inv, 0, k.half(), k.half()), {}, "dtype"),
-            ((x, 8, 4, w, w, 1e-6, inv, 0, k, k), {"first_row": -1}, "first_row")):
+            ((x, 8, 4, w, w, 1e-6, inv, 0, k, k), {"first_row": -1}, "first_row"),
+            ((x, 8, 4, w, w, 1e-6, inv, 0, k, k), {"first_row": 62}, "first_row"),
+            ((x, 8, 4, w, w, 1e-6, inv, 0, k, k), {"first_row": 2**32}, "first_row"),
+            ((x, 8, 4, w, w, 1e-6, inv, 62, k, k), {}, "outside"),
+            ((x, 8, 4, w, w, 1e-6, inv, 2**32, k, k), {"first_row": 0}, "outside")):
         with pytest.raises(RuntimeError, match=match):
             kv.rope_append(*args, **kw)
     c = pkg.KV8Cache.empty(4, 100, batch=2, device="cpu")
@@ -200,6 +220,11 @@ def test_python_refuses(pkg, monkeypatch):
         kv.kv8_append(kk[:, :, :2], kk[:, :, :2], c, 0)
     with pytest.raises(RuntimeError, match="agree"):
         kv.kv8_append(kk, kk.half(), c, 0)
+    for pos in (-1, 126, 2**32):
+        with pytest.raises(RuntimeError, match="outside"):
+            kv.kv8_append(kk, kk, c, pos)
+        with pytest.raises(RuntimeError, match="outside"):
+            kv.attn_kv8(q, c, pos)
     t = list(c._t)
     for i, bad, match in ((0, t[0].view(torch.uint8), "int8 or float8"), (0, t[0][:, :, 0], "k is"),
                           (1, t[1].transpose(3, 4), "v must"), (2, t[2].double(), "float32"),
