@@ -88,8 +88,7 @@ __device__ inline void stage16(uint64_t k, uint64_t v, int j0, int last, u32 str
 // 5000-token one over 8 bits.
 //
 // Tried and slower: the next tile's scores computed between this tile's exponentials within
-// a wave (11 % more cycles: a second set of scores leaves fewer operands read ahead).  The
-// weights' sum as dot products of the packed weights: no difference.
+// a wave (11 % more cycles: a second set of scores leaves fewer operands read ahead).
 
 // A fence for the scheduler: LDS reads are issued two products ahead of their use, which it
 // would undo to save registers (a wave then waits out LDS's latency at every product).
@@ -149,7 +148,17 @@ __device__ inline void tile_max(TileAcc& acc, const f32x16 (&s)[2], float c) {
     for (int t = 0; t < 4; ++t) acc.o[t] *= f;
   }
 }
-// scores -> weights times 2^lift in place; returns their sum
+// the weights of 16 keys (step ks of the tile's four) as the product's operand
+template <int PT> __device__ inline u32x4 weights16(const f32x16 (&s)[2], int ks) {
+  const f32x16& x = s[ks >> 1];
+  const int o = 8 * (ks & 1);
+  return u32x4{pack2<PT>(x[o], x[o + 1]), pack2<PT>(x[o + 2], x[o + 3]),
+               pack2<PT>(x[o + 4], x[o + 5]), pack2<PT>(x[o + 6], x[o + 7])};
+}
+// scores -> weights times 2^lift in place; returns their sum.  ROUNDED: as they enter the
+// product, so that what rounding adds to the weights is divided out again (two an instruction,
+// in the time that the fp32 additions take)
+template <int PT, bool ROUNDED>
 __device__ inline float tile_weights(const TileAcc& acc, f32x16 (&s)[2], float c, float lift) {
   // a row that has seen nothing yet has m = -inf and scores -inf: weights 0
   const float base = acc.m == -__builtin_inff() ? lift : lift - acc.m;
@@ -159,8 +168,17 @@ __device__ inline float tile_weights(const TileAcc& acc, f32x16 (&s)[2], float c
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, base));
-      sum[i & 3] += s[t][i];
+      if constexpr (!ROUNDED) sum[i & 3] += s[t][i];
     }
+  if constexpr (ROUNDED) {
+    constexpr u32 ones = PT == I4_F16 ? 0x3C003C00u : 0x3F803F80u;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      const u32x4 b = weights16<PT>(s, ks);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[ks] = Half<PT>::dot2(b[i], ones, sum[ks]);
+    }
+  }
   return (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
 // v where the row does not see the key; key0: the tile's first position + 4 h
@@ -174,13 +192,6 @@ __device__ inline void tile_mask(f32x16 (&s)[2], int key0, int p, const Bounds& 
     }
 }
 
-// the weights of 16 keys (step ks of the tile's four) as the product's operand
-template <int PT> __device__ inline u32x4 weights16(const f32x16 (&s)[2], int ks) {
-  const f32x16& x = s[ks >> 1];
-  const int o = 8 * (ks & 1);
-  return u32x4{pack2<PT>(x[o], x[o + 1]), pack2<PT>(x[o + 2], x[o + 3]),
-               pack2<PT>(x[o + 4], x[o + 5]), pack2<PT>(x[o + 6], x[o + 7])};
-}
 // O^T += V^T P^T for a 16-bit tile
 template <int XT>
 __device__ inline void tile_values16(TileAcc& acc, const f32x16 (&s)[2], const lds_t* v,
@@ -367,7 +378,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       tile_scores<XT>(buf, q, s, n, h);
       if (edge) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
       tile_max(acc, s, a.c2);
-      acc.l += tile_weights(acc, s, a.c2, kLift);
+      acc.l += tile_weights<XT, true>(acc, s, a.c2, kLift);
       tile_values16<XT>(acc, s, buf + TBYTES, lane);
     };
     if constexpr (FMT < 0) {
@@ -437,7 +448,11 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
             }
             r = vs / unit;
           }
-          acc.l = fmaf(tile_weights(acc, s, a.c2 * ks, kLift + log2f(r)), 1.0f / r, acc.l);
+          // (an fp16 block's sum is of the fp32 weights: in units of a larger block they may
+          // round to 0)
+          const float sum =
+              tile_weights<XT, XT == I4_BF16>(acc, s, a.c2 * ks, kLift + log2f(r));
+          acc.l = fmaf(sum, 1.0f / r, acc.l);
           tile_values8<XT>(acc, s, buf + TBYTES, n, h);
         } else if (j0 <= p && (min(j0 + KBLK - 1, p) > p - a.w.window || j0 < a.w.sinks)) {
           acc.l = __builtin_nanf("");  // a block that reads as NaN, for a row that sees a key
