@@ -282,10 +282,11 @@ __device__ inline void values8(RowAcc<NT>& acc, const Block8& x, f32x4 (&s)[NT][
 
 // Parts go past the caches of this XCD (sc1), as the workgroup that merges them may run on
 // another: stored through, counted when the stores are done, read from memory.
-__device__ inline void put_part(float* p, float a, float b) {
-  const uint64_t v = (uint64_t)__builtin_bit_cast(u32, a) | (uint64_t)__builtin_bit_cast(u32, b)
-                                                                 << 32;
-  __hip_atomic_store((uint64_t*)p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+__device__ inline void put_part(rsrc_t r, u32 at, float a, float b, float c, float d) {
+  __builtin_amdgcn_raw_buffer_store_b128(
+      u32x4{__builtin_bit_cast(u32, a), __builtin_bit_cast(u32, b), __builtin_bit_cast(u32, c),
+            __builtin_bit_cast(u32, d)},
+      r, at, 0, kCoherent);
 }
 
 // The contexts shared out: every workgroup gets up to q tiles of one kv head, and kv head
@@ -560,11 +561,17 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
         for (int i = 0; i < 8; ++i) o[i] = fmaf(s_o[v][row][d0 + i], f, o[i]);
       }
       if (parts > 1 && t < sq.fit) {
-        const int64_t at = (int64_t)blockIdx.x * (16 * NT) + r;
-        if (d0 == 0) put_part(a.ml + 2 * at, M, L);
-        if (L != 0.f) {  // an empty part is skipped by its sum
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) put_part(a.part + at * KHD + d0 + i, o[i], o[i + 1]);
+        // this workgroup's rows; an empty part is skipped by its sum
+        const int64_t at = (int64_t)blockIdx.x * (16 * NT);
+        const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * 16 * NT);
+        const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * 16 * NT);
+        if (d0 == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(
+              u32x2{__builtin_bit_cast(u32, M), __builtin_bit_cast(u32, L)}, ml, 8u * r, 0,
+              kCoherent);
+        if (L != 0.f) {
+          put_part(part, 4u * (KHD * r + d0), o[0], o[1], o[2], o[3]);
+          put_part(part, 4u * (KHD * r + d0 + 4), o[4], o[5], o[6], o[7]);
         }
       } else if (parts == 1) {
         const float inv = t < sq.fit ? 1.0f / L : __builtin_nanf("");
