@@ -359,12 +359,11 @@ __device__ inline bool find_share(const CtxArgs& a, int wg, int head, int* s_n, 
 }
 
 // The rows of a kv head from the parts of its workgroups, by one of them: a row to each half
-// of a wave, whose lanes take 4 dims, with 16 parts in flight (a round of loads past the
+// of a wave, whose lanes take 4 dims, with U parts in flight (a round of loads past the
 // caches takes 1.2 us).
-template <int XT, int ROWS>
-__device__ inline void merge_share(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
+template <int XT, int ROWS, int U>
+__device__ inline void merge_rows(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
   const int d = 4 * (threadIdx.x & 31);
-  constexpr int U = 16;
   const int64_t at = (int64_t)sh.first * ROWS;
   const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * ROWS * sh.n);
   const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * ROWS * sh.n);
@@ -412,6 +411,13 @@ __device__ inline void merge_share(const CtxArgs& a, const Share& sh, const CtxS
 __device__ inline const uint16_t* query_row(const CtxArgs& a, int b, int g, int r) {
   const int t = udiv(r, a.G);
   return a.q + b * a.qbs + t * a.qts + (int64_t)(g * a.G + r - t * a.G) * a.qhs;
+}
+
+// few parts: little code; many: one round of loads (a token over 8191 8-bit positions has 32)
+template <int XT, int ROWS>
+__device__ inline void merge_share(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
+  if (sh.n <= 8) merge_rows<XT, ROWS, 8>(a, sh, sq);
+  else merge_rows<XT, ROWS, 32>(a, sh, sq);
 }
 
 // A workgroup takes its share of the context of one kv head, all of whose rows fit into 16 NT.

@@ -104,10 +104,10 @@ _STREAM_WS: dict = {}
 
 
 def _scratch(workspace: Workspace | None, need: int,
-             dev: torch.device) -> tuple[int, int | None]:
-    """The addresses of `need` bytes and of the counters: of the caller's workspace, else of
-    one per stream, whose calls run in order; under capture one of the call's own, which the
-    graph then owns."""
+             dev: torch.device) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """`need` bytes and the counters: of the caller's workspace, else of one per stream, whose
+    calls run in order; under capture one of the call's own, which the graph then owns.  The
+    caller holds them until its call is queued (another thread's may grow the workspace)."""
     if workspace is None:
         if torch.cuda.is_current_stream_capturing():
             workspace = Workspace()
@@ -116,8 +116,8 @@ def _scratch(workspace: Workspace | None, need: int,
             workspace = _STREAM_WS.get(key) or _STREAM_WS.setdefault(key, Workspace())
             buf, counters = workspace.buf, workspace._counters
             if buf is not None and buf.numel() >= need and counters is not None:
-                return buf.data_ptr(), counters.data_ptr()
-    return workspace.get(need, dev).data_ptr(), _lib.ptr(workspace.counters(dev))
+                return buf, counters
+    return workspace.get(need, dev), workspace.counters(dev)
 
 
 def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torch.Tensor,
@@ -194,7 +194,8 @@ def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
     s0, s1, s2, _ = x.stride()
     _call(dev, entry, x.data_ptr(), _lib.half_code(x.dtype), T, s0, s1, s2, nh, ctypes.byref(cc),
           pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
-          hd ** -0.5 if scale is None else scale, y.data_ptr(), ws, need, counters)
+          hd ** -0.5 if scale is None else scale, y.data_ptr(), _lib.ptr(ws), need,
+          _lib.ptr(counters))
     return y
 
 
