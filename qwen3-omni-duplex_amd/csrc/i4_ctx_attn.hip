@@ -37,7 +37,7 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
     int64_t w = heads <= 128 ? 512 : heads <= 256 ? 1024 : 2048;
     if (w > heads * ((tiles + 3) / 4)) w = heads * ((tiles + 3) / 4);
     if (w <= heads || heads > kShared) w = heads;
-    return {1, (int)w, w > heads ? w * (R <= 16 ? 16 : 32) : 0};
+    return {1, (int)w, w > heads ? w * kFewRows : 0};
   }
   // Two workgroups fit a CU: 512 take 2.1 us a tile together, 256 that have their CU to
   // themselves 1.3 us.  Parts cost 1040 bytes a row, written and read, and a launch.

@@ -1,5 +1,5 @@
-// Attention of few query rows (at most 32 per kv head: one token of up to 32 query heads per
-// kv head, or a few tokens) over a long cached context.  Bound by the bytes of the keys and
+// Attention of few query rows (at most 16 per kv head: one token of up to 16 query heads per
+// kv head, or two of 8) over a long cached context.  Bound by the bytes of the keys and
 // values, so those stream from memory straight into the matrix operands' registers: no LDS,
 // no transposition through it.
 //
@@ -34,9 +34,9 @@ __device__ inline int udiv(int n, int d) {
   return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)d));
 }
 
-template <int NT> struct RowAcc {
-  f32x4 o[NT][8];
-  float m[NT], l[NT];  // l: this lane's keys alone
+struct RowAcc {
+  f32x4 o[8];
+  float m, l;  // l: this lane's keys alone
 };
 
 __device__ inline float max_qd(float v) {  // over the lanes of a row (qd)
@@ -50,49 +50,36 @@ __device__ inline float sum_qd(float v) {
 
 // scores (in place) -> weights; c: scale log2(e) (times the keys' scale); key0: the lane's
 // first key, key0 + 4 k + i the others
-template <int NT, int NK>
-__device__ inline void weights(RowAcc<NT>& acc, f32x4 (&s)[NT][NK], float c, bool partial,
-                               int key0, const int (&p)[NT], const Bounds& w) {
-  bool raise = false;
-  float top[NT];
+template <int NK>
+__device__ inline void weights(RowAcc& acc, f32x4 (&s)[NK], float c, bool partial, int key0, int p,
+                               const Bounds& w) {
+  float top = -__builtin_inff();
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    float mx = -__builtin_inff();
+  for (int k = 0; k < NK; ++k)
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = s[n][k][i] * c;
-        if (partial) x = sees(w, p[n], key0 + 4 * k + i) ? x : -__builtin_inff();
-        s[n][k][i] = x;
-        mx = fmaxf(mx, x);
-      }
-    top[n] = mx;
-    raise |= mx > acc.m[n] + kLazy;
-  }
-  if (__builtin_amdgcn_ballot_w64(raise)) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float m = fmaxf(acc.m[n], max_qd(top[n]));
-      const float f = m > acc.m[n] ? __builtin_amdgcn_exp2f(acc.m[n] - m) : 1.f;
-      acc.m[n] = m;
-      acc.l[n] *= f;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) acc.o[n][t] *= f;
+    for (int i = 0; i < 4; ++i) {
+      float x = s[k][i] * c;
+      if (partial) x = sees(w, p, key0 + 4 * k + i) ? x : -__builtin_inff();
+      s[k][i] = x;
+      top = fmaxf(top, x);
     }
+  if (__builtin_amdgcn_ballot_w64(top > acc.m + kLazy)) {
+    const float m = fmaxf(acc.m, max_qd(top));
+    const float f = m > acc.m ? __builtin_amdgcn_exp2f(acc.m - m) : 1.f;
+    acc.m = m;
+    acc.l *= f;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) acc.o[t] *= f;
   }
+  // a row that has seen nothing yet has m = -inf and scores -inf: weights 0
+  const float base = acc.m == -__builtin_inff() ? 0.f : acc.m - kLift;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    // a row that has seen nothing yet has m = -inf and scores -inf: weights 0
-    const float base = acc.m[n] == -__builtin_inff() ? 0.f : acc.m[n] - kLift;
+  for (int k = 0; k < NK; ++k)
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[n][k][i] = __builtin_amdgcn_exp2f(s[n][k][i] - base);
-        acc.l[n] += s[n][k][i];
-      }
-  }
+    for (int i = 0; i < 4; ++i) {
+      s[k][i] = __builtin_amdgcn_exp2f(s[k][i] - base);
+      acc.l += s[k][i];
+    }
 }
 
 // eight weights as two operands that sum to them
@@ -129,26 +116,23 @@ __device__ inline void load_v16(Half16& h, rsrc_t vr, int row0, u32 stride, int 
     h.v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, (u32)(row0 + 8 * qd + j) * stride + 16u * m,
                                                    0, kStream);
 }
-template <int XT, int NT>
-__device__ inline void scores16(const Half16& h, const u32x4 (&q)[NT][4], f32x4 (&s)[NT][2]) {
+template <int XT>
+__device__ inline void scores16(const Half16& h, const u32x4 (&q)[4], f32x4 (&s)[2]) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int t = 0; t < 2; ++t) {
+    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      s[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) s[n][t] = mfma16<XT>(h.k[t][c], q[n][c], s[n][t]);
-    }
+    for (int c = 0; c < 4; ++c) s[t] = mfma16<XT>(h.k[t][c], q[c], s[t]);
+  }
 }
 
 // Values that a row does not see must not reach it (0 times an infinity is NaN): before the
 // product of a tile that is not seen in full, the values of keys that no row sees are
 // cleared; where rows differ, infinities and NaN are taken out and added to the rows that
 // see them.
-template <int XT, int NT>
-__device__ inline void clean16(RowAcc<NT>& acc, Half16& h, rsrc_t vr, int row0, u32 stride,
-                               int key0, int m, int qd, int plo, int phi, const int (&p)[NT],
-                               const Bounds& w) {
+template <int XT>
+__device__ inline void clean16(RowAcc& acc, Half16& h, rsrc_t vr, int row0, u32 stride, int key0,
+                               int m, int qd, int plo, int phi, int p, const Bounds& w) {
   bool bad = false;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -169,29 +153,25 @@ __device__ inline void clean16(RowAcc<NT>& acc, Half16& h, rsrc_t vr, int row0, 
 #pragma unroll
     for (int e = 0; e < 4; ++e) h.v[j][e] = finite_pair<XT>(h.v[j][e]);
   for (int j = 0; j < 32; ++j) {
+    const bool see = sees(w, p, key0 + j);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // dims 32 qd + 8 i + t
       const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(
           vr, (u32)(row0 + j) * stride + 64u * qd + 16u * i, 0, 0);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const bool see = sees(w, p[n], key0 + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float a = lo_f32<XT>(x[e]), b = hi_f32<XT>(x[e]);
-          if (see && !(fabsf(a) < __builtin_inff())) acc.o[n][2 * e][i] += a;
-          if (see && !(fabsf(b) < __builtin_inff())) acc.o[n][2 * e + 1][i] += b;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float a = lo_f32<XT>(x[e]), b = hi_f32<XT>(x[e]);
+        if (see && !(fabsf(a) < __builtin_inff())) acc.o[2 * e][i] += a;
+        if (see && !(fabsf(b) < __builtin_inff())) acc.o[2 * e + 1][i] += b;
       }
     }
   }
 }
 
-template <int XT, int NT>
-__device__ inline void values16(RowAcc<NT>& acc, const Half16& h, const f32x4 (&s)[NT][2]) {
-  u32x4 hi[NT], lo[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) split8<XT>(s[n][0], s[n][1], hi[n], lo[n]);
+template <int XT>
+__device__ inline void values16(RowAcc& acc, const Half16& h, const f32x4 (&s)[2]) {
+  u32x4 hi, lo;
+  split8<XT>(s[0], s[1], hi, lo);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     u32x4 a, b;  // dims 8 m + 2 e and 8 m + 2 e + 1 of the lane's 8 keys
@@ -200,13 +180,10 @@ __device__ inline void values16(RowAcc<NT>& acc, const Half16& h, const f32x4 (&
       a[j] = __builtin_amdgcn_perm(h.v[2 * j + 1][e], h.v[2 * j][e], 0x05040100u);
       b[j] = __builtin_amdgcn_perm(h.v[2 * j + 1][e], h.v[2 * j][e], 0x07060302u);
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      acc.o[n][2 * e] = mfma16<XT>(a, hi[n], acc.o[n][2 * e]);
-      acc.o[n][2 * e] = mfma16<XT>(a, lo[n], acc.o[n][2 * e]);
-      acc.o[n][2 * e + 1] = mfma16<XT>(b, hi[n], acc.o[n][2 * e + 1]);
-      acc.o[n][2 * e + 1] = mfma16<XT>(b, lo[n], acc.o[n][2 * e + 1]);
-    }
+    acc.o[2 * e] = mfma16<XT>(a, hi, acc.o[2 * e]);
+    acc.o[2 * e + 1] = mfma16<XT>(b, hi, acc.o[2 * e + 1]);
+    acc.o[2 * e] = mfma16<XT>(a, lo, acc.o[2 * e]);
+    acc.o[2 * e + 1] = mfma16<XT>(b, lo, acc.o[2 * e + 1]);
   }
 }
 
@@ -229,53 +206,41 @@ __device__ inline void load_v8(Block8& x, const Cache8& c, int64_t blk, int m, i
   for (int t = 0; t < 8; ++t) x.v[t] = __builtin_nontemporal_load((const u32x4*)(v + t * KBLK));
   x.vs = c.vs[blk];
 }
-template <int XT, int FMT, int NT>
-__device__ inline void scores8(const Block8& x, const u32x4 (&q)[NT][4], f32x4 (&s)[NT][4]) {
+template <int XT, int FMT>
+__device__ inline void scores8(const Block8& x, const u32x4 (&q)[4], f32x4 (&s)[4]) {
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const u32x4 a = cvt8<FMT, XT>(x.k[t][u][0], x.k[t][u][1]);
-      const u32x4 b = cvt8<FMT, XT>(x.k[t][u][2], x.k[t][u][3]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        s[n][t] = mfma16<XT>(a, q[n][2 * u], s[n][t]);
-        s[n][t] = mfma16<XT>(b, q[n][2 * u + 1], s[n][t]);
-      }
+      s[t] = mfma16<XT>(cvt8<FMT, XT>(x.k[t][u][0], x.k[t][u][1]), q[2 * u], s[t]);
+      s[t] = mfma16<XT>(cvt8<FMT, XT>(x.k[t][u][2], x.k[t][u][3]), q[2 * u + 1], s[t]);
     }
     __builtin_amdgcn_sched_barrier(0);  // one key group's conversions at a time
   }
 }
 // The weights take the values' scale; both enter the product as bf16, whose range holds any
 // scale.  A block with scale NaN is NaN for the rows that see one of its keys.
-template <int FMT, int NT>
-__device__ inline void values8(RowAcc<NT>& acc, const Block8& x, f32x4 (&s)[NT][4], bool partial,
-                               int key0, const int (&p)[NT], const Bounds& w) {
-  u32x4 hi[NT][2], lo[NT][2];
+template <int FMT>
+__device__ inline void values8(RowAcc& acc, const Block8& x, f32x4 (&s)[4], bool partial, int key0,
+                               int p, const Bounds& w) {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+  for (int k = 0; k < 4; ++k) {
+    s[k] *= x.vs;
+    if (partial)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      s[n][k] *= x.vs;
-      if (partial)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][k][i] = sees(w, p[n], key0 + 4 * k + i) ? s[n][k][i] : 0.f;
-    }
-    split8<I4_BF16>(s[n][0], s[n][1], hi[n][0], lo[n][0]);
-    split8<I4_BF16>(s[n][2], s[n][3], hi[n][1], lo[n][1]);
+      for (int i = 0; i < 4; ++i) s[k][i] = sees(w, p, key0 + 4 * k + i) ? s[k][i] : 0.f;
   }
+  u32x4 hi[2], lo[2];
+  split8<I4_BF16>(s[0], s[1], hi[0], lo[0]);
+  split8<I4_BF16>(s[2], s[3], hi[1], lo[1]);
 #pragma unroll
   for (int t = 0; t < 8; ++t)
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       const u32x4 a = cvt8<FMT, I4_BF16>(x.v[t][2 * g], x.v[t][2 * g + 1]);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        acc.o[n][t] = mfma16<I4_BF16>(a, hi[n][g], acc.o[n][t]);
-        acc.o[n][t] = mfma16<I4_BF16>(a, lo[n][g], acc.o[n][t]);
-      }
+      acc.o[t] = mfma16<I4_BF16>(a, hi[g], acc.o[t]);
+      acc.o[t] = mfma16<I4_BF16>(a, lo[g], acc.o[t]);
       __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -361,12 +326,12 @@ __device__ inline bool find_share(const CtxArgs& a, int wg, int head, int* s_n, 
 // The rows of a kv head from the parts of its workgroups, by one of them: a row to each half
 // of a wave, whose lanes take 4 dims, with U parts in flight (a round of loads past the
 // caches takes 1.2 us).
-template <int XT, int ROWS, int U>
+template <int XT, int U>
 __device__ inline void merge_rows(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
   const int d = 4 * (threadIdx.x & 31);
-  const int64_t at = (int64_t)sh.first * ROWS;
-  const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * ROWS * sh.n);
-  const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * ROWS * sh.n);
+  const int64_t at = (int64_t)sh.first * kFewRows;
+  const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * kFewRows * sh.n);
+  const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * kFewRows * sh.n);
 #pragma unroll 1
   for (int r = threadIdx.x >> 5; r < a.R; r += 8) {
     float M = -__builtin_inff(), L = 0.f;
@@ -377,7 +342,7 @@ __device__ inline void merge_rows(const CtxArgs& a, const Share& sh, const CtxSe
       u32x4 w[U];
 #pragma unroll
       for (int i = 0; i < U; ++i) {  // reads past the parts are zeros: an empty part
-        const u32 row = ROWS * (s0 + i) + r;
+        const u32 row = kFewRows * (s0 + i) + r;
         v[i] = __builtin_amdgcn_raw_buffer_load_b64(ml, 8u * row, 0, kCoherent);
         w[i] = __builtin_amdgcn_raw_buffer_load_b128(part, 4u * (KHD * row + d), 0, kCoherent);
       }
@@ -414,15 +379,15 @@ __device__ inline const uint16_t* query_row(const CtxArgs& a, int b, int g, int 
 }
 
 // few parts: little code; many: one round of loads (a token over 8191 8-bit positions has 32)
-template <int XT, int ROWS>
+template <int XT>
 __device__ inline void merge_share(const CtxArgs& a, const Share& sh, const CtxSeq& sq) {
-  if (sh.n <= 8) merge_rows<XT, ROWS, 8>(a, sh, sq);
-  else merge_rows<XT, ROWS, 32>(a, sh, sq);
+  if (sh.n <= 8) merge_rows<XT, 8>(a, sh, sq);
+  else merge_rows<XT, 32>(a, sh, sq);
 }
 
-// A workgroup takes its share of the context of one kv head, all of whose rows fit into 16 NT.
-template <int XT, int FMT, int NT>
-__global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(CtxArgs a) {
+// A workgroup takes its share of the context of one kv head and all of its rows.
+template <int XT, int FMT>
+__global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
   __shared__ __align__(16) float s_o[4][16][KHD + 4];
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ int s_last;
@@ -435,27 +400,20 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, qd = lane >> 4;
   const CtxSeq sq = ctx_seq(a, b);
   const int thi = sq.fit - 1;  // the last token with something to attend
-  RowAcc<NT> acc;
-  int p[NT];  // this lane's rows' positions; -1 sees nothing
+  RowAcc acc;
+  acc.m = -__builtin_inff();
+  acc.l = 0.f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int t = udiv(16 * n + m, a.G);
-    p[n] = 16 * n + m < a.R && t < sq.fit ? sq.p0 + t : -1;
-    acc.m[n] = -__builtin_inff();
-    acc.l[n] = 0.f;
-#pragma unroll
-    for (int t8 = 0; t8 < 8; ++t8) acc.o[n][t8] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int t = 0; t < 8; ++t) acc.o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int tm = udiv(m, a.G);  // this lane's row's token
+  const int p = m < a.R && tm < sq.fit ? sq.p0 + tm : -1;  // its position; -1 sees nothing
   if (thi >= 0) {
     const int plo = sq.p0, phi = sq.p0 + thi;
-    u32x4 q[NT][4];
+    const uint16_t* row = query_row(a, b, g, p < 0 ? 0 : m);  // one that exists
+    u32x4 q[4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const uint16_t* row = query_row(a, b, g, p[n] < 0 ? 0 : 16 * n + m);  // one that exists
-#pragma unroll
-      for (int c = 0; c < 4; ++c)  // dims as the keys' lanes hold them
-        q[n][c] = ldg16(row + (FMT < 0 ? 32 * c + 8 * qd : 64 * (c >> 1) + 16 * qd + 8 * (c & 1)));
-    }
+    for (int c = 0; c < 4; ++c)  // dims as the keys' lanes hold them
+      q[c] = ldg16(row + (FMT < 0 ? 32 * c + 8 * qd : 64 * (c >> 1) + 16 * qd + 8 * (c & 1)));
     const CtxTiles ct = ctx_tiles(a.w, plo, phi);
     // this workgroup's tiles, dealt to its waves in turn
     const int each = udiv(ct.n, parts), more = ct.n - each * parts;
@@ -476,13 +434,13 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
       for (; x < e; x += 4) {
         const int j0 = pos0(x);
         const bool partial = !all_see(a.w, plo, phi, j0, 32);
-        f32x4 s[NT][2];
-        scores16<XT, NT>(h, q, s);
+        f32x4 s[2];
+        scores16<XT>(h, q, s);
         const int jn = pos0(min(x + 4, e - 1));
         if (x + 4 < e) load_k16(h, kr, jn, stride, m, qd);
-        weights<NT, 2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
-        if (partial) clean16<XT, NT>(acc, h, vr, j0, stride, j0, m, qd, plo, phi, p, a.w);
-        values16<XT, NT>(acc, h, s);
+        weights<2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
+        if (partial) clean16<XT>(acc, h, vr, j0, stride, j0, m, qd, plo, phi, p, a.w);
+        values16<XT>(acc, h, s);
         if (x + 4 < e) load_v16(h, vr, jn, stride, m, qd);
       }
     } else {
@@ -500,13 +458,13 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
       for (; x < e; x += 4) {
         const int j0 = 64 * ct.at(x);
         const bool partial = !all_see(a.w, plo, phi, j0, 64);
-        f32x4 s[NT][4];
-        scores8<XT, FMT, NT>(x8, q, s);
+        f32x4 s[4];
+        scores8<XT, FMT>(x8, q, s);
         const float c = a.c2 * x8.ks;
         const int64_t nb = hblk + ct.at(min(x + 4, e - 1));
         if (x + 4 < e) load_k8(x8, a.c8, nb, m, qd);
-        weights<NT, 4>(acc, s, c, partial, j0 + 16 * qd, p, a.w);
-        values8<FMT, NT>(acc, x8, s, partial, j0 + 16 * qd, p, a.w);
+        weights<4>(acc, s, c, partial, j0 + 16 * qd, p, a.w);
+        values8<FMT>(acc, x8, s, partial, j0 + 16 * qd, p, a.w);
         if (x + 4 < e) load_v8(x8, a.c8, nb, m, qd);
       }
       if (tail && wave >= 2) {  // its halves, by the two waves that have the least to do
@@ -515,78 +473,70 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
           const u32 stride = KHD * 2u, bytes = (u32)(phi - full * KBLK + 1) * stride;
           const int64_t base = ((int64_t)b * a.nkv + g) * (KBLK * KHD);
           const rsrc_t kr = rsrc(a.c8.kt + base, bytes), vr = rsrc(a.c8.vt + base, bytes);
-          u32x4 qn[NT][4];  // dims in the 16-bit order
+          u32x4 qn[4];  // dims in the 16-bit order
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint16_t* row = query_row(a, b, g, p[n] < 0 ? 0 : 16 * n + m);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) qn[n][c] = ldg16(row + 32 * c + 8 * qd);
-          }
+          for (int c = 0; c < 4; ++c) qn[c] = ldg16(row + 32 * c + 8 * qd);
           Half16 h;
           const int row0 = 32 * (wave - 2);
           load_k16(h, kr, row0, stride, m, qd);
           load_v16(h, vr, row0, stride, m, qd);
-          f32x4 s[NT][2];
-          scores16<XT, NT>(h, qn, s);
-          weights<NT, 2>(acc, s, a.c2, true, j0 + 8 * qd, p, a.w);
-          clean16<XT, NT>(acc, h, vr, row0, stride, j0, m, qd, plo, phi, p, a.w);
-          values16<XT, NT>(acc, h, s);
+          f32x4 s[2];
+          scores16<XT>(h, qn, s);
+          weights<2>(acc, s, a.c2, true, j0 + 8 * qd, p, a.w);
+          clean16<XT>(acc, h, vr, row0, stride, j0, m, qd, plo, phi, p, a.w);
+          values16<XT>(acc, h, s);
         }
       }
     }
   }
   // merge the waves: thread t takes row t / 16, dims 8 (t % 16) .. + 7
-  const int row = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15);
+  const int r = threadIdx.x >> 4, d0 = 8 * (threadIdx.x & 15), t = udiv(r, a.G);
+  __syncthreads();  // s_o has been read
+  const float l = sum_qd(acc.l);
+  if (qd == 0) {
+    s_m[wave][m] = acc.m;
+    s_l[wave][m] = l;
+  }
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    __syncthreads();  // s_o has been read
-    const float l = sum_qd(acc.l[n]);
-    if (qd == 0) {
-      s_m[wave][m] = acc.m[n];
-      s_l[wave][m] = l;
-    }
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int e = 0; e < 8; e += 4)
+      *(f32x4*)&s_o[wave][m][32 * qd + 8 * i + e] =
+          f32x4{acc.o[e][i], acc.o[e + 1][i], acc.o[e + 2][i], acc.o[e + 3][i]};
+  __syncthreads();
+  if (r < a.R && t < sq.have) {
+    float M = -__builtin_inff(), L = 0.f, o[8];
 #pragma unroll
-      for (int t = 0; t < 8; t += 4)
-        *(f32x4*)&s_o[wave][m][32 * qd + 8 * i + t] =
-            f32x4{acc.o[n][t][i], acc.o[n][t + 1][i], acc.o[n][t + 2][i], acc.o[n][t + 3][i]};
-    __syncthreads();
-    const int r = 16 * n + row, t = udiv(r, a.G);
-    if (r < a.R && t < sq.have) {
-      float M = -__builtin_inff(), L = 0.f, o[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = 0.f;
-      for (int v = 0; v < 4; ++v) M = fmaxf(M, s_m[v][row]);
+    for (int i = 0; i < 8; ++i) o[i] = 0.f;
+    for (int v = 0; v < 4; ++v) M = fmaxf(M, s_m[v][r]);
 #pragma unroll 1
-      for (int v = 0; v < 4; ++v) {
-        if (s_m[v][row] == -__builtin_inff() && s_l[v][row] == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(s_m[v][row] - M);
-        L = fmaf(s_l[v][row], f, L);
+    for (int v = 0; v < 4; ++v) {
+      if (s_m[v][r] == -__builtin_inff() && s_l[v][r] == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(s_m[v][r] - M);
+      L = fmaf(s_l[v][r], f, L);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = fmaf(s_o[v][row][d0 + i], f, o[i]);
+      for (int i = 0; i < 8; ++i) o[i] = fmaf(s_o[v][r][d0 + i], f, o[i]);
+    }
+    if (parts > 1 && t < sq.fit) {
+      // this workgroup's rows; an empty part is skipped by its sum
+      const int64_t at = (int64_t)blockIdx.x * kFewRows;
+      const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * kFewRows);
+      const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * kFewRows);
+      if (d0 == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(
+            u32x2{__builtin_bit_cast(u32, M), __builtin_bit_cast(u32, L)}, ml, 8u * r, 0,
+            kCoherent);
+      if (L != 0.f) {
+        put_part(part, 4u * (KHD * r + d0), o[0], o[1], o[2], o[3]);
+        put_part(part, 4u * (KHD * r + d0 + 4), o[4], o[5], o[6], o[7]);
       }
-      if (parts > 1 && t < sq.fit) {
-        // this workgroup's rows; an empty part is skipped by its sum
-        const int64_t at = (int64_t)blockIdx.x * (16 * NT);
-        const rsrc_t ml = rsrc(a.ml + 2 * at, 8u * 16 * NT);
-        const rsrc_t part = rsrc(a.part + at * KHD, 4u * KHD * 16 * NT);
-        if (d0 == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(
-              u32x2{__builtin_bit_cast(u32, M), __builtin_bit_cast(u32, L)}, ml, 8u * r, 0,
-              kCoherent);
-        if (L != 0.f) {
-          put_part(part, 4u * (KHD * r + d0), o[0], o[1], o[2], o[3]);
-          put_part(part, 4u * (KHD * r + d0 + 4), o[4], o[5], o[6], o[7]);
-        }
-      } else if (parts == 1) {
-        const float inv = t < sq.fit ? 1.0f / L : __builtin_nanf("");
-        u32x4 y;
+    } else if (parts == 1) {
+      const float inv = 1.0f / L;
+      u32x4 y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = pack2<XT>(o[2 * i] * inv, o[2 * i + 1] * inv);
-        if (!(t < sq.fit)) y = u32x4{} + (u32)Half<XT>::QNAN * 0x10001u;
-        *(u32x4*)(a.out + ctx_out_of(a, b, g, r, t) + d0) = y;
-      }
+      for (int i = 0; i < 4; ++i) y[i] = pack2<XT>(o[2 * i] * inv, o[2 * i + 1] * inv);
+      if (t >= sq.fit) y = u32x4{} + (u32)Half<XT>::QNAN * 0x10001u;
+      *(u32x4*)(a.out + ctx_out_of(a, b, g, r, t) + d0) = y;
     }
   }
   if (parts == 1 || !a.counters) return;
@@ -601,23 +551,20 @@ __global__ __launch_bounds__(256, FMT >= 0 && NT == 2 ? 1 : 2) void k_ctx_rows(C
   if (!s_last) return;
   if (threadIdx.x == 0)
     __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  merge_share<XT, 16 * NT>(a, sh, sq);
+  merge_share<XT>(a, sh, sq);
 }
 
 // The same merge as a launch of its own, a workgroup for each kv head.
-template <int XT, int ROWS> __global__ __launch_bounds__(256) void k_ctx_rows_merge(CtxArgs a) {
+template <int XT> __global__ __launch_bounds__(256) void k_ctx_rows_merge(CtxArgs a) {
   __shared__ int s_n[kShared];
   Share sh;
   if (!find_share(a, 0, blockIdx.x, s_n, sh) || sh.n == 1) return;
-  merge_share<XT, ROWS>(a, sh, ctx_seq(a, sh.b));
+  merge_share<XT>(a, sh, ctx_seq(a, sh.b));
 }
 
 template <int XT, int FMT> static void rows_go(const CtxArgs& a, hipStream_t s) {
-  if (a.R <= 16) k_ctx_rows<XT, FMT, 1><<<a.wgs, 256, 0, s>>>(a);
-  else k_ctx_rows<XT, FMT, 2><<<a.wgs, 256, 0, s>>>(a);
-  if (a.wgs == a.B * a.nkv || a.counters) return;
-  if (a.R <= 16) k_ctx_rows_merge<XT, 16><<<a.B * a.nkv, 256, 0, s>>>(a);
-  else k_ctx_rows_merge<XT, 32><<<a.B * a.nkv, 256, 0, s>>>(a);
+  k_ctx_rows<XT, FMT><<<a.wgs, 256, 0, s>>>(a);
+  if (a.wgs > a.B * a.nkv && !a.counters) k_ctx_rows_merge<XT><<<a.B * a.nkv, 256, 0, s>>>(a);
 }
 
 }  // namespace i4
