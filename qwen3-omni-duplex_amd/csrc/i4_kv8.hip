@@ -48,7 +48,7 @@ template <int XT> __device__ inline void widen8(u32x4 x, float (&f)[8]) {
 // Thread t holds dims 8 (t % 16) .. + 7 of tokens 4 (t / 16) .. + 3: whole rows in a wave's
 // loads; a key row's 8 bytes are stored as they are, four tokens of a value dim make a word,
 // which LDS brings into rows.  Bound by the divisions (about 10 instructions an element) for
-// prompts: 4001 tokens of four heads take 7 us.
+// prompts: 4001 tokens of four heads take 8 us.
 template <int XT, int FMT>
 __global__ __launch_bounds__(256) void k_kv8_append(const uint16_t* __restrict__ k,
                                                     const uint16_t* __restrict__ v, int64_t bs,
