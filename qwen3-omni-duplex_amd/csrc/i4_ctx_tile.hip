@@ -155,22 +155,26 @@ template <int PT> __device__ inline u32x4 weights16(const f32x16 (&s)[2], int ks
   return u32x4{pack2<PT>(x[o], x[o + 1]), pack2<PT>(x[o + 2], x[o + 3]),
                pack2<PT>(x[o + 4], x[o + 5]), pack2<PT>(x[o + 6], x[o + 7])};
 }
-// scores -> weights times 2^lift in place; returns their sum.  ROUNDED: as they enter the
+// scores -> weights times 2^lift in place; returns their sum.  rounded: as they enter the
 // product, so that what rounding adds to the weights is divided out again (two an instruction,
 // in the time that the fp32 additions take)
-template <int PT, bool ROUNDED>
-__device__ inline float tile_weights(const TileAcc& acc, f32x16 (&s)[2], float c, float lift) {
+template <int PT>
+__device__ inline float tile_weights(const TileAcc& acc, f32x16 (&s)[2], float c, float lift,
+                                     bool rounded = true) {
   // a row that has seen nothing yet has m = -inf and scores -inf: weights 0
   const float base = acc.m == -__builtin_inff() ? lift : lift - acc.m;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 16; ++i)
       s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], c, base));
-      if constexpr (!ROUNDED) sum[i & 3] += s[t][i];
-    }
-  if constexpr (ROUNDED) {
+  if (!rounded) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[i & 3] += s[t][i];
+  } else {
     constexpr u32 ones = PT == I4_F16 ? 0x3C003C00u : 0x3F803F80u;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       tile_scores<XT>(buf, q, s, n, h);
       if (edge) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
       tile_max(acc, s, a.c2);
-      acc.l += tile_weights<XT, true>(acc, s, a.c2, kLift);
+      acc.l += tile_weights<XT>(acc, s, a.c2, kLift);
       tile_values16<XT>(acc, s, buf + TBYTES, lane);
     };
     if constexpr (FMT < 0) {
@@ -448,10 +452,10 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
             }
             r = vs / unit;
           }
-          // (an fp16 block's sum is of the fp32 weights: in units of a larger block they may
-          // round to 0)
-          const float sum =
-              tile_weights<XT, XT == I4_BF16>(acc, s, a.c2 * ks, kLift + log2f(r));
+          // (in units of a much larger block an fp16 block's weights may round to 0: then the
+          // sum is of the fp32 ones)
+          const float sum = tile_weights<XT>(acc, s, a.c2 * ks, kLift + log2f(r),
+                                             XT == I4_BF16 || r > 0.125f);
           acc.l = fmaf(sum, 1.0f / r, acc.l);
           tile_values8<XT>(acc, s, buf + TBYTES, n, h);
         } else if (j0 <= p && (min(j0 + KBLK - 1, p) > p - a.w.window || j0 < a.w.sinks)) {

@@ -480,6 +480,27 @@ def test_attn_kv8_block_scales(pkg, dev, dtype, kind, T, nh):
         check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
 
 
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,nh", [(1, 4), (6, 4), (130, 2)])
+def test_attn_kv8_of_one_key(pkg, dev, dtype, kind, T, nh):
+    """A token that sees itself alone gets its value: the weight cancels, rounded or not.
+
+    Left are the output's rounding (half a step) and 2^-16, what a sum of two bf16 numbers is
+    off by; 2^-20 holds the fp32 operations."""
+    total = 64 * 6
+    kv = history(dev, 1, 1, total, dtype, seed=6)
+    cache = pkg.KV8Cache.empty(1, total, dtype=dtype, kind=kind, device=dev)
+    want8 = ref.Cache8(1, 1, cache.max_len // 64, kind, dtype)
+    pkg.kv8_append(kv[0], kv[1], cache, 0)
+    want8.append(kv, [0], [total])
+    q = rand(dev, 1, T, nh, HD, seed=8, dtype=dtype)
+    got = pkg.attn_kv8(q, cache, total - T, window=1).double().cpu()
+    want = want8.rows([total])[1][0, 0, total - T:total].double().cpu()[None, :, None]
+    tol = want.abs() * (torch.finfo(dtype).eps / 2 + 2.0 ** -16 + 2.0 ** -20) + 2.0 ** -25
+    assert ((got - want).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("T,nh", [(1, 8), (2, 8), (5, 24), (120, 8)])
 def test_attn_kv8_padding_outside_and_bad_blocks(pkg, dev, kind, T, nh):
