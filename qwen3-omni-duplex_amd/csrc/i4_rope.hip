@@ -16,14 +16,16 @@ struct RopeFreq {
   float f[KHD / 2];
 };
 
-// cos and sin of p f as the sum of two floats: the product's rounding error (up to 2^-25 of
-// an angle that grows with the position) is carried to first order.
+// cos and sin of p f as the sum of two floats, hi + lo exactly: lo is up to 2^-24 of an angle
+// that grows with the position (half a radian at position 2^24), so the rotation by hi is
+// followed by a whole one by lo.
 __device__ inline void angle(float p, float f, float& c, float& s) {
   const float hi = p * f, lo = fmaf(p, f, -hi);
-  float s0, c0;
+  float s0, c0, s1, c1;
   sincosf(hi, &s0, &c0);
-  c = fmaf(-lo, s0, c0);
-  s = fmaf(lo, c0, s0);
+  sincosf(lo, &s1, &c1);
+  c = fmaf(c0, c1, -s0 * s1);
+  s = fmaf(s0, c1, c0 * s1);
 }
 
 __device__ inline float half_row(float v) {  // the value 8 lanes away within 16

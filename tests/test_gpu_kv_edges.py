@@ -1,0 +1,62 @@
+"""The cache operators at the edges of their ranges: far positions, value blocks of extreme and
+zero scales, splits beyond one round of the merges, what 8 bits do to a prompt."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from tests import _kv_ref as ref
+
+pytestmark = pytest.mark.gpu
+HD = 128
+DTS = [torch.bfloat16, torch.float16]
+KINDS = [torch.int8, torch.float8_e4m3fn]
+
+
+def rand(dev, *shape, seed=0, dtype=torch.bfloat16, gain=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=dev) * gain).to(dtype)
+
+
+def i32(dev, values):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def check(got, want, tol):
+    got = got.double().cpu()
+    assert torch.isfinite(got).all()
+    off = (got - want).abs()
+    assert (off <= tol).all(), f"off by {(off / tol).max().item():.2f} times the tolerance"
+
+
+def caches(pkg, dev, kv, kind, room=0):
+    """An 8-bit cache of the tokens kv [2, B, T, n, 128] and its reference."""
+    _, B, T, n, _ = kv.shape
+    cache = pkg.KV8Cache.empty(n, T + room, batch=B, dtype=kv.dtype, kind=kind, device=dev)
+    want = ref.Cache8(B, n, cache.max_len // 64, kind, kv.dtype)
+    pkg.kv8_append(kv[0], kv[1], cache, 0)
+    want.append(kv, [0] * B, [T] * B)
+    return cache, want
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("pos", [1 << 17, 1 << 20, (1 << 22) + 12345, (1 << 24) - 5])
+def test_rope_far_positions(pkg, dev, dtype, pos):
+    """The rotation up to the last position that fp32 holds exactly."""
+    T, nh, nkv = 5, 3, 1
+    qkv = rand(dev, 1, T, (nh + 2 * nkv) * HD, seed=1, dtype=dtype)
+    qw, kw = ((1 + 0.2 * rand(dev, HD, seed=s).float()).to(dtype) for s in (2, 3))
+    inv = pkg.rope_inv_freq(HD, 1e6)
+    k, v = (torch.zeros(1, nkv, T, HD, dtype=dtype, device=dev) for _ in range(2))
+    x = qkv.cpu().view(1, T, nh + 2 * nkv, HD)
+    p = torch.arange(pos, pos + T)[None, :, None]
+    for at in (pos, i32(dev, [pos])):
+        q = pkg.rope_append(qkv, nh, nkv, qw, kw, 1e-6, inv, at, k, v, first_row=0)
+        for lo, n, w, got in ((0, nh, qw, q), (nh, nkv, kw, k.transpose(1, 2))):
+            want, size = ref.rope(x[:, :, lo:lo + n], w.cpu(), p, inv, 1e-6)
+            # the norm's sum, root and quotient 2^-20, the sines and cosines of the product's
+            # two parts 2^-21; then one rounding
+            err = 2.0 ** -19 * size
+            check(got, want, err + ref.half_step(dtype) * (want.abs() + err) + 1e-7)
