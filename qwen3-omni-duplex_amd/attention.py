@@ -110,7 +110,8 @@ class ThinkerAttention(nn.Module):
         ops.weights_changed()
 
     def forward(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
-        """h [T, H] (T tokens at cache positions pos, pos + 1, ...) -> h + o_proj(attn(norm(h))).
+        """h [T, H] or [1, T, H] (T tokens of one sequence at cache positions pos, pos + 1, ...)
+        -> h + o_proj(attn(norm(h))).
 
         pos is an int, or an int32 device tensor of one element that the kernels read (a
         decode step captured in a hipGraph then serves every token; a position outside the
@@ -118,6 +119,8 @@ class ThinkerAttention(nn.Module):
         T = h.numel() // h.shape[-1]
         if T < 1:
             raise ValueError("no token")
+        if h.dim() > 2 and h.shape[-2] != T:  # [B, T, H]: several sequences share no cache
+            raise ValueError(f"h {tuple(h.shape)} holds tokens of several sequences")
         if not isinstance(pos, torch.Tensor) and not 0 <= pos <= self.max_len - T:
             raise ValueError(f"positions {pos} to {pos + T - 1} outside the cache "
                              f"(max_len {self.max_len})")

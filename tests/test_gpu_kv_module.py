@@ -137,3 +137,14 @@ def test_module_refuses(pkg, dev):
     for bad in ({"window": 0}, {"sinks": 2}, {"window": 4, "sinks": -1}):
         with pytest.raises(ValueError, match="window"):
             build(pkg, dev, **bad)
+
+
+def test_leading_dimension_of_one(pkg, dev):
+    """[1, T, H] is [T, H], for a prompt and for one token."""
+    a, b = (build(pkg, dev, layers=2) for _ in range(2))
+    h = tokens(dev, 9)
+    for x, pos in ((h[:8], 0), (h[8:], 8)):
+        got, want = a.step(x[None], pos), b.step(x, pos)
+        assert got.shape == (1, *want.shape) and torch.equal(got[0], want)
+    with pytest.raises(ValueError, match="several sequences"):
+        a.step(h[:2, None], 0)

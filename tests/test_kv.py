@@ -255,3 +255,19 @@ def test_reference_visibility():
     assert ref.see(5, 8, None, 0).tolist() == [True] * 6 + [False] * 2
     assert ref.see(5, 8, 2, 1).nonzero()[:, 0].tolist() == [0, 4, 5]
     assert ref.see(0, 3, 1, 9).nonzero()[:, 0].tolist() == [0]
+
+
+def test_module_refuses_several_sequences(pkg):
+    """A batch of sequences is not read as the tokens of one (made before any launch)."""
+    attn = pkg.ThinkerAttention.__new__(pkg.ThinkerAttention)
+    torch.nn.Module.__init__(attn)
+    attn.max_len = 64
+    layer = pkg.ThinkerDecoderLayer.__new__(pkg.ThinkerDecoderLayer)
+    torch.nn.Module.__init__(layer)
+    layer.attn = attn
+    for shape in ((2, 1, 16), (2, 3, 16), (2, 1, 1, 16)):
+        for call in (attn, layer.unfused, pkg.ThinkerDecoder([layer]).unfused):
+            with pytest.raises(ValueError, match="several sequences"):
+                call(torch.zeros(shape), 0)
+    with pytest.raises(ValueError, match="no token"):
+        attn(torch.zeros(1, 0, 16), 0)
