@@ -74,7 +74,7 @@ class ThinkerAttention(nn.Module):
         self.register_buffer("_v_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
         self.max_len = int(max_len)
         self.workspace = ops.Workspace()
-        self.context_workspace = ops.Workspace()  # of _attend: its counters stay with it
+        self.context_workspace = ops.Workspace()  # of _attend, where the caller brings none
 
     # The caches are written in place by the kernels and their addresses are held by the
     # decoder's layer structs, so they cannot be replaced: fill them in place
@@ -109,13 +109,16 @@ class ThinkerAttention(nn.Module):
         super().__setattr__(name, value)
         ops.weights_changed()
 
-    def forward(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
+    def forward(self, h: torch.Tensor, pos: int | torch.Tensor,
+                context_workspace: ops.Workspace | None = None) -> torch.Tensor:
         """h [T, H] or [1, T, H] (T tokens of one sequence at cache positions pos, pos + 1, ...)
         -> h + o_proj(attn(norm(h))).
 
         pos is an int, or an int32 device tensor of one element that the kernels read (a
         decode step captured in a hipGraph then serves every token; a position outside the
-        cache gives NaN and leaves the cache untouched)."""
+        cache gives NaN and leaves the cache untouched).  context_workspace: scratch of the
+        attention over several tokens, a bounded context or an 8-bit cache, shared by layers
+        that run one after the other (default: the module's own)."""
         T = h.numel() // h.shape[-1]
         if T < 1:
             raise ValueError("no token")
@@ -125,7 +128,7 @@ class ThinkerAttention(nn.Module):
             raise ValueError(f"positions {pos} to {pos + T - 1} outside the cache "
                              f"(max_len {self.max_len})")
         if T > 1 or not self.whole_context():
-            return self._attend(h, pos)
+            return self._attend(h, pos, context_workspace or self.context_workspace)
         if self.o_proj.w.layout == "ct":
             # input_layernorm + q|k|v inside the attention chunk launch, then the head
             # merge and o_proj (+ the residual) in one more
@@ -142,7 +145,8 @@ class ThinkerAttention(nn.Module):
         return ops.linear(a.view(1, -1), self.o_proj.w, bias=h.reshape(-1)).view(h.shape)
 
 
-    def _attend(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
+    def _attend(self, h: torch.Tensor, pos: int | torch.Tensor,
+                workspace: ops.Workspace) -> torch.Tensor:
         """Several tokens, a bounded context or an 8-bit cache, launch by launch."""
         H, n, hd = h.shape[-1], self.n_kv_heads, self.head_dim
         x = h.reshape(-1, H)
@@ -154,7 +158,7 @@ class ThinkerAttention(nn.Module):
             k, v = self.k_cache, self.v_cache
         q = kv.rope_append(qkv, self.n_heads, n, self.q_norm_w, self.k_norm_w, self.eps,
                            self.inv_freq, pos, k, v, first_row=0 if eight else None)
-        bounds = {"window": self.window, "sinks": self.sinks, "workspace": self.context_workspace}
+        bounds = {"window": self.window, "sinks": self.sinks, "workspace": workspace}
         if eight:
             kv.kv8_append(k.transpose(0, 1), v.transpose(0, 1), self.kv8, pos)
             a = kv.attn_kv8(q, self.kv8, pos, **bounds)
@@ -188,7 +192,8 @@ class ThinkerDecoderLayer(nn.Module):
                                            m.hidden, m.down.K, m.gate_up.E, m.top_k))
         return self._fused
 
-    def forward(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
+    def forward(self, h: torch.Tensor, pos: int | torch.Tensor,
+                context_workspace: ops.Workspace | None = None) -> torch.Tensor:
         if h.numel() == h.shape[-1] and self.fused():
             a, m = self.attn, self.moe
             if not isinstance(pos, torch.Tensor) and not 0 <= pos < a.max_len:
@@ -198,11 +203,12 @@ class ThinkerDecoderLayer(nn.Module):
                 a.k_norm_w, a.inv_freq, pos, a.k_cache, a.v_cache, a.o_proj.w, m.gate_up,
                 m.down, m.top_k, m.router_w, m.norm_weight, m.norm_eps, m.norm_topk_prob,
                 a.workspace)
-        return self.unfused(h, pos)
+        return self.unfused(h, pos, context_workspace)
 
-    def unfused(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
+    def unfused(self, h: torch.Tensor, pos: int | torch.Tensor,
+                context_workspace: ops.Workspace | None = None) -> torch.Tensor:
         """The attention block, then the MoE block (each its own entry points)."""
-        h = self.attn(h, pos)
+        h = self.attn(h, pos, context_workspace)
         return self.moe(h, residual=h)
 
 
@@ -215,6 +221,7 @@ class ThinkerDecoder(nn.Module):
         super().__init__()
         self.layers = nn.ModuleList(layers)
         self.workspace = ops.Workspace()
+        self.context_workspace = ops.Workspace()  # of the layers' attention, one by one
         self._fused: bool | None = None
         self._layers_c, self._layers_refs, self._layers_gen = None, None, -1
 
@@ -268,7 +275,7 @@ class ThinkerDecoder(nn.Module):
     def unfused(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
         """Layer by layer (each its own i4_thinker_layer_decode or module calls)."""
         for layer in self.layers:
-            h = layer(h, pos)
+            h = layer(h, pos, self.context_workspace)
         return h
 
     forward = step

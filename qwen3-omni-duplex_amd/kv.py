@@ -102,12 +102,21 @@ def _call(dev: torch.device, entry, *args) -> None:
 
 _STREAM_WS: dict = {}
 
+# Scratch up to which a workspace keeps it from call to call.  Calls of few query rows need at
+# most 17 MB; the parts of a long chunk's rows (30 MB for 300 tokens at 32000 positions and the
+# Thinker's heads, 339 MB for 2912 at 65536) are memory of that call.
+KEPT_BYTES = 1 << 25
+
 
 def _scratch(workspace: Workspace | None, need: int,
              dev: torch.device) -> tuple[torch.Tensor, torch.Tensor | None]:
     """`need` bytes and the counters: of the caller's workspace, else of one per stream, whose
-    calls run in order; under capture one of the call's own, which the graph then owns.  The
-    caller holds them until its call is queued (another thread's may grow the workspace)."""
+    calls run in order; under capture one of the call's own, which the graph then owns.  More
+    than KEPT_BYTES are the call's own throughout (stream ordered, without counters: only calls
+    of few rows count).  The caller holds them until its call is queued (another thread's may
+    grow the workspace)."""
+    if need > KEPT_BYTES:
+        return torch.empty(need, dtype=torch.uint8, device=dev), None
     if workspace is None:
         if torch.cuda.is_current_stream_capturing():
             workspace = Workspace()

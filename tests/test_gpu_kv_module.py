@@ -148,3 +148,26 @@ def test_leading_dimension_of_one(pkg, dev):
         assert got.shape == (1, *want.shape) and torch.equal(got[0], want)
     with pytest.raises(ValueError, match="several sequences"):
         a.step(h[:2, None], 0)
+
+
+@pytest.mark.parametrize("context", [{}, {"kv_dtype": torch.int8}])
+def test_scratch_of_a_decoder(pkg, dev, context):
+    """A long chunk far into a conversation leaves no scratch behind, and steps share one."""
+    dec = build(pkg, dev, layers=3, max_len=65536, **context)
+    T, pos = 1040, 64 * 936  # a whole block: the chunk can be appended twice
+    need = pkg.lib().i4_attn_window_workspace_bytes(1, T, NH, NKV, pos + T, 0, 0)
+    assert need > 1 << 25
+    h = tokens(dev, T)
+    for l in dec.layers:
+        if l.attn.kv8 is not None:  # a cache of zeros
+            l.attn.kv8.k_scale.fill_(1.0), l.attn.kv8.v_scale.fill_(1.0)
+    first = dec.step(h, pos)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    again = dec.step(h, pos)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() - held < need // 2  # the result
+    assert torch.equal(first, again)
+    dec.step(h[:2], pos)  # few rows: kept, once
+    assert all(l.attn.context_workspace.buf is None for l in dec.layers)
+    assert 0 < dec.context_workspace.buf.numel() <= 1 << 25

@@ -271,3 +271,32 @@ def test_module_refuses_several_sequences(pkg):
                 call(torch.zeros(shape), 0)
     with pytest.raises(ValueError, match="no token"):
         attn(torch.zeros(1, 0, 16), 0)
+
+
+def test_scratch_of_long_chunks_is_the_calls_own(pkg):
+    """What a workspace keeps is bounded, and a decoder's layers share one."""
+    from qwen3_omni_duplex_amd import kv
+
+    ws, cpu = pkg.Workspace(), torch.device("cpu")
+    big, counters = kv._scratch(ws, kv.KEPT_BYTES + 1, cpu)
+    assert big.numel() > kv.KEPT_BYTES and counters is None and ws.buf is None
+    small, counters = kv._scratch(ws, 1000, cpu)
+    assert ws.buf is small and counters is not None
+    size = pkg.lib().i4_attn_window_workspace_bytes
+    for B in (1, 3, 70, 256, 600):  # calls that count their parts
+        for T, nh, nkv in ((1, 32, 4), (16, 2, 2), (2, 32, 4), (1, 16, 1)):
+            assert size(B, T, nh, nkv, 1 << 20, 0, 0) <= kv.KEPT_BYTES
+
+    class Attn(torch.nn.Module):
+        def forward(self, h, pos, workspace=None):
+            seen.append(workspace)
+            return h
+
+    seen = []
+    layer = pkg.ThinkerDecoderLayer.__new__(pkg.ThinkerDecoderLayer)
+    torch.nn.Module.__init__(layer)
+    layer.attn, layer._fused = Attn(), False
+    layer.moe = lambda h, residual: h
+    dec = pkg.ThinkerDecoder([layer, layer])
+    dec.step(torch.zeros(3, 16), 0)
+    assert seen == [dec.context_workspace] * 2
