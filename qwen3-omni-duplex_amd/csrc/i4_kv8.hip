@@ -18,8 +18,9 @@ __device__ inline float quotient_to_odd(float x, float s, float inv) {
   t = fmaf(fmaf(-t, s, x), inv, t);
   const float r = fmaf(-t, s, x);
   const u32 b = __builtin_bit_cast(u32, t);
-  // an even last bit and a remainder: the odd neighbour on the remainder's side
-  const u32 odd = (r > 0.f) == (t > 0.f) ? b + 1 : b - 1;
+  // an even last bit and a remainder: the odd neighbour on the remainder's side (by the sign
+  // bit, as t may have underflowed to a zero of x's sign: away from it then)
+  const u32 odd = (r > 0.f) == ((b >> 31) == 0) ? b + 1 : b - 1;
   return __builtin_bit_cast(float, r == 0.f || (b & 1) ? b : odd);
 }
 // four elements in a word

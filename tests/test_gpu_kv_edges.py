@@ -60,3 +60,23 @@ def test_rope_far_positions(pkg, dev, dtype, pos):
             # two parts 2^-21; then one rounding
             err = 2.0 ** -19 * size
             check(got, want, err + ref.half_step(dtype) * (want.abs() + err) + 1e-7)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_append_quotients_that_underflow(pkg, dev, kind):
+    """Elements so far below their block's largest that x / scale is below fp32's range."""
+    x = torch.zeros(2, 1, 128, 1, HD, dtype=torch.bfloat16, device=dev)
+    x[:, 0, 0] = 1e30
+    small = [1e-20, -1e-20, 9.2e-41, -9.2e-41, 1e-38, -1e-38, 1e-8, -1e-8, 0.0, -0.0]
+    for i, e in enumerate(small):
+        x[:, 0, 1 + i] = e
+    x[:, 0, 64] = 1e9
+    for i, e in enumerate(small):
+        x[:, 0, 65 + i, 0, ::2] = e
+    cache, want = caches(pkg, dev, x, kind)
+    for s, (got, sc) in enumerate(zip(cache.values(), (cache.k_scale, cache.v_scale))):
+        assert torch.equal(sc.cpu(), want.scale[s].float())
+        vals = (want.elem[s].float() * sc.cpu()[..., None, None]).reshape(got.shape)
+        assert torch.equal(got.cpu(), vals)
+    q = rand(dev, 1, 2, 4, HD, seed=1)
+    assert torch.isfinite(pkg.attn_kv8(1e-30 * q, cache, 126)).all()
