@@ -443,10 +443,10 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
           tile_max(acc, s, a.c2 * ks);
           float r = vs;
           if constexpr (XT == I4_F16) {
+            // the power of two above vs; every block's counts among the largest
+            const float near = as_f32((__builtin_bit_cast(u32, vs) & 0x7F800000u) + 0x00800000u);
+            top = fmaxf(top, near);
             if (!(vs <= unit && vs > 0.125f * unit)) {
-              // the power of two above vs
-              const float near = as_f32((__builtin_bit_cast(u32, vs) & 0x7F800000u) + 0x00800000u);
-              top = fmaxf(top, near);
               const float u = fmaxf(near, 0x1p-30f * top);
               if (u != unit) set_unit(u);
             }

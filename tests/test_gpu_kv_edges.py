@@ -80,3 +80,24 @@ def test_append_quotients_that_underflow(pkg, dev, kind):
         assert torch.equal(got.cpu(), vals)
     q = rand(dev, 1, 2, 4, HD, seed=1)
     assert torch.isfinite(pkg.attn_kv8(1e-30 * q, cache, 126)).all()
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,nh,n,more", [(1, 4, 20, 6), (6, 4, 20, 6), (130, 2, 20, 6),
+                                         (50, 4, 6, 0)])  # the last: one split
+def test_zero_block_behind_large_blocks(pkg, dev, dtype, kind, T, nh, n, more):
+    """n blocks of scales up to 1 with a sum that grows along the context, then a block of
+    zeros, then ordinary ones."""
+    total = 64 * (n + 1 + more) + T
+    kv = rand(dev, 2, 1, total, 1, HD, seed=4, dtype=torch.float32)
+    big = 127.0 if kind == torch.int8 else 400.0
+    kv[1, :, :64 * n, :, 17] = big
+    kv[1, :, 64 * n:64 * n + 64] = 0
+    kv = kv.to(dtype)
+    cache, want8 = caches(pkg, dev, kv, kind)
+    q = rand(dev, 1, T, nh, HD, seed=8, dtype=dtype, gain=0.01)
+    k, v = want8.rows([total])
+    for window, sinks in ((None, 0), (64 * 10, 64)):
+        want, tol = ref.attention(q, k, v, [total - T], [T], window, sinks)
+        check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
