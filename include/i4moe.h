@@ -680,7 +680,9 @@ typedef struct i4_kvcache {
  * head: value = element * scale.  Blocks are rounded once, when their last token arrives;
  * the tokens of the unfinished block wait in the tail in 16 bits and are attended there.
  * Value blocks are kept [head_dim][token], the operand order of the product with the
- * softmax's weights.  Every array is dense and 16-byte aligned; blocks <= 2^14. */
+ * softmax's weights.  Elements are finite and scales positive, or NaN for a block that reads
+ * as NaN; a scale below 2^-100 / 448 (the zeros of an empty cache) reads as that.  Every
+ * array is dense and 16-byte aligned; blocks <= 2^14. */
 #define I4_KV8_BLOCK 64
 #define I4_KV8_INT8  0       /* element = RNE(x / scale), scale = max |x| / 127 */
 #define I4_KV8_E4M3  1       /* OCP e4m3fn, scale = max |x| / 448 */

@@ -224,9 +224,10 @@ __device__ inline void scores8(const Block8& x, const u32x4 (&q)[4], f32x4 (&s)[
 template <int FMT>
 __device__ inline void values8(RowAcc& acc, const Block8& x, f32x4 (&s)[4], bool partial, int key0,
                                int p, const Bounds& w) {
+  const float vs = block_scale(x.vs);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    s[k] *= x.vs;
+    s[k] *= vs;
     if (partial)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[k][i] = sees(w, p, key0 + 4 * k + i) ? s[k][i] : 0.f;
@@ -460,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
         const bool partial = !all_see(a.w, plo, phi, j0, 64);
         f32x4 s[4];
         scores8<XT, FMT>(x8, q, s);
-        const float c = a.c2 * x8.ks;
+        const float c = a.c2 * block_scale(x8.ks);
         const int64_t nb = hblk + ct.at(min(x + 4, e - 1));
         if (x + 4 < e) load_k8(x8, a.c8, nb, m, qd);
         weights<4>(acc, s, c, partial, j0 + 16 * qd, p, a.w);

@@ -430,7 +430,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       if (i0 < e) {
         load8(s8, a.c8, hblk + ct.at(i0), tid);
         store8<XT, FMT>(s8, lds, tid);
-        ks = s8.ks, vs = s8.vs;
+        ks = block_scale(s8.ks), vs = block_scale(s8.vs);
       }
       for (int i = i0; i < e; ++i) {
         const int cur = (i - i0) & 1, j0 = 64 * ct.at(i);
@@ -440,7 +440,8 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
         if (ks + vs == ks + vs) {
           tile_scores<XT>(buf, q, s, n, h);
           if (!whole(i)) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
-          tile_max(acc, s, a.c2 * ks);
+          const float c = fmaxf(a.c2 * ks, 0x1p-126f);  // above 0: masked scores stay -inf
+          tile_max(acc, s, c);
           float r = vs;
           if constexpr (XT == I4_F16) {
             // the power of two above vs; every block's counts among the largest
@@ -454,7 +455,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
           }
           // (in units of a much larger block an fp16 block's weights may round to 0: then the
           // sum is of the fp32 ones)
-          const float sum = tile_weights<XT>(acc, s, a.c2 * ks, kLift + log2f(r),
+          const float sum = tile_weights<XT>(acc, s, c, kLift + log2f(r),
                                              XT == I4_BF16 || r > 0.125f);
           acc.l = fmaf(sum, 1.0f / r, acc.l);
           tile_values8<XT>(acc, s, buf + TBYTES, n, h);
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
         }
         if (i + 1 < e) {
           store8<XT, FMT>(s8, lds + (cur ^ 1) * 2 * TBYTES, tid);
-          ks = s8.ks, vs = s8.vs;
+          ks = block_scale(s8.ks), vs = block_scale(s8.vs);
         }
       }
       if (XT == I4_F16 && unit != 1.f) set_unit(1.f);

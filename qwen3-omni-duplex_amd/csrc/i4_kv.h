@@ -48,6 +48,15 @@ struct Cache8 {
   int32_t blocks;
 };
 
+// A block's scale from what is stored: at least the smallest that the append writes, so that
+// nothing is divided by a scale of 0 (an empty cache's, or another quantiser's for a block of
+// zeros); NaN stays.  Taken where the scale is used, not where it is loaded: there it would
+// wait for the block's loads (a 300-token chunk 40 -> 43.6 us).
+__device__ inline float block_scale(float x) {
+  constexpr float least = KV8_TINY / 448.f;
+  return x < least ? least : x;
+}
+
 // 8-bit elements: FMT is I4_KV8_INT8 or I4_KV8_E4M3.
 template <int FMT> __device__ inline float from_8bit(uint8_t b) {
   if constexpr (FMT == I4_KV8_INT8) return (float)(int8_t)b;

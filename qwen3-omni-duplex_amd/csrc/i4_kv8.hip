@@ -144,14 +144,14 @@ __global__ __launch_bounds__(256) void k_kv8_values(Cache8 c, float* __restrict_
   };
   if (blockIdx.y == 0) {
     const u32* src = (const u32*)(c.k + blk * KBLK * KHD);
-    const float s = c.ks[blk];
+    const float s = block_scale(c.ks[blk]);
     f32x4* dst = (f32x4*)(ko + blk * KBLK * KHD);
 #pragma unroll
     for (int j = 0; j < 8; ++j) dst[256 * j + tid] = four(src[256 * j + tid], s);
     return;
   }
   const u32* src = (const u32*)(c.v + blk * KBLK * KHD);
-  const float s = c.vs[blk];
+  const float s = block_scale(c.vs[blk]);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int w = 256 * j + tid;

@@ -101,3 +101,24 @@ def test_zero_block_behind_large_blocks(pkg, dev, dtype, kind, T, nh, n, more):
     for window, sinks in ((None, 0), (64 * 10, 64)):
         want, tol = ref.attention(q, k, v, [total - T], [T], window, sinks)
         check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("which", ["k", "v", "both"])
+@pytest.mark.parametrize("T,nh", [(2, 8), (3, 8), (90, 4)])
+def test_blocks_of_scale_zero(pkg, dev, dtype, kind, which, T, nh):
+    """A scale of 0 (an empty cache's, or another quantiser's for zeros): the block's values are
+    zeros, also where a row sees part of the block alone."""
+    total = 64 * 8 + T
+    cache, want8 = caches(pkg, dev, rand(dev, 2, 1, total, 1, HD, seed=4, dtype=dtype), kind)
+    for i in (0, 2, 5, 6):
+        for s, (name, sc) in enumerate((("k", cache.k_scale), ("v", cache.v_scale))):
+            if which in (name, "both"):
+                sc[..., i] = 0
+                want8.scale[s, ..., i] = 0
+    q = rand(dev, 1, T, nh, HD, seed=8, dtype=dtype)
+    k, v = want8.rows([total])
+    for window, sinks in ((None, 0), (90, 0), (150, 20), (1, 0)):
+        want, tol = ref.attention(q, k, v, [total - T], [T], window, sinks)
+        check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
