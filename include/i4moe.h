@@ -722,7 +722,8 @@ int    i4_rope_append(const void* qkv, int x_dtype, int T, int64_t batch_stride,
  * j <= p, and with window > 0 only j > p - window or j < sinks (the first tokens stay
  * visible); query head h reads kv head h / (n_heads / n_kv_heads).  window == 0: no bound
  * (sinks must be 0).  Keys and values that a query does not see do not reach its row, be
- * they infinite or NaN.  q at q + b q_batch_stride + t q_token_stride + h q_head_stride
+ * they infinite or NaN; a value that is not finite makes the rows that see it infinite or NaN
+ * there, and finite ones overflow only where sum_j e^(s_j - max s) |v_j| passes fp32.  q at q + b q_batch_stride + t q_token_stride + h q_head_stride
  * (elements, 16-byte aligned rows), x_dtype == cache->dtype; out dense
  * [B][T][n_heads][head_dim], rounded once from fp32.  Workspace:
  * i4_attn_window_workspace_bytes with keys = pos + T, or max_len for a device position;
@@ -759,7 +760,8 @@ int    i4_kv8_values(const i4_kv8cache* cache, float* k_out, float* v_out, hipSt
 
 /* i4_attn_window over an 8-bit cache that holds the queries' own tokens too (appended
  * first): positions in finished blocks of the pos + count tokens are read in 8 bits, the
- * unfinished block from the tail.  Workspace: i4_attn_window_workspace_bytes, keys =
+ * unfinished block from the tail.  Blocks whose values are below 2^-30 (fp16; bf16: 2^-80) of the
+ * largest block's of the call may be lost beside it.  Workspace: i4_attn_window_workspace_bytes, keys =
  * pos + T, or 64 blocks for a device position. */
 int    i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    int64_t q_token_stride, int64_t q_head_stride, int n_heads,

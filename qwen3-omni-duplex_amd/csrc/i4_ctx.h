@@ -117,9 +117,11 @@ template <int XT> __device__ inline float hi_f32(u32 x) {
   return Half<XT>::to_f32((uint16_t)(x >> 16));
 }
 
-// Weights are 2^(x - m + kLift): with m at most kLazy below the true maximum they reach
-// 2^(kLift + kLazy) < 65504 and stay normal fp16 numbers down to 2^-21 of the largest.
-static constexpr float kLift = 7.f, kLazy = 8.f;
+// Weights are 2^(x - m + lift) with m at most kLazy below the true maximum.  In fp16 they reach
+// 2^(7 + 8) < 65504 and stay normal numbers down to 2^-21 of the largest.  In bf16 they are at
+// most 1, so that sums overflow only where those of the plain form do.
+static constexpr float kLazy = 8.f;
+template <int XT> static constexpr float kLift = XT == I4_F16 ? 7.f : -kLazy;
 
 // Byte N of w as a signed integer, converted: one instruction.  Written out because the
 // compiler otherwise splits the loaded words into bytes as soon as they arrive and carries

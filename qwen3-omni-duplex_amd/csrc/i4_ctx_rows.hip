@@ -50,7 +50,7 @@ __device__ inline float sum_qd(float v) {
 
 // scores (in place) -> weights; c: scale log2(e) (times the keys' scale); key0: the lane's
 // first key, key0 + 4 k + i the others
-template <int NK>
+template <int XT, int NK>
 __device__ inline void weights(RowAcc& acc, f32x4 (&s)[NK], float c, bool partial, int key0, int p,
                                const Bounds& w) {
   float top = -__builtin_inff();
@@ -72,7 +72,7 @@ __device__ inline void weights(RowAcc& acc, f32x4 (&s)[NK], float c, bool partia
     for (int t = 0; t < 8; ++t) acc.o[t] *= f;
   }
   // a row that has seen nothing yet has m = -inf and scores -inf: weights 0
-  const float base = acc.m == -__builtin_inff() ? 0.f : acc.m - kLift;
+  const float base = acc.m == -__builtin_inff() ? 0.f : acc.m - kLift<XT>;
 #pragma unroll
   for (int k = 0; k < NK; ++k)
 #pragma unroll
@@ -220,7 +220,9 @@ __device__ inline void scores8(const Block8& x, const u32x4 (&q)[4], f32x4 (&s)[
   }
 }
 // The weights take the values' scale; both enter the product as bf16, whose range holds any
-// scale.  A block with scale NaN is NaN for the rows that see one of its keys.
+// scale: bf16's weights of at most 1 times up to 2^121, fp16's of 2^15 times up to 2^10.  Below
+// 2^-133 a product is lost, 2^-125 of the largest weight: with the smallest scale, 2^-109, that
+// is an output off by up to 2^-117 a position.  A block with scale NaN is NaN for the rows that see one of its keys.
 template <int FMT>
 __device__ inline void values8(RowAcc& acc, const Block8& x, f32x4 (&s)[4], bool partial, int key0,
                                int p, const Bounds& w) {
@@ -439,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
         scores16<XT>(h, q, s);
         const int jn = pos0(min(x + 4, e - 1));
         if (x + 4 < e) load_k16(h, kr, jn, stride, m, qd);
-        weights<2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
+        weights<XT, 2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
         if (partial) clean16<XT>(acc, h, vr, j0, stride, j0, m, qd, plo, phi, p, a.w);
         values16<XT>(acc, h, s);
         if (x + 4 < e) load_v16(h, vr, jn, stride, m, qd);
@@ -464,7 +466,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
         const float c = a.c2 * block_scale(x8.ks);
         const int64_t nb = hblk + ct.at(min(x + 4, e - 1));
         if (x + 4 < e) load_k8(x8, a.c8, nb, m, qd);
-        weights<4>(acc, s, c, partial, j0 + 16 * qd, p, a.w);
+        weights<XT, 4>(acc, s, c, partial, j0 + 16 * qd, p, a.w);
         values8<FMT>(acc, x8, s, partial, j0 + 16 * qd, p, a.w);
         if (x + 4 < e) load_v8(x8, a.c8, nb, m, qd);
       }
@@ -483,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
           load_v16(h, vr, row0, stride, m, qd);
           f32x4 s[2];
           scores16<XT>(h, qn, s);
-          weights<2>(acc, s, a.c2, true, j0 + 8 * qd, p, a.w);
+          weights<XT, 2>(acc, s, a.c2, true, j0 + 8 * qd, p, a.w);
           clean16<XT>(acc, h, vr, row0, stride, j0, m, qd, plo, phi, p, a.w);
           values16<XT>(acc, h, s);
         }

@@ -382,7 +382,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       tile_scores<XT>(buf, q, s, n, h);
       if (edge) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
       tile_max(acc, s, a.c2);
-      acc.l += tile_weights<XT>(acc, s, a.c2, kLift);
+      acc.l += tile_weights<XT>(acc, s, a.c2, kLift<XT>);
       tile_values16<XT>(acc, s, buf + TBYTES, lane);
     };
     if constexpr (FMT < 0) {
@@ -416,16 +416,22 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       Stage8 s8;
       float ks = 0.f, vs = 0.f;
       // The weights that enter the product take the values' scale, in the exponent; their sum
-      // gives it back.  In fp16, whose range does not hold any scale, the scale is taken in
-      // units of a power of two near it, and the sums so far follow when the unit changes.
-      // It stays above 2^-30 of the largest one there was: what a block of so much smaller
-      // values adds is lost only to rows that met larger ones (and their sums would overflow).
-      float unit = 1.f, top = 0.f;
+      // gives it back.  As the 16-bit types' ranges do not hold every scale, it is taken in units
+      // of a power of two near it, and the sums so far follow when the unit changes: in fp16
+      // where a scale is above it or below an eighth of it, in bf16 above 2^10 or below 2^-60.
+      // The unit stays above 2^-30 (bf16: 2^-80) of the largest scale there was, so that the sums
+      // do not overflow: what a block of so much smaller values adds is lost to rows that met
+      // the larger ones, and to rows of this workgroup that did not see them.
+      constexpr bool F16 = XT == I4_F16;
+      constexpr float kUp = F16 ? 1.f : 0x1p10f, kDown = F16 ? 0.125f : 0x1p-60f;
+      constexpr float kFloor = F16 ? 0x1p-30f : 0x1p-80f;
+      float unit = 1.f, per = 1.f, top = 0.f;  // per = 1 / unit
       auto set_unit = [&](float u) {
         const float f = unit / u;
 #pragma unroll
         for (int t = 0; t < 4; ++t) acc.o[t] *= f;
         unit = u;
+        per = 1.0f / u;
       };
       if (i0 < e) {
         load8(s8, a.c8, hblk + ct.at(i0), tid);
@@ -442,21 +448,17 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
           if (!whole(i)) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
           const float c = fmaxf(a.c2 * ks, 0x1p-126f);  // above 0: masked scores stay -inf
           tile_max(acc, s, c);
-          float r = vs;
-          if constexpr (XT == I4_F16) {
-            // the power of two above vs; every block's counts among the largest
-            const float near = as_f32((__builtin_bit_cast(u32, vs) & 0x7F800000u) + 0x00800000u);
-            top = fmaxf(top, near);
-            if (!(vs <= unit && vs > 0.125f * unit)) {
-              const float u = fmaxf(near, 0x1p-30f * top);
-              if (u != unit) set_unit(u);
-            }
-            r = vs / unit;
+          // the power of two above vs; every block's counts among the largest
+          const float near = as_f32((__builtin_bit_cast(u32, vs) & 0x7F800000u) + 0x00800000u);
+          top = fmaxf(top, near);
+          if (!(vs <= kUp * unit && vs > kDown * unit)) {
+            const float u = fmaxf(near, kFloor * top);
+            if (u != unit) set_unit(u);
           }
+          const float r = F16 ? vs * per : fmaxf(vs * per, 0x1p-100f);
           // (in units of a much larger block an fp16 block's weights may round to 0: then the
           // sum is of the fp32 ones)
-          const float sum = tile_weights<XT>(acc, s, c, kLift + log2f(r),
-                                             XT == I4_BF16 || r > 0.125f);
+          const float sum = tile_weights<XT>(acc, s, c, kLift<XT> + log2f(r), !F16 || r > 0.125f);
           acc.l = fmaf(sum, 1.0f / r, acc.l);
           tile_values8<XT>(acc, s, buf + TBYTES, n, h);
         } else if (j0 <= p && (min(j0 + KBLK - 1, p) > p - a.w.window || j0 < a.w.sinks)) {
@@ -467,7 +469,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
           ks = block_scale(s8.ks), vs = block_scale(s8.vs);
         }
       }
-      if (XT == I4_F16 && unit != 1.f) set_unit(1.f);
+      if (unit != 1.f) set_unit(1.f);
       if (tail) {
         const int64_t at = (int64_t)hb * (KBLK * KHD);
         const int rows = phi - full * KBLK + 1;

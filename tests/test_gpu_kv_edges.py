@@ -122,3 +122,63 @@ def test_blocks_of_scale_zero(pkg, dev, dtype, kind, which, T, nh):
     for window, sinks in ((None, 0), (90, 0), (150, 20), (1, 0)):
         want, tol = ref.attention(q, k, v, [total - T], [T], window, sinks)
         check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
+
+
+@pytest.mark.parametrize("kind", [None] + KINDS)
+@pytest.mark.parametrize("T,nh", [(1, 4), (6, 4), (130, 2)])
+def test_values_near_the_end_of_bf16(pkg, dev, kind, T, nh):
+    """bf16 values up to 2.5e38: the average is finite where the sum of the values under weights
+    of at most 1 is; scores that grow along the context make the running maximum late."""
+    total, pos = 64 * 6 + T, 64 * 6
+    kv = rand(dev, 2, 1, total, 1, HD, seed=4, dtype=torch.float32)
+    kv[1] = kv[1].clamp(-3, 3) * 1e37
+    kv[1, :, ::7, :, 5] = 2.5e38
+    kv[0, ..., 0] = torch.linspace(0, 12, total, device=dev)[None, :, None]
+    kv = kv.to(torch.bfloat16)
+    q = rand(dev, 1, T, nh, HD, seed=8, gain=0.1)
+    q[..., 0] = 3.0
+    if kind is None:
+        k, v = (x.transpose(1, 2).contiguous() for x in kv)
+        go = lambda **b: pkg.attn_window(q, k, v, pos, **b)  # noqa: E731
+    else:
+        cache, want8 = caches(pkg, dev, kv, kind)
+        k, v = want8.rows([total])
+        go = lambda **b: pkg.attn_kv8(q, cache, pos, **b)  # noqa: E731
+    for window, sinks in ((1, 0), (3, 0), (2, 1)):
+        want, tol = ref.attention(q, k, v, [pos], [T], window, sinks)
+        check(go(window=window, sinks=sinks), want, tol)
+    # rows of small weights on many large values of both signs: each sum stays in fp32
+    kv[1] = torch.where(kv[1].abs() > 2e38, kv[1] / 4, kv[1])
+    kv[1, :, 1::2] = -kv[1, :, 0:total - 1:2][:, :kv[1, :, 1::2].shape[1]]
+    if kind is None:
+        k, v = (x.transpose(1, 2).contiguous() for x in kv)
+        go = lambda **b: pkg.attn_window(q, k, v, pos, **b)  # noqa: E731
+    else:
+        cache, want8 = caches(pkg, dev, kv, kind)
+        k, v = want8.rows([total])
+        go = lambda **b: pkg.attn_kv8(q, cache, pos, **b)  # noqa: E731
+    want, tol = ref.attention(q, k, v, [pos], [T], 40, 4)
+    check(go(window=40, sinks=4), want, tol)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,nh", [(1, 4), (6, 4), (130, 2)])
+def test_bf16_blocks_of_very_different_magnitudes(pkg, dev, kind, T, nh):
+    """Value blocks from 2^-90 to 2^100 in one cache, upwards, downwards and mixed."""
+    total = 64 * 14 + T
+    base = rand(dev, 2, 1, total, 1, HD, seed=4, dtype=torch.float32)
+    mixed = [0, -90, 100, None, -90, -40, 60, 0, 100, -60, None, 20, -90, 100, 0, 0, 0]
+    for steps in (mixed, sorted((s or 0) for s in mixed), sorted(((s or 0) for s in mixed),
+                                                                  reverse=True), [-90] * 17):
+        kv = base.clone()
+        for i, p in enumerate(steps):
+            kv[1, :, 64 * i:64 * i + 64] *= 0.0 if p is None else 2.0 ** p
+        cache, want8 = caches(pkg, dev, kv.to(torch.bfloat16), kind)
+        q = rand(dev, 1, T, nh, HD, seed=8, gain=0.5)
+        k, v = want8.rows([total])
+        for window, sinks in ((None, 0), (130, 64)):
+            want, tol = ref.attention(q, k, v, [total - T], [T], window, sinks)
+            # a workgroup's rows share the unit of their sums: what a row sees is kept to 2^-60
+            # of the largest value among the cache's blocks
+            tol += 2.0 ** -60 * v.abs().max().item()
+            check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
