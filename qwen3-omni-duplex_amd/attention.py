@@ -96,9 +96,12 @@ class ThinkerAttention(nn.Module):
 
     def _apply(self, fn, *args, **kwargs):
         super()._apply(fn, *args, **kwargs)
-        dev = self.input_norm_w.device
-        if self.kv8 is not None and self.kv8.k.device != dev:
-            self.kv8 = kv.KV8Cache(*(t.to(dev) for t in self.kv8.tensors))
+        w = self.input_norm_w
+        if self.kv8 is not None:
+            *blocks, k_tail, v_tail = self.kv8.tensors
+            if (k_tail.device, k_tail.dtype) != (w.device, w.dtype):
+                self.kv8 = kv.KV8Cache(*(t.to(w.device) for t in blocks),
+                                       k_tail.to(w.device, w.dtype), v_tail.to(w.device, w.dtype))
         return self
 
     def whole_context(self) -> bool:

@@ -171,3 +171,18 @@ def test_scratch_of_a_decoder(pkg, dev, context):
     dec.step(h[:2], pos)  # few rows: kept, once
     assert all(l.attn.context_workspace.buf is None for l in dec.layers)
     assert 0 < dec.context_workspace.buf.numel() <= 1 << 25
+
+
+def test_8_bit_cache_follows_the_dtype(pkg, dev):
+    """half() moves the unfinished block with the norms; the finished ones have no dtype."""
+    h = tokens(dev, 100, dtype=torch.float16)
+    a, b = (build(pkg, dev, kv_dtype=t).layers[0].attn for t in (torch.int8, None))
+    a.half(), b.half()
+    assert a.kv8.k_tail.dtype == a.kv8.v_tail.dtype == torch.float16
+    for lo, hi in ((0, 60), (60, 61)):  # all of them still in 16 bits
+        assert near(a(h[lo:hi], lo), b(h[lo:hi], lo), torch.float16)
+    k8 = a.kv8.tensors
+    a.bfloat16()
+    assert a.kv8.k.data_ptr() == k8[0].data_ptr() and a.kv8.k_tail.dtype == torch.bfloat16
+    assert torch.equal(a.kv8.k_tail, k8[4].bfloat16())
+    assert torch.isfinite(a(h[61:].bfloat16(), 61)).all()
