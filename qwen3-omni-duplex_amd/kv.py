@@ -29,7 +29,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import Workspace
+from .ops import Workspace, _capturing
 
 KV8_BLOCK = 64
 _FORMATS = {torch.int8: 0, torch.float8_e4m3fn: 1}
@@ -118,7 +118,7 @@ def _scratch(workspace: Workspace | None, need: int,
     if need > KEPT_BYTES:
         return torch.empty(need, dtype=torch.uint8, device=dev), None
     if workspace is None:
-        if torch.cuda.is_current_stream_capturing():
+        if _capturing(dev):
             workspace = Workspace()
         else:
             key = (dev.index, _lib.stream(dev))

@@ -278,7 +278,14 @@ def moe_weights_c(gate_up: QWeight, down: QWeight, router_w: torch.Tensor | None
 
 
 def _capturing(device: torch.device) -> bool:
-    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+    """Whether the device's own current stream is being captured (torch asks the current
+    device's)."""
+    if device.type != "cuda":
+        return False
+    if device.index in (None, torch.cuda.current_device()):
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
 
 
 class Workspace:

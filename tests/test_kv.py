@@ -300,3 +300,35 @@ def test_scratch_of_long_chunks_is_the_calls_own(pkg):
     dec = pkg.ThinkerDecoder([layer, layer])
     dec.step(torch.zeros(3, 16), 0)
     assert seen == [dec.context_workspace] * 2
+
+
+def test_capture_on_another_device_than_the_current_one(pkg, monkeypatch):
+    """Scratch of a call on cuda:1 goes by cuda:1's stream while cuda:0 is current."""
+    import contextlib
+
+    from qwen3_omni_duplex_amd import _lib, kv, ops
+
+    now = [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        old, now[0] = now[0], d.index
+        yield
+        now[0] = old
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] in capturing)
+    monkeypatch.setattr(_lib, "stream", lambda dev: 7)
+    monkeypatch.setattr(kv, "_STREAM_WS", {})
+    for capturing, want in (({1}, (False, True)), ({0}, (True, False)), (set(), (False, False))):
+        for i in (0, 1):
+            dev = torch.device("cuda", i)
+            assert ops._capturing(dev) is want[i] and now[0] == 0
+            got = []
+            monkeypatch.setattr(kv.Workspace, "get", lambda self, n, d: got.append(self))
+            monkeypatch.setattr(kv.Workspace, "counters", lambda self, d: None)
+            kv._scratch(None, 100, dev)
+            kept = kv._STREAM_WS.get((i, 7))
+            assert (got[0] is not kept) == want[i]
+    assert not ops._capturing(torch.device("cpu"))
