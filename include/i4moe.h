@@ -662,7 +662,9 @@ int    i4_dmoe_down_wait(const void* x, int x_dtype, const i4_dmoe_weights* weig
  * of the T tokens sequence b has (clamped to [0, T]): the others are padding, for which
  * nothing is read or written.  A position outside the cache, which only a device position
  * can give, writes nothing to it and NaN to the token's output row.  head_dim == 128; any
- * n_heads that is a multiple of n_kv_heads, at most 1024; B T n_heads < 2^31. */
+ * n_heads that is a multiple of n_kv_heads, at most 1024; B T (n_heads + 2 n_kv_heads) < 2^31,
+ * and fewer than 2^24 workgroups a launch (i4_rope_append: tokens; i4_kv8_values: blocks of all
+ * heads; the attention: kv heads, or tiles of 128 of their rows). */
 
 /* A 16-bit cache: k and v [batch][n_kv_heads][max_len][head_dim] with strides in elements
  * (the same for k and v; a row's head_dim values adjacent, every row 16-byte aligned), so

@@ -62,6 +62,8 @@ static int launch(CtxArgs& a, int xt, int fmt, int keys, const i4_span& w, hipSt
   a.ml = a.part + sp.parts * KHD;
   a.counters = w.counters;
   a.tiles = (a.R + kTileRows - 1) / kTileRows;
+  const int64_t grid = a.R <= kFewRows ? sp.wgs : (int64_t)a.tiles * sp.S * a.B * a.nkv;
+  if (grid > kMaxGrid) return I4_ERR_SHAPE;
   return a.R <= kFewRows ? i4_launch_ctx_rows(a, xt, fmt, stream)
                          : i4_launch_ctx_tile(a, xt, fmt, stream);
 }

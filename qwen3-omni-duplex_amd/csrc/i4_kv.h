@@ -10,6 +10,7 @@ static constexpr int KHD = 128;                // head_dim
 static constexpr int KBLK = I4_KV8_BLOCK;      // tokens per 8-bit block
 static constexpr int KV_MAX_LEN = 1 << 20;     // positions of a cache
 static constexpr int ROPE_MAX_POS = 1 << 24;   // positions that fp32 holds exactly
+static constexpr int kMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads: fewer than 2^32
 static constexpr float KV8_TINY = 0x1p-100f;   // floor of a block's largest magnitude
 
 // The tokens of the call's sequences: where each begins and how many it has.

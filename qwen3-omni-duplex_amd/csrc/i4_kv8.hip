@@ -276,7 +276,9 @@ extern "C" int i4_kv8_values(const i4_kv8cache* cache, float* k_out, float* v_ou
   const int rc = i4_check_kv8cache(cache);
   if (rc) return rc;
   if (((uintptr_t)k_out & 15) || ((uintptr_t)v_out & 15)) return I4_ERR_ALIGN;
-  const dim3 grid((unsigned)(cache->batch * cache->n_kv_heads * cache->blocks), 2);
+  const int64_t blocks = (int64_t)cache->batch * cache->n_kv_heads * cache->blocks;
+  if (blocks > kMaxGrid) return I4_ERR_SHAPE;
+  const dim3 grid((unsigned)blocks, 2);
   if (cache->format == I4_KV8_E4M3)
     k_kv8_values<I4_KV8_E4M3><<<grid, 256, 0, stream>>>(cache8(cache), k_out, v_out);
   else

@@ -122,6 +122,7 @@ extern "C" int i4_rope_append(const void* qkv, int x_dtype, int T, int64_t batch
   rc = i4_check_tokens(B, T, n_heads, nkv, pos_dev, pos, counts, limit);
   if (rc) return rc;
   if (first_row >= 0 && first_row > cache->max_len - T) return I4_ERR_SHAPE;
+  if ((int64_t)B * T > kMaxGrid) return I4_ERR_SHAPE;
   const int64_t width = (int64_t)(n_heads + 2 * nkv) * KHD;
   if ((T > 1 && token_stride < width) || (B > 1 && batch_stride < width)) return I4_ERR_STRIDE;
   if (((uintptr_t)qkv & 15) || ((uintptr_t)q_norm_w & 15) || ((uintptr_t)k_norm_w & 15) ||

@@ -332,3 +332,18 @@ def test_capture_on_another_device_than_the_current_one(pkg, monkeypatch):
             kept = kv._STREAM_WS.get((i, 7))
             assert (got[0] is not kept) == want[i]
     assert not ops._capturing(torch.device("cpu"))
+
+
+def test_launches_past_the_grid_limit_are_refused(lb, pkg):
+    """2^24 workgroups of 256 threads are more than a launch holds."""
+    lib = pkg.lib()
+    c = cache(lb, batch=16, max_len=1 << 20, head_stride=128 << 20, batch_stride=512 << 20)
+    assert call_rope(lb, lib, c, T=1 << 20, bs=2048 << 20) == SHAPE
+    for batch, T in ((1 << 14, 1), (1 << 14, 17)):  # few rows, and tiles of them
+        many = dict(batch=batch, n_kv_heads=1024)
+        big = cache(lb, **many, head_stride=256 * 128, batch_stride=1024 * 256 * 128)
+        a = dict(T=T, nh=1024, ts=1024 * 128, bs=1024 * 128 * T)
+        assert call_attn(lb, lib, big, **a) == SHAPE
+        assert call_attn(lb, lib, cache8(lb, **many), eight=True, **a) == SHAPE
+    c8 = cache8(lb, batch=1024, n_kv_heads=1024, blocks=16)
+    assert lib.i4_kv8_values(ctypes.byref(c8), P, P, None) == SHAPE
