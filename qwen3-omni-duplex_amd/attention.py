@@ -40,8 +40,8 @@ class ThinkerAttention(nn.Module):
 
     window: a token attends the last `window` positions (its own among them) and the first
     `sinks` ones; None: every position.  kv_dtype torch.int8 or torch.float8_e4m3fn: the cache
-    is a KV8Cache (self.kv8) instead of the 16-bit k_cache / v_cache, and tokens arrive in
-    order."""
+    is a KV8Cache (self.kv8) instead of the 16-bit k_cache / v_cache, tokens arrive in order,
+    and max_len is rounded up to whole blocks of 64."""
 
     def __init__(self, qkv: PackedQKV, o_proj: PackedLinear, q_norm_w: torch.Tensor,
                  k_norm_w: torch.Tensor, input_norm_w: torch.Tensor, n_heads: int,
@@ -72,7 +72,7 @@ class ThinkerAttention(nn.Module):
         shape = (n_kv_heads, max_len if kv_dtype is None else 0, head_dim)
         self.register_buffer("_k_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
         self.register_buffer("_v_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
-        self.max_len = int(max_len)
+        self.max_len = int(max_len) if self.kv8 is None else self.kv8.max_len
         self.workspace = ops.Workspace()
         self.context_workspace = ops.Workspace()  # of _attend, where the caller brings none
 

@@ -186,3 +186,16 @@ def test_8_bit_cache_follows_the_dtype(pkg, dev):
     assert a.kv8.k.data_ptr() == k8[0].data_ptr() and a.kv8.k_tail.dtype == torch.bfloat16
     assert torch.equal(a.kv8.k_tail, k8[4].bfloat16())
     assert torch.isfinite(a(h[61:].bfloat16(), 61)).all()
+
+
+def test_end_of_an_8_bit_cache(pkg, dev):
+    """Host and device positions end at the same one: max_len in whole blocks."""
+    h = tokens(dev, 128)
+    for step in (lambda p: p, lambda p: torch.tensor([p], dtype=torch.int32, device=dev)):
+        attn = build(pkg, dev, max_len=100, kv_dtype=torch.int8).layers[0].attn
+        assert attn.max_len == 128
+        attn(h[:127], 0)
+        assert torch.isfinite(attn(h[127:], step(127))).all()
+    assert torch.isnan(attn(h[127:], step(128))).all()
+    with pytest.raises(ValueError, match="outside the cache"):
+        attn(h[127:], 128)
