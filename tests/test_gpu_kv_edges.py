@@ -182,3 +182,123 @@ def test_bf16_blocks_of_very_different_magnitudes(pkg, dev, kind, T, nh):
             # of the largest value among the cache's blocks
             tol += 2.0 ** -60 * v.abs().max().item()
             check(pkg.attn_kv8(q, cache, total - T, window=window, sinks=sinks), want, tol)
+
+
+def splits(pkg, B, T, nh, nkv, keys, rows):
+    need = pkg.lib().i4_attn_window_workspace_bytes(B, T, nh, nkv, keys, 0, 0)
+    return need / ((HD + 2) * 4 * rows)
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("T,nh,pos,least", [(4, 8, 8000, 17), (20, 4, 8000, 17), (33, 2, 6000, 17),
+                                            (3, 6, 30000, 33)])
+def test_merge_of_many_splits(pkg, dev, dtype, eight, T, nh, pos, least):
+    """More splits than one round of the merge's loads, with a workgroup a row."""
+    assert splits(pkg, 1, T, nh, 1, pos + T, T * nh) >= least
+    kv = rand(dev, 2, 1, pos + T, 1, HD, seed=T, dtype=dtype)
+    q = rand(dev, 1, T, nh, HD, seed=8, dtype=dtype)
+    if eight:
+        cache, want8 = caches(pkg, dev, kv, torch.int8)
+        k, v = want8.rows([pos + T])
+        got = pkg.attn_kv8(q, cache, pos)
+    else:
+        k, v = (x.transpose(1, 2).contiguous() for x in kv)
+        got = pkg.attn_window(q, k, v, pos)
+    want, tol = ref.attention(q, k, v, [pos], [T], None, 0)
+    check(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("counted", [True, False])
+@pytest.mark.parametrize("B,nh,nkv,pos", [(1, 8, 1, 9000), (1, 4, 2, 32000), (2, 16, 1, 16500)])
+def test_merge_of_many_parts(pkg, dev, dtype, eight, counted, B, nh, nkv, pos):
+    """More parts than one round of the few-row merge, by the last workgroup or in a launch."""
+    assert splits(pkg, B, 1, nh, nkv, pos + 1, 16 * B * nkv) > 32
+    kv = rand(dev, 2, B, pos + 1, nkv, HD, seed=B, dtype=dtype)
+    q = rand(dev, B, 1, nh, HD, seed=8, dtype=dtype)
+    ws = pkg.Workspace()
+    if not counted:
+        ws.counters = lambda device: None
+    first = [pos - 700 * b for b in range(B)]
+    if eight:
+        cache, want8 = caches(pkg, dev, kv, torch.int8)
+        k, v = want8.rows([p + 1 for p in first])
+        for b in range(B):  # each sequence's own unfinished block
+            cache.k_tail[b] = kv[0, b, first[b] // 64 * 64:][:64].transpose(0, 1)[
+                :, torch.arange(64) % (first[b] % 64 + 1)]
+            cache.v_tail[b] = kv[1, b, first[b] // 64 * 64:][:64].transpose(0, 1)[
+                :, torch.arange(64) % (first[b] % 64 + 1)]
+            for s, x in enumerate((k, v)):
+                n = first[b] % 64 + 1
+                x[b, :, first[b] // 64 * 64:first[b] + 1] = (
+                    (cache.k_tail, cache.v_tail)[s][b, :, :n].double().cpu())
+        got = pkg.attn_kv8(q, cache, i32(dev, first), workspace=ws)
+    else:
+        k, v = (x.transpose(1, 2).contiguous() for x in kv)
+        got = pkg.attn_window(q, k, v, i32(dev, first), workspace=ws)
+    want, tol = ref.attention(q, k, v, first, [1] * B, None, 0)
+    check(got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("kind", [None] + KINDS)
+@pytest.mark.parametrize("T,nh,window", [(1, 8, 2), (2, 8, 9), (16, 1, 20)])
+def test_few_rows_keep_their_weights(pkg, dev, dtype, kind, T, nh, window):
+    """Up to 16 rows of a kv head: a weight is a sum of two 16-bit numbers, off by the square of
+    half a step.  Values that cancel under the weights leave the output's rounding out of it; the
+    oracle with weights of one number is off by more than the tolerance."""
+    total, pos = 64 * 6 + T - 1, 64 * 6 - 1
+    kv = rand(dev, 2, 1, total, 1, HD, seed=4, dtype=torch.float32)
+    q = rand(dev, 1, T, nh, HD, seed=8, dtype=dtype, gain=0.1)
+    kk = kv[0, 0, :, 0].to(dtype).double()
+    w = torch.softmax(kk[pos - window + 1:pos + 1] @ q[0, 0, 0].double() / math.sqrt(HD), 0)
+    # the last of the first row's values cancels the others
+    vv = kv[1, 0, pos - window + 1:pos + 1, 0].to(dtype).double()
+    kv[1, 0, pos, 0] = (-(w[:-1, None] * vv[:-1]).sum(0) / w[-1]).float()
+    kv = kv.to(dtype)
+    if kind is None:
+        k, v = (x.transpose(1, 2).contiguous() for x in kv)
+        got = pkg.attn_window(q, k, v, pos, window=window)
+    else:
+        cache, want8 = caches(pkg, dev, kv, kind)
+        k, v = want8.rows([total])
+        got = pkg.attn_kv8(q, cache, pos, window=window)
+    u = 2.0 ** -8 if kind is not None else ref.half_step(dtype)  # 8-bit values: bf16 weights
+    two, one = torch.empty(T, nh, HD, dtype=torch.float64), 0.0
+    tol = two.clone()
+    for t in range(T):
+        j = ref.see(pos + t, pos + t + 1, window, 0).nonzero()[:, 0]
+        kd, vd = (x.double().cpu()[0, 0][j] for x in (k, v))
+        s = q[0, t].double().cpu() @ kd.T / math.sqrt(HD)
+        e = torch.exp(s - s.amax(-1, keepdim=True))
+        mass = e @ vd.abs() / e.sum(-1, keepdim=True)
+        size = (q[0, t].double().cpu().abs() @ kd.abs().T).amax(-1, keepdim=True) / math.sqrt(HD)
+        two[t] = e @ vd / e.sum(-1, keepdim=True)
+        # as in the reference's tolerance, with u^2 in the place of u for the weights
+        off = (u * u + 2.0 ** -16 * size + 2.0 ** -18) * mass
+        tol[t] = off + ref.half_step(dtype) * (two[t].abs() + off) + 2.0 ** -25
+        r = e.to(torch.bfloat16 if kind is not None else dtype).double()
+        one = max(one, (((r @ vd / e.sum(-1, keepdim=True)) - two[t]).abs() / tol[t]).max().item())
+    assert one > 1.5
+    check(got[0], two, tol)
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("B,T,nh,nkv,pos,window,sinks", [
+    (3, 300, 32, 4, 5000, 2048, 4), (1, 1500, 16, 4, 0, None, 0), (1, 200, 32, 4, 3000, 2000, 64)])
+def test_tiles_repeat(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
+    """Prompts and chunks over both caches give the same bits on every call."""
+    kv = rand(dev, 2, B, pos + T, nkv, HD, seed=T, dtype=dtype)
+    q = rand(dev, B, T, nh, HD, seed=8, dtype=dtype)
+    k, v = (x.transpose(1, 2).contiguous() for x in kv)
+    cache = pkg.KV8Cache.empty(nkv, pos + T, batch=B, dtype=dtype, device=dev)
+    pkg.kv8_append(kv[0], kv[1], cache, 0)
+    first = None
+    for _ in range(4):
+        got = (pkg.attn_window(q, k, v, pos, window=window, sinks=sinks),
+               pkg.attn_kv8(q, cache, pos, window=window, sinks=sinks))
+        if first is None:
+            first = got
+        assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, first))
