@@ -41,7 +41,8 @@ class ThinkerAttention(nn.Module):
     window: a token attends the last `window` positions (its own among them) and the first
     `sinks` ones; None: every position.  kv_dtype torch.int8 or torch.float8_e4m3fn: the cache
     is a KV8Cache (self.kv8) instead of the 16-bit k_cache / v_cache, tokens arrive in order,
-    and max_len is rounded up to whole blocks of 64."""
+    and max_len is rounded up to whole blocks of 64.  A prompt over it differs from the same
+    tokens one by one by what 8 bits do to the blocks that it finishes (kv.attn_kv8)."""
 
     def __init__(self, qkv: PackedQKV, o_proj: PackedLinear, q_norm_w: torch.Tensor,
                  k_norm_w: torch.Tensor, input_norm_w: torch.Tensor, n_heads: int,

@@ -332,7 +332,9 @@ def attn_kv8(q: torch.Tensor, cache: KV8Cache, pos: int | torch.Tensor, *,
              workspace: Workspace | None = None) -> torch.Tensor:
     """attn_window over an 8-bit cache whose last tokens are the queries' own (kv8_append):
     positions in the finished blocks of the pos + T (or counts) tokens are read in 8 bits, the
-    unfinished block from the tail (i4_attn_kv8)."""
+    unfinished block from the tail (i4_attn_kv8).  A query of several therefore reads its own
+    block, if the call finished it, in 8 bits with a scale that later tokens have a part in
+    (one that is not finite makes the block NaN); token by token it is read in 16 bits."""
     dev = _lib.require_device(q, cache._t[0], counts, out)
     return _attend(_lib.lib().i4_attn_kv8, cache._c, cache.max_len, q, dev, pos, window, sinks,
                    scale, counts, out, workspace)

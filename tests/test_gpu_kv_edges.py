@@ -302,3 +302,37 @@ def test_tiles_repeat(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
         if first is None:
             first = got
         assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_prompt_over_8_bits_reads_whole_blocks(pkg, dev, kind):
+    """A prompt's queries read the blocks that their call finished in 8 bits, their own among
+    them, with later tokens in the scale; token by token the unfinished block is in 16 bits."""
+    T, nh = 100, 2
+    kv = rand(dev, 2, 1, T, 1, HD, seed=4)
+    q = rand(dev, 1, T, nh, HD, seed=8)
+    cache, whole8 = caches(pkg, dev, kv, kind)
+    k, v = whole8.rows([T])
+    want, tol = ref.attention(q, k, v, [0], [T], None, 0)
+    prompt = pkg.attn_kv8(q, cache, 0)
+    check(prompt, want, tol)
+    one = pkg.KV8Cache.empty(1, T, kind=kind, device=dev)
+    one8 = ref.Cache8(1, 1, 2, kind, torch.bfloat16)
+    for t in range(T):
+        pkg.kv8_append(kv[0, :, t:t + 1], kv[1, :, t:t + 1], one, t)
+        one8.append(kv[:, :, t:t + 1], [t], [1])
+        k, v = one8.rows([t + 1])
+        wt, tt = ref.attention(q[:, t:t + 1], k, v, [t], [1], None, 0)
+        check(pkg.attn_kv8(q[:, t:t + 1], one, t), wt, tt)
+    assert torch.equal(one.k, cache.k) and torch.equal(one.v_scale, cache.v_scale)
+    # a later token's infinity: all rows of its finished block, none of a tail's earlier rows
+    for at in (60, 90):
+        x = kv.clone()
+        x[1, 0, at, 0, 3] = math.inf
+        cache, _ = caches(pkg, dev, x, kind)
+        got = pkg.attn_kv8(q, cache, 0)
+        if at == 60:
+            assert got.isnan().all()
+        else:
+            assert torch.equal(got[:, :at], prompt[:, :at])
+            assert not torch.isfinite(got[:, at:, :, 3]).any()
