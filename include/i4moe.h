@@ -711,7 +711,7 @@ typedef struct i4_kv8cache {
  *   cache  row (first_row or p's own) + t of each kv head receives the token's rotated key
  *          and its value.  first_row < 0: the row is the position; >= 0: token t goes to row
  *          first_row + t (<= max_len), and positions reach to 2^24.
- * inv_freq is a host array [head_dim / 2].  Computed in fp32 (the angle p inv_freq as a sum
+ * inv_freq is a host array [head_dim / 2].  Computed in fp32 (the angle p inv_freq is a sum
  * of two floats) and rounded once. */
 int    i4_rope_append(const void* qkv, int x_dtype, int T, int64_t batch_stride,
                       int64_t token_stride, int n_heads, const void* q_norm_w,
@@ -725,9 +725,13 @@ int    i4_rope_append(const void* qkv, int x_dtype, int T, int64_t batch_stride,
  * visible); query head h reads kv head h / (n_heads / n_kv_heads).  window == 0: no bound
  * (sinks must be 0).  Keys and values that a query does not see do not reach its row, be
  * they infinite or NaN; a value that is not finite makes the rows that see it infinite or NaN
- * there, and finite ones overflow only where sum_j e^(s_j - max s) |v_j| passes fp32.  q at q + b q_batch_stride + t q_token_stride + h q_head_stride
- * (elements, 16-byte aligned rows), x_dtype == cache->dtype; out dense
- * [B][T][n_heads][head_dim], rounded once from fp32.  Workspace:
+ * there, and finite ones overflow only where sum_j e^(s_j - max s) |v_j| passes fp32.  q at
+ * q + b q_batch_stride + t q_token_stride + h q_head_stride (elements, 16-byte aligned rows),
+ * x_dtype == cache->dtype; out dense [B][T][n_heads][head_dim].  Scores, maxima and sums are
+ * fp32 and the output is rounded once; the weights e^(s - max) are rounded on their way into
+ * the product with v: up to 16 rows of a kv head (T n_heads / n_kv_heads) to a sum of two
+ * numbers of x_dtype (two bf16 ones over 8-bit blocks), more rows to one, whose sum over j is
+ * then of the rounded ones.  Workspace:
  * i4_attn_window_workspace_bytes with keys = pos + T, or max_len for a device position;
  * no initial contents, 256-byte aligned; calls sharing one must not overlap.  counters
  * (nullable): I4_CTX_COUNTERS int32, zero when they are allocated and left zero by every

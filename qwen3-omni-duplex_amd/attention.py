@@ -17,6 +17,8 @@ transformers' growing DynamicCache.
 
 Prompts and chunks of several tokens, a bounded context (window, sinks) and an 8-bit cache
 (kv_dtype) run launch by launch instead, on rope_append and attn_window / attn_kv8 (kv.py).
+Those round less often than the decode entries: a cache that holds a prompt's keys and later
+tokens' keys holds both roundings, several half steps of the dtype apart.
 """
 from __future__ import annotations
 
@@ -171,6 +173,7 @@ class ThinkerAttention(nn.Module):
         a = a.view(x.shape[0], -1)
         if x.shape[0] == 1:  # the residual enters the o_proj launch as its bias
             return ops.linear(a, self.o_proj.w, bias=x.reshape(-1)).view(h.shape)
+        # (several tokens: o_proj's output is rounded, then the sum with the residual)
         return self.o_proj(a).add_(x).view(h.shape)
 
 

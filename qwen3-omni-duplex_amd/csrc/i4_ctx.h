@@ -11,9 +11,10 @@
 namespace i4 {
 
 // Rows of a kv head up to which k_ctx_rows takes a call: as many as a 16-row product holds.
-// With a second one (32 rows) it took 138 us against k_ctx_tile's 160 for 16 sequences of 4
-// tokens over 32000 16-bit positions, but 26 against 16 for one sequence over 8000 (the parts
-// of 32 rows are merged by one workgroup) and 35 against 22 for 32 over 1000 8-bit ones.
+// With a second one (32 rows) it took 138 us against k_ctx_tile's 156 for 16 sequences of 4
+// tokens over 32000 16-bit positions (143 against 152 over 8-bit ones), but 26 against 16 for
+// one sequence over 8000 (the parts of 32 rows are merged by one workgroup) and 35 against 22
+// for 32 over 1000 8-bit ones.  The rule does not look at the batch: the large ones pay for it.
 static constexpr int kFewRows = 16;
 static constexpr int kShared = I4_CTX_COUNTERS;  // kv heads whose contexts are shared out
 static constexpr int kTileRows = 128;    // of a workgroup of k_ctx_tile

@@ -4,7 +4,8 @@
 // no transposition through it.
 //
 // A wave takes context tiles of its own with a softmax state of its own; the waves of a
-// workgroup and then the S splits of the context are merged at the end.
+// workgroup and then the workgroups that share a kv head's context (Share, below) are merged
+// at the end.
 //   S^T = K Q^T   (16 keys x 16 rows x 32 dims, v_mfma 16x16x32): lane (m = lane % 16, qd =
 //                 lane / 16) supplies key m's dims, and gets the scores of query row m with
 //                 keys 4 qd + i of the 16.  The keys of a tile are dealt to the 16-key groups
@@ -18,7 +19,7 @@
 // Product t of the eight covers dims 8 m + t; a lane's sums are dims 32 qd + 8 i + t.
 //
 // The weights enter the product as a sum of two 16-bit numbers (the matrix cores are idle
-// most of the time here), so their rounding does not add to the output's; sums are fp32.
+// most of the time here), off by the square of half a step; sums are fp32.
 // The running maximum is only raised when a score exceeds it by 2^kLazy.
 #include "i4_ctx.h"
 

@@ -13,7 +13,8 @@
 // LDS read; an 8-bit value block is [dim][token] already and is stored that way, converted,
 // its tokens in the order of the product's k index.
 // LDS rows are 256 bytes (K, 16-bit V) or 128 (8-bit V); 16-byte chunk c of row r lies at
-// c ^ f(r), so that neither read has bank conflicts.
+// c ^ f(r), so that the rows of a read spread over the banks.  Conflicts are left all the same:
+// a third of the cycles in which LDS is active (18.3 of 55.0 million for a 6001-token prompt).
 #include "i4_ctx.h"
 
 namespace i4 {
@@ -148,7 +149,12 @@ __device__ inline void tile_max(TileAcc& acc, const f32x16 (&s)[2], float c) {
     for (int t = 0; t < 4; ++t) acc.o[t] *= f;
   }
 }
-// the weights of 16 keys (step ks of the tile's four) as the product's operand
+// The weights of 16 keys (step ks of the tile's four) as the product's operand: one 16-bit number
+// each.  A second one for what the rounding leaves, as the kernel for few rows has, would make
+// the second product twice as long here, where the matrix cores are the bound.  With the sum of
+// the rounded weights the error against 64 bits is that of weights and values in fp32 to within
+// 2 % where a row sees many keys (relative 0.0017 in bf16 either way, most of it the output's
+// own rounding) and 1.2 times it where a window holds few.
 template <int PT> __device__ inline u32x4 weights16(const f32x16 (&s)[2], int ks) {
   const f32x16& x = s[ks >> 1];
   const int o = 8 * (ks & 1);

@@ -48,8 +48,9 @@ template <int XT> __device__ inline void widen8(u32x4 x, float (&f)[8]) {
 // workgroup does the last, unfinished block too, behind its own.
 // Thread t holds dims 8 (t % 16) .. + 7 of tokens 4 (t / 16) .. + 3: whole rows in a wave's
 // loads; a key row's 8 bytes are stored as they are, four tokens of a value dim make a word,
-// which LDS brings into rows.  Bound by the divisions (about 10 instructions an element) for
-// prompts: 4001 tokens of four heads take 8 us.
+// which LDS brings into rows.  4001 tokens of four heads take 8 us, for 2.6 of bytes and some 1
+// of quotients (10 instructions an element): two workgroups a CU, each a chain of its own of
+// loads, maximum, barrier, quotients, LDS and stores, do not hide each other's waits.
 template <int XT, int FMT>
 __global__ __launch_bounds__(256) void k_kv8_append(const uint16_t* __restrict__ k,
                                                     const uint16_t* __restrict__ v, int64_t bs,

@@ -20,7 +20,8 @@ B elements, optional) says how many of the T tokens each sequence has; the rest 
 whose output rows are left as they are.  A device position outside the cache writes nothing
 to it and NaN to the token's output row; an int is refused.
 
-Every op enqueues on torch's current stream of the tensors' device and never synchronises.
+Every op enqueues on torch's current stream of the tensors' device and does not synchronise,
+with one exception: an inv_freq that is on the device is copied to the host, which waits.
 """
 from __future__ import annotations
 
@@ -139,7 +140,9 @@ def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torc
     the rotated queries [T, n_heads, head_dim] (or [B, T, ...]) and writes each token's
     rotated key and its value to the caches ([n_kv_heads, max_len, head_dim] or [B, ...]):
     at the row of its position, or at first_row + t when first_row is given.  inv_freq is the
-    host fp32 table [head_dim / 2].  fp32 inside, rounded once (i4_rope_append)."""
+    host fp32 table [head_dim / 2].  fp32 inside, rounded once (i4_rope_append); attn_decode
+    and the other one-token entries round the norm, the sines and each product to the dtype, as
+    the model's own code does, so their keys differ from these by several half steps."""
     dev = _lib.require_device(qkv, q_norm_w, k_norm_w, k_cache, v_cache, counts, out)
     x = _batched(qkv, 3, "qkv")
     cc = _cache_c(k_cache, v_cache)
@@ -217,7 +220,9 @@ def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     pos + t over caches [n_kv_heads, max_len, head_dim] (or [B, ...]) that hold the tokens up
     to and including theirs (rope_append): softmax(scale q k^T) v over the positions j <= p
     and, with a window, j > p - window or j < sinks.  scale defaults to head_dim ** -0.5.
-    fp32 inside, rounded once to the activation dtype (i4_attn_window)."""
+    Scores, maxima and sums are fp32 and the output is rounded once; the weights are rounded
+    on their way into the second product: to a sum of two numbers of the activation dtype for
+    up to 16 rows of a kv head (T n_heads / n_kv_heads), to one for more (i4_attn_window)."""
     dev = _lib.require_device(q, k_cache, v_cache, counts, out)
     cc = _cache_c(k_cache, v_cache)
     return _attend(_lib.lib().i4_attn_window, cc, cc.max_len, q, dev, pos, window, sinks, scale,
