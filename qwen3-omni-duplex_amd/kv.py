@@ -109,17 +109,17 @@ _STREAM_WS: dict = {}
 KEPT_BYTES = 1 << 25
 
 
-def _scratch(workspace: Workspace | None, need: int,
-             dev: torch.device) -> tuple[torch.Tensor, torch.Tensor | None]:
+def _scratch(workspace: Workspace | None, need: int, dev: torch.device,
+             current: bool = False) -> tuple[torch.Tensor, torch.Tensor | None]:
     """`need` bytes and the counters: of the caller's workspace, else of one per stream, whose
     calls run in order; under capture one of the call's own, which the graph then owns.  More
     than KEPT_BYTES are the call's own throughout (stream ordered, without counters: only calls
     of few rows count).  The caller holds them until its call is queued (another thread's may
-    grow the workspace)."""
+    grow the workspace).  current: dev is the current device, which need not be asked again."""
     if need > KEPT_BYTES:
         return torch.empty(need, dtype=torch.uint8, device=dev), None
     if workspace is None:
-        if _capturing(dev):
+        if torch.cuda.is_current_stream_capturing() if current else _capturing(dev):
             workspace = Workspace()
         else:
             key = (dev.index, _lib.stream(dev))
@@ -200,14 +200,19 @@ def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
     on_dev = isinstance(pos, torch.Tensor)
     pd, ph = (_int32(pos, B, dev, "pos"), 0) if on_dev else (None, _host_pos(pos, T, keys))
     w = 0 if window is None else min(window, 2**31 - 1)
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _attend(entry, cc, keys, q, dev, pos, window, sinks, scale, counts, y, workspace)
     need = _lib.lib().i4_attn_window_workspace_bytes(
         B, T, nh, cc.n_kv_heads, keys if on_dev else ph + T, w, sinks)
-    ws, counters = _scratch(workspace, need, dev) if need else (None, None)
+    ws, counters = _scratch(workspace, need, dev, True) if need else (None, None)
     s0, s1, s2, _ = x.stride()
-    _call(dev, entry, x.data_ptr(), _lib.half_code(x.dtype), T, s0, s1, s2, nh, ctypes.byref(cc),
-          pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
-          hd ** -0.5 if scale is None else scale, y.data_ptr(), _lib.ptr(ws), need,
-          _lib.ptr(counters))
+    rc = entry(x.data_ptr(), _lib.half_code(x.dtype), T, s0, s1, s2, nh, ctypes.byref(cc),
+               pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
+               hd ** -0.5 if scale is None else scale, y.data_ptr(), _lib.ptr(ws), need,
+               _lib.ptr(counters), _lib.stream(dev))
+    if rc:
+        _lib.check(rc)
     return y
 
 

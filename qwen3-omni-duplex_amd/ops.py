@@ -282,7 +282,8 @@ def _capturing(device: torch.device) -> bool:
     device's)."""
     if device.type != "cuda":
         return False
-    if device.index in (None, torch.cuda.current_device()):
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
         return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
