@@ -770,7 +770,8 @@ int    i4_kv8_values(const i4_kv8cache* cache, float* k_out, float* v_out, hipSt
  * has finished it, with a scale that later tokens have a part in: a prompt differs from its
  * tokens one by one by what 8 bits do to that block, and an infinity or a NaN in a later
  * token of the block makes the block, and the row, NaN.  Blocks whose values are below 2^-30
- * (fp16; bf16: 2^-80) of the largest block's of the call may be lost beside it.  Workspace: i4_attn_window_workspace_bytes, keys =
+ * (fp16; bf16: 2^-80) of the largest block's of the call may be lost beside it.  Workspace:
+ * i4_attn_window_workspace_bytes, keys =
  * pos + T, or 64 blocks for a device position. */
 int    i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    int64_t q_token_stride, int64_t q_head_stride, int n_heads,

@@ -223,7 +223,8 @@ __device__ inline void scores8(const Block8& x, const u32x4 (&q)[4], f32x4 (&s)[
 // The weights take the values' scale; both enter the product as bf16, whose range holds any
 // scale: bf16's weights of at most 1 times up to 2^121, fp16's of 2^15 times up to 2^10.  Below
 // 2^-133 a product is lost, 2^-125 of the largest weight: with the smallest scale, 2^-109, that
-// is an output off by up to 2^-117 a position.  A block with scale NaN is NaN for the rows that see one of its keys.
+// is an output off by up to 2^-117 a position.  A block with scale NaN is NaN for the rows
+// that see one of its keys.
 template <int FMT>
 __device__ inline void values8(RowAcc& acc, const Block8& x, f32x4 (&s)[4], bool partial, int key0,
                                int p, const Bounds& w) {

@@ -85,7 +85,7 @@ def test_append_quotients_that_underflow(pkg, dev, kind):
 @pytest.mark.parametrize("dtype", DTS)
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("T,nh,n,more", [(1, 4, 20, 6), (6, 4, 20, 6), (130, 2, 20, 6),
-                                         (50, 4, 6, 0)])  # the last: one split
+                                         (50, 4, 6, 0), (50, 4, 5, 0)])  # the last: one split
 def test_zero_block_behind_large_blocks(pkg, dev, dtype, kind, T, nh, n, more):
     """n blocks of scales up to 1 with a sum that grows along the context, then a block of
     zeros, then ordinary ones."""
