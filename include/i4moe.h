@@ -781,6 +781,94 @@ int    i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                    hipStream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Many sessions on one key/value cache: rotary embeddings of any model, a cache in pages, and
+ * attention over it.  No counterpart in the reference beyond the attention itself.  B, T,
+ * pos_dev, pos and counts are as above (of a sequence whose pos_dev is outside the cache, every
+ * token is). */
+
+/* A rotary embedding: pair i < pairs of a head's first 2 pairs dims turns by the angle
+ * p inv_freq[i] (finite, at most 16), and cos and sin are multiplied by factor (the attention factor of tables that
+ * were scaled for long contexts; 1 otherwise); dims behind them stay as they are.  axes (host,
+ * nullable): which of the positions that a token is given pair i turns by (images and video);
+ * a token with one position turns all pairs by it. */
+#define I4_ROPE_HALF        0   /* pair i: dims i and i + pairs     */
+#define I4_ROPE_INTERLEAVED 1   /* pair i: dims 2 i and 2 i + 1     */
+#define I4_ROPE_MAX_PAIRS   128
+typedef struct i4_rotary {
+  const float*   inv_freq;   /* host [pairs] */
+  const uint8_t* axes;       /* host [pairs], each < turn->axes where that is more than 1 */
+  float   factor;
+  int32_t pairs;             /* 1 .. I4_ROPE_MAX_PAIRS */
+  int32_t layout;            /* I4_ROPE_* */
+} i4_rotary;
+
+/* Positions given for each token: int32 [axes][B][T] on the device (strides in elements, tokens
+ * adjacent), for angles alone; several axes need rotary->axes.  |position| < 2^24; one outside
+ * makes the token's rows NaN.  Negative ones turn back. */
+typedef struct i4_turn {
+  const int32_t* pos;
+  int64_t axis_stride, batch_stride;
+  int32_t axes;              /* 1 .. 4 */
+} i4_turn;
+
+/* Rows of heads that a rotation reads and writes: token t, head h of sequence b at
+ * x + b xb + t xt + h xh (elements), and y likewise; y is x itself (the same strides: in place)
+ * or does not overlap it. */
+typedef struct i4_heads {
+  const void* x;
+  void*       y;
+  int64_t xb, xt, xh, yb, yt, yh;
+  int32_t heads;
+} i4_heads;
+
+/* The rotary embedding of the heads in q and, if given, k, in fp32 and rounded once.  head_dim
+ * even, 2 pairs <= head_dim <= 256, heads <= 1024.  Positions: turn, or (turn NULL) pos + t as
+ * above, each within (-2^24, 2^24).  Rows at any alignment of their elements (16-byte rows are
+ * fastest). */
+int    i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B, int T, int head_dim,
+               const i4_rotary* rotary, const int32_t* pos_dev, int pos, const i4_turn* turn,
+               const int32_t* counts, hipStream_t stream);
+
+/* A 16-bit cache in pages: position j of sequence b is row j % page of page
+ * table[b][j / page], k and v [pages][n_kv_heads][page][head_dim] with strides in elements (the
+ * same for k and v, any order; the page head_dim values of a head's page adjacent, 16-byte
+ * aligned).  Entries that no visible position needs are not used and may hold anything.  An
+ * entry outside [0, pages) where one is needed is never followed: the append writes nothing and
+ * gives a NaN row, the attention a NaN row to the queries that see such a position.  Several
+ * sequences may hold a page; who appends to one holds it alone.  head_dim == 128, page a power
+ * of two from 16 to 1024, table_len page <= 2^20. */
+typedef struct i4_pagedcache {
+  void*   k;
+  void*   v;
+  const int32_t* table;      /* [batch][table_len], device */
+  int64_t page_stride, head_stride, table_stride;
+  int32_t batch, n_kv_heads, pages, page, table_len, head_dim;
+  int32_t dtype;             /* I4_F16 / I4_BF16 */
+} i4_pagedcache;
+
+/* i4_rope_append into pages, with any rotary embedding of head_dim 128 (I4_ROPE_HALF: pairs a
+ * multiple of 8, at most 64): the fused rows qkv [n_heads + 2 n_kv_heads][128] of token t of
+ * sequence b at qkv + b batch_stride + t token_stride; the queries' and keys' RMSNorm where
+ * q_norm_w / k_norm_w are given (nullable, each on its own); rotated queries to q_out
+ * [B][T][n_heads][128], rotated keys and values to the pages of positions pos + t.  turn
+ * (nullable): the angles' positions, where they are not pos + t.  fp32 inside, rounded once. */
+int    i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batch_stride,
+                       int64_t token_stride, int n_heads, const void* q_norm_w,
+                       const void* k_norm_w, float eps, const i4_rotary* rotary,
+                       const int32_t* pos_dev, int pos, const i4_turn* turn,
+                       const int32_t* counts, void* q_out, const i4_pagedcache* cache,
+                       hipStream_t stream);
+
+/* i4_attn_window over pages.  Workspace: i4_attn_window_workspace_bytes, keys = pos + T, or
+ * table_len page for a device position. */
+int    i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
+                     int64_t q_token_stride, int64_t q_head_stride, int n_heads,
+                     const i4_pagedcache* cache, const int32_t* pos_dev, int pos,
+                     const int32_t* counts, int window, int sinks, float scale, void* out,
+                     void* workspace, size_t workspace_bytes, int32_t* counters,
+                     hipStream_t stream);
+
+/* ------------------------------------------------------------------------
  * No counterpart in the reference.  For callers that cannot allocate device
  * memory (code under hipGraph capture, tight serving loops, harnesses that
  * forbid hipMalloc): i4_moe_forward with its workspace taken from a static

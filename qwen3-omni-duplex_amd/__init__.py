@@ -11,6 +11,8 @@ Drop-in replacements for thecodacus/qwen3-omni-duplex's quantized compute:
                             (clock.py:164-172): attention with KV cache + MoE per layer
   attn_window, attn_kv8  <- the same attention for prompt chunks and several sessions, under
                             a sliding window, over a 16-bit or an 8-bit cache (kv.py)
+  paged_append, attn_paged <- the same for many sessions on one pool of pages (paged.py)
+  rope                   <- rotary embeddings of either pairing, part of a head, several axes
   FusedMoE               <- src/duplex/streaming/fused_moe.py:40 (16-bit / int8
                             experts + gated shared expert: the Talker's block)
   fuse_moe_blocks        <- fused_moe.py:144
@@ -34,6 +36,8 @@ from .ops import (dequant, dequant_gemv, linear, moe_down_combine, moe_down_wait
                   thinker_layer_fits, thinker_layer_c, thinker_decode_step, dmoe_forward,
                   dmoe_status, dmoe_down_wait, StackLayerX)
 from .kv import KV8Cache, attn_kv8, attn_window, kv8_append, rope_append
+from .paged import PagedCache, attn_paged, paged_append
+from .rotary import Rotary, rope
 from .weights import QWeight, repack_awq_to_ct, repack_tile
 
 lib = _lib.lib
@@ -54,4 +58,5 @@ __all__ = [
     "FusedMoE", "fuse_moe_blocks", "quantize_q8", "dmoe_forward", "dmoe_status",
     "dmoe_down_wait", "StackLayerX",
     "KV8Cache", "attn_kv8", "attn_window", "kv8_append", "rope_append",
+    "PagedCache", "paged_append", "attn_paged", "Rotary", "rope",
 ]

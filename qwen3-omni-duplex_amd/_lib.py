@@ -93,6 +93,37 @@ class KV8CacheC(ctypes.Structure):
                 ("dtype", c_int32), ("format", c_int32)]
 
 
+class RotaryC(ctypes.Structure):
+    """struct i4_rotary"""
+
+    _fields_ = [("inv_freq", c_void_p), ("axes", c_void_p), ("factor", ctypes.c_float),
+                ("pairs", c_int32), ("layout", c_int32)]
+
+
+class TurnC(ctypes.Structure):
+    """struct i4_turn"""
+
+    _fields_ = [("pos", c_void_p), ("axis_stride", c_int64), ("batch_stride", c_int64),
+                ("axes", c_int32)]
+
+
+class HeadsC(ctypes.Structure):
+    """struct i4_heads"""
+
+    _fields_ = [("x", c_void_p), ("y", c_void_p), ("xb", c_int64), ("xt", c_int64),
+                ("xh", c_int64), ("yb", c_int64), ("yt", c_int64), ("yh", c_int64),
+                ("heads", c_int32)]
+
+
+class PagedCacheC(ctypes.Structure):
+    """struct i4_pagedcache"""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("table", c_void_p), ("page_stride", c_int64),
+                ("head_stride", c_int64), ("table_stride", c_int64), ("batch", c_int32),
+                ("n_kv_heads", c_int32), ("pages", c_int32), ("page", c_int32),
+                ("table_len", c_int32), ("head_dim", c_int32), ("dtype", c_int32)]
+
+
 # name -> (restype, argtypes); every function declared in include/i4moe.h
 SIGNATURES = {
     "i4_abi_version": (c_int, []),
@@ -195,6 +226,15 @@ SIGNATURES = {
     "i4_attn_kv8": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
                             POINTER(KV8CacheC), c_void_p, c_int, c_void_p, c_int, c_int,
                             ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "i4_rope": (c_int, [POINTER(HeadsC), POINTER(HeadsC), c_int, c_int, c_int, c_int,
+                        POINTER(RotaryC), c_void_p, c_int, POINTER(TurnC), c_void_p, c_void_p]),
+    "i4_paged_append": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int, c_void_p,
+                                c_void_p, ctypes.c_float, POINTER(RotaryC), c_void_p, c_int,
+                                POINTER(TurnC), c_void_p, c_void_p, POINTER(PagedCacheC),
+                                c_void_p]),
+    "i4_attn_paged": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
+                              POINTER(PagedCacheC), c_void_p, c_int, c_void_p, c_int, c_int,
+                              ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "i4_dmoe_forward": (c_int, [c_void_p, c_int, c_int, POINTER(DmoeWeightsC), c_int, c_int,
                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                 c_size_t, c_void_p]),

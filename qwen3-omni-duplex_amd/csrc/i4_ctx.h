@@ -37,7 +37,12 @@ struct CtxArgs {
   float* part;            // [B nkv R][S] or [wgs][rows], [128] sums of e v each, then
   float* ml;              // [2] each: maximum and sum
   int32_t* counters;      // nullable: parts of a kv head that are done, 0 between calls
+  Pages pg;               // the 16-bit cache in pages
 };
+
+// What a kernel reads: FMT is I4_KV8_* or one of these.
+static constexpr int kDense = -1;  // the 16-bit cache c
+static constexpr int kPaged = -2;  // the pages pg
 
 // All of the arguments' cache lines asked for at once, at a kernel's start: the compiler
 // loads each group of them where it is used, and every such load is a trip to host memory.
@@ -176,6 +181,6 @@ template <int XT> __device__ inline u32 finite_pair(u32 x) {
 
 }  // namespace i4
 
-// i4_ctx_rows.hip / i4_ctx_tile.hip; fmt: -1 (16-bit cache) or I4_KV8_*
+// i4_ctx_rows.hip / i4_ctx_tile.hip; fmt: kDense, kPaged or I4_KV8_*
 int i4_launch_ctx_tile(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s);
 int i4_launch_ctx_rows(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s);

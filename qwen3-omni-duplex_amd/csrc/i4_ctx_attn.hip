@@ -1,6 +1,6 @@
 // Attention over a conversation's cached context: B x T queries over a 16-bit cache
-// (i4_attn_window) or an 8-bit one (i4_attn_kv8), under an optional sliding window whose
-// first tokens stay visible.
+// (i4_attn_window), one in pages (i4_attn_paged) or an 8-bit one (i4_attn_kv8), under an optional
+// sliding window whose first tokens stay visible.
 //   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  s_j = scale q . k_j,
 // over the visible j in one pass, with a running maximum m and sum.
 #include "i4_ctx.h"
@@ -150,7 +150,7 @@ int i4_attn_window(const void* q, int x_dtype, int T, int64_t q_batch_stride,
   a.c = Cache16{(uint16_t*)cache->k, (uint16_t*)cache->v, cache->batch_stride,
                 cache->head_stride, cache->row_stride, cache->max_len};
   a.len = cache->max_len;
-  return launch(a, x_dtype, -1, keys, i4_span{window, sinks, workspace, counters}, stream);
+  return launch(a, x_dtype, kDense, keys, i4_span{window, sinks, workspace, counters}, stream);
 }
 
 int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64_t q_token_stride,
@@ -176,6 +176,30 @@ int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64
   a.len = len;
   return launch(a, x_dtype, cache->format, keys, i4_span{window, sinks, workspace, counters},
                 stream);
+}
+
+int i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
+                  int64_t q_token_stride, int64_t q_head_stride, int n_heads,
+                  const i4_pagedcache* cache, const int32_t* pos_dev, int pos,
+                  const int32_t* counts, int window, int sinks, float scale, void* out,
+                  void* workspace, size_t workspace_bytes, int32_t* counters,
+                  hipStream_t stream) {
+  using namespace i4;
+  int rc = i4_check_pagedcache(cache);
+  if (rc) return rc;
+  const int B = cache->batch, nkv = cache->n_kv_heads, len = cache->table_len * cache->page;
+  const int keys = call_keys(pos_dev, pos, T, len);
+  rc = query_check(q, x_dtype, cache->dtype, B, T, q_batch_stride, q_token_stride, q_head_stride,
+                   n_heads, nkv, pos_dev, pos, counts, len, window, sinks, scale, out, workspace,
+                   workspace_bytes,
+                   i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
+                   counters);
+  if (rc) return rc;
+  CtxArgs a = ctx_args(q, B, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
+                       pos, counts, window, sinks, scale, out);
+  a.pg = i4_pages_of(cache);
+  a.len = len;
+  return launch(a, x_dtype, kPaged, keys, i4_span{window, sinks, workspace, counters}, stream);
 }
 
 }  // extern "C"

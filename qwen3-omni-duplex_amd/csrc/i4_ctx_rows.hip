@@ -117,6 +117,36 @@ __device__ inline void load_v16(Half16& h, rsrc_t vr, int row0, u32 stride, int 
     h.v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, (u32)(row0 + 8 * qd + j) * stride + 16u * m,
                                                    0, kStream);
 }
+// the same of 32 positions in pages, 16 of them at a and 16 at b; rows past the last one that a
+// query sees hold anything
+__device__ inline void load_k16(Half16& h, const void* k, const PageRows& a, const PageRows& b,
+                                int m, int qd) {
+  const char* row = (const char*)k + (m & 8 ? b.at : a.at) + (8 * ((m >> 2) & 1) + (m & 3)) * 256 +
+                    16 * qd;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) h.k[t][c] = ldg16(row + 1024 * t + 64 * c);
+}
+__device__ inline void load_v16(Half16& h, const void* v, const PageRows& a, const PageRows& b,
+                                int m, int qd) {
+  const char* row = (const char*)v + (qd & 2 ? b.at : a.at) + (qd & 1) * 2048 + 16 * m;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    h.v[j] = __builtin_nontemporal_load((const u32x4*)(row + 256 * j));
+}
+// where a page is missing: keys of NaN, so that the rows that see one are NaN, and values of 0
+template <int XT>
+__device__ inline void poison16(Half16& h, const PageRows& a, const PageRows& b, int m, int qd) {
+  if (m & 8 ? b.bad : a.bad)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) h.k[t][c] = u32x4{} + (u32)Half<XT>::QNAN * 0x10001u;
+  if (qd & 2 ? b.bad : a.bad)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) h.v[j] = u32x4{};
+}
 template <int XT>
 __device__ inline void scores16(const Half16& h, const u32x4 (&q)[4], f32x4 (&s)[2]) {
 #pragma unroll
@@ -130,10 +160,10 @@ __device__ inline void scores16(const Half16& h, const u32x4 (&q)[4], f32x4 (&s)
 // Values that a row does not see must not reach it (0 times an infinity is NaN): before the
 // product of a tile that is not seen in full, the values of keys that no row sees are
 // cleared; where rows differ, infinities and NaN are taken out and added to the rows that
-// see them.
-template <int XT>
-__device__ inline void clean16(RowAcc& acc, Half16& h, rsrc_t vr, int row0, u32 stride, int key0,
-                               int m, int qd, int plo, int phi, int p, const Bounds& w) {
+// see them.  value(j, at): 16 bytes at byte `at` of key j's values.
+template <int XT, class Value>
+__device__ inline void clean16(RowAcc& acc, Half16& h, Value value, int key0, int m, int qd,
+                               int plo, int phi, int p, const Bounds& w) {
   bool bad = false;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -157,8 +187,7 @@ __device__ inline void clean16(RowAcc& acc, Half16& h, rsrc_t vr, int row0, u32 
     const bool see = sees(w, p, key0 + j);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {  // dims 32 qd + 8 i + t
-      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(
-          vr, (u32)(row0 + j) * stride + 64u * qd + 16u * i, 0, 0);
+      const u32x4 x = value(j, 64u * qd + 16u * i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float a = lo_f32<XT>(x[e]), b = hi_f32<XT>(x[e]);
@@ -423,7 +452,44 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
     // this workgroup's tiles, dealt to its waves in turn
     const int each = udiv(ct.n, parts), more = ct.n - each * parts;
     const int i0 = split * each + min(split, more), i1 = i0 + each + (split < more ? 1 : 0);
-    if constexpr (FMT < 0) {
+    if constexpr (FMT == kPaged) {
+      const int32_t* table = a.pg.table + b * a.pg.ts;
+      Half16 h;
+      // halves of 32 positions as below; the pages of the half after the next are looked up
+      // while the next one's rows are loaded
+      const int e = 2 * i1;
+      int x = 2 * i0 + __builtin_amdgcn_readfirstlane(wave);
+      auto pos0 = [&](int y) { return 64 * ct.at(y >> 1) + 32 * (y & 1); };
+      // positions behind the last row's own may have no page: that row's serves for them
+      auto rows_at = [&](int j) { return page_rows(a.pg, table, g, min(j, phi) & ~15); };
+      PageRows c0{}, c1{}, n0{}, n1{};
+      if (x < e) {
+        const int j = pos0(x);
+        c0 = rows_at(j), c1 = rows_at(j + 16);
+        load_k16(h, a.pg.k, c0, c1, m, qd);
+        load_v16(h, a.pg.v, c0, c1, m, qd);
+        const int jn = pos0(min(x + 4, e - 1));
+        n0 = rows_at(jn), n1 = rows_at(jn + 16);
+      }
+      for (; x < e; x += 4) {
+        const int j0 = pos0(x);
+        const bool partial = !all_see(a.w, plo, phi, j0, 32);
+        if (c0.bad || c1.bad) poison16<XT>(h, c0, c1, m, qd);
+        f32x4 s[2];
+        scores16<XT>(h, q, s);
+        if (x + 4 < e) load_k16(h, a.pg.k, n0, n1, m, qd);
+        weights<XT, 2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
+        if (partial)
+          clean16<XT>(acc, h, [&](int j, u32 at) {
+            return ldg16((const char*)a.pg.v + (j & 16 ? c1.at : c0.at) + (j & 15) * 256 + at);
+          }, j0, m, qd, plo, phi, p, a.w);
+        values16<XT>(acc, h, s);
+        if (x + 4 < e) load_v16(h, a.pg.v, n0, n1, m, qd);
+        c0 = n0, c1 = n1;
+        const int jn = pos0(min(x + 8, e - 1));
+        n0 = rows_at(jn), n1 = rows_at(jn + 16);
+      }
+    } else if constexpr (FMT == kDense) {
       const u32 stride = (u32)a.c.rs * 2u, bytes = (u32)phi * stride + KHD * 2u;
       const int64_t base = b * a.c.bs + g * a.c.hs;
       const rsrc_t kr = rsrc(a.c.k + base, bytes), vr = rsrc(a.c.v + base, bytes);
@@ -444,7 +510,10 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
         const int jn = pos0(min(x + 4, e - 1));
         if (x + 4 < e) load_k16(h, kr, jn, stride, m, qd);
         weights<XT, 2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
-        if (partial) clean16<XT>(acc, h, vr, j0, stride, j0, m, qd, plo, phi, p, a.w);
+        if (partial)
+          clean16<XT>(acc, h, [&](int j, u32 at) {
+            return __builtin_amdgcn_raw_buffer_load_b128(vr, (u32)(j0 + j) * stride + at, 0, 0);
+          }, j0, m, qd, plo, phi, p, a.w);
         values16<XT>(acc, h, s);
         if (x + 4 < e) load_v16(h, vr, jn, stride, m, qd);
       }
@@ -488,7 +557,9 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
           f32x4 s[2];
           scores16<XT>(h, qn, s);
           weights<XT, 2>(acc, s, a.c2, true, j0 + 8 * qd, p, a.w);
-          clean16<XT>(acc, h, vr, row0, stride, j0, m, qd, plo, phi, p, a.w);
+          clean16<XT>(acc, h, [&](int j, u32 at) {
+            return __builtin_amdgcn_raw_buffer_load_b128(vr, (u32)(row0 + j) * stride + at, 0, 0);
+          }, j0, m, qd, plo, phi, p, a.w);
           values16<XT>(acc, h, s);
         }
       }
@@ -577,11 +648,13 @@ template <int XT, int FMT> static void rows_go(const CtxArgs& a, hipStream_t s) 
 int i4_launch_ctx_rows(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s) {
   using namespace i4;
   if (xt == I4_F16) {
-    if (fmt < 0) rows_go<I4_F16, -1>(a, s);
+    if (fmt == kDense) rows_go<I4_F16, kDense>(a, s);
+    else if (fmt == kPaged) rows_go<I4_F16, kPaged>(a, s);
     else if (fmt == I4_KV8_INT8) rows_go<I4_F16, I4_KV8_INT8>(a, s);
     else rows_go<I4_F16, I4_KV8_E4M3>(a, s);
   } else {
-    if (fmt < 0) rows_go<I4_BF16, -1>(a, s);
+    if (fmt == kDense) rows_go<I4_BF16, kDense>(a, s);
+    else if (fmt == kPaged) rows_go<I4_BF16, kPaged>(a, s);
     else if (fmt == I4_KV8_INT8) rows_go<I4_BF16, I4_KV8_INT8>(a, s);
     else rows_go<I4_BF16, I4_KV8_E4M3>(a, s);
   }

@@ -84,6 +84,28 @@ __device__ inline void stage16(uint64_t k, uint64_t v, int j0, int last, u32 str
   }
 }
 
+// The same from pages: this wave's 16 rows, which lie in one page (u), from position j on.  A
+// missing page's keys are NaN, so that the rows that see one are NaN, and its values 0.
+template <int XT>
+__device__ inline void stage_pages(const Pages& pg, const PageRows& u, int j, int last, u32 lds,
+                                   int wave, int lane) {
+  const int r4 = lane >> 4, c = lane & 15;
+  const uint64_t k = uniform((const char*)pg.k + u.at), v = uniform((const char*)pg.v + u.at);
+  const int most = last - min(j, last & ~15);  // the last row that anything sees
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const u32 row = (u32)min(4 * i + r4, most) * (KHD * 2u);
+    const u32 dst = lds + 1024u * (4 * wave + i);
+    if (u.bad) {
+      lds_put((lds_t*)(uintptr_t)(dst + 16u * lane), u32x4{} + (u32)Half<XT>::QNAN * 0x10001u);
+      lds_put((lds_t*)(uintptr_t)(dst + TBYTES + 16u * lane), u32x4{});
+    } else {
+      load_lds16(k, row + 16u * (c ^ (4 * i + r4)), dst);
+      load_lds16(v, row + 16u * (c ^ ((4 * (i & 1) + r4) << 1)), dst + TBYTES);
+    }
+  }
+}
+
 // While a wave is among its products it goes before the other one of its SIMD (s_setprio),
 // whose vector work fits in between: 293 -> 291 us for a 6001-token prompt, 228 -> 226 for a
 // 5000-token one over 8 bits.
@@ -258,13 +280,13 @@ template <int XT> __device__ inline bool clear_not_finite(lds_t* v, int tid) {
   return bad;
 }
 // and added to the rows that see them when all tiles are done: whatever they meet, they stay.
-// v: the rows of the tile at position j0, of which `rows` exist
-template <int XT>
-__device__ inline void add_not_finite(TileAcc& acc, const uint16_t* v, u32 stride, int rows,
-                                      int j0, int p, int h, const Bounds& w) {
+// row(key): the values of a key of the tile at position j0, of which `rows` exist
+template <int XT, class Row>
+__device__ inline void add_not_finite(TileAcc& acc, Row row, int rows, int j0, int p, int h,
+                                      const Bounds& w) {
   for (int key = 0; key < rows; ++key) {
     const bool see = sees(w, p, j0 + key);
-    const char* r = (const char*)v + (int64_t)key * stride + 8 * h;
+    const char* r = row(key) + 8 * h;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -391,7 +413,38 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       acc.l += tile_weights<XT>(acc, s, a.c2, kLift<XT>);
       tile_values16<XT>(acc, s, buf + TBYTES, lane);
     };
-    if constexpr (FMT < 0) {
+    if constexpr (FMT == kPaged) {
+      const int32_t* table = a.pg.table + b * a.pg.ts;
+      // this wave's 16 positions of tile i; behind the last row's own, that row's
+      auto rows_at = [&](int i) {
+        return page_rows(a.pg, table, g, min(64 * ct.at(i) + 16 * wave, phi) & ~15);
+      };
+      PageRows next{};  // looked up a tile before its rows are loaded
+      if (i0 < i1) {
+        stage_pages<XT>(a.pg, rows_at(i0), 64 * ct.at(i0) + 16 * wave, phi, lds0, wave, lane);
+        next = rows_at(min(i0 + 1, i1 - 1));
+      }
+      for (int i = i0; i < i1; ++i) {
+        const int cur = (i - i0) & 1;
+        wait_loads();
+        __syncthreads();  // the tile is here, and its other half is free
+        if (i + 1 < i1) {
+          stage_pages<XT>(a.pg, next, 64 * ct.at(i + 1) + 16 * wave, phi,
+                          lds0 + (cur ^ 1) * 2 * TBYTES, wave, lane);
+          next = rows_at(min(i + 2, i1 - 1));
+        }
+        attend16(lds + cur * 2 * TBYTES, 64 * ct.at(i), !whole(i));
+      }
+      if (bad)
+        for (int i = i0; i < i1; ++i) {
+          const int j0 = 64 * ct.at(i);
+          if (!whole(i))
+            add_not_finite<XT>(acc, [&](int key) {
+              const int j = __builtin_amdgcn_readfirstlane(j0 + key);
+              return (const char*)a.pg.v + page_rows(a.pg, table, g, j & ~15).at + (j & 15) * 256;
+            }, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
+        }
+    } else if constexpr (FMT == kDense) {
       const u32 stride = (u32)a.c.rs * 2u;
       const uint16_t* k = a.c.k + b * a.c.bs + g * a.c.hs;
       const uint16_t* v = a.c.v + b * a.c.bs + g * a.c.hs;
@@ -410,8 +463,9 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
         for (int i = i0; i < i1; ++i) {
           const int j0 = 64 * ct.at(i);
           if (!whole(i))
-            add_not_finite<XT>(acc, (const uint16_t*)((const char*)v + (int64_t)j0 * stride),
-                               stride, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
+            add_not_finite<XT>(acc, [&](int key) {
+              return (const char*)v + (int64_t)(j0 + key) * stride;
+            }, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
         }
     } else {
       const int end = sq.p0 + sq.fit, full = end / KBLK;  // finished blocks, then the tail
@@ -486,7 +540,9 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
         __syncthreads();
         attend16(lds, full * KBLK, true);
         if (bad)
-          add_not_finite<XT>(acc, a.c8.vt + at, KHD * 2u, rows, full * KBLK, p, h, a.w);
+          add_not_finite<XT>(acc, [&](int key) {
+            return (const char*)(a.c8.vt + at) + key * (KHD * 2);
+          }, rows, full * KBLK, p, h, a.w);
       }
     }
     if (mine) {
@@ -608,11 +664,13 @@ int i4_launch_ctx_tile(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s) {
   const dim3 grid((unsigned)(a.tiles * a.S * a.B * a.nkv));
   auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a); };
   if (xt == I4_F16) {
-    if (fmt < 0) go(k_ctx_tile<I4_F16, -1>);
+    if (fmt == kDense) go(k_ctx_tile<I4_F16, kDense>);
+    else if (fmt == kPaged) go(k_ctx_tile<I4_F16, kPaged>);
     else if (fmt == I4_KV8_INT8) go(k_ctx_tile<I4_F16, I4_KV8_INT8>);
     else go(k_ctx_tile<I4_F16, I4_KV8_E4M3>);
   } else {
-    if (fmt < 0) go(k_ctx_tile<I4_BF16, -1>);
+    if (fmt == kDense) go(k_ctx_tile<I4_BF16, kDense>);
+    else if (fmt == kPaged) go(k_ctx_tile<I4_BF16, kPaged>);
     else if (fmt == I4_KV8_INT8) go(k_ctx_tile<I4_BF16, I4_KV8_INT8>);
     else go(k_ctx_tile<I4_BF16, I4_KV8_E4M3>);
   }

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "i4_common.h"
+#include "i4_page.h"
 
 namespace i4 {
 
@@ -49,6 +50,21 @@ struct Cache8 {
   int32_t blocks;
 };
 
+// A 16-bit cache in pages: position j of sequence b is row j % page of page
+// table[b ts + j / page], a page 2^shift rows of KHD values a head.
+struct Pages {
+  uint16_t *k, *v;
+  const int32_t* table;
+  int64_t ps, hs, ts;  // strides of k and v in bytes, of the table in entries
+  int32_t pages, table_len, shift;
+};
+// where position j of a sequence lies for head g (row: its table); the same j in all lanes
+__device__ inline PageRows page_rows(const Pages& pg, const int32_t* row, int g, int j) {
+  // a scalar load: the table is not written while a kernel runs
+  const int id = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)row)[j >> pg.shift];
+  return page_rows_of(id, pg.pages, pg.ps, pg.hs, pg.shift, KHD * 2, g, j);
+}
+
 // A block's scale from what is stored: at least the smallest that the append writes, so that
 // nothing is divided by a scale of 0 (an empty cache's, or another quantiser's for a block of
 // zeros); NaN stays.  Taken where the scale is used, not where it is loaded: there it would
@@ -71,3 +87,5 @@ int i4_check_tokens(int B, int T, int n_heads, int n_kv_heads, const int32_t* po
                     const int32_t* counts, int limit);
 int i4_check_kvcache(const i4_kvcache* c);
 int i4_check_kv8cache(const i4_kv8cache* c);
+int i4_check_pagedcache(const i4_pagedcache* c);  // i4_pages.hip
+i4::Pages i4_pages_of(const i4_pagedcache* c);

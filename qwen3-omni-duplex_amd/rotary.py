@@ -1,0 +1,194 @@
+"""Rotary embeddings of any model's queries and keys.
+
+    Rotary   a rotation as the kernels take it: which dims pair, how fast each pair turns
+    rope     queries and keys turned by their positions
+
+rope_append (kv.py) turns the Thinker's heads by a plain table on their way into a cache; these
+take neighbouring pairs, part of a head, tables scaled for long contexts, positions given for
+each token, and the several positions of an image's or a video's tokens (the reference's model
+turns its pairs by three axes then: Qwen3OmniMoeThinkerTextRotaryEmbedding, transformers 5.15).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Sequence
+
+import torch
+
+from . import _lib
+from .kv import _batched, _call, _int32
+
+LAYOUTS = {"half": 0, "interleaved": 1}
+MAX_PAIRS = 128
+MAX_POS = 1 << 24
+
+
+class Rotary:
+    """Pair i of a head's first 2 len(inv_freq) dims turns by the angle position * inv_freq[i]:
+    dims i and i + len(inv_freq) (layout "half") or 2 i and 2 i + 1 ("interleaved").  factor
+    multiplies cos and sin (the attention factor of a scaled table).  axes: for tokens that are
+    given several positions, which of them each pair turns by.  The table is copied to the host."""
+
+    __slots__ = ("inv_freq", "layout", "factor", "axes", "_bytes", "_c")
+
+    def __init__(self, inv_freq: torch.Tensor, *, layout: str = "half", factor: float = 1.0,
+                 axes: Sequence[int] | None = None):
+        f = inv_freq.detach().to("cpu", torch.float32).clone().contiguous()
+        n = f.numel()
+        if f.dim() != 1 or not 1 <= n <= MAX_PAIRS:
+            raise RuntimeError(f"inv_freq holds 1 to {MAX_PAIRS} values, got {tuple(f.shape)}")
+        if not bool((f.abs() <= 16).all()):
+            raise RuntimeError("inverse frequencies are finite and at most 16")
+        if layout not in LAYOUTS:
+            raise RuntimeError(f"layout is one of {sorted(LAYOUTS)}, got {layout!r}")
+        if not math.isfinite(factor):
+            raise RuntimeError(f"factor is {factor}")
+        if axes is not None and (len(axes) != n or not all(0 <= a < 4 for a in axes)):
+            raise RuntimeError(f"axes: {n} numbers from 0 to 3")
+        self.inv_freq, self.layout, self.factor = f, layout, float(factor)
+        self.axes = None if axes is None else tuple(int(a) for a in axes)
+        self._bytes = None if axes is None else (ctypes.c_uint8 * n)(*self.axes)
+        self._c = _lib.RotaryC(f.data_ptr(), None if axes is None else
+                               ctypes.addressof(self._bytes), self.factor, n, LAYOUTS[layout])
+
+    @classmethod
+    def plain(cls, dims: int, theta: float, **kw) -> "Rotary":
+        """The default table of `dims` turning dims: theta ** (-2 i / dims)."""
+        return cls(1.0 / theta ** (torch.arange(0, dims, 2, dtype=torch.float) / dims), **kw)
+
+    @classmethod
+    def scaled(cls, dims: int, theta: float, scale: float, trained: int | None = None, *,
+               slow: float = 1.0, fast: float = 32.0, factor: float | None = None,
+               **kw) -> "Rotary":
+        """A table for contexts `scale` times as long as the model was trained for.
+
+        trained None: every position is divided by scale.  Else by parts (arXiv 2309.00071): a
+        pair that turns more than `fast` times within `trained` positions keeps its frequency,
+        one that turns less than `slow` times has it divided by scale, and those between are
+        blended by their number of turns; factor defaults to 0.1 ln(scale) + 1."""
+        if scale < 1 or not fast > slow:
+            raise RuntimeError("scale is at least 1, and fast above slow")
+        f = theta ** (-torch.arange(0, dims, 2, dtype=torch.double) / dims)
+        if trained is None:
+            f = f / scale
+        else:
+            keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+            f = f * keep + f / scale * (1 - keep)
+            factor = 0.1 * math.log(scale) + 1 if factor is None else factor
+        return cls(f.float(), factor=1.0 if factor is None else factor, **kw)
+
+    @property
+    def dims(self) -> int:
+        """How many dims of a head turn."""
+        return 2 * self.inv_freq.numel()
+
+    def __repr__(self) -> str:
+        return (f"Rotary(dims={self.dims}, layout={self.layout!r}, factor={self.factor}"
+                + (f", axes={self.axes}" if self.axes else "") + ")")
+
+
+def _turn_c(turn: torch.Tensor, rotary: Rotary, batched: bool, B: int, T: int,
+            dev: torch.device) -> _lib.TurnC:
+    """struct i4_turn of given positions [B, T] or [axes, B, T] ([T] or [axes, T] for tokens
+    without a batch)."""
+    t = turn if batched else turn.unsqueeze(-2) if turn.dim() else turn
+    shape = tuple(t.shape)
+    if shape[-2:] != (B, T) or len(shape) > 3:
+        raise RuntimeError(f"given positions {tuple(turn.shape)} for {B} x {T} tokens")
+    axes = shape[0] if len(shape) == 3 else 1
+    if axes > 1 and (axes > 4 or rotary.axes is None or max(rotary.axes) >= axes):
+        raise RuntimeError(f"positions on {axes} axes for a rotary embedding with "
+                           f"{'none' if rotary.axes is None else max(rotary.axes) + 1}")
+    if turn.dtype != torch.int32 or turn.device != dev or (T > 1 and t.stride(-1) != 1):
+        raise RuntimeError("given positions are int32 on the tensors' device, tokens adjacent")
+    return _lib.TurnC(turn.data_ptr(), t.stride(0) if axes > 1 else 0,
+                      t.stride(-2) if B > 1 else 0, axes)
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The first and last byte that a tensor covers."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() - 1
+
+
+def _heads_c(x: torch.Tensor, y: torch.Tensor) -> _lib.HeadsC:
+    a, b = x.stride(), y.stride()
+    return _lib.HeadsC(x.data_ptr(), y.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], x.shape[2])
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x as it is, or a copy where its rows are not dense or lie on each other."""
+    hd = x.shape[3]
+    return x if x.stride(3) == 1 and all(
+        n == 1 or s >= hd for n, s in zip(x.shape[:3], x.stride())) else x.contiguous()
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotary: Rotary, *,
+         counts: torch.Tensor | None = None,
+         out: tuple[torch.Tensor, torch.Tensor | None] | None = None):
+    """The rotary embedding of queries q [T, heads, head_dim] (or [B, T, ...]) and, if given, of
+    keys k with heads of their own: (q, k) turned, or q alone where k is None.  fp32 inside (the
+    angles as good as exact for every position within 2^24), rounded once (i4_rope).
+
+    pos: an int or int32 [B] on the device, the position of each sequence's first token; or the
+    positions of the tokens themselves, int32 [B, T] on the device, or [axes, B, T] for a rotary
+    embedding with axes ([T] or [axes, T] for tokens without a batch); with one position a token
+    every pair turns by it, as text tokens do.  Negative positions turn
+    back: rope(rope(x, p), -p) is x to rounding, and the gradient of rope(x, p) is that of its
+    output turned by -p.  A position at or behind +-2^24 gives NaN, an int is refused.  q and k
+    may have any strides above a dense last dimension, and so may out, a pair of tensors that
+    are q and k themselves (in place) or do not overlap them."""
+    dev = _lib.require_device(q, k, counts)
+    code = _lib.half_code(q.dtype)
+    x = _batched(q, 4, "q")
+    B, T, _, hd = x.shape
+    if k is not None and k.dtype != q.dtype:
+        raise RuntimeError("q and k must have one dtype")
+    xs = [x] if k is None else [x, _batched(k, 4, "k")]
+    if xs[-1].shape[:2] != x.shape[:2] or xs[-1].shape[3] != hd or k is not None \
+            and k.dim() != q.dim():
+        raise RuntimeError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
+    if out is None:
+        xs = [_rows(t) for t in xs]
+        make = torch.zeros if counts is not None else torch.empty
+        ys = [make(t.shape, dtype=t.dtype, device=dev) for t in xs]
+    else:
+        outs = [t for t in out if t is not None]
+        if len(outs) != len(xs):
+            raise RuntimeError("out holds a tensor for each input")
+        _lib.require_device(q, *outs)
+        ys = [_batched(t, 4, "out") for t in outs]
+        for y, x in zip(ys, xs):
+            if y.shape != x.shape or y.dtype != x.dtype or y.dim() != x.dim():
+                raise RuntimeError(f"out must be a {tuple(x.shape)} tensor of {x.dtype}")
+            if _rows(y) is not y:
+                raise RuntimeError("out's rows must be dense and lie apart")
+        for y, x in zip(ys, xs):
+            if y.data_ptr() == x.data_ptr() and y.stride() == x.stride():
+                continue
+            lo, hi = _span(y)
+            for z in xs:
+                a, b = _span(z)
+                if lo <= b and a <= hi:
+                    raise RuntimeError("out is its input itself or does not overlap the inputs")
+        xs = [x if x.data_ptr() == y.data_ptr() else _rows(x) for x, y in zip(xs, ys)]
+    if rotary.dims > hd:
+        raise RuntimeError(f"{rotary.dims} dims turn, the heads have {hd}")
+    turn = pd = None
+    ph = 0
+    if not isinstance(pos, torch.Tensor):
+        ph = int(pos)
+        if not -MAX_POS < ph <= MAX_POS - T:
+            raise RuntimeError(f"positions {ph} to {ph + T - 1} outside (-2^24, 2^24)")
+    elif pos.dim() == 1 and (q.dim() == 4 or pos.numel() == 1):
+        pd = _int32(pos, B, dev, "pos")
+    else:
+        turn = _turn_c(pos, rotary, q.dim() == 4, B, T, dev)
+    cs = [_heads_c(x, y) for x, y in zip(xs, ys)]
+    _call(dev, _lib.lib().i4_rope, cs[0], cs[1] if len(cs) > 1 else None, code, B, T, hd, rotary._c,
+          pd, ph, turn, _int32(counts, B, dev, "counts"))
+    if out is not None:
+        return out[0] if k is None else tuple(out)
+    ys = [y if q.dim() == 4 else y[0] for y in ys]
+    return ys[0] if k is None else tuple(ys)
