@@ -859,7 +859,7 @@ int    i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batch_stride
                        const int32_t* counts, void* q_out, const i4_pagedcache* cache,
                        hipStream_t stream);
 
-/* i4_attn_window over pages.  Workspace: i4_attn_window_workspace_bytes, keys = pos + T, or
+/* i4_attn_window over pages.  Workspace: i4_attn_paged_workspace_bytes, keys = pos + T, or
  * table_len page for a device position. */
 int    i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                      int64_t q_token_stride, int64_t q_head_stride, int n_heads,
@@ -867,6 +867,8 @@ int    i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                      const int32_t* counts, int window, int sinks, float scale, void* out,
                      void* workspace, size_t workspace_bytes, int32_t* counters,
                      hipStream_t stream);
+size_t i4_attn_paged_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
+                                     int window, int sinks);
 
 /* ------------------------------------------------------------------------
  * No counterpart in the reference.  For callers that cannot allocate device

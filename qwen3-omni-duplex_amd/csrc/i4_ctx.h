@@ -38,6 +38,28 @@ struct CtxArgs {
   float* ml;              // [2] each: maximum and sum
   int32_t* counters;      // nullable: parts of a kv head that are done, 0 between calls
   Pages pg;               // the 16-bit cache in pages
+  int32_t* plan;          // of a call whose tiles are shared out (k_ctx_tile), or null
+};
+
+// Row tiles up to which their context tiles are shared out; the plan of a call: the context
+// tiles before each row tile of one kv head ([0, M], M = B tiles), then the workgroups.
+static constexpr int kPlanned = 1024;
+
+// how many runs `total` tiles are cut into: at least four tiles each, as many on every XCD
+__host__ __device__ inline int64_t runs_of(int64_t total) {
+  const int64_t w = total / 4;
+  return w >= 512 ? 512 : w >= 8 ? w & ~7 : w > 1 ? w : 1;
+}
+// The context tiles of all row tiles as one list, kv head after kv head, cut into `wgs` runs of
+// the same length: run w has tiles [w total / wgs, (w + 1) total / wgs).
+struct Runs {
+  int64_t total;
+  int wgs;  // at most `total`, so that no run is empty
+  __host__ __device__ inline int64_t first(int w) const { return total * w / wgs; }
+  // the run that tile u is in
+  __host__ __device__ inline int of(int64_t u) const {
+    return (int)(((u + 1) * wgs - 1) / total);
+  }
 };
 
 // What a kernel reads: FMT is I4_KV8_* or one of these.
@@ -183,4 +205,5 @@ template <int XT> __device__ inline u32 finite_pair(u32 x) {
 
 // i4_ctx_rows.hip / i4_ctx_tile.hip; fmt: kDense, kPaged or I4_KV8_*
 int i4_launch_ctx_tile(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s);
+int i4_launch_ctx_shared(const i4::CtxArgs& a, int xt, hipStream_t s);
 int i4_launch_ctx_rows(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s);

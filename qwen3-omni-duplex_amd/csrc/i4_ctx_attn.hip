@@ -14,13 +14,22 @@ struct i4_span {
 
 namespace i4 {
 
+// Row tiles of all kv heads up to which a call's context tiles are shared out.
+static constexpr int kSharedTiles = 1024;
+
 // How a call is split: a rule on its sizes alone (no device value), so that the workspace
 // can be named before the call.
 struct CtxSplit {
-  int S, wgs;      // k_ctx_tile's splits; k_ctx_rows' workgroups
+  int S, wgs;      // k_ctx_tile's splits; k_ctx_rows' workgroups, or those of a shared-out call
   int64_t parts;   // rows that are written as parts
+  int plan;        // entries of a shared-out call's plan, or 0
+  size_t bytes() const {
+    return (size_t)parts * ((KHD + 2) * 4) + ((size_t)plan * 4 + 255) / 256 * 256;
+  }
 };
-static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, int sinks) {
+// share: whether the caller's kernel can share the tiles out
+static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, int sinks,
+                          bool share) {
   const int R = T * (nq / nkv);
   const bool few = R <= kFewRows;
   // the context tiles of 64 that one row tile sees at most
@@ -37,7 +46,12 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
     int64_t w = heads <= 128 ? 512 : heads <= 256 ? 1024 : 2048;
     if (w > heads * ((tiles + 3) / 4)) w = heads * ((tiles + 3) / 4);
     if (w <= heads || heads > kShared) w = heads;
-    return {1, (int)w, w > heads ? w * kFewRows : 0};
+    return {1, (int)w, w > heads ? w * kFewRows : 0, 0};
+  }
+  const int64_t tiled = (R + kTileRows - 1) / kTileRows;
+  if (share && B * tiled <= kPlanned && heads * tiled <= kSharedTiles) {
+    const int64_t w = runs_of(heads * tiled * tiles);
+    return {1, (int)w, 2 * w * kTileRows, (int)(B * tiled) + 2};
   }
   // Two workgroups fit a CU: 512 take 2.1 us a tile together, 256 that have their CU to
   // themselves 1.3 us.  Parts cost 1040 bytes a row, written and read, and a launch.
@@ -51,17 +65,19 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
     if (c > 1) t += 4 + (double)rows * c * 1040 / 4e6;
     if (c == 1 || t < best) best = t, s = c;
   }
-  return {s, 0, s > 1 ? rows * s : 0};
+  return {s, 0, s > 1 ? rows * s : 0, 0};
 }
 
 static int launch(CtxArgs& a, int xt, int fmt, int keys, const i4_span& w, hipStream_t stream) {
-  const CtxSplit sp = ctx_split(a.B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks);
+  const CtxSplit sp = ctx_split(a.B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks, fmt == kPaged);
   a.S = sp.S;
   a.wgs = sp.wgs;
   a.part = (float*)w.workspace;
   a.ml = a.part + sp.parts * KHD;
   a.counters = w.counters;
+  a.plan = (int32_t*)(a.ml + 2 * sp.parts);
   a.tiles = (a.R + kTileRows - 1) / kTileRows;
+  if (sp.plan) return i4_launch_ctx_shared(a, xt, stream);
   const int64_t grid = a.R <= kFewRows ? sp.wgs : (int64_t)a.tiles * sp.S * a.B * a.nkv;
   if (grid > kMaxGrid) return I4_ERR_SHAPE;
   return a.R <= kFewRows ? i4_launch_ctx_rows(a, xt, fmt, stream)
@@ -70,16 +86,24 @@ static int launch(CtxArgs& a, int xt, int fmt, int keys, const i4_span& w, hipSt
 
 }  // namespace i4
 
-extern "C" {
-
-size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
-                                      int window, int sinks) {
+static size_t ctx_bytes(int B, int T, int n_heads, int n_kv_heads, int keys, int window, int sinks,
+                        bool share) {
   if (B < 1 || T < 1 || T > i4::KV_MAX_LEN || n_kv_heads < 1 || n_heads < n_kv_heads ||
       n_heads > 1024 || n_heads % n_kv_heads || keys < 1 || window < 0 || sinks < 0)
     return 0;
   if (n_kv_heads > 1024 || B > 65535) return 0;
-  return (size_t)i4::ctx_split(B, T, n_heads, n_kv_heads, keys, window, sinks).parts *
-         ((i4::KHD + 2) * 4);
+  return i4::ctx_split(B, T, n_heads, n_kv_heads, keys, window, sinks, share).bytes();
+}
+
+extern "C" {
+
+size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
+                                      int window, int sinks) {
+  return ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, false);
+}
+size_t i4_attn_paged_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
+                                     int window, int sinks) {
+  return ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true);
 }
 
 // the positions that a call may attend (a host position is checked after this)
@@ -192,7 +216,7 @@ int i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
   rc = query_check(q, x_dtype, cache->dtype, B, T, q_batch_stride, q_token_stride, q_head_stride,
                    n_heads, nkv, pos_dev, pos, counts, len, window, sinks, scale, out, workspace,
                    workspace_bytes,
-                   i4_attn_window_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
+                   i4_attn_paged_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
                    counters);
   if (rc) return rc;
   CtxArgs a = ctx_args(q, B, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,

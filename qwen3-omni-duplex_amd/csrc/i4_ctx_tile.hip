@@ -366,216 +366,294 @@ template <int XT, int FMT> __device__ inline void store8(const Stage8& st, lds_t
   }
 }
 
+// The list of context tiles that a call's row tiles see, by all threads of a workgroup: the
+// tiles of one kv head before each row tile m = b a.tiles + rt to s_at [0, M].
+__device__ inline Runs plan_runs(const CtxArgs& a, int* s_at, int* s_sum, int most) {
+  const int M = a.B * a.tiles, tid = threadIdx.x, each = (M + 255) / 256;
+  int sum = 0;
+  for (int m = tid * each; m < min(M, (tid + 1) * each); ++m) {
+    const int b = m / a.tiles, tlo = (m - b * a.tiles) * kTileRows / a.G;
+    const CtxSeq sq = ctx_seq(a, b);
+    const int thi = min(((m - b * a.tiles + 1) * kTileRows - 1) / a.G, sq.fit - 1);
+    s_at[m] = sum;
+    if (sq.fit > tlo) sum += ctx_tiles(a.w, sq.p0 + tlo, sq.p0 + thi).n;
+  }
+  const int end = wave_incl_scan(sum);
+  if ((tid & 63) == 63) s_sum[tid >> 6] = end;
+  __syncthreads();
+  int before = end - sum, all = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < tid >> 6) before += s_sum[w];
+    all += s_sum[w];
+  }
+  all = __builtin_amdgcn_readfirstlane(all);
+  for (int m = tid * each; m < min(M, (tid + 1) * each); ++m) s_at[m] += before;
+  if (tid == 0) s_at[M] = all;
+  Runs r;
+  r.total = (int64_t)all * a.nkv;
+  r.wgs = (int)min(runs_of(r.total), (int64_t)most);
+  __syncthreads();
+  return r;
+}
+
 // Workgroup (row tile, split, kv head of a sequence); the last rows, which see the most of
 // a context, come first.
-template <int XT, int FMT>
+// SHARED: every workgroup takes a run of the list of all row tiles' context tiles instead, so
+// that all end together however long the sequences are and however many rows are padding.  A row
+// tile that lies in one run is done there; of the others each run leaves a part, at most two:
+// number 2 w of a row tile that began before run w, 2 w + 1 of one that ends behind it.
+template <int XT, int FMT, bool SHARED>
 __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
   __shared__ __align__(1024) unsigned char s_tile[2][2 * TBYTES];
-  const int heads = (int)gridDim.x / (a.S * a.tiles);  // kv heads of all sequences
-  const int hb = blockIdx.x % heads, b = hb / a.nkv, g = hb % a.nkv;
-  const int split = blockIdx.x / heads % a.S, rt = a.tiles - 1 - (int)(blockIdx.x / heads / a.S);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int n = lane & 31, h = lane >> 5;
-  const CtxSeq sq = ctx_seq(a, b);
-  const int r0 = rt * kTileRows, r = r0 + 32 * wave + n;
-  const int tlo = r0 / a.G, thi = min(min(r0 + kTileRows, a.R) - 1, sq.fit * a.G - 1) / a.G;
-  const int t = r / a.G;
-  const bool mine = r < a.R && t < sq.fit;  // a row with something to attend
-  if (sq.fit > tlo) {
-    const int plo = sq.p0 + tlo, phi = sq.p0 + thi;
-    const int p = mine ? sq.p0 + t : -1;  // -1 sees nothing
-    const int rq = mine ? r : r0;         // any row that exists
-    const uint16_t* qrow =
-        a.q + b * a.qbs + (rq / a.G) * a.qts + (int64_t)(g * a.G + rq % a.G) * a.qhs;
-    u32x4 q[8];
+  int hb, b, g, split = 0, rt;
+  [[maybe_unused]] int run = 0;
+  [[maybe_unused]] int64_t at = 0, stop = 0;
+  [[maybe_unused]] int* s_at = nullptr;
+  if constexpr (SHARED) {
+    __shared__ int s_plan[kPlanned + 1], s_sum[4];
+    s_at = s_plan;
+    const Runs runs = plan_runs(a, s_plan, s_sum, gridDim.x);
+    const int M = a.B * a.tiles;
+    if (blockIdx.x == 0) {  // for the merge
+      for (int m = tid; m <= M; m += 256) a.plan[m] = s_plan[m];
+      if (tid == 0) a.plan[M + 1] = runs.wgs;
+    }
+    // one XCD's workgroups take runs that are neighbours: they read the same contexts
+    const int per = runs.wgs >> 3;
+    run = per ? (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3) : blockIdx.x;
+    if (per ? (int)(blockIdx.x >> 3) >= per : run >= runs.wgs) return;
+    at = runs.first(run);
+    stop = runs.first(run + 1);
+  } else {
+    const int heads = (int)gridDim.x / (a.S * a.tiles);  // kv heads of all sequences
+    hb = blockIdx.x % heads, b = hb / a.nkv, g = hb % a.nkv;
+    split = blockIdx.x / heads % a.S, rt = a.tiles - 1 - (int)(blockIdx.x / heads / a.S);
+  }
+  do {
+    [[maybe_unused]] int from = 0, to = 0;  // SHARED: the context tiles of this row tile
+    if constexpr (SHARED) {
+      if (at >= stop) break;
+      const int M = a.B * a.tiles, one = __builtin_amdgcn_readfirstlane(s_at[M]);
+      g = (int)(at / one);
+      const int u = (int)(at - (int64_t)g * one);
+      int lo = 0, hi = M;  // the row tile that tile u is of: s_at[lo] <= u < s_at[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__builtin_amdgcn_readfirstlane(s_at[mid]) <= u) lo = mid;
+        else hi = mid;
+      }
+      const int begin = __builtin_amdgcn_readfirstlane(s_at[lo]);
+      const int end = __builtin_amdgcn_readfirstlane(s_at[lo + 1]);
+      b = lo / a.tiles, rt = lo - b * a.tiles, hb = b * a.nkv + g;
+      from = u - begin;
+      to = (int)min((int64_t)(end - begin), from + (stop - at));
+      at += to - from;
+      __syncthreads();  // the tiles of the row tile before have been read
+    }
+    const CtxSeq sq = ctx_seq(a, b);
+    const int r0 = rt * kTileRows, r = r0 + 32 * wave + n;
+    const int tlo = r0 / a.G, thi = min(min(r0 + kTileRows, a.R) - 1, sq.fit * a.G - 1) / a.G;
+    const int t = r / a.G;
+    const bool mine = r < a.R && t < sq.fit;  // a row with something to attend
+    if (sq.fit > tlo) {
+      const int plo = sq.p0 + tlo, phi = sq.p0 + thi;
+      const int p = mine ? sq.p0 + t : -1;  // -1 sees nothing
+      const int rq = mine ? r : r0;         // any row that exists
+      const uint16_t* qrow =
+          a.q + b * a.qbs + (rq / a.G) * a.qts + (int64_t)(g * a.G + rq % a.G) * a.qhs;
+      u32x4 q[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) q[c] = ldg16(qrow + 16 * c + 8 * h);
-    TileAcc acc;
-    acc.m = -__builtin_inff();
-    acc.l = 0.f;
+      for (int c = 0; c < 8; ++c) q[c] = ldg16(qrow + 16 * c + 8 * h);
+      TileAcc acc;
+      acc.m = -__builtin_inff();
+      acc.l = 0.f;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc.o[u][i] = 0.f;
-    const CtxTiles ct = ctx_tiles(a.w, plo, phi);
-    const int i0 = (int)((int64_t)ct.n * split / a.S);
-    const int i1 = (int)((int64_t)ct.n * (split + 1) / a.S);
-    lds_t* lds = (lds_t*)&s_tile[0][0];
-    const u32 lds0 = __builtin_amdgcn_readfirstlane((u32)(uintptr_t)lds);
-    f32x16 s[2];
-    bool bad = false;  // values that are not finite in a tile that not all rows see in full
-    auto whole = [&](int i) { return all_see(a.w, plo, phi, 64 * ct.at(i), TKEYS); };
-    auto attend16 = [&](lds_t* buf, int j0, bool edge) {
-      if (edge) bad |= __syncthreads_or(clear_not_finite<XT>(buf + TBYTES, tid));
-      tile_scores<XT>(buf, q, s, n, h);
-      if (edge) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
-      tile_max(acc, s, a.c2);
-      acc.l += tile_weights<XT>(acc, s, a.c2, kLift<XT>);
-      tile_values16<XT>(acc, s, buf + TBYTES, lane);
-    };
-    if constexpr (FMT == kPaged) {
-      const int32_t* table = a.pg.table + b * a.pg.ts;
-      // this wave's 16 positions of tile i; behind the last row's own, that row's
-      auto rows_at = [&](int i) {
-        return page_rows(a.pg, table, g, min(64 * ct.at(i) + 16 * wave, phi) & ~15);
+        for (int i = 0; i < 16; ++i) acc.o[u][i] = 0.f;
+      const CtxTiles ct = ctx_tiles(a.w, plo, phi);
+      const int i0 = SHARED ? from : (int)((int64_t)ct.n * split / a.S);
+      const int i1 = SHARED ? to : (int)((int64_t)ct.n * (split + 1) / a.S);
+      lds_t* lds = (lds_t*)&s_tile[0][0];
+      const u32 lds0 = __builtin_amdgcn_readfirstlane((u32)(uintptr_t)lds);
+      f32x16 s[2];
+      bool bad = false;  // values that are not finite in a tile that not all rows see in full
+      auto whole = [&](int i) { return all_see(a.w, plo, phi, 64 * ct.at(i), TKEYS); };
+      auto attend16 = [&](lds_t* buf, int j0, bool edge) {
+        if (edge) bad |= __syncthreads_or(clear_not_finite<XT>(buf + TBYTES, tid));
+        tile_scores<XT>(buf, q, s, n, h);
+        if (edge) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
+        tile_max(acc, s, a.c2);
+        acc.l += tile_weights<XT>(acc, s, a.c2, kLift<XT>);
+        tile_values16<XT>(acc, s, buf + TBYTES, lane);
       };
-      PageRows next{};  // looked up a tile before its rows are loaded
-      if (i0 < i1) {
-        stage_pages<XT>(a.pg, rows_at(i0), 64 * ct.at(i0) + 16 * wave, phi, lds0, wave, lane);
-        next = rows_at(min(i0 + 1, i1 - 1));
-      }
-      for (int i = i0; i < i1; ++i) {
-        const int cur = (i - i0) & 1;
-        wait_loads();
-        __syncthreads();  // the tile is here, and its other half is free
-        if (i + 1 < i1) {
-          stage_pages<XT>(a.pg, next, 64 * ct.at(i + 1) + 16 * wave, phi,
-                          lds0 + (cur ^ 1) * 2 * TBYTES, wave, lane);
-          next = rows_at(min(i + 2, i1 - 1));
+      if constexpr (FMT == kPaged) {
+        const int32_t* table = a.pg.table + b * a.pg.ts;
+        // this wave's 16 positions of tile i; behind the last row's own, that row's
+        auto rows_at = [&](int i) {
+          return page_rows(a.pg, table, g, min(64 * ct.at(i) + 16 * wave, phi) & ~15);
+        };
+        PageRows next{};  // looked up a tile before its rows are loaded
+        if (i0 < i1) {
+          stage_pages<XT>(a.pg, rows_at(i0), 64 * ct.at(i0) + 16 * wave, phi, lds0, wave, lane);
+          next = rows_at(min(i0 + 1, i1 - 1));
         }
-        attend16(lds + cur * 2 * TBYTES, 64 * ct.at(i), !whole(i));
-      }
-      if (bad)
         for (int i = i0; i < i1; ++i) {
-          const int j0 = 64 * ct.at(i);
-          if (!whole(i))
-            add_not_finite<XT>(acc, [&](int key) {
-              const int j = __builtin_amdgcn_readfirstlane(j0 + key);
-              return (const char*)a.pg.v + page_rows(a.pg, table, g, j & ~15).at + (j & 15) * 256;
-            }, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
-        }
-    } else if constexpr (FMT == kDense) {
-      const u32 stride = (u32)a.c.rs * 2u;
-      const uint16_t* k = a.c.k + b * a.c.bs + g * a.c.hs;
-      const uint16_t* v = a.c.v + b * a.c.bs + g * a.c.hs;
-      const uint64_t ku = uniform(k), vu = uniform(v);
-      if (i0 < i1) stage16(ku, vu, 64 * ct.at(i0), phi, stride, lds0, wave, lane);
-      for (int i = i0; i < i1; ++i) {
-        const int cur = (i - i0) & 1;
-        wait_loads();
-        __syncthreads();  // the tile is here, and its other half is free
-        if (i + 1 < i1)
-          stage16(ku, vu, 64 * ct.at(i + 1), phi, stride, lds0 + (cur ^ 1) * 2 * TBYTES, wave,
-                  lane);
-        attend16(lds + cur * 2 * TBYTES, 64 * ct.at(i), !whole(i));
-      }
-      if (bad)
-        for (int i = i0; i < i1; ++i) {
-          const int j0 = 64 * ct.at(i);
-          if (!whole(i))
-            add_not_finite<XT>(acc, [&](int key) {
-              return (const char*)v + (int64_t)(j0 + key) * stride;
-            }, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
-        }
-    } else {
-      const int end = sq.p0 + sq.fit, full = end / KBLK;  // finished blocks, then the tail
-      const int64_t hblk = (int64_t)hb * a.c8.blocks;
-      // the tail's tile is the last one of the list if it is there at all
-      const bool tail = i1 == ct.n && i1 > i0 && ct.at(ct.n - 1) >= full;
-      const int e = i1 - (tail ? 1 : 0);
-      Stage8 s8;
-      float ks = 0.f, vs = 0.f;
-      // The weights that enter the product take the values' scale, in the exponent; their sum
-      // gives it back.  As the 16-bit types' ranges do not hold every scale, it is taken in units
-      // of a power of two near it, and the sums so far follow when the unit changes: in fp16
-      // where a scale is above it or below an eighth of it, in bf16 above 2^10 or below 2^-60.
-      // The unit stays above 2^-30 (bf16: 2^-80) of the largest scale there was, so that the sums
-      // do not overflow: what a block of so much smaller values adds is lost to rows that met
-      // the larger ones, and to rows of this workgroup that did not see them.
-      constexpr bool F16 = XT == I4_F16;
-      constexpr float kUp = F16 ? 1.f : 0x1p10f, kDown = F16 ? 0.125f : 0x1p-60f;
-      constexpr float kFloor = F16 ? 0x1p-30f : 0x1p-80f;
-      float unit = 1.f, per = 1.f, top = 0.f;  // per = 1 / unit
-      auto set_unit = [&](float u) {
-        const float f = unit / u;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc.o[t] *= f;
-        unit = u;
-        per = 1.0f / u;
-      };
-      if (i0 < e) {
-        load8(s8, a.c8, hblk + ct.at(i0), tid);
-        store8<XT, FMT>(s8, lds, tid);
-        ks = block_scale(s8.ks), vs = block_scale(s8.vs);
-      }
-      for (int i = i0; i < e; ++i) {
-        const int cur = (i - i0) & 1, j0 = 64 * ct.at(i);
-        __syncthreads();
-        if (i + 1 < e) load8(s8, a.c8, hblk + ct.at(i + 1), tid);
-        const lds_t* buf = lds + cur * 2 * TBYTES;
-        if (ks + vs == ks + vs) {
-          tile_scores<XT>(buf, q, s, n, h);
-          if (!whole(i)) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
-          const float c = fmaxf(a.c2 * ks, 0x1p-126f);  // above 0: masked scores stay -inf
-          tile_max(acc, s, c);
-          // the power of two above vs; every block's counts among the largest
-          const float near = as_f32((__builtin_bit_cast(u32, vs) & 0x7F800000u) + 0x00800000u);
-          top = fmaxf(top, near);
-          if (!(vs <= kUp * unit && vs > kDown * unit)) {
-            const float u = fmaxf(near, kFloor * top);
-            if (u != unit) set_unit(u);
+          const int cur = (i - i0) & 1;
+          wait_loads();
+          __syncthreads();  // the tile is here, and its other half is free
+          if (i + 1 < i1) {
+            stage_pages<XT>(a.pg, next, 64 * ct.at(i + 1) + 16 * wave, phi,
+                            lds0 + (cur ^ 1) * 2 * TBYTES, wave, lane);
+            next = rows_at(min(i + 2, i1 - 1));
           }
-          const float r = F16 ? vs * per : fmaxf(vs * per, 0x1p-100f);
-          // (in units of a much larger block an fp16 block's weights may round to 0: then the
-          // sum is of the fp32 ones)
-          const float sum = tile_weights<XT>(acc, s, c, kLift<XT> + log2f(r), !F16 || r > 0.125f);
-          acc.l = fmaf(sum, 1.0f / r, acc.l);
-          tile_values8<XT>(acc, s, buf + TBYTES, n, h);
-        } else if (j0 <= p && (min(j0 + KBLK - 1, p) > p - a.w.window || j0 < a.w.sinks)) {
-          acc.l = __builtin_nanf("");  // a block that reads as NaN, for a row that sees a key
+          attend16(lds + cur * 2 * TBYTES, 64 * ct.at(i), !whole(i));
         }
-        if (i + 1 < e) {
-          store8<XT, FMT>(s8, lds + (cur ^ 1) * 2 * TBYTES, tid);
+        if (bad)
+          for (int i = i0; i < i1; ++i) {
+            const int j0 = 64 * ct.at(i);
+            if (!whole(i))
+              add_not_finite<XT>(acc, [&](int key) {
+                const int j = __builtin_amdgcn_readfirstlane(j0 + key);
+                return (const char*)a.pg.v + page_rows(a.pg, table, g, j & ~15).at + (j & 15) * 256;
+              }, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
+          }
+      } else if constexpr (FMT == kDense) {
+        const u32 stride = (u32)a.c.rs * 2u;
+        const uint16_t* k = a.c.k + b * a.c.bs + g * a.c.hs;
+        const uint16_t* v = a.c.v + b * a.c.bs + g * a.c.hs;
+        const uint64_t ku = uniform(k), vu = uniform(v);
+        if (i0 < i1) stage16(ku, vu, 64 * ct.at(i0), phi, stride, lds0, wave, lane);
+        for (int i = i0; i < i1; ++i) {
+          const int cur = (i - i0) & 1;
+          wait_loads();
+          __syncthreads();  // the tile is here, and its other half is free
+          if (i + 1 < i1)
+            stage16(ku, vu, 64 * ct.at(i + 1), phi, stride, lds0 + (cur ^ 1) * 2 * TBYTES, wave,
+                    lane);
+          attend16(lds + cur * 2 * TBYTES, 64 * ct.at(i), !whole(i));
+        }
+        if (bad)
+          for (int i = i0; i < i1; ++i) {
+            const int j0 = 64 * ct.at(i);
+            if (!whole(i))
+              add_not_finite<XT>(acc, [&](int key) {
+                return (const char*)v + (int64_t)(j0 + key) * stride;
+              }, min(TKEYS, phi - j0 + 1), j0, p, h, a.w);
+          }
+      } else {
+        const int end = sq.p0 + sq.fit, full = end / KBLK;  // finished blocks, then the tail
+        const int64_t hblk = (int64_t)hb * a.c8.blocks;
+        // the tail's tile is the last one of the list if it is there at all
+        const bool tail = i1 == ct.n && i1 > i0 && ct.at(ct.n - 1) >= full;
+        const int e = i1 - (tail ? 1 : 0);
+        Stage8 s8;
+        float ks = 0.f, vs = 0.f;
+        // The weights that enter the product take the values' scale, in the exponent; their sum
+        // gives it back.  As the 16-bit types' ranges do not hold every scale, it is taken in units
+        // of a power of two near it, and the sums so far follow when the unit changes: in fp16
+        // where a scale is above it or below an eighth of it, in bf16 above 2^10 or below 2^-60.
+        // The unit stays above 2^-30 (bf16: 2^-80) of the largest scale there was, so that the sums
+        // do not overflow: what a block of so much smaller values adds is lost to rows that met
+        // the larger ones, and to rows of this workgroup that did not see them.
+        constexpr bool F16 = XT == I4_F16;
+        constexpr float kUp = F16 ? 1.f : 0x1p10f, kDown = F16 ? 0.125f : 0x1p-60f;
+        constexpr float kFloor = F16 ? 0x1p-30f : 0x1p-80f;
+        float unit = 1.f, per = 1.f, top = 0.f;  // per = 1 / unit
+        auto set_unit = [&](float u) {
+          const float f = unit / u;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) acc.o[t] *= f;
+          unit = u;
+          per = 1.0f / u;
+        };
+        if (i0 < e) {
+          load8(s8, a.c8, hblk + ct.at(i0), tid);
+          store8<XT, FMT>(s8, lds, tid);
           ks = block_scale(s8.ks), vs = block_scale(s8.vs);
         }
+        for (int i = i0; i < e; ++i) {
+          const int cur = (i - i0) & 1, j0 = 64 * ct.at(i);
+          __syncthreads();
+          if (i + 1 < e) load8(s8, a.c8, hblk + ct.at(i + 1), tid);
+          const lds_t* buf = lds + cur * 2 * TBYTES;
+          if (ks + vs == ks + vs) {
+            tile_scores<XT>(buf, q, s, n, h);
+            if (!whole(i)) tile_mask(s, j0 + 4 * opaque(h), opaque(p), a.w, -__builtin_inff());
+            const float c = fmaxf(a.c2 * ks, 0x1p-126f);  // above 0: masked scores stay -inf
+            tile_max(acc, s, c);
+            // the power of two above vs; every block's counts among the largest
+            const float near = as_f32((__builtin_bit_cast(u32, vs) & 0x7F800000u) + 0x00800000u);
+            top = fmaxf(top, near);
+            if (!(vs <= kUp * unit && vs > kDown * unit)) {
+              const float u = fmaxf(near, kFloor * top);
+              if (u != unit) set_unit(u);
+            }
+            const float r = F16 ? vs * per : fmaxf(vs * per, 0x1p-100f);
+            // (in units of a much larger block an fp16 block's weights may round to 0: then the
+            // sum is of the fp32 ones)
+            const float sum = tile_weights<XT>(acc, s, c, kLift<XT> + log2f(r), !F16 || r > 0.125f);
+            acc.l = fmaf(sum, 1.0f / r, acc.l);
+            tile_values8<XT>(acc, s, buf + TBYTES, n, h);
+          } else if (j0 <= p && (min(j0 + KBLK - 1, p) > p - a.w.window || j0 < a.w.sinks)) {
+            acc.l = __builtin_nanf("");  // a block that reads as NaN, for a row that sees a key
+          }
+          if (i + 1 < e) {
+            store8<XT, FMT>(s8, lds + (cur ^ 1) * 2 * TBYTES, tid);
+            ks = block_scale(s8.ks), vs = block_scale(s8.vs);
+          }
+        }
+        if (unit != 1.f) set_unit(1.f);
+        if (tail) {
+          const int64_t at = (int64_t)hb * (KBLK * KHD);
+          const int rows = phi - full * KBLK + 1;
+          __syncthreads();
+          stage16(uniform(a.c8.kt + at), uniform(a.c8.vt + at), 0, rows - 1, KHD * 2u, lds0, wave,
+                  lane);
+          wait_loads();
+          __syncthreads();
+          attend16(lds, full * KBLK, true);
+          if (bad)
+            add_not_finite<XT>(acc, [&](int key) {
+              return (const char*)(a.c8.vt + at) + key * (KHD * 2);
+            }, rows, full * KBLK, p, h, a.w);
+        }
       }
-      if (unit != 1.f) set_unit(1.f);
-      if (tail) {
-        const int64_t at = (int64_t)hb * (KBLK * KHD);
-        const int rows = phi - full * KBLK + 1;
-        __syncthreads();
-        stage16(uniform(a.c8.kt + at), uniform(a.c8.vt + at), 0, rows - 1, KHD * 2u, lds0, wave,
-                lane);
-        wait_loads();
-        __syncthreads();
-        attend16(lds, full * KBLK, true);
-        if (bad)
-          add_not_finite<XT>(acc, [&](int key) {
-            return (const char*)(a.c8.vt + at) + key * (KHD * 2);
-          }, rows, full * KBLK, p, h, a.w);
-      }
-    }
-    if (mine) {
-      const float l = acc.l + __shfl_xor(acc.l, 32);
-      if (a.S > 1) {
-        const int64_t at = ((int64_t)hb * a.R + r) * a.S + split;
-        if (h == 0) *(float2*)(a.ml + 2 * at) = float2{acc.m, l};
-        if (l != 0.f)
+      if (mine) {
+        const float l = acc.l + __shfl_xor(acc.l, 32);
+        if (SHARED ? from > 0 || to < ct.n : a.S > 1) {
+          const int64_t at = SHARED ? (2 * run + (from == 0)) * kTileRows + (r - r0)
+                                    : ((int64_t)hb * a.R + r) * a.S + split;
+          if (h == 0) *(float2*)(a.ml + 2 * at) = float2{acc.m, l};
+          if (l != 0.f)
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *(f32x4*)(a.part + at * KHD + 32 * u + 8 * i + 4 * h) =
+                    f32x4{acc.o[u][4 * i], acc.o[u][4 * i + 1], acc.o[u][4 * i + 2],
+                          acc.o[u][4 * i + 3]};
+        } else {
+          uint16_t* y = a.out + ctx_out(a, b, g, r);
+          const float inv = 1.0f / l;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              *(f32x4*)(a.part + at * KHD + 32 * u + 8 * i + 4 * h) =
-                  f32x4{acc.o[u][4 * i], acc.o[u][4 * i + 1], acc.o[u][4 * i + 2],
-                        acc.o[u][4 * i + 3]};
-      } else {
-        uint16_t* y = a.out + ctx_out(a, b, g, r);
-        const float inv = 1.0f / l;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *(u32x2v*)(y + 32 * u + 8 * i + 4 * h) =
-                u32x2v{pack2<XT>(acc.o[u][4 * i] * inv, acc.o[u][4 * i + 1] * inv),
-                       pack2<XT>(acc.o[u][4 * i + 2] * inv, acc.o[u][4 * i + 3] * inv)};
+              *(u32x2v*)(y + 32 * u + 8 * i + 4 * h) =
+                  u32x2v{pack2<XT>(acc.o[u][4 * i] * inv, acc.o[u][4 * i + 1] * inv),
+                         pack2<XT>(acc.o[u][4 * i + 2] * inv, acc.o[u][4 * i + 3] * inv)};
+        }
       }
     }
-  }
-  // tokens whose position is outside the cache (the merge writes them when there is one)
-  if (a.S == 1 && r < a.R && t >= sq.fit && t < sq.have) {
-    u32* y = (u32*)(a.out + ctx_out(a, b, g, r)) + 32 * h;
-    for (int i = 0; i < 32; ++i) y[i] = (u32)Half<XT>::QNAN * 0x10001u;
-  }
+    // tokens whose position is outside the cache (the merge writes them when there is one)
+    if (!SHARED && a.S == 1 && r < a.R && t >= sq.fit && t < sq.have) {
+      u32* y = (u32*)(a.out + ctx_out(a, b, g, r)) + 32 * h;
+      for (int i = 0; i < 32; ++i) y[i] = (u32)Half<XT>::QNAN * 0x10001u;
+    }
+  } while (SHARED);
 }
 
 // The splits of rows merged: 32 P lanes a row, each dims 4 (t % 32) .. + 3 of every P-th
@@ -643,7 +721,69 @@ template <int XT, int P> __global__ __launch_bounds__(256) void k_ctx_merge(CtxA
   else *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
 }
 
+// The parts of row tiles that several runs share, and the rows of tokens outside the cache: eight
+// rows a workgroup, a row to 32 lanes of 4 dims.
+template <int XT> __global__ __launch_bounds__(256) void k_ctx_join(CtxArgs a) {
+  const int M = a.B * a.tiles, g = blockIdx.y / M, m = blockIdx.y - g * M;
+  const int b = m / a.tiles, rt = m - b * a.tiles, d = 4 * (threadIdx.x & 31);
+  const int row = 8 * blockIdx.x + (threadIdx.x >> 5), r = rt * kTileRows + row, t = r / a.G;
+  const CtxSeq sq = ctx_seq(a, b);
+  if (r >= a.R || t >= sq.have) return;
+  u32x2* y = (u32x2*)(a.out + ctx_out(a, b, g, r) + d);
+  if (t >= sq.fit) {
+    *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
+    return;
+  }
+  const int one = a.plan[M], begin = a.plan[m], end = a.plan[m + 1];
+  const Runs runs{(int64_t)one * a.nkv, a.plan[M + 1]};
+  const int64_t u = (int64_t)g * one;
+  const int w0 = runs.of(u + begin), w1 = runs.of(u + end - 1);
+  if (w0 == w1) return;
+  float top = -__builtin_inff(), L = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;
+  for (int w = w0; w <= w1; w += U) {
+    float2 v[U];
+    f32x4 x[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = min(w + i, w1);
+      const int64_t at = (int64_t)(2 * k + (k == w0)) * kTileRows + row;
+      v[i] = ((const float2*)a.ml)[at];
+      x[i] = *(const f32x4*)(a.part + at * KHD + d);
+      if (w + i > w1) v[i].y = 0.f;
+    }
+    float mb = top;  // a sum of 0: nothing seen there, no part written
+#pragma unroll
+    for (int i = 0; i < U; ++i) mb = v[i].y == 0.f ? mb : fmaxf(mb, v[i].x);
+    const float f0 = top == mb ? 1.f : exp2f(top - mb);
+    L *= f0;
+    o *= f0;
+    top = mb;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (v[i].y == 0.f) continue;
+      const float f = exp2f(v[i].x - top);
+      L = fmaf(v[i].y, f, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], f, o[e]);
+    }
+  }
+  *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
+}
+
 }  // namespace i4
+
+int i4_launch_ctx_shared(const i4::CtxArgs& a, int xt, hipStream_t s) {
+  using namespace i4;
+  const dim3 join(kTileRows / 8, (unsigned)(a.B * a.tiles * a.nkv));
+  if (xt == I4_F16) k_ctx_tile<I4_F16, kPaged, true><<<a.wgs, 256, 0, s>>>(a);
+  else k_ctx_tile<I4_BF16, kPaged, true><<<a.wgs, 256, 0, s>>>(a);
+  if (hipGetLastError() != hipSuccess) return I4_ERR_LAUNCH;
+  if (xt == I4_F16) k_ctx_join<I4_F16><<<join, 256, 0, s>>>(a);
+  else k_ctx_join<I4_BF16><<<join, 256, 0, s>>>(a);
+  return hipGetLastError() == hipSuccess ? I4_OK : I4_ERR_LAUNCH;
+}
 
 static int launch_merge(const i4::CtxArgs& a, int xt, hipStream_t s) {
   const int64_t rows = (int64_t)a.B * a.nkv * a.R;
@@ -664,15 +804,15 @@ int i4_launch_ctx_tile(const i4::CtxArgs& a, int xt, int fmt, hipStream_t s) {
   const dim3 grid((unsigned)(a.tiles * a.S * a.B * a.nkv));
   auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a); };
   if (xt == I4_F16) {
-    if (fmt == kDense) go(k_ctx_tile<I4_F16, kDense>);
-    else if (fmt == kPaged) go(k_ctx_tile<I4_F16, kPaged>);
-    else if (fmt == I4_KV8_INT8) go(k_ctx_tile<I4_F16, I4_KV8_INT8>);
-    else go(k_ctx_tile<I4_F16, I4_KV8_E4M3>);
+    if (fmt == kDense) go(k_ctx_tile<I4_F16, kDense, false>);
+    else if (fmt == kPaged) go(k_ctx_tile<I4_F16, kPaged, false>);
+    else if (fmt == I4_KV8_INT8) go(k_ctx_tile<I4_F16, I4_KV8_INT8, false>);
+    else go(k_ctx_tile<I4_F16, I4_KV8_E4M3, false>);
   } else {
-    if (fmt == kDense) go(k_ctx_tile<I4_BF16, kDense>);
-    else if (fmt == kPaged) go(k_ctx_tile<I4_BF16, kPaged>);
-    else if (fmt == I4_KV8_INT8) go(k_ctx_tile<I4_BF16, I4_KV8_INT8>);
-    else go(k_ctx_tile<I4_BF16, I4_KV8_E4M3>);
+    if (fmt == kDense) go(k_ctx_tile<I4_BF16, kDense, false>);
+    else if (fmt == kPaged) go(k_ctx_tile<I4_BF16, kPaged, false>);
+    else if (fmt == I4_KV8_INT8) go(k_ctx_tile<I4_BF16, I4_KV8_INT8, false>);
+    else go(k_ctx_tile<I4_BF16, I4_KV8_E4M3, false>);
   }
   if (hipGetLastError() != hipSuccess) return I4_ERR_LAUNCH;
   return a.S > 1 ? launch_merge(a, xt, s) : I4_OK;

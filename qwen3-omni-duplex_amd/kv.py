@@ -83,7 +83,7 @@ def _out(out: torch.Tensor | None, like: torch.Tensor, shape: tuple[int, ...],
             return torch.zeros(shape, dtype=like.dtype, device=like.device)
         if like.shape == shape and like.is_contiguous():
             return torch.empty_like(like)  # 0.5 us less than spelling it out
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+        return like.new_empty(shape)  # 0.7 us less than torch.empty
     if tuple(out.shape) != shape or out.dtype != like.dtype or not out.is_contiguous():
         raise RuntimeError(f"out must be a contiguous {shape} tensor of {like.dtype}")
     return out
@@ -182,8 +182,9 @@ def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torc
 def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
             pos: int | torch.Tensor, window: int | None, sinks: int, scale: float | None,
             counts: torch.Tensor | None, out: torch.Tensor | None,
-            workspace: Workspace | None) -> torch.Tensor:
-    """The call that attn_window and attn_kv8 share; keys: the positions of the cache."""
+            workspace: Workspace | None, sizes=None) -> torch.Tensor:
+    """The call that attn_window, attn_kv8 and attn_paged share; keys: the positions of the
+    cache; sizes: what names the workspace's."""
     x = _batched(q, 4, "q")
     B, T, nh, hd = x.shape
     if B != cc.batch or hd != cc.head_dim:
@@ -202,8 +203,9 @@ def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
     w = 0 if window is None else min(window, 2**31 - 1)
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
-            return _attend(entry, cc, keys, q, dev, pos, window, sinks, scale, counts, y, workspace)
-    need = _lib.lib().i4_attn_window_workspace_bytes(
+            return _attend(entry, cc, keys, q, dev, pos, window, sinks, scale, counts, y,
+                           workspace, sizes)
+    need = (sizes or _lib.lib().i4_attn_window_workspace_bytes)(
         B, T, nh, cc.n_kv_heads, keys if on_dev else ph + T, w, sinks)
     ws, counters = _scratch(workspace, need, dev, True) if need else (None, None)
     s0, s1, s2, _ = x.stride()

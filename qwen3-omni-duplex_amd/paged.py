@@ -66,14 +66,15 @@ class PagedCache:
 
     def _with(self, table: torch.Tensor, B: int, dev: torch.device) -> _lib.PagedCacheC:
         """struct i4_pagedcache of this pool under a call's table."""
-        t = table if table.dim() == 2 else table.unsqueeze(0) if table.dim() == 1 else None
-        if t is None or t.dtype != torch.int32 or t.device != dev or t.shape[0] != B \
-                or t.shape[1] < 1 or t.stride(1) != 1 and t.shape[1] > 1:
+        shape, stride = table.shape, table.stride()
+        if len(shape) not in (1, 2) or (shape[0] if len(shape) == 2 else 1) != B \
+                or table.dtype != torch.int32 or table.device != dev or shape[-1] < 1 \
+                or stride[-1] != 1 and shape[-1] > 1:
             raise RuntimeError(f"the table is int32 [{B}, n] on the tensors' device, a sequence's "
                                f"entries adjacent")
         pages, page, n, hd, k, v, ps, hs, dt = self._c
-        return _lib.PagedCacheC(k, v, t.data_ptr(), ps, hs, t.stride(0) if B > 1 else 0, B, n,
-                                pages, page, t.shape[1], hd, dt)
+        return _lib.PagedCacheC(k, v, table.data_ptr(), ps, hs, stride[0] if B > 1 else 0, B, n,
+                                pages, page, shape[-1], hd, dt)
 
 
 def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
@@ -98,12 +99,9 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
         raise RuntimeError("the pages must have the activation dtype")
     if width != (n_heads + 2 * cc.n_kv_heads) * hd:
         raise RuntimeError("qkv's width does not match the head counts")
-    norms = []
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dtype != x.dtype or w.numel() != hd):
-            raise RuntimeError(f"the norm weights hold head_dim = {hd} values of the activation "
-                               "dtype")
-        norms.append(w if w is None else w.contiguous())
+        if w is not None and (w.dtype != x.dtype or w.shape != (hd,) or w.stride(0) != 1):
+            raise RuntimeError(f"a norm weight is {hd} adjacent values of the activation dtype")
     if rotary.dims > hd or rotary.layout == "half" and rotary.dims % 16:
         raise RuntimeError(f"{rotary.dims} of {hd} dims turn: at most all, and with the layout "
                            "'half' a multiple of 16")
@@ -114,7 +112,7 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
     on_dev = isinstance(pos, torch.Tensor)
     tc = None if turn is None else _turn_c(turn, rotary, qkv.dim() == 3, B, T, dev)
     _call(dev, _lib.lib().i4_paged_append, x.data_ptr(), cc.dtype, T, x.stride(0), x.stride(1),
-          n_heads, _lib.ptr(norms[0]), _lib.ptr(norms[1]), eps, rotary._c,
+          n_heads, _lib.ptr(q_norm_w), _lib.ptr(k_norm_w), eps, rotary._c,
           _int32(pos, B, dev, "pos") if on_dev else None,
           0 if on_dev else _host_pos(pos, T, cc.table_len * cc.page), tc,
           _int32(counts, B, dev, "counts"), q.data_ptr(), ctypes.byref(cc))
@@ -132,5 +130,6 @@ def attn_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor,
     as attn_window (i4_attn_paged)."""
     dev = _lib.require_device(q, cache.k, counts, out)
     cc = cache._with(table, q.shape[0] if q.dim() == 4 else 1, dev)
-    return _attend(_lib.lib().i4_attn_paged, cc, cc.table_len * cc.page, q, dev, pos, window,
-                   sinks, scale, counts, out, workspace)
+    lib = _lib.lib()
+    return _attend(lib.i4_attn_paged, cc, cc.table_len * cc.page, q, dev, pos, window, sinks, scale,
+                   counts, out, workspace, lib.i4_attn_paged_workspace_bytes)

@@ -30,7 +30,7 @@ class Rotary:
     multiplies cos and sin (the attention factor of a scaled table).  axes: for tokens that are
     given several positions, which of them each pair turns by.  The table is copied to the host."""
 
-    __slots__ = ("inv_freq", "layout", "factor", "axes", "_bytes", "_c")
+    __slots__ = ("inv_freq", "layout", "factor", "axes", "dims", "_bytes", "_c")
 
     def __init__(self, inv_freq: torch.Tensor, *, layout: str = "half", factor: float = 1.0,
                  axes: Sequence[int] | None = None):
@@ -47,6 +47,7 @@ class Rotary:
         if axes is not None and (len(axes) != n or not all(0 <= a < 4 for a in axes)):
             raise RuntimeError(f"axes: {n} numbers from 0 to 3")
         self.inv_freq, self.layout, self.factor = f, layout, float(factor)
+        self.dims = 2 * n  # of a head that turn
         self.axes = None if axes is None else tuple(int(a) for a in axes)
         self._bytes = None if axes is None else (ctypes.c_uint8 * n)(*self.axes)
         self._c = _lib.RotaryC(f.data_ptr(), None if axes is None else
@@ -78,11 +79,6 @@ class Rotary:
             factor = 0.1 * math.log(scale) + 1 if factor is None else factor
         return cls(f.float(), factor=1.0 if factor is None else factor, **kw)
 
-    @property
-    def dims(self) -> int:
-        """How many dims of a head turn."""
-        return 2 * self.inv_freq.numel()
-
     def __repr__(self) -> str:
         return (f"Rotary(dims={self.dims}, layout={self.layout!r}, factor={self.factor}"
                 + (f", axes={self.axes}" if self.axes else "") + ")")
@@ -112,16 +108,54 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() - 1
 
 
-def _heads_c(x: torch.Tensor, y: torch.Tensor) -> _lib.HeadsC:
-    a, b = x.stride(), y.stride()
-    return _lib.HeadsC(x.data_ptr(), y.data_ptr(), a[0], a[1], a[2], b[0], b[1], b[2], x.shape[2])
+def _apart(shape: tuple[int, ...], stride: tuple[int, ...]) -> bool:
+    """Whether the rows [B, T, heads, head_dim] are dense and lie apart."""
+    hd = shape[3]
+    return stride[3] == 1 and (shape[2] == 1 or stride[2] >= hd) and (
+        shape[1] == 1 or stride[1] >= hd) and (shape[0] == 1 or stride[0] >= hd)
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x as it is, or a copy where its rows are not dense or lie on each other."""
-    hd = x.shape[3]
-    return x if x.stride(3) == 1 and all(
-        n == 1 or s >= hd for n, s in zip(x.shape[:3], x.stride())) else x.contiguous()
+def _new(x: torch.Tensor, zeros: bool, held: list[torch.Tensor]) -> _lib.HeadsC:
+    """A dense output for x [B, T, heads, head_dim], appended to held, and struct i4_heads of
+    both.  What the struct points at is held until the call is queued."""
+    shape, a = x.shape, x.stride()
+    if not _apart(shape, a):
+        x = x.contiguous()
+        a = x.stride()
+        held.insert(0, x)
+    y = (torch.zeros_like if zeros else torch.empty_like)(
+        x, memory_format=torch.contiguous_format)
+    _, T, n, hd = shape
+    held.append(y)
+    return _lib.HeadsC(x.data_ptr(), y.data_ptr(), a[0], a[1], a[2], T * n * hd, n * hd, hd, n)
+
+
+def _into(xs: list[torch.Tensor], out: tuple[torch.Tensor | None, ...],
+          held: list[torch.Tensor]) -> list[_lib.HeadsC]:
+    """struct i4_heads of the inputs and the given outputs, checked."""
+    outs = [t for t in out if t is not None]
+    if len(outs) != len(xs):
+        raise RuntimeError("out holds a tensor for each input")
+    _lib.require_device(*xs, *outs)
+    cs = []
+    for t, x in zip(outs, xs):
+        y = _batched(t, 4, "out")
+        if y.shape != x.shape or y.dtype != x.dtype:
+            raise RuntimeError(f"out must be a {tuple(x.shape)} tensor of {x.dtype}")
+        if not _apart(y.shape, y.stride()):
+            raise RuntimeError("out's rows must be dense and lie apart")
+        if y.data_ptr() != x.data_ptr() or y.stride() != x.stride():  # not in place
+            lo, hi = _span(y)
+            for z in xs:
+                a, b = _span(z)
+                if lo <= b and a <= hi:
+                    raise RuntimeError("out is its input itself or does not overlap the inputs")
+            if not _apart(x.shape, x.stride()):
+                x = x.contiguous()
+                held.append(x)
+        cs.append(_lib.HeadsC(x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3],
+                              x.shape[2]))
+    return cs
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotary: Rotary, *,
@@ -141,38 +175,17 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
     are q and k themselves (in place) or do not overlap them."""
     dev = _lib.require_device(q, k, counts)
     code = _lib.half_code(q.dtype)
-    x = _batched(q, 4, "q")
+    batched = q.dim() == 4
+    x = q if batched else _batched(q, 4, "q")
     B, T, _, hd = x.shape
-    if k is not None and k.dtype != q.dtype:
-        raise RuntimeError("q and k must have one dtype")
-    xs = [x] if k is None else [x, _batched(k, 4, "k")]
-    if xs[-1].shape[:2] != x.shape[:2] or xs[-1].shape[3] != hd or k is not None \
-            and k.dim() != q.dim():
-        raise RuntimeError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
-    if out is None:
-        xs = [_rows(t) for t in xs]
-        make = torch.zeros if counts is not None else torch.empty
-        ys = [make(t.shape, dtype=t.dtype, device=dev) for t in xs]
-    else:
-        outs = [t for t in out if t is not None]
-        if len(outs) != len(xs):
-            raise RuntimeError("out holds a tensor for each input")
-        _lib.require_device(q, *outs)
-        ys = [_batched(t, 4, "out") for t in outs]
-        for y, x in zip(ys, xs):
-            if y.shape != x.shape or y.dtype != x.dtype or y.dim() != x.dim():
-                raise RuntimeError(f"out must be a {tuple(x.shape)} tensor of {x.dtype}")
-            if _rows(y) is not y:
-                raise RuntimeError("out's rows must be dense and lie apart")
-        for y, x in zip(ys, xs):
-            if y.data_ptr() == x.data_ptr() and y.stride() == x.stride():
-                continue
-            lo, hi = _span(y)
-            for z in xs:
-                a, b = _span(z)
-                if lo <= b and a <= hi:
-                    raise RuntimeError("out is its input itself or does not overlap the inputs")
-        xs = [x if x.data_ptr() == y.data_ptr() else _rows(x) for x, y in zip(xs, ys)]
+    xs = [x]
+    if k is not None:
+        z = k if batched else k.unsqueeze(0)
+        if z.dim() != 4 or z.shape[0] != B or z.shape[1] != T or z.shape[3] != hd:
+            raise RuntimeError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not match")
+        if k.dtype != q.dtype:
+            raise RuntimeError("q and k must have one dtype")
+        xs.append(z)
     if rotary.dims > hd:
         raise RuntimeError(f"{rotary.dims} dims turn, the heads have {hd}")
     turn = pd = None
@@ -181,14 +194,18 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
         ph = int(pos)
         if not -MAX_POS < ph <= MAX_POS - T:
             raise RuntimeError(f"positions {ph} to {ph + T - 1} outside (-2^24, 2^24)")
-    elif pos.dim() == 1 and (q.dim() == 4 or pos.numel() == 1):
+    elif pos.dim() == 1 and (batched or pos.numel() == 1):
         pd = _int32(pos, B, dev, "pos")
     else:
-        turn = _turn_c(pos, rotary, q.dim() == 4, B, T, dev)
-    cs = [_heads_c(x, y) for x, y in zip(xs, ys)]
-    _call(dev, _lib.lib().i4_rope, cs[0], cs[1] if len(cs) > 1 else None, code, B, T, hd, rotary._c,
-          pd, ph, turn, _int32(counts, B, dev, "counts"))
-    if out is not None:
-        return out[0] if k is None else tuple(out)
-    ys = [y if q.dim() == 4 else y[0] for y in ys]
+        turn = _turn_c(pos, rotary, batched, B, T, dev)
+    held: list[torch.Tensor] = []  # the new outputs are its last elements
+    if out is None:
+        cs = [_new(t, counts is not None, held) for t in xs]
+    else:
+        cs = _into(xs, out, held)
+    _call(dev, _lib.lib().i4_rope, cs[0], cs[1] if k is not None else None, code, B, T, hd,
+          rotary._c, pd, ph, turn, None if counts is None else _int32(counts, B, dev, "counts"))
+    ys = held[-len(xs):] if out is None else [t for t in out if t is not None]
+    if not batched and out is None:
+        ys = [y[0] for y in ys]
     return ys[0] if k is None else tuple(ys)

@@ -83,9 +83,10 @@ def test_attention_matches_64_bits(pkg, dev, dtype, page, B, T, nh, nkv, pos, wi
 @pytest.mark.parametrize("page", [16, 32, 128, 1024])
 @pytest.mark.parametrize("B,T,nh,nkv,pos,window,sinks", [
     (1, 1, 32, 4, 8191, None, 0), (4, 1, 32, 4, 3000, None, 0), (2, 2, 16, 2, 777, 256, 20),
-    (1, 300, 16, 2, 1000, None, 0), (2, 70, 8, 8, 333, 100, 7)])
+    (1, 4110, 32, 4, 100, 300, 5), (2, 2100, 64, 8, 77, None, 0)])
 def test_attention_is_that_over_rows(pkg, dev, dtype, page, B, T, nh, nkv, pos, window, sinks):
-    """The bits of attn_window over the same rows, for host and device positions."""
+    """The bits of attn_window over the same rows, for host and device positions: for few rows,
+    and for so many that their context tiles are not shared out."""
     n = -(-(pos + T) // page) * page
     q, rows = case(dev, B, T, nh, nkv, n, dtype)
     cache, table = pool_of(pkg, dev, rows, [n] * B, page, seed=1)
@@ -161,7 +162,7 @@ def test_pages_behind_the_window_may_be_gone(pkg, dev, T):
 @pytest.mark.parametrize("T", [1, 2, 40])
 def test_shared_pages(pkg, dev, T):
     """Sequences whose first pages are the same, with tails of their own; the same sequence
-    twice in one call."""
+    twice in one call (with the same bits where a context is not cut for the whole batch)."""
     page, common, pos, B = 32, 160, 300, 3
     q, rows = case(dev, B, T, 8, 2, pos + T, torch.bfloat16)
     rows[:, 1:, :, :common] = rows[:, :1, :, :common]
@@ -172,7 +173,10 @@ def test_shared_pages(pkg, dev, T):
     assert same(pkg.attn_paged(q, cache, one, pos), want)
     twice = table[[0, 0, 2]]
     got = pkg.attn_paged(q[[0, 0, 2]], cache, twice, pos)
-    assert same(got[0], got[1]) and same(got[0], want[0]) and same(got[2], want[2])
+    assert same(got[0], want[0]) and same(got[2], want[2])
+    assert T == 40 or same(got[0], got[1])
+    check(got, *(x[[0, 0, 2]] for x in kvref.attention(q, rows[0], rows[1], [pos] * B, [T] * B,
+                                                       None, 0)))
 
 
 @pytest.mark.parametrize("T,pos,window", [(1, 100, None), (2, 90, 33), (5, 60, None), (50, 70, 40)])
@@ -244,6 +248,34 @@ def test_pool_views(pkg, dev):
     assert same(pkg.attn_paged(view, cache, table, 60), want)
     # one sequence without a batch
     assert same(pkg.attn_paged(q[1], cache, table[1], 60), want[1])
+
+
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("B,T,nh,nkv,pos,window,sinks", [
+    (1, 33, 32, 4, 3000, None, 0),    # many runs for each row tile
+    (3, 90, 16, 2, 700, None, 0),     # row tiles that runs cut
+    (9, 50, 8, 8, 260, 100, 3),       # runs of several row tiles
+    (2, 18, 8, 1, 0, None, 0),        # fewer tiles than a run of four for each XCD
+    (40, 24, 8, 2, 90, None, 0)])
+def test_shared_out_tiles(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
+    """Padded batches of several rows whose context tiles are shared out, against 64 bits: ages
+    and counts that differ, none among them; the same bits again and from a larger workspace."""
+    at = starts(pos, B)
+    counts = [T if b == 0 else (T - 7 * b) % (T + 1) for b in range(B)]
+    q, rows = case(dev, B, T, nh, nkv, pos + T, dtype)
+    cache, table = pool_of(pkg, dev, rows, [p + n for p, n in zip(at, counts)], 16)
+    bounds = dict(window=window, sinks=sinks, counts=i32(dev, counts))
+    out = torch.full_like(q, 5.0)
+    got = pkg.attn_paged(q, cache, table, i32(dev, at), out=out, **bounds)
+    want, tol = kvref.attention(q, rows[0], rows[1], at, counts, window, sinks)
+    check(got, want, tol)
+    for b, n in enumerate(counts):
+        assert (out[b, n:] == 5.0).all()
+    ws = pkg.Workspace()
+    ws.get(1 << 25, dev).fill_(0xFF)
+    again = pkg.attn_paged(q, cache, table, i32(dev, at), workspace=ws, **bounds)
+    for b, n in enumerate(counts):
+        assert same(again[b, :n], got[b, :n])
 
 
 # ------------------------------------------------------------------- append
