@@ -41,22 +41,25 @@ struct CtxArgs {
   int32_t* plan;          // of a call whose tiles are shared out (k_ctx_tile), or null
 };
 
-// Row tiles up to which their context tiles are shared out; the plan of a call: the context
-// tiles before each row tile of one kv head ([0, M], M = B tiles), then the workgroups.
+// Row tiles up to which their context tiles are shared out; the plan of a call: the list's
+// length before each row tile of one kv head ([0, M], M = B tiles), then the workgroups.
 static constexpr int kPlanned = 1024;
+// What a row tile takes besides its context tiles (its queries, the first loads, its output), in
+// context tiles: it has as many places in the list in front of them.
+static constexpr int kRowTile = 2;
 
-// how many runs `total` tiles are cut into: at least four tiles each, as many on every XCD
+// how many runs `total` places are cut into: at least four places each, as many on every XCD
 __host__ __device__ inline int64_t runs_of(int64_t total) {
   const int64_t w = total / 4;
   return w >= 512 ? 512 : w >= 8 ? w & ~7 : w > 1 ? w : 1;
 }
 // The context tiles of all row tiles as one list, kv head after kv head, cut into `wgs` runs of
-// the same length: run w has tiles [w total / wgs, (w + 1) total / wgs).
+// the same length: run w has places [w total / wgs, (w + 1) total / wgs).
 struct Runs {
   int64_t total;
   int wgs;  // at most `total`, so that no run is empty
   __host__ __device__ inline int64_t first(int w) const { return total * w / wgs; }
-  // the run that tile u is in
+  // the run that place u is in
   __host__ __device__ inline int of(int64_t u) const {
     return (int)(((u + 1) * wgs - 1) / total);
   }

@@ -14,8 +14,16 @@ struct i4_span {
 
 namespace i4 {
 
-// Row tiles of all kv heads up to which a call's context tiles are shared out.
-static constexpr int kSharedTiles = 1024;
+// When the context tiles of many rows are shared out: several sequences whose lengths the host
+// does not know (device positions, counts), up to kSharedTiles row tiles of all kv heads, and at
+// least kSharedSpan context tiles that a row tile may see.  Measured, shared out against split by
+// ctx_split's cost, us: 4 x 400 padded tokens behind up to 9001 positions 184 / 257, 16 x 100
+// behind 8000 114 / 209, 16 x 17 behind 16000 103 / 134, 3 x 1000 behind 2000 106 / 102.  The
+// parts that runs leave (66 KB each, up to 1024) cost it some 25 us: fewer context tiles, 4 x 400
+// behind 1000: 48 / 43, 40 x 8 behind 900: 39 / 32; more row tiles, 8 x 300 of 56 heads behind
+// 1000: 105 / 81; and one prompt, whose row tiles the longest-first order evens out: 3000 tokens
+// 115 / 84.
+static constexpr int kSharedTiles = 1024, kSharedSpan = 32;
 
 // How a call is split: a rule on its sizes alone (no device value), so that the workspace
 // can be named before the call.
@@ -27,7 +35,7 @@ struct CtxSplit {
     return (size_t)parts * ((KHD + 2) * 4) + ((size_t)plan * 4 + 255) / 256 * 256;
   }
 };
-// share: whether the caller's kernel can share the tiles out
+// share: whether the tiles may be shared out
 static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, int sinks,
                           bool share) {
   const int R = T * (nq / nkv);
@@ -49,8 +57,9 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
     return {1, (int)w, w > heads ? w * kFewRows : 0, 0};
   }
   const int64_t tiled = (R + kTileRows - 1) / kTileRows;
-  if (share && B * tiled <= kPlanned && heads * tiled <= kSharedTiles) {
-    const int64_t w = runs_of(heads * tiled * tiles);
+  if (share && B > 1 && B * tiled <= kPlanned && heads * tiled <= kSharedTiles &&
+      tiles >= kSharedSpan) {
+    const int64_t w = runs_of(heads * tiled * (tiles + kRowTile));
     return {1, (int)w, 2 * w * kTileRows, (int)(B * tiled) + 2};
   }
   // Two workgroups fit a CU: 512 take 2.1 us a tile together, 256 that have their CU to
@@ -69,7 +78,8 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
 }
 
 static int launch(CtxArgs& a, int xt, int fmt, int keys, const i4_span& w, hipStream_t stream) {
-  const CtxSplit sp = ctx_split(a.B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks, fmt == kPaged);
+  const CtxSplit sp = ctx_split(a.B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks,
+                                fmt == kPaged && (a.tk.pos_dev || a.tk.counts));
   a.S = sp.S;
   a.wgs = sp.wgs;
   a.part = (float*)w.workspace;
@@ -103,7 +113,9 @@ size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads,
 }
 size_t i4_attn_paged_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                      int window, int sinks) {
-  return ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true);
+  const size_t split = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, false);
+  const size_t shared = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true);
+  return split > shared ? split : shared;
 }
 
 // the positions that a call may attend (a host position is checked after this)

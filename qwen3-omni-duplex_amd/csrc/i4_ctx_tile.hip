@@ -89,6 +89,15 @@ __device__ inline void stage16(uint64_t k, uint64_t v, int j0, int last, u32 str
 template <int XT>
 __device__ inline void stage_pages(const Pages& pg, const PageRows& u, int j, int last, u32 lds,
                                    int wave, int lane) {
+  if (u.bad) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lds_t* dst = (lds_t*)(uintptr_t)(lds + 1024u * (4 * wave + i) + 16u * lane);
+      lds_put(dst, u32x4{} + (u32)Half<XT>::QNAN * 0x10001u);
+      lds_put(dst + TBYTES, u32x4{});
+    }
+    return;
+  }
   const int r4 = lane >> 4, c = lane & 15;
   const uint64_t k = uniform((const char*)pg.k + u.at), v = uniform((const char*)pg.v + u.at);
   const int most = last - min(j, last & ~15);  // the last row that anything sees
@@ -96,13 +105,8 @@ __device__ inline void stage_pages(const Pages& pg, const PageRows& u, int j, in
   for (int i = 0; i < 4; ++i) {
     const u32 row = (u32)min(4 * i + r4, most) * (KHD * 2u);
     const u32 dst = lds + 1024u * (4 * wave + i);
-    if (u.bad) {
-      lds_put((lds_t*)(uintptr_t)(dst + 16u * lane), u32x4{} + (u32)Half<XT>::QNAN * 0x10001u);
-      lds_put((lds_t*)(uintptr_t)(dst + TBYTES + 16u * lane), u32x4{});
-    } else {
-      load_lds16(k, row + 16u * (c ^ (4 * i + r4)), dst);
-      load_lds16(v, row + 16u * (c ^ ((4 * (i & 1) + r4) << 1)), dst + TBYTES);
-    }
+    load_lds16(k, row + 16u * (c ^ (4 * i + r4)), dst);
+    load_lds16(v, row + 16u * (c ^ ((4 * (i & 1) + r4) << 1)), dst + TBYTES);
   }
 }
 
@@ -366,8 +370,8 @@ template <int XT, int FMT> __device__ inline void store8(const Stage8& st, lds_t
   }
 }
 
-// The list of context tiles that a call's row tiles see, by all threads of a workgroup: the
-// tiles of one kv head before each row tile m = b a.tiles + rt to s_at [0, M].
+// The list of context tiles that a call's row tiles see, by all threads of a workgroup: its
+// length for one kv head before each row tile m = b a.tiles + rt to s_at [0, M].
 __device__ inline Runs plan_runs(const CtxArgs& a, int* s_at, int* s_sum, int most) {
   const int M = a.B * a.tiles, tid = threadIdx.x, each = (M + 255) / 256;
   int sum = 0;
@@ -376,7 +380,7 @@ __device__ inline Runs plan_runs(const CtxArgs& a, int* s_at, int* s_sum, int mo
     const CtxSeq sq = ctx_seq(a, b);
     const int thi = min(((m - b * a.tiles + 1) * kTileRows - 1) / a.G, sq.fit - 1);
     s_at[m] = sum;
-    if (sq.fit > tlo) sum += ctx_tiles(a.w, sq.p0 + tlo, sq.p0 + thi).n;
+    if (sq.fit > tlo) sum += kRowTile + ctx_tiles(a.w, sq.p0 + tlo, sq.p0 + thi).n;
   }
   const int end = wave_incl_scan(sum);
   if ((tid & 63) == 63) s_sum[tid >> 6] = end;
@@ -438,18 +442,19 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
       const int M = a.B * a.tiles, one = __builtin_amdgcn_readfirstlane(s_at[M]);
       g = (int)(at / one);
       const int u = (int)(at - (int64_t)g * one);
-      int lo = 0, hi = M;  // the row tile that tile u is of: s_at[lo] <= u < s_at[hi]
+      int lo = 0, hi = M;  // the row tile that place u is of: s_at[lo] <= u < s_at[hi]
       while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (__builtin_amdgcn_readfirstlane(s_at[mid]) <= u) lo = mid;
         else hi = mid;
       }
-      const int begin = __builtin_amdgcn_readfirstlane(s_at[lo]);
+      const int begin = __builtin_amdgcn_readfirstlane(s_at[lo]) + kRowTile;
       const int end = __builtin_amdgcn_readfirstlane(s_at[lo + 1]);
       b = lo / a.tiles, rt = lo - b * a.tiles, hb = b * a.nkv + g;
-      from = u - begin;
-      to = (int)min((int64_t)(end - begin), from + (stop - at));
-      at += to - from;
+      const int last = (int)min((int64_t)end, u + (stop - at));
+      at += last - u;
+      from = max(u - begin, 0), to = last - begin;
+      if (to <= from) continue;
       __syncthreads();  // the tiles of the row tile before have been read
     }
     const CtxSeq sq = ctx_seq(a, b);
@@ -734,7 +739,7 @@ template <int XT> __global__ __launch_bounds__(256) void k_ctx_join(CtxArgs a) {
     *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
     return;
   }
-  const int one = a.plan[M], begin = a.plan[m], end = a.plan[m + 1];
+  const int one = a.plan[M], begin = a.plan[m] + kRowTile, end = a.plan[m + 1];
   const Runs runs{(int64_t)one * a.nkv, a.plan[M + 1]};
   const int64_t u = (int64_t)g * one;
   const int w0 = runs.of(u + begin), w1 = runs.of(u + end - 1);

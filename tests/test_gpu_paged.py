@@ -252,18 +252,22 @@ def test_pool_views(pkg, dev):
 
 @pytest.mark.parametrize("dtype", DTS)
 @pytest.mark.parametrize("B,T,nh,nkv,pos,window,sinks", [
-    (1, 33, 32, 4, 3000, None, 0),    # many runs for each row tile
+    (2, 33, 32, 4, 3000, None, 0),    # many runs for each row tile
     (3, 90, 16, 2, 700, None, 0),     # row tiles that runs cut
-    (9, 50, 8, 8, 260, 100, 3),       # runs of several row tiles
+    (9, 50, 8, 8, 260, 100, 3),       # runs of several row tiles, under a window
+    (9, 50, 8, 8, 260, 5000, 3),
     (2, 18, 8, 1, 0, None, 0),        # fewer tiles than a run of four for each XCD
+    (2, 18, 8, 1, 300, None, 0),
     (40, 24, 8, 2, 90, None, 0)])
 def test_shared_out_tiles(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
-    """Padded batches of several rows whose context tiles are shared out, against 64 bits: ages
-    and counts that differ, none among them; the same bits again and from a larger workspace."""
+    """Padded batches of several rows whose context tiles are shared out (a wide table: it goes by
+    what the table could hold), against 64 bits: ages and counts that differ, none among them;
+    the same bits again and from a larger workspace."""
     at = starts(pos, B)
     counts = [T if b == 0 else (T - 7 * b) % (T + 1) for b in range(B)]
     q, rows = case(dev, B, T, nh, nkv, pos + T, dtype)
-    cache, table = pool_of(pkg, dev, rows, [p + n for p, n in zip(at, counts)], 16)
+    cache, table = pool_of(pkg, dev, rows, [p + n for p, n in zip(at, counts)], 16,
+                           width=max(130, -(-(pos + T) // 16)))
     bounds = dict(window=window, sinks=sinks, counts=i32(dev, counts))
     out = torch.full_like(q, 5.0)
     got = pkg.attn_paged(q, cache, table, i32(dev, at), out=out, **bounds)
@@ -276,6 +280,67 @@ def test_shared_out_tiles(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
     again = pkg.attn_paged(q, cache, table, i32(dev, at), workspace=ws, **bounds)
     for b, n in enumerate(counts):
         assert same(again[b, :n], got[b, :n])
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (90, 20)])
+def test_shared_out_missing_pages(pkg, dev, window, sinks):
+    """As above where the context tiles are shared out: NaN in exactly the rows that see one of
+    the missing page's positions; the other sequence as it was."""
+    T, pos, page = 40, 400, 16
+    q, rows = case(dev, 2, T, 8, 2, pos + T, torch.bfloat16)
+    cache, table = pool_of(pkg, dev, rows, [pos + T] * 2, page, width=130, fill=0.5)
+    at, bounds = i32(dev, [pos, pos]), dict(window=window, sinks=sinks)
+    clean = pkg.attn_paged(q, cache, table, at, **bounds)
+    for i in (0, 1, 5, 19, 20, 24, 25, 26, 27):
+        broken = table.clone()
+        broken[1, i] = [-1, cache.pages, 2**31 - 1][i % 3]
+        got = pkg.attn_paged(q, cache, broken, at, **bounds)
+        assert same(got[0], clean[0])
+        for t in range(T):
+            if kvref.see(pos + t, pos + T, window, sinks)[i * page:(i + 1) * page].any():
+                assert torch.isnan(got[1, t]).all()
+            else:
+                assert same(got[1, t], clean[1, t])
+
+
+@pytest.mark.parametrize("window", [None, 70])
+def test_shared_out_values_that_are_not_finite(pkg, dev, window):
+    T, pos = 40, 300
+    q, rows = case(dev, 2, T, 8, 2, pos + T, torch.bfloat16)
+    want, tol = kvref.attention(q, rows[0], rows[1], [pos] * 2, [T] * 2, window, 0)
+    for j in (0, 250, pos, pos + 17, pos + T - 1):
+        bad = rows.clone()
+        bad[1, 1, 1, j, 5] = math.inf
+        bad[1, 1, 1, j, 77] = QNAN
+        cache, table = pool_of(pkg, dev, bad, [pos + T] * 2, 16, width=130)
+        got = pkg.attn_paged(q, cache, table, i32(dev, [pos, pos]), window=window).double().cpu()
+        rest = torch.ones_like(got, dtype=torch.bool)
+        for t in range(T):
+            if kvref.see(pos + t, pos + T, window, 0)[j]:
+                rest[1, t, 4:, [5, 77]] = False
+        assert torch.equal(torch.isfinite(got), rest)
+        assert ((got - want).abs() <= tol)[rest].all()
+
+
+def test_shared_out_positions_outside(pkg, dev):
+    """Rows past the table are NaN, padding stays, where the context tiles are shared out; also
+    when no sequence has a token inside."""
+    B, T, page, width = 5, 40, 16, 130
+    end = page * width
+    pos, counts = [end - 20, -1, end, 100, 2**31 - 1], [40, 40, 7, 33, 40]
+    q, rows = case(dev, B, T, 8, 2, end, torch.float16)
+    cache, table = pool_of(pkg, dev, rows, [end] * B, page)
+    out = torch.full_like(q, 5.0)
+    pkg.attn_paged(q, cache, table, i32(dev, pos), counts=i32(dev, counts), out=out)
+    fit = [20, 0, 0, 33, 0]
+    want, tol = kvref.attention(q, rows[0], rows[1], pos, fit, None, 0)
+    for b in range(B):
+        check(out[b:b + 1, :fit[b]], want[b:b + 1, :fit[b]], tol[b:b + 1, :fit[b]])
+        assert torch.isnan(out[b, fit[b]:counts[b]]).all() and (out[b, counts[b]:] == 5.0).all()
+    out.fill_(5.0)
+    pkg.attn_paged(q, cache, table, i32(dev, [-1] * B), counts=i32(dev, [0, 1, 2, 40, 9]), out=out)
+    for b, n in enumerate([0, 1, 2, 40, 9]):
+        assert torch.isnan(out[b, :n]).all() and (out[b, n:] == 5.0).all()
 
 
 # ------------------------------------------------------------------- append
