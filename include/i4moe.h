@@ -784,7 +784,7 @@ int    i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride,
  * Many sessions on one key/value cache: rotary embeddings of any model, a cache in pages, and
  * attention over it.  No counterpart in the reference beyond the attention itself.  B, T,
  * pos_dev, pos and counts are as above (of a sequence whose pos_dev is outside the cache, every
- * token is). */
+ * token is); zero_padding != 0 sets the padding's output rows to zero instead of leaving them. */
 
 /* A rotary embedding: pair i < pairs of a head's first 2 pairs dims turns by the angle
  * p inv_freq[i] (finite, at most 16), and cos and sin are multiplied by factor (the attention factor of tables that
@@ -827,7 +827,7 @@ typedef struct i4_heads {
  * fastest). */
 int    i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B, int T, int head_dim,
                const i4_rotary* rotary, const int32_t* pos_dev, int pos, const i4_turn* turn,
-               const int32_t* counts, hipStream_t stream);
+               const int32_t* counts, int zero_padding, hipStream_t stream);
 
 /* A 16-bit cache in pages: position j of sequence b is row j % page of page
  * table[b][j / page], k and v [pages][n_kv_heads][page][head_dim] with strides in elements (the
@@ -856,16 +856,16 @@ int    i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batch_stride
                        int64_t token_stride, int n_heads, const void* q_norm_w,
                        const void* k_norm_w, float eps, const i4_rotary* rotary,
                        const int32_t* pos_dev, int pos, const i4_turn* turn,
-                       const int32_t* counts, void* q_out, const i4_pagedcache* cache,
-                       hipStream_t stream);
+                       const int32_t* counts, int zero_padding, void* q_out,
+                       const i4_pagedcache* cache, hipStream_t stream);
 
 /* i4_attn_window over pages.  Workspace: i4_attn_paged_workspace_bytes, keys = pos + T, or
  * table_len page for a device position. */
 int    i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                      int64_t q_token_stride, int64_t q_head_stride, int n_heads,
                      const i4_pagedcache* cache, const int32_t* pos_dev, int pos,
-                     const int32_t* counts, int window, int sinks, float scale, void* out,
-                     void* workspace, size_t workspace_bytes, int32_t* counters,
+                     const int32_t* counts, int zero_padding, int window, int sinks, float scale,
+                     void* out, void* workspace, size_t workspace_bytes, int32_t* counters,
                      hipStream_t stream);
 size_t i4_attn_paged_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                      int window, int sinks);

@@ -227,14 +227,15 @@ SIGNATURES = {
                             POINTER(KV8CacheC), c_void_p, c_int, c_void_p, c_int, c_int,
                             ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "i4_rope": (c_int, [POINTER(HeadsC), POINTER(HeadsC), c_int, c_int, c_int, c_int,
-                        POINTER(RotaryC), c_void_p, c_int, POINTER(TurnC), c_void_p, c_void_p]),
+                        POINTER(RotaryC), c_void_p, c_int, POINTER(TurnC), c_void_p, c_int,
+                        c_void_p]),
     "i4_paged_append": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int, c_void_p,
                                 c_void_p, ctypes.c_float, POINTER(RotaryC), c_void_p, c_int,
-                                POINTER(TurnC), c_void_p, c_void_p, POINTER(PagedCacheC),
-                                c_void_p]),
+                                POINTER(TurnC), c_void_p, c_int, c_void_p,
+                                POINTER(PagedCacheC), c_void_p]),
     "i4_attn_paged": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
                               POINTER(PagedCacheC), c_void_p, c_int, c_void_p, c_int, c_int,
-                              ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+                              c_int, ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "i4_attn_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int,
                                                  c_int]),
     "i4_dmoe_forward": (c_int, [c_void_p, c_int, c_int, POINTER(DmoeWeightsC), c_int, c_int,

@@ -38,6 +38,7 @@ struct CtxArgs {
   float* ml;              // [2] each: maximum and sum
   int32_t* counters;      // nullable: parts of a kv head that are done, 0 between calls
   Pages pg;               // the 16-bit cache in pages
+  int32_t zero;           // whether the padding's rows are set to zero (pages)
   int32_t* plan;          // of a call whose tiles are shared out (k_ctx_tile), or null
 };
 

@@ -217,8 +217,8 @@ int i4_attn_kv8(const void* q, int x_dtype, int T, int64_t q_batch_stride, int64
 int i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                   int64_t q_token_stride, int64_t q_head_stride, int n_heads,
                   const i4_pagedcache* cache, const int32_t* pos_dev, int pos,
-                  const int32_t* counts, int window, int sinks, float scale, void* out,
-                  void* workspace, size_t workspace_bytes, int32_t* counters,
+                  const int32_t* counts, int zero_padding, int window, int sinks, float scale,
+                  void* out, void* workspace, size_t workspace_bytes, int32_t* counters,
                   hipStream_t stream) {
   using namespace i4;
   int rc = i4_check_pagedcache(cache);
@@ -234,6 +234,7 @@ int i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
   CtxArgs a = ctx_args(q, B, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,
                        pos, counts, window, sinks, scale, out);
   a.pg = i4_pages_of(cache);
+  a.zero = zero_padding;
   a.len = len;
   return launch(a, x_dtype, kPaged, keys, i4_span{window, sinks, workspace, counters}, stream);
 }

@@ -580,6 +580,9 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
       *(f32x4*)&s_o[wave][m][32 * qd + 8 * i + e] =
           f32x4{acc.o[e][i], acc.o[e + 1][i], acc.o[e + 2][i], acc.o[e + 3][i]};
   __syncthreads();
+  if constexpr (FMT == kPaged)
+    if (a.zero && split == 0 && r < a.R && t >= sq.have)
+      *(u32x4*)(a.out + ctx_out_of(a, b, g, r, t) + d0) = u32x4{};
   if (r < a.R && t < sq.have) {
     float M = -__builtin_inff(), L = 0.f, o[8];
 #pragma unroll

@@ -653,6 +653,11 @@ __global__ __launch_bounds__(256, 2) void k_ctx_tile(CtxArgs a) {
         }
       }
     }
+    if constexpr (FMT == kPaged && !SHARED)
+      if (a.zero && split == 0 && r < a.R && t >= sq.have) {
+        u32* y = (u32*)(a.out + ctx_out(a, b, g, r)) + 32 * h;
+        for (int i = 0; i < 32; ++i) y[i] = 0;
+      }
     // tokens whose position is outside the cache (the merge writes them when there is one)
     if (!SHARED && a.S == 1 && r < a.R && t >= sq.fit && t < sq.have) {
       u32* y = (u32*)(a.out + ctx_out(a, b, g, r)) + 32 * h;
@@ -726,15 +731,19 @@ template <int XT, int P> __global__ __launch_bounds__(256) void k_ctx_merge(CtxA
   else *y = u32x2{pack2<XT>(o[0] / L, o[1] / L), pack2<XT>(o[2] / L, o[3] / L)};
 }
 
-// The parts of row tiles that several runs share, and the rows of tokens outside the cache: eight
+// The parts of row tiles that several runs share, and the rows of other tokens: eight
 // rows a workgroup, a row to 32 lanes of 4 dims.
 template <int XT> __global__ __launch_bounds__(256) void k_ctx_join(CtxArgs a) {
   const int M = a.B * a.tiles, g = blockIdx.y / M, m = blockIdx.y - g * M;
   const int b = m / a.tiles, rt = m - b * a.tiles, d = 4 * (threadIdx.x & 31);
   const int row = 8 * blockIdx.x + (threadIdx.x >> 5), r = rt * kTileRows + row, t = r / a.G;
   const CtxSeq sq = ctx_seq(a, b);
-  if (r >= a.R || t >= sq.have) return;
+  if (r >= a.R) return;
   u32x2* y = (u32x2*)(a.out + ctx_out(a, b, g, r) + d);
+  if (t >= sq.have) {
+    if (a.zero) *y = u32x2{};
+    return;
+  }
   if (t >= sq.fit) {
     *y = u32x2{} + (u32)Half<XT>::QNAN * 0x10001u;
     return;

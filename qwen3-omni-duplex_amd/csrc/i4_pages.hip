@@ -20,6 +20,7 @@ struct PagedAppend {
   Tokens tk;
   Turn turn;
   int32_t nq, nkv;
+  int32_t zero;  // whether the padding's rows are set to zero
   float eps;
 };
 
@@ -27,7 +28,8 @@ template <int XT, int FORM>
 __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a, RotaryTable<KHD / 2> rt) {
   __shared__ __align__(16) float s_c[KHD / 2], s_s[KHD / 2];
   const int b = blockIdx.x / a.tk.T, t = blockIdx.x % a.tk.T;
-  if (t >= count_of(a.tk, b)) return;
+  const bool have = t < count_of(a.tk, b);
+  if (!have && !a.zero) return;
   const int heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 15;
   const int p0 = first_pos(a.tk, b), len = a.pg.table_len << a.pg.shift;
   // p0 is checked before t is added: a device position may be anything
@@ -37,8 +39,9 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a, RotaryTable
   ok = ok && !slot.bad && turns(a.turn, b, t, p);
   u32x4* q_row = (u32x4*)(a.q_out + (int64_t)blockIdx.x * a.nq * KHD) + lane;
   int h = threadIdx.x >> 4;
-  if (!ok) {
-    for (; h < a.nq; h += 16) q_row[h * (KHD / 8)] = u32x4{} + (u32)Half<XT>::QNAN * 0x10001u;
+  if (!ok || !have) {
+    const u32 fill = have ? (u32)Half<XT>::QNAN * 0x10001u : 0u;
+    for (; h < a.nq; h += 16) q_row[h * (KHD / 8)] = u32x4{} + fill;
     return;
   }
   const u32x4* x_row = (const u32x4*)(a.qkv + b * a.bs + t * a.ts) + lane;
@@ -158,8 +161,8 @@ extern "C" int i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batc
                                int64_t token_stride, int n_heads, const void* q_norm_w,
                                const void* k_norm_w, float eps, const i4_rotary* rotary,
                                const int32_t* pos_dev, int pos, const i4_turn* turn,
-                               const int32_t* counts, void* q_out, const i4_pagedcache* cache,
-                               hipStream_t stream) {
+                               const int32_t* counts, int zero_padding, void* q_out,
+                               const i4_pagedcache* cache, hipStream_t stream) {
   using namespace i4;
   if (!qkv || !q_out) return I4_ERR_NULL;
   int rc = i4_check_pagedcache(cache);
@@ -178,7 +181,7 @@ extern "C" int i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batc
     return I4_ERR_ALIGN;
   PagedAppend a{(const uint16_t*)qkv, batch_stride, token_stride, (const uint16_t*)q_norm_w,
                 (const uint16_t*)k_norm_w, (uint16_t*)q_out, i4_pages_of(cache),
-                Tokens{pos_dev, counts, pos, T}, turn_of(turn), n_heads, nkv, eps};
+                Tokens{pos_dev, counts, pos, T}, turn_of(turn), n_heads, nkv, zero_padding, eps};
   const RotaryTable<KHD / 2> rt = rotary_table<KHD / 2>(rotary);
   auto go = [&](auto kern) { kern<<<(unsigned)(B * T), 256, 0, stream>>>(a, rt); };
   const bool f16 = x_dtype == I4_F16;

@@ -36,6 +36,7 @@ struct RopeCall {
   int32_t each;   // of them a workgroup
   int32_t hd;     // head_dim
   int32_t items;  // of a head
+  int32_t zero;   // whether the padding's rows are set to zero
 };
 
 template <int XT, int V, int LAYOUT>
@@ -59,7 +60,8 @@ __global__ __launch_bounds__(256) void k_rope(RopeCall a, RotaryTable<kPairs> rt
   for (int i = threadIdx.x; i < total; i += 256) {
     const int rh = i / a.items, c = i - rh * a.items;
     const int r = rh / heads, h = rh - r * heads, b = (row0 + r) / a.tk.T, t = (row0 + r) % a.tk.T;
-    if (t >= count_of(a.tk, b)) continue;
+    const bool have = t < count_of(a.tk, b);
+    if (!have && !a.zero) continue;
     const bool key = h >= a.q.heads;
     const Heads& g = key ? a.k : a.q;
     const int hh = key ? h - a.q.heads : h;
@@ -76,10 +78,12 @@ __global__ __launch_bounds__(256) void k_rope(RopeCall a, RotaryTable<kPairs> rt
     }
     typedef typename Vec<V>::type vec;
     Bits<V> u{}, w{};
-    u.v = *(const vec*)(x + d0);
     const bool two = d1 < a.hd;
-    if (two) w.v = *(const vec*)(x + d1);
-    if (!s_ok[r]) {
+    if (have) {
+      u.v = *(const vec*)(x + d0);
+      if (two) w.v = *(const vec*)(x + d1);
+    }
+    if (have && !s_ok[r]) {
 #pragma unroll
       for (int e = 0; e < V; ++e) u.e[e] = w.e[e] = Half<XT>::QNAN;
     } else {
@@ -165,7 +169,8 @@ int i4_check_rotary(const i4_rotary* r, const i4_turn* t) {
 
 extern "C" int i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B, int T,
                        int head_dim, const i4_rotary* rotary, const int32_t* pos_dev, int pos,
-                       const i4_turn* turn, const int32_t* counts, hipStream_t stream) {
+                       const i4_turn* turn, const int32_t* counts, int zero_padding,
+                       hipStream_t stream) {
   using namespace i4;
   if (!q) return I4_ERR_NULL;
   if (x_dtype != I4_F16 && x_dtype != I4_BF16) return I4_ERR_DTYPE;
@@ -194,6 +199,7 @@ extern "C" int i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B,
   a.rows = B * T;
   a.each = a.rows >= 4096 ? 4 : a.rows >= 2048 ? 2 : 1;
   a.hd = head_dim;
+  a.zero = zero_padding;
   a.items = rotary->layout == I4_ROPE_HALF ? n / v + (head_dim - 2 * n + 2 * v - 1) / (2 * v)
                                            : (head_dim + 2 * v - 1) / (2 * v);
   const RotaryTable<kPairs> rt = rotary_table<kPairs>(rotary);

@@ -182,9 +182,10 @@ def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torc
 def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
             pos: int | torch.Tensor, window: int | None, sinks: int, scale: float | None,
             counts: torch.Tensor | None, out: torch.Tensor | None,
-            workspace: Workspace | None, sizes=None) -> torch.Tensor:
+            workspace: Workspace | None, sizes=None, zero: tuple[bool, ...] = ()) -> torch.Tensor:
     """The call that attn_window, attn_kv8 and attn_paged share; keys: the positions of the
-    cache; sizes: what names the workspace's."""
+    cache; sizes: what names the workspace's; zero: (whether the entry is to set the padding's
+    rows to zero,) of an entry that can."""
     x = _batched(q, 4, "q")
     B, T, nh, hd = x.shape
     if B != cc.batch or hd != cc.head_dim:
@@ -197,20 +198,21 @@ def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
         raise RuntimeError("sinks are the first tokens outside a window: give the window too")
     if x.stride(3) != 1:
         x = x.contiguous()
-    y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd), counts is not None)
+    y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd),
+             counts is not None and not zero)
     on_dev = isinstance(pos, torch.Tensor)
     pd, ph = (_int32(pos, B, dev, "pos"), 0) if on_dev else (None, _host_pos(pos, T, keys))
     w = 0 if window is None else min(window, 2**31 - 1)
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return _attend(entry, cc, keys, q, dev, pos, window, sinks, scale, counts, y,
-                           workspace, sizes)
+                           workspace, sizes, zero)
     need = (sizes or _lib.lib().i4_attn_window_workspace_bytes)(
         B, T, nh, cc.n_kv_heads, keys if on_dev else ph + T, w, sinks)
     ws, counters = _scratch(workspace, need, dev, True) if need else (None, None)
     s0, s1, s2, _ = x.stride()
     rc = entry(x.data_ptr(), _lib.half_code(x.dtype), T, s0, s1, s2, nh, ctypes.byref(cc),
-               pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
+               pd, ph, _int32(counts, B, dev, "counts"), *zero, w, sinks,
                hd ** -0.5 if scale is None else scale, y.data_ptr(), _lib.ptr(ws), need,
                _lib.ptr(counters), _lib.stream(dev))
     if rc:

@@ -14,8 +14,8 @@ that needed it are NaN.
 
 Tokens, positions and counts are those of kv.py: [T, ...] of one sequence (a table [n]) or
 [B, T, ...] of B, token t of sequence b at position pos + t, pos an int or int32 [B] on the
-device.  Every op enqueues on torch's current stream of the tensors' device and does not
-synchronise.
+device.  The padding's rows are zeros in a new output and left as they are in a given one.
+Every op enqueues on torch's current stream of the tensors' device and does not synchronise.
 """
 from __future__ import annotations
 
@@ -108,14 +108,14 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
     if x.stride(2) != 1:
         x = x.contiguous()
     shape = (B, T, n_heads, hd)
-    q = _out(out, x, shape if qkv.dim() == 3 else shape[1:], counts is not None)
+    q = _out(out, x, shape if qkv.dim() == 3 else shape[1:], False)
     on_dev = isinstance(pos, torch.Tensor)
     tc = None if turn is None else _turn_c(turn, rotary, qkv.dim() == 3, B, T, dev)
     _call(dev, _lib.lib().i4_paged_append, x.data_ptr(), cc.dtype, T, x.stride(0), x.stride(1),
           n_heads, _lib.ptr(q_norm_w), _lib.ptr(k_norm_w), eps, rotary._c,
           _int32(pos, B, dev, "pos") if on_dev else None,
           0 if on_dev else _host_pos(pos, T, cc.table_len * cc.page), tc,
-          _int32(counts, B, dev, "counts"), q.data_ptr(), ctypes.byref(cc))
+          _int32(counts, B, dev, "counts"), out is None, q.data_ptr(), ctypes.byref(cc))
     return q
 
 
@@ -132,4 +132,4 @@ def attn_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor,
     cc = cache._with(table, q.shape[0] if q.dim() == 4 else 1, dev)
     lib = _lib.lib()
     return _attend(lib.i4_attn_paged, cc, cc.table_len * cc.page, q, dev, pos, window, sinks, scale,
-                   counts, out, workspace, lib.i4_attn_paged_workspace_bytes)
+                   counts, out, workspace, lib.i4_attn_paged_workspace_bytes, (out is None,))

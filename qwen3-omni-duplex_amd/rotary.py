@@ -19,6 +19,8 @@ import torch
 from . import _lib
 from .kv import _batched, _call, _int32
 
+_HeadsC, _empty = _lib.HeadsC, torch.empty_like
+_DENSE = torch.contiguous_format
 LAYOUTS = {"half": 0, "interleaved": 1}
 MAX_PAIRS = 128
 MAX_POS = 1 << 24
@@ -115,26 +117,27 @@ def _apart(shape: tuple[int, ...], stride: tuple[int, ...]) -> bool:
         shape[1] == 1 or stride[1] >= hd) and (shape[0] == 1 or stride[0] >= hd)
 
 
-def _new(x: torch.Tensor, zeros: bool, held: list[torch.Tensor]) -> _lib.HeadsC:
-    """A dense output for x [B, T, heads, head_dim], appended to held, and struct i4_heads of
-    both.  What the struct points at is held until the call is queued."""
-    shape, a = x.shape, x.stride()
-    if not _apart(shape, a):
+def _new(x: torch.Tensor, T: int, hd: int, held: list[torch.Tensor]) -> _lib.HeadsC:
+    """A dense output for x [B, T, heads, hd], appended to held, and struct i4_heads of both.
+    What the struct points at is held until the call is queued."""
+    B, _, n, _ = x.shape
+    a, b, c, d = x.stride()
+    if d != 1 or c < hd and n > 1 or b < hd and T > 1 or a < hd and B > 1:
         x = x.contiguous()
-        a = x.stride()
+        a, b, c, _ = x.stride()
         held.insert(0, x)
-    y = (torch.zeros_like if zeros else torch.empty_like)(
-        x, memory_format=torch.contiguous_format)
-    _, T, n, hd = shape
+    y = _empty(x, memory_format=_DENSE)
     held.append(y)
-    return _lib.HeadsC(x.data_ptr(), y.data_ptr(), a[0], a[1], a[2], T * n * hd, n * hd, hd, n)
+    return _HeadsC(x.data_ptr(), y.data_ptr(), a, b, c, T * n * hd, n * hd, hd, n)
 
 
 def _into(xs: list[torch.Tensor], out: tuple[torch.Tensor | None, ...],
-          held: list[torch.Tensor]) -> list[_lib.HeadsC]:
+          held: list[torch.Tensor]) -> list[_lib.HeadsC | None]:
     """struct i4_heads of the inputs and the given outputs, checked."""
-    outs = [t for t in out if t is not None]
-    if len(outs) != len(xs):
+    outs = list(out)
+    if len(outs) == 2 and len(xs) == 1 and outs[1] is None:
+        outs.pop()
+    if len(outs) != len(xs) or any(t is None for t in outs):
         raise RuntimeError("out holds a tensor for each input")
     _lib.require_device(*xs, *outs)
     cs = []
@@ -155,7 +158,7 @@ def _into(xs: list[torch.Tensor], out: tuple[torch.Tensor | None, ...],
                 held.append(x)
         cs.append(_lib.HeadsC(x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3],
                               x.shape[2]))
-    return cs
+    return cs if len(cs) > 1 else [cs[0], None]
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotary: Rotary, *,
@@ -172,7 +175,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
     back: rope(rope(x, p), -p) is x to rounding, and the gradient of rope(x, p) is that of its
     output turned by -p.  A position at or behind +-2^24 gives NaN, an int is refused.  q and k
     may have any strides above a dense last dimension, and so may out, a pair of tensors that
-    are q and k themselves (in place) or do not overlap them."""
+    are q and k themselves (in place) or do not overlap them.  Padding (counts,
+    int32 [B] on the device) is zeros in new outputs and left as it is in given ones."""
     dev = _lib.require_device(q, k, counts)
     code = _lib.half_code(q.dtype)
     batched = q.dim() == 4
@@ -200,12 +204,14 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
         turn = _turn_c(pos, rotary, batched, B, T, dev)
     held: list[torch.Tensor] = []  # the new outputs are its last elements
     if out is None:
-        cs = [_new(t, counts is not None, held) for t in xs]
+        qc = _new(x, T, hd, held)
+        kc = None if k is None else _new(xs[1], T, hd, held)
     else:
-        cs = _into(xs, out, held)
-    _call(dev, _lib.lib().i4_rope, cs[0], cs[1] if k is not None else None, code, B, T, hd,
-          rotary._c, pd, ph, turn, None if counts is None else _int32(counts, B, dev, "counts"))
-    ys = held[-len(xs):] if out is None else [t for t in out if t is not None]
-    if not batched and out is None:
-        ys = [y[0] for y in ys]
-    return ys[0] if k is None else tuple(ys)
+        qc, kc = _into(xs, out, held)
+    _call(dev, _lib.lib().i4_rope, qc, kc, code, B, T, hd, rotary._c, pd, ph, turn,
+          None if counts is None else _int32(counts, B, dev, "counts"), out is None)
+    if out is not None:
+        return out[0] if k is None else (out[0], out[1])
+    if not batched:
+        held = [y[0] for y in held]
+    return held[-1] if k is None else (held[-2], held[-1])

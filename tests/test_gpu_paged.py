@@ -42,6 +42,33 @@ def case(dev, B, T, nh, nkv, n, dtype, seed=0):
     return q, rows
 
 
+def dirty(x):
+    """Leaves memory of x's size, not zeros, to the next allocation."""
+    torch.full_like(x, 5.0, memory_format=torch.contiguous_format)
+
+
+@pytest.mark.parametrize("T,nh,pos", [(1, 8, 100), (1, 8, 9000), (2, 8, 500), (40, 8, 100),
+                                      (40, 8, 9000)])
+def test_padding_of_a_new_output_is_zeros(pkg, dev, T, nh, pos):
+    """On every path: one part and several, few rows and many, one sequence (split by its cost)
+    and two (shared out); appended rows too."""
+    for B in (1, 2):
+        q, rows = case(dev, B, T, nh, 2, pos + T, torch.bfloat16)
+        cache, table = pool_of(pkg, dev, rows, [pos + T] * B, 64)
+        for counts in ([T, 0][:B], [0, T - 1][:B], [T // 2, T][:B]):
+            dirty(q)
+            got = pkg.attn_paged(q, cache, table, i32(dev, [pos] * B), counts=i32(dev, counts))
+            want = pkg.attn_paged(q, cache, table, i32(dev, [pos] * B), counts=i32(dev, counts),
+                                  out=torch.full_like(q, 5.0))
+            qkv = rand(dev, B, T, (nh + 4) * HD, seed=3)
+            dirty(q)
+            new = pkg.paged_append(qkv, nh, None, None, 1e-6, pkg.Rotary.plain(HD, 1e4),
+                                   i32(dev, [pos] * B), cache, table, counts=i32(dev, counts))
+            for b, n in enumerate(counts):
+                assert same(got[b, :n], want[b, :n]) and not got[b, n:].any()
+                assert (want[b, n:] == 5.0).all() and not new[b, n:].any() and new[b, :n].any() == (n > 0)
+
+
 # ------------------------------------------------------------------- attention
 
 SHAPES = [
@@ -118,6 +145,7 @@ def test_padding_and_positions_outside(pkg, dev, T):
     for b in range(B):
         check(got[b:b + 1, :fit[b]], want[b:b + 1, :fit[b]], tol[b:b + 1, :fit[b]])
         assert torch.isnan(got[b, fit[b]:have[b]]).all() and (got[b, have[b]:] == 5.0).all()
+    dirty(q)
     fresh = pkg.attn_paged(q, cache, table, i32(dev, pos), counts=i32(dev, counts))
     assert all(same(fresh[b, :have[b]], got[b, :have[b]]) and not fresh[b, have[b]:].any()
                for b in range(B))
@@ -277,9 +305,10 @@ def test_shared_out_tiles(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
         assert (out[b, n:] == 5.0).all()
     ws = pkg.Workspace()
     ws.get(1 << 25, dev).fill_(0xFF)
+    dirty(q)
     again = pkg.attn_paged(q, cache, table, i32(dev, at), workspace=ws, **bounds)
     for b, n in enumerate(counts):
-        assert same(again[b, :n], got[b, :n])
+        assert same(again[b, :n], got[b, :n]) and not again[b, n:].any()
 
 
 @pytest.mark.parametrize("window,sinks", [(None, 0), (90, 20)])

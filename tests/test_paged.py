@@ -52,7 +52,7 @@ def heads(lb, **kw):
 def call_rope(lb, lib, q=None, k=None, r=None, turn=None, **kw):
     a = {**dict(xt=2, B=2, T=4, hd=128, pos_dev=None, pos=0, counts=None), **kw}
     return lib.i4_rope(q or heads(lb), k, a["xt"], a["B"], a["T"], a["hd"], r or rotary(lb),
-                       a["pos_dev"], a["pos"], turn, a["counts"], None)
+                       a["pos_dev"], a["pos"], turn, a["counts"], 0, None)
 
 
 def call_append(lb, lib, c=None, r=None, turn=None, **kw):
@@ -60,7 +60,7 @@ def call_append(lb, lib, c=None, r=None, turn=None, **kw):
                 counts=None, out=P), **kw}
     return lib.i4_paged_append(a["qkv"], a["xt"], a["T"], a["bs"], a["ts"], a["nh"], a["qw"],
                                a["kw"], 1e-6, r or rotary(lb), a["pos_dev"], a["pos"], turn,
-                               a["counts"], a["out"], c or cache(lb), None)
+                               a["counts"], 0, a["out"], c or cache(lb), None)
 
 
 def call_attn(lb, lib, c=None, **kw):
@@ -68,7 +68,7 @@ def call_attn(lb, lib, c=None, **kw):
                 counts=None, window=0, sinks=0, scale=0.1, out=P, ws=P, wsb=1 << 40,
                 counters=None), **kw}
     return lib.i4_attn_paged(a["q"], a["xt"], a["T"], a["bs"], a["ts"], a["hs"], a["nh"],
-                             c or cache(lb), a["pos_dev"], a["pos"], a["counts"], a["window"],
+                             c or cache(lb), a["pos_dev"], a["pos"], a["counts"], 0, a["window"],
                              a["sinks"], a["scale"], a["out"], a["ws"], a["wsb"], a["counters"],
                              None)
 
