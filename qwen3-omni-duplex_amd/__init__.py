@@ -37,7 +37,7 @@ from .ops import (dequant, dequant_gemv, linear, moe_down_combine, moe_down_wait
                   dmoe_status, dmoe_down_wait, StackLayerX)
 from .kv import KV8Cache, attn_kv8, attn_window, kv8_append, rope_append
 from .paged import PagedCache, attn_paged, paged_append
-from .rotary import Rotary, rope
+from .rotary import Rotary, interleaved_axes, rope
 from .weights import QWeight, repack_awq_to_ct, repack_tile
 
 lib = _lib.lib
@@ -58,5 +58,5 @@ __all__ = [
     "FusedMoE", "fuse_moe_blocks", "quantize_q8", "dmoe_forward", "dmoe_status",
     "dmoe_down_wait", "StackLayerX",
     "KV8Cache", "attn_kv8", "attn_window", "kv8_append", "rope_append",
-    "PagedCache", "paged_append", "attn_paged", "Rotary", "rope",
+    "PagedCache", "paged_append", "attn_paged", "Rotary", "interleaved_axes", "rope",
 ]

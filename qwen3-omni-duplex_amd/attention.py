@@ -16,7 +16,8 @@ i4_attn_decode_qkv_o.  The KV cache is preallocated
 transformers' growing DynamicCache.
 
 Prompts and chunks of several tokens, a bounded context (window, sinks) and an 8-bit cache
-(kv_dtype) run launch by launch instead, on rope_append and attn_window / attn_kv8 (kv.py).
+(kv_dtype) run launch by launch instead, on rope_append and attn_window / attn_kv8 (kv.py), and
+so do many sessions on one pool of pages (paged_append and attn_paged, paged.py).
 Those round less often than the decode entries: a cache that holds a prompt's keys and later
 tokens' keys holds both roundings, several half steps of the dtype apart.
 """
@@ -28,6 +29,8 @@ import torch.nn as nn
 from . import _lib, kv, ops
 from .linear import PackedLinear, PackedQKV
 from .moe import FusedPackedMoE
+from .paged import PagedCache, attn_paged, paged_append
+from .rotary import Rotary
 
 
 def rope_inv_freq(head_dim: int, theta: float) -> torch.Tensor:
@@ -44,15 +47,25 @@ class ThinkerAttention(nn.Module):
     `sinks` ones; None: every position.  kv_dtype torch.int8 or torch.float8_e4m3fn: the cache
     is a KV8Cache (self.kv8) instead of the 16-bit k_cache / v_cache, tokens arrive in order,
     and max_len is rounded up to whole blocks of 64.  A prompt over it differs from the same
-    tokens one by one by what 8 bits do to the blocks that it finishes (kv.attn_kv8)."""
+    tokens one by one by what 8 bits do to the blocks that it finishes (kv.attn_kv8).
+
+    pages: the cache is a pool (self.paged, a PagedCache) of that many pages of `page` positions
+    instead; a call then takes B sequences and says with `table` which pages are theirs, and
+    max_len is no bound (a sequence's is its table's width).  rotary: another rotary embedding
+    than the plain one of rope_theta; it needs pages."""
 
     def __init__(self, qkv: PackedQKV, o_proj: PackedLinear, q_norm_w: torch.Tensor,
                  k_norm_w: torch.Tensor, input_norm_w: torch.Tensor, n_heads: int,
                  n_kv_heads: int, head_dim: int = 128, eps: float = 1e-6,
                  rope_theta: float = 1_000_000.0, max_len: int = 4096,
                  window: int | None = None, sinks: int = 0,
-                 kv_dtype: torch.dtype | None = None):
+                 kv_dtype: torch.dtype | None = None, pages: int | None = None, page: int = 64,
+                 rotary: Rotary | None = None):
         super().__init__()
+        if pages is not None and kv_dtype is not None:
+            raise ValueError("pages hold 16 bits: no kv_dtype")
+        if pages is None and rotary is not None:
+            raise ValueError("another rotary embedding needs a cache in pages")
         if window is not None and window < 1 or sinks < 0 or (window is None and sinks):
             raise ValueError("window must be at least 1, and sinks need a window")
         if qkv.lin.w.layout != "ct":
@@ -72,7 +85,10 @@ class ThinkerAttention(nn.Module):
         self.window, self.sinks = window, int(sinks)
         self.kv8 = None if kv_dtype is None else kv.KV8Cache.empty(
             n_kv_heads, max_len, head_dim, dtype=dt, kind=kv_dtype, device=dev)
-        shape = (n_kv_heads, max_len if kv_dtype is None else 0, head_dim)
+        self.paged = None if pages is None else PagedCache.empty(
+            n_kv_heads, pages, page, head_dim, dtype=dt, device=dev)
+        self.rotary = Rotary(self.inv_freq) if pages is not None and rotary is None else rotary
+        shape = (n_kv_heads, max_len if kv_dtype is None and pages is None else 0, head_dim)
         self.register_buffer("_k_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
         self.register_buffer("_v_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
         self.max_len = int(max_len) if self.kv8 is None else self.kv8.max_len
@@ -96,6 +112,9 @@ class ThinkerAttention(nn.Module):
         self._v_cache.zero_()
         if self.kv8 is not None:
             self.kv8.reset()
+        if self.paged is not None:
+            self.paged.k.zero_()
+            self.paged.v.zero_()
 
     def _apply(self, fn, *args, **kwargs):
         super()._apply(fn, *args, **kwargs)
@@ -105,20 +124,33 @@ class ThinkerAttention(nn.Module):
             if (k_tail.device, k_tail.dtype) != (w.device, w.dtype):
                 self.kv8 = kv.KV8Cache(*(t.to(w.device) for t in blocks),
                                        k_tail.to(w.device, w.dtype), v_tail.to(w.device, w.dtype))
+        if self.paged is not None:
+            k, v = self.paged.k, self.paged.v
+            if (k.device, k.dtype) != (w.device, w.dtype):
+                self.paged = PagedCache(k.to(w.device, w.dtype), v.to(w.device, w.dtype))
         return self
 
     def whole_context(self) -> bool:
-        """Whether tokens attend a 16-bit cache without a bound, as the decode entries do."""
-        return self.window is None and self.kv8 is None
+        """Whether tokens attend one run of 16-bit rows without a bound, as the decode entries
+        do."""
+        return self.window is None and self.kv8 is None and self.paged is None
 
     def __setattr__(self, name, value):
         super().__setattr__(name, value)
         ops.weights_changed()
 
     def forward(self, h: torch.Tensor, pos: int | torch.Tensor,
-                context_workspace: ops.Workspace | None = None) -> torch.Tensor:
+                context_workspace: ops.Workspace | None = None, *,
+                table: torch.Tensor | None = None, counts: torch.Tensor | None = None,
+                turn: torch.Tensor | None = None) -> torch.Tensor:
         """h [T, H] or [1, T, H] (T tokens of one sequence at cache positions pos, pos + 1, ...)
         -> h + o_proj(attn(norm(h))).
+
+        With a cache in pages h is [T, H] of one sequence or [B, T, H] of B, pos an int or int32
+        [B] on the device, table [n] or [B, n] the sequences' pages, counts (int32 [B] on the
+        device) how many of the tokens each has (the rest is padding, whose rows of the result
+        mean nothing), and turn the rotary embedding's positions where they are not the tokens'
+        own (paged.paged_append).
 
         pos is an int, or an int32 device tensor of one element that the kernels read (a
         decode step captured in a hipGraph then serves every token; a position outside the
@@ -128,6 +160,13 @@ class ThinkerAttention(nn.Module):
         T = h.numel() // h.shape[-1]
         if T < 1:
             raise ValueError("no token")
+        if (self.paged is None) != (table is None):
+            raise ValueError("a table goes with a cache in pages, and the other way round")
+        if self.paged is not None:
+            return self._attend_pages(h, pos, table, counts, turn,
+                                      context_workspace or self.context_workspace)
+        if counts is not None or turn is not None:
+            raise ValueError("counts and turn need a cache in pages")
         if h.dim() > 2 and h.shape[-2] != T:  # [B, T, H]: several sequences share no cache
             raise ValueError(f"h {tuple(h.shape)} holds tokens of several sequences")
         if not isinstance(pos, torch.Tensor) and not 0 <= pos <= self.max_len - T:
@@ -170,11 +209,29 @@ class ThinkerAttention(nn.Module):
             a = kv.attn_kv8(q, self.kv8, pos, **bounds)
         else:
             a = kv.attn_window(q, k, v, pos, **bounds)
+        return self._out(a, x).view(h.shape)
+
+    def _attend_pages(self, h: torch.Tensor, pos: int | torch.Tensor, table: torch.Tensor,
+                      counts: torch.Tensor | None, turn: torch.Tensor | None,
+                      workspace: ops.Workspace) -> torch.Tensor:
+        """Tokens of one sequence or several over the pages, launch by launch."""
+        if h.dim() not in (2, 3):
+            raise ValueError(f"h {tuple(h.shape)} is not [T, H] or [B, T, H]")
+        x = h.reshape(-1, h.shape[-1])
+        qkv = self.qkv.lin(ops.rmsnorm(x, self.input_norm_w, self.eps))
+        q = paged_append(qkv.view(*h.shape[:-1], -1), self.n_heads, self.q_norm_w, self.k_norm_w,
+                         self.eps, self.rotary, pos, self.paged, table, turn=turn, counts=counts)
+        a = attn_paged(q, self.paged, table, pos, window=self.window, sinks=self.sinks,
+                       counts=counts, workspace=workspace)
+        return self._out(a, x).view(h.shape)
+
+    def _out(self, a: torch.Tensor, x: torch.Tensor) -> torch.Tensor:
+        """x + o_proj of the tokens' heads."""
         a = a.view(x.shape[0], -1)
         if x.shape[0] == 1:  # the residual enters the o_proj launch as its bias
-            return ops.linear(a, self.o_proj.w, bias=x.reshape(-1)).view(h.shape)
+            return ops.linear(a, self.o_proj.w, bias=x.reshape(-1))
         # (several tokens: o_proj's output is rounded, then the sum with the residual)
-        return self.o_proj(a).add_(x).view(h.shape)
+        return self.o_proj(a).add_(x)
 
 
 class ThinkerDecoderLayer(nn.Module):
@@ -200,8 +257,9 @@ class ThinkerDecoderLayer(nn.Module):
         return self._fused
 
     def forward(self, h: torch.Tensor, pos: int | torch.Tensor,
-                context_workspace: ops.Workspace | None = None) -> torch.Tensor:
-        if h.numel() == h.shape[-1] and self.fused():
+                context_workspace: ops.Workspace | None = None, **pages) -> torch.Tensor:
+        """pages: ThinkerAttention's table, counts and turn, with a cache in pages."""
+        if h.numel() == h.shape[-1] and not pages and self.fused():
             a, m = self.attn, self.moe
             if not isinstance(pos, torch.Tensor) and not 0 <= pos < a.max_len:
                 raise ValueError(f"position {pos} outside the cache (max_len {a.max_len})")
@@ -210,19 +268,21 @@ class ThinkerDecoderLayer(nn.Module):
                 a.k_norm_w, a.inv_freq, pos, a.k_cache, a.v_cache, a.o_proj.w, m.gate_up,
                 m.down, m.top_k, m.router_w, m.norm_weight, m.norm_eps, m.norm_topk_prob,
                 a.workspace)
-        return self.unfused(h, pos, context_workspace)
+        return self.unfused(h, pos, context_workspace, **pages)
 
     def unfused(self, h: torch.Tensor, pos: int | torch.Tensor,
-                context_workspace: ops.Workspace | None = None) -> torch.Tensor:
+                context_workspace: ops.Workspace | None = None, **pages) -> torch.Tensor:
         """The attention block, then the MoE block (each its own entry points)."""
-        h = self.attn(h, pos, context_workspace)
+        h = self.attn(h, pos, context_workspace, **pages)
         return self.moe(h, residual=h)
 
 
 class ThinkerDecoder(nn.Module):
     """Thinker[0:n] decode: step(h, pos) runs every layer on one token, or on the several
     tokens of a prompt, and returns the hidden state after the last layer (the clock path's
-    layer-24 tap, clock.py:168)."""
+    layer-24 tap, clock.py:168).  With caches in pages step(h, pos, table=...) takes several
+    sequences (ThinkerAttention.forward): every layer has a pool of its own, and one table serves
+    them all."""
 
     def __init__(self, layers: list[ThinkerDecoderLayer]):
         super().__init__()
@@ -268,8 +328,9 @@ class ThinkerDecoder(nn.Module):
                 sizes(l) == sizes(ls[0]) for l in ls)
         return self._fused
 
-    def step(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
-        if h.numel() == h.shape[-1] and self.fused():
+    def step(self, h: torch.Tensor, pos: int | torch.Tensor, **pages) -> torch.Tensor:
+        """pages: ThinkerAttention's table, counts and turn, with caches in pages."""
+        if h.numel() == h.shape[-1] and not pages and self.fused():
             a0, m0 = self.layers[0].attn, self.layers[0].moe
             if not isinstance(pos, torch.Tensor) and not 0 <= pos < a0.max_len:
                 raise ValueError(f"position {pos} outside the cache (max_len {a0.max_len})")
@@ -277,12 +338,12 @@ class ThinkerDecoder(nn.Module):
                 h, self._structs(), len(self.layers), a0.n_heads, a0.n_kv_heads, a0.head_dim,
                 a0.inv_freq, pos, a0.max_len, m0.hidden, m0.down.K, m0.gate_up.E, m0.top_k,
                 m0.norm_topk_prob, self.workspace)
-        return self.unfused(h, pos)
+        return self.unfused(h, pos, **pages)
 
-    def unfused(self, h: torch.Tensor, pos: int | torch.Tensor) -> torch.Tensor:
+    def unfused(self, h: torch.Tensor, pos: int | torch.Tensor, **pages) -> torch.Tensor:
         """Layer by layer (each its own i4_thinker_layer_decode or module calls)."""
         for layer in self.layers:
-            h = layer(h, pos, self.context_workspace)
+            h = layer(h, pos, self.context_workspace, **pages)
         return h
 
     forward = step

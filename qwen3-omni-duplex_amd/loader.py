@@ -32,9 +32,10 @@ from pathlib import Path
 
 import torch
 
-from .attention import ThinkerAttention, ThinkerDecoder, ThinkerDecoderLayer
+from .attention import ThinkerAttention, ThinkerDecoder, ThinkerDecoderLayer, rope_inv_freq
 from .linear import PackedLinear, PackedQKV
 from .moe import FusedPackedMoE
+from .rotary import Rotary, interleaved_axes
 from .weights import QWeight
 
 PREFIX = "thinker.model.layers"
@@ -223,17 +224,33 @@ def rope_theta(tc: dict) -> float:
     return 10000.0
 
 
+def thinker_rotary(tc: dict, head_dim: int) -> Rotary:
+    """The rotary embedding of a text config: the default table, and where it has interleaved
+    sections (mrope_section) the axes of the tokens of images, video and audio."""
+    sections, interleaved = None, False
+    for src in (tc.get("rope_parameters") or {}, tc.get("rope_scaling") or {}):
+        sections = src.get("mrope_section", sections)
+        interleaved |= bool(src.get("mrope_interleaved") or src.get("interleaved"))
+    table = rope_inv_freq(head_dim, rope_theta(tc))
+    if not interleaved or not sections or sum(sections) != table.numel():
+        return Rotary(table)
+    return Rotary(table, axes=interleaved_axes(sections))
+
+
 def load_thinker_layer(ckpt: Checkpoint, layer: int, device="cuda", dtype=torch.bfloat16,
                        max_len: int = 4096, layouts: str = "both",
                        **context) -> ThinkerDecoderLayer:
-    """One Thinker decoder layer for decode (context: ThinkerAttention's window, sinks and
-    kv_dtype): attention (input_layernorm, q|k|v in one
+    """One Thinker decoder layer for decode (context: ThinkerAttention's window, sinks,
+    kv_dtype, pages, page and rotary, with pages by default the config's with its axes):
+    attention (input_layernorm, q|k|v in one
     launch, q_norm / k_norm, rotary, KV cache of max_len positions, o_proj) and the MoE
     block with its post_attention_layernorm (clock.py:45-103 loads the same tensors)."""
     tc = ckpt.text_config()
     base = f"{PREFIX}.{layer}"
     nh, nkv = int(tc["num_attention_heads"]), int(tc["num_key_value_heads"])
     hd = int(tc.get("head_dim") or tc["hidden_size"] // nh)
+    if context.get("pages") is not None and context.get("rotary") is None:
+        context = {**context, "rotary": thinker_rotary(tc, hd)}
     proj = load_attention(ckpt, layer, device, fuse_qkv=True)
     attn = ThinkerAttention(
         proj["qkv"], proj["o"],
@@ -248,7 +265,7 @@ def load_thinker_decoder(root: str | Path, n_layers: int = 24, device="cuda",
                          dtype=torch.bfloat16, max_len: int = 4096,
                          **context) -> ThinkerDecoder:
     """Thinker[0:n_layers] for decode steps and prompts (the clock path's prefix); context:
-    ThinkerAttention's window, sinks and kv_dtype."""
+    ThinkerAttention's window, sinks, kv_dtype, pages, page and rotary."""
     ckpt = Checkpoint(root)
     return ThinkerDecoder([load_thinker_layer(ckpt, layer, device, dtype, max_len, **context)
                            for layer in range(n_layers)])

@@ -86,6 +86,16 @@ class Rotary:
                 + (f", axes={self.axes}" if self.axes else "") + ")")
 
 
+def interleaved_axes(sections: Sequence[int]) -> tuple[int, ...]:
+    """The axes of a multimodal rotary embedding whose sections are interleaved: the pairs take
+    the axes in turn, axis a > 0 for its sections[a] first turns, and axis 0 otherwise."""
+    axes = [0] * sum(sections)
+    for a in range(1, len(sections)):
+        for i in range(a, min(len(axes), len(sections) * sections[a]), len(sections)):
+            axes[i] = a
+    return tuple(axes)
+
+
 def _turn_c(turn: torch.Tensor, rotary: Rotary, batched: bool, B: int, T: int,
             dev: torch.device) -> _lib.TurnC:
     """struct i4_turn of given positions [B, T] or [axes, B, T] ([T] or [axes, T] for tokens
