@@ -1,9 +1,9 @@
 // Rows of the fused q|k|v projection into a cache in pages: RMSNorm of the queries and keys (if
 // the model has it), rotary embedding, and keys and values to the rows of their positions'
-// pages.  fp32 inside, rounded once.  Bound by the rows' bytes.  A workgroup takes one token:
-// its angles are computed once, for all heads; a head is 16 lanes of 8 dims, so that a half
-// pair's other dim is in a lane pairs / 8 away (8 for a whole head: half a DPP row), and a
-// neighbour's is in the same lane.
+// pages.  fp32 inside, rounded once.  Bound by the rows' bytes.  A workgroup takes one token
+// (several share its heads where tokens are few): its angles are computed once; a head is 16
+// lanes of 8 dims, so that a half pair's other dim is in a lane pairs / 8 away (8 for a whole
+// head: half a DPP row), and a neighbour's is in the same lane.
 #include "i4_rotary.h"
 
 namespace i4 {
@@ -30,7 +30,13 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a, RotaryTable
   const int b = blockIdx.x / a.tk.T, t = blockIdx.x % a.tk.T;
   const bool have = t < count_of(a.tk, b);
   if (!have && !a.zero) return;
-  const int heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 15;
+  const int heads = a.nq + 2 * a.nkv, lane = threadIdx.x & 15, step = 16 * gridDim.y;
+  int h = 16 * blockIdx.y + (threadIdx.x >> 4);
+  // on their way while the position, then its page are looked up and the angles computed
+  const u32x4* x_row = (const u32x4*)(a.qkv + b * a.bs + t * a.ts) + lane;
+  u32x4 raw = have && h < heads ? x_row[h * (KHD / 8)] : u32x4{};
+  const u32x4 qn = a.qw ? ((const u32x4*)a.qw)[lane] : u32x4{};
+  const u32x4 kn = a.kw ? ((const u32x4*)a.kw)[lane] : u32x4{};
   const int p0 = first_pos(a.tk, b), len = a.pg.table_len << a.pg.shift;
   // p0 is checked before t is added: a device position may be anything
   bool ok = p0 >= 0 && p0 < len && t < len - p0;
@@ -38,16 +44,11 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a, RotaryTable
   const PageRows slot = page_rows(a.pg, a.pg.table + b * a.pg.ts, 0, p);
   ok = ok && !slot.bad && turns(a.turn, b, t, p);
   u32x4* q_row = (u32x4*)(a.q_out + (int64_t)blockIdx.x * a.nq * KHD) + lane;
-  int h = threadIdx.x >> 4;
   if (!ok || !have) {
     const u32 fill = have ? (u32)Half<XT>::QNAN * 0x10001u : 0u;
-    for (; h < a.nq; h += 16) q_row[h * (KHD / 8)] = u32x4{} + fill;
+    for (; h < a.nq; h += step) q_row[h * (KHD / 8)] = u32x4{} + fill;
     return;
   }
-  const u32x4* x_row = (const u32x4*)(a.qkv + b * a.bs + t * a.ts) + lane;
-  u32x4 raw = h < heads ? x_row[h * (KHD / 8)] : u32x4{};
-  const u32x4 qn = a.qw ? ((const u32x4*)a.qw)[lane] : u32x4{};
-  const u32x4 kn = a.kw ? ((const u32x4*)a.kw)[lane] : u32x4{};
   const int n = rt.n;
   if (threadIdx.x < KHD / 2) {
     const int i = threadIdx.x;
@@ -76,8 +77,8 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a, RotaryTable
     cs[i] = s_c[j];
     sn[i] = FORM != kNext && low ? -s_s[j] : s_s[j];
   }
-  for (; h < heads; h += 16) {
-    const u32x4 next = h + 16 < heads ? x_row[(h + 16) * (KHD / 8)] : u32x4{};
+  for (; h < heads; h += step) {
+    const u32x4 next = h + step < heads ? x_row[(h + step) * (KHD / 8)] : u32x4{};
     u32x4 out = raw;
     if (h < a.nq + a.nkv) {
       const bool norm = h < a.nq ? a.qw != nullptr : a.kw != nullptr;
@@ -183,7 +184,12 @@ extern "C" int i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batc
                 (const uint16_t*)k_norm_w, (uint16_t*)q_out, i4_pages_of(cache),
                 Tokens{pos_dev, counts, pos, T}, turn_of(turn), n_heads, nkv, zero_padding, eps};
   const RotaryTable<KHD / 2> rt = rotary_table<KHD / 2>(rotary);
-  auto go = [&](auto kern) { kern<<<(unsigned)(B * T), 256, 0, stream>>>(a, rt); };
+  // the heads of few tokens are shared out: AAA
+  const int heads = n_heads + 2 * nkv;
+  int shares = 1;
+  while (shares * 16 < heads && (int64_t)B * T * (shares + 1) <= 512) ++shares;
+  const dim3 grid((unsigned)(B * T), (unsigned)shares);
+  auto go = [&](auto kern) { kern<<<grid, 256, 0, stream>>>(a, rt); };
   const bool f16 = x_dtype == I4_F16;
   if (rotary->layout == I4_ROPE_INTERLEAVED) {
     if (f16) go(k_paged_append<I4_F16, kNext>);

@@ -28,91 +28,120 @@ template <int V> union Bits {
   uint16_t e[V];
 };
 
+static constexpr int kTokens = 4;  // of a workgroup at most
+
 struct RopeCall {
   Heads q, k;
   Tokens tk;
   Turn turn;
   int32_t rows;   // tokens of all sequences
   int32_t each;   // of them a workgroup
+  int32_t shares;  // workgroups that share the heads of the same tokens
   int32_t hd;     // head_dim
   int32_t items;  // of a head
   int32_t zero;   // whether the padding's rows are set to zero
 };
 
+// n / d for 0 <= n < 2^22, d > 0: the reciprocal is off by 2^-23 of the quotient, less than the
+// half that is added
+__device__ inline int quotient(int n, int d) {
+  return (int)(((float)n + 0.5f) * __builtin_amdgcn_rcpf((float)d));
+}
+
 template <int XT, int V, int LAYOUT>
 __global__ __launch_bounds__(256) void k_rope(RopeCall a, RotaryTable<kPairs> rt) {
-  __shared__ float s_c[4 * kPairs], s_s[4 * kPairs];
-  __shared__ int s_ok[4];
+  __shared__ __align__(16) float s_c[kTokens * kPairs], s_s[kTokens * kPairs];
+  __shared__ int s_state[kTokens];  // of a token: padding, in range, out of range
+  enum { kPadding, kGood, kOutside };
+  typedef typename Vec<V>::type vec;
   const int n = rt.n, heads = a.q.heads + a.k.heads, row0 = blockIdx.x * a.each;
-  const int rows = min(a.each, a.rows - row0);
-  for (int i = threadIdx.x; i < rows * n; i += 256) {
-    const int r = i / n, j = i - r * n, b = (row0 + r) / a.tk.T, t = (row0 + r) % a.tk.T;
-    // the sum wraps where a start is near the ends of its type: out of range either way
-    const int p = (int)((u32)first_pos(a.tk, b) + (u32)t);
-    if (j == 0) s_ok[r] = turns(a.turn, b, t, p);
-    float c, s;
-    angle_of(turn_pos(a.turn, rt.axis[j], b, t, p), rt.f[j], c, s);
-    s_c[i] = c * rt.factor;
-    s_s[i] = s * rt.factor;
-  }
-  __syncthreads();
-  const int total = rows * heads * a.items;
-  for (int i = threadIdx.x; i < total; i += 256) {
-    const int rh = i / a.items, c = i - rh * a.items;
-    const int r = rh / heads, h = rh - r * heads, b = (row0 + r) / a.tk.T, t = (row0 + r) % a.tk.T;
-    const bool have = t < count_of(a.tk, b);
-    if (!have && !a.zero) continue;
+  const int rows = min(a.each, a.rows - row0), total = rows * heads * a.items;
+  const int b0 = row0 / a.tk.T, t0 = row0 - b0 * a.tk.T;
+  struct Item {
+    Bits<V> u, w;
+    uint16_t* y;
+    int d0, d1, pair, r;
+  };
+  auto load = [&](int i) {
+    Item m{};
+    const int rh = quotient(i, a.items), c = i - rh * a.items;
+    const int r = quotient(rh, heads), h = rh - r * heads;
+    const int over = quotient(t0 + r, a.tk.T), b = b0 + over, t = t0 + r - over * a.tk.T;
     const bool key = h >= a.q.heads;
     const Heads& g = key ? a.k : a.q;
     const int hh = key ? h - a.q.heads : h;
     const uint16_t* x = g.x + b * g.xb + t * g.xt + hh * g.xh;
-    uint16_t* y = g.y + b * g.yb + t * g.yt + hh * g.yh;
-    // the item's first pair and its dims
-    int d0, d1, pair = V * c;
-    if (LAYOUT == I4_ROPE_HALF && pair < n) {
-      d0 = pair, d1 = pair + n;
-    } else if (LAYOUT == I4_ROPE_HALF) {
-      d0 = 2 * n + 2 * (pair - n), d1 = d0 + V;
-    } else {
-      d0 = 2 * pair, d1 = d0 + V;
+    m.y = g.y + b * g.yb + t * g.yt + hh * g.yh;
+    m.r = r;
+    m.pair = V * c;  // the first one, and its dims
+    if (LAYOUT == I4_ROPE_HALF && m.pair < n) {
+      m.d0 = m.pair, m.d1 = m.pair + n;
+    } else {  // neighbours, or dims behind the turned ones
+      m.d0 = 2 * m.pair, m.d1 = m.d0 + V;
     }
-    typedef typename Vec<V>::type vec;
-    Bits<V> u{}, w{};
-    const bool two = d1 < a.hd;
-    if (have) {
-      u.v = *(const vec*)(x + d0);
-      if (two) w.v = *(const vec*)(x + d1);
+    if (t < count_of(a.tk, b)) {
+      m.u.v = *(const vec*)(x + m.d0);
+      if (m.d1 < a.hd) m.w.v = *(const vec*)(x + m.d1);
     }
-    if (have && !s_ok[r]) {
+    return m;
+  };
+  const int step = 256 * gridDim.y;
+  int i = 256 * blockIdx.y + threadIdx.x;
+  Item m{};
+  if (i < total) m = load(i);  // on its way while the angles are computed
+  for (int j = threadIdx.x; j < rows * n; j += 256) {
+    const int r = quotient(j, n), e = j - r * n;
+    const int over = quotient(t0 + r, a.tk.T), b = b0 + over, t = t0 + r - over * a.tk.T;
+    // the sum wraps where a start is near the ends of its type: out of range either way
+    const int p = (int)((u32)first_pos(a.tk, b) + (u32)t);
+    if (e == 0)
+      s_state[r] = t >= count_of(a.tk, b) ? kPadding : turns(a.turn, b, t, p) ? kGood : kOutside;
+    float c, s;
+    angle_of(turn_pos(a.turn, rt.axis[e], b, t, p), rt.f[e], c, s);
+    s_c[j] = c * rt.factor;
+    s_s[j] = s * rt.factor;
+  }
+  __syncthreads();
+  for (; i < total; i += step) {
+    Item next{};
+    if (i + step < total) next = load(i + step);
+    const int state = s_state[m.r];
+    if (state != kGood) {
+      const uint16_t fill = state == kPadding ? (uint16_t)0 : Half<XT>::QNAN;
 #pragma unroll
-      for (int e = 0; e < V; ++e) u.e[e] = w.e[e] = Half<XT>::QNAN;
-    } else {
+      for (int e = 0; e < V; ++e) m.u.e[e] = m.w.e[e] = fill;
+    } else if (LAYOUT != I4_ROPE_HALF || m.pair < n) {
+      const int at = m.r * n + m.pair;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         uint16_t *pa, *pb;
         if constexpr (LAYOUT == I4_ROPE_HALF) {
-          pa = &u.e[e], pb = &w.e[e];
+          pa = &m.u.e[e], pb = &m.w.e[e];
         } else {
-          pa = 2 * e < V ? &u.e[2 * e % V] : &w.e[2 * e % V];
-          pb = 2 * e + 1 < V ? &u.e[(2 * e + 1) % V] : &w.e[(2 * e + 1) % V];
+          pa = 2 * e < V ? &m.u.e[2 * e % V] : &m.w.e[2 * e % V];
+          pb = 2 * e + 1 < V ? &m.u.e[(2 * e + 1) % V] : &m.w.e[(2 * e + 1) % V];
         }
-        if (pair + e < n) {
-          const float cs = s_c[r * n + pair + e], sn = s_s[r * n + pair + e];
+        if (LAYOUT == I4_ROPE_HALF || m.pair + e < n) {
+          const float cs = s_c[at + e], sn = s_s[at + e];
           const float fa = Half<XT>::to_f32(*pa), fb = Half<XT>::to_f32(*pb);
           *pa = Half<XT>::from_f32(fmaf(fa, cs, -(fb * sn)));
           *pb = Half<XT>::from_f32(fmaf(fb, cs, fa * sn));
         }
       }
     }
-    *(vec*)(y + d0) = u.v;
-    if (two) *(vec*)(y + d1) = w.v;
+    if (state != kPadding || a.zero) {
+      *(vec*)(m.y + m.d0) = m.u.v;
+      if (m.d1 < a.hd) *(vec*)(m.y + m.d1) = m.w.v;
+    }
+    m = next;
   }
 }
 
 template <int V>
 static void rope_go(const RopeCall& a, const RotaryTable<kPairs>& rt, int layout, bool f16,
                     hipStream_t s) {
-  auto go = [&](auto kern) { kern<<<(unsigned)((a.rows + a.each - 1) / a.each), 256, 0, s>>>(a, rt); };
+  const dim3 grid((unsigned)((a.rows + a.each - 1) / a.each), (unsigned)a.shares);
+  auto go = [&](auto kern) { kern<<<grid, 256, 0, s>>>(a, rt); };
   if (layout == I4_ROPE_HALF) {
     if (f16) go(k_rope<I4_F16, V, I4_ROPE_HALF>);
     else go(k_rope<I4_BF16, V, I4_ROPE_HALF>);
@@ -197,11 +226,19 @@ extern "C" int i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B,
   a.tk = Tokens{pos_dev, counts, pos, T};
   a.turn = turn_of(turn);
   a.rows = B * T;
-  a.each = a.rows >= 4096 ? 4 : a.rows >= 2048 ? 2 : 1;
   a.hd = head_dim;
   a.zero = zero_padding;
   a.items = rotary->layout == I4_ROPE_HALF ? n / v + (head_dim - 2 * n + 2 * v - 1) / (2 * v)
                                            : (head_dim + 2 * v - 1) / (2 * v);
+  // A token a workgroup, or the heads of one shared out where the chip has room: 24 tokens of 72
+  // heads of 256 dims 6.7 us with one workgroup a token, 3.3 with five.  Two tokens where there
+  // are many (3000 of 36 heads of 128: 12.1, 10.7, 11.3 us with one, two, four), four where a token
+  // is less than half a workgroup's items (3000 of 2 heads: 5.5, 4.2, 3.7), one again where it
+  // is several rounds of them (3000 of 72 heads of 256: 44.1, 46.6, 48.9).
+  const int items = (a.q.heads + a.k.heads) * a.items;
+  a.each = a.rows < 1536 || items > 512 ? 1 : items < 128 ? 4 : 2;
+  a.shares = 1;
+  while (a.shares * 256 < items && (int64_t)a.rows * (a.shares + 1) <= 512) ++a.shares;
   const RotaryTable<kPairs> rt = rotary_table<kPairs>(rotary);
   const bool f16 = x_dtype == I4_F16;
   if (v == 8) rope_go<8>(a, rt, rotary->layout, f16, stream);
