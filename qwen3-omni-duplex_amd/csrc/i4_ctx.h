@@ -140,10 +140,6 @@ template <int XT> __device__ inline f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                    __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <int XT> __device__ inline u32 pack2(float a, float b) {
-  if constexpr (XT == I4_F16) return __builtin_bit_cast(u32, f16x2{(_Float16)a, (_Float16)b});
-  else return __builtin_bit_cast(u32, bf16x2{(__bf16)a, (__bf16)b});
-}
 template <int XT> __device__ inline float lo_f32(u32 x) { return Half<XT>::to_f32((uint16_t)x); }
 template <int XT> __device__ inline float hi_f32(u32 x) {
   return Half<XT>::to_f32((uint16_t)(x >> 16));

@@ -14,6 +14,12 @@ static constexpr int ROPE_MAX_POS = 1 << 24;   // positions that fp32 holds exac
 static constexpr int kMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads: fewer than 2^32
 static constexpr float KV8_TINY = 0x1p-100f;   // floor of a block's largest magnitude
 
+// two values rounded, as a pair
+template <int XT> __device__ inline u32 pack2(float a, float b) {
+  if constexpr (XT == I4_F16) return __builtin_bit_cast(u32, f16x2{(_Float16)a, (_Float16)b});
+  else return __builtin_bit_cast(u32, bf16x2{(__bf16)a, (__bf16)b});
+}
+
 // The tokens of the call's sequences: where each begins and how many it has.
 struct Tokens {
   const int32_t* pos_dev;  // nullable: pos for every sequence

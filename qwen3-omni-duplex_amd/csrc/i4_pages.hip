@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a, RotaryTable
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) ss += x[2 * i] * x[2 * i] + x[2 * i + 1] * x[2 * i + 1];
-        const float r = 1.0f / sqrtf(group_sum<16>(ss) * (1.0f / KHD) + a.eps);
+        const float r = rsqrtf(group_sum<16>(ss) * (1.0f / KHD) + a.eps);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           x[2 * i] *= r * Half<XT>::to_f32((uint16_t)w[i]);
@@ -116,8 +116,7 @@ __global__ __launch_bounds__(256) void k_paged_append(PagedAppend a, RotaryTable
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        out[i] = (u32)Half<XT>::from_f32(y[2 * i]) | ((u32)Half<XT>::from_f32(y[2 * i + 1]) << 16);
+      for (int i = 0; i < 4; ++i) out[i] = pack2<XT>(y[2 * i], y[2 * i + 1]);
     }
     if (h < a.nq) {
       q_row[h * (KHD / 8)] = out;

@@ -26,9 +26,19 @@ template <> struct Vec<1> { typedef uint16_t type; };
 template <int V> union Bits {
   typename Vec<V>::type v;
   uint16_t e[V];
+  u32 pair[(V + 1) / 2];
 };
 
 static constexpr int kTokens = 4;  // of a workgroup at most
+
+template <int XT, int V> __device__ inline void put(Bits<V>& y, const float* x) {
+  if constexpr (V == 1) {
+    y.e[0] = Half<XT>::from_f32(x[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) y.pair[i] = pack2<XT>(x[2 * i], x[2 * i + 1]);
+  }
+}
 
 struct RopeCall {
   Heads q, k;
@@ -110,23 +120,35 @@ __global__ __launch_bounds__(256) void k_rope(RopeCall a, RotaryTable<kPairs> rt
       const uint16_t fill = state == kPadding ? (uint16_t)0 : Half<XT>::QNAN;
 #pragma unroll
       for (int e = 0; e < V; ++e) m.u.e[e] = m.w.e[e] = fill;
-    } else if (LAYOUT != I4_ROPE_HALF || m.pair < n) {
+    } else if (m.pair < n) {
       const int at = m.r * n + m.pair;
+      float x[2 * V];  // u's elements, then w's
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        uint16_t *pa, *pb;
-        if constexpr (LAYOUT == I4_ROPE_HALF) {
-          pa = &m.u.e[e], pb = &m.w.e[e];
-        } else {
-          pa = 2 * e < V ? &m.u.e[2 * e % V] : &m.w.e[2 * e % V];
-          pb = 2 * e + 1 < V ? &m.u.e[(2 * e + 1) % V] : &m.w.e[(2 * e + 1) % V];
-        }
-        if (LAYOUT == I4_ROPE_HALF || m.pair + e < n) {
-          const float cs = s_c[at + e], sn = s_s[at + e];
-          const float fa = Half<XT>::to_f32(*pa), fb = Half<XT>::to_f32(*pb);
-          *pa = Half<XT>::from_f32(fmaf(fa, cs, -(fb * sn)));
-          *pb = Half<XT>::from_f32(fmaf(fb, cs, fa * sn));
-        }
+        x[e] = Half<XT>::to_f32(m.u.e[e]);
+        x[V + e] = Half<XT>::to_f32(m.w.e[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float& fa = x[LAYOUT == I4_ROPE_HALF ? e : 2 * e];
+        float& fb = x[LAYOUT == I4_ROPE_HALF ? V + e : 2 * e + 1];
+        const int p = LAYOUT == I4_ROPE_HALF ? at + e : min(at + e, m.r * n + n - 1);
+        const float cs = s_c[p], sn = s_s[p], u = fa;
+        fa = fmaf(u, cs, -(fb * sn));
+        fb = fmaf(fb, cs, u * sn);
+      }
+      const Bits<V> u = m.u, w = m.w;
+      put<XT, V>(m.u, x);
+      put<XT, V>(m.w, x + V);
+      if (LAYOUT != I4_ROPE_HALF && m.pair + V > n) {  // neighbours behind the turned dims
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (m.pair + e >= n) {
+            if (2 * e < V) m.u.e[2 * e % V] = u.e[2 * e % V];
+            else m.w.e[2 * e % V] = w.e[2 * e % V];
+            if (2 * e + 1 < V) m.u.e[(2 * e + 1) % V] = u.e[(2 * e + 1) % V];
+            else m.w.e[(2 * e + 1) % V] = w.e[(2 * e + 1) % V];
+          }
       }
     }
     if (state != kPadding || a.zero) {
