@@ -47,7 +47,7 @@ struct CtxArgs {
 static constexpr int kPlanned = 1024;
 // What a row tile takes besides its context tiles (its queries, the first loads, its output), in
 // context tiles: it has as many places in the list in front of them.
-static constexpr int kRowTile = 2;
+static constexpr int kRowTile = 3;
 
 // how many runs `total` places are cut into: at least four places each, as many on every XCD
 __host__ __device__ inline int64_t runs_of(int64_t total) {
