@@ -54,6 +54,8 @@ class ThinkerAttention(nn.Module):
     max_len is no bound (a sequence's is its table's width).  rotary: another rotary embedding
     than the plain one of rope_theta; it needs pages."""
 
+    paged: PagedCache | None = None
+
     def __init__(self, qkv: PackedQKV, o_proj: PackedLinear, q_norm_w: torch.Tensor,
                  k_norm_w: torch.Tensor, input_norm_w: torch.Tensor, n_heads: int,
                  n_kv_heads: int, head_dim: int = 128, eps: float = 1e-6,
@@ -85,8 +87,8 @@ class ThinkerAttention(nn.Module):
         self.window, self.sinks = window, int(sinks)
         self.kv8 = None if kv_dtype is None else kv.KV8Cache.empty(
             n_kv_heads, max_len, head_dim, dtype=dt, kind=kv_dtype, device=dev)
-        self.paged = None if pages is None else PagedCache.empty(
-            n_kv_heads, pages, page, head_dim, dtype=dt, device=dev)
+        if pages is not None:
+            self.paged = PagedCache.empty(n_kv_heads, pages, page, head_dim, dtype=dt, device=dev)
         self.rotary = Rotary(self.inv_freq) if pages is not None and rotary is None else rotary
         shape = (n_kv_heads, max_len if kv_dtype is None and pages is None else 0, head_dim)
         self.register_buffer("_k_cache", torch.zeros(shape, dtype=dt, device=dev), persistent=False)
