@@ -26,7 +26,7 @@ import torch
 from . import _lib
 from .kv import _attend, _batched, _call, _host_pos, _int32, _out
 from .ops import Workspace
-from .rotary import Rotary, _turn_c
+from .rotary import Rotary, _turn_c, overlaps
 
 
 class PagedCache:
@@ -45,6 +45,8 @@ class PagedCache:
         pages, n, page, hd = k.shape
         if k.stride(3) != 1 or k.stride(2) != hd:
             raise RuntimeError("the rows of a head's page must be dense")
+        if k.data_ptr() == v.data_ptr():
+            raise RuntimeError("k and v must be pools of their own")
         if page < 16 or page > 1024 or page & (page - 1):
             raise RuntimeError(f"a page holds 16 to 1024 positions, a power of two, got {page}")
         self.k, self.v = k, v
@@ -58,6 +60,9 @@ class PagedCache:
         """A pool of zeros."""
         return cls(*(torch.zeros(pages, n_kv_heads, page, head_dim, dtype=dtype, device=device)
                      for _ in range(2)))
+
+    def __reduce__(self):  # a copy holds its own tensors' addresses
+        return PagedCache, (self.k, self.v)
 
     pages = property(lambda self: self._c[0])
     page = property(lambda self: self._c[1])
@@ -109,6 +114,8 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
         x = x.contiguous()
     shape = (B, T, n_heads, hd)
     q = _out(out, x, shape if qkv.dim() == 3 else shape[1:], False)
+    if out is not None and overlaps(q.view(B, T, n_heads, hd), x.unflatten(2, (-1, hd))):
+        raise RuntimeError("out must not overlap qkv")
     on_dev = isinstance(pos, torch.Tensor)
     tc = None if turn is None else _turn_c(turn, rotary, qkv.dim() == 3, B, T, dev)
     _call(dev, _lib.lib().i4_paged_append, x.data_ptr(), cc.dtype, T, x.stride(0), x.stride(1),
@@ -130,6 +137,9 @@ def attn_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor,
     as attn_window (i4_attn_paged)."""
     dev = _lib.require_device(q, cache.k, counts, out)
     cc = cache._with(table, q.shape[0] if q.dim() == 4 else 1, dev)
+    if out is not None and out.dim() == q.dim() and overlaps(
+            *(_batched(t, 4, "q") for t in (out, q))):
+        raise RuntimeError("out must not overlap q")
     lib = _lib.lib()
     return _attend(lib.i4_attn_paged, cc, cc.table_len * cc.page, q, dev, pos, window, sinks, scale,
                    counts, out, workspace, lib.i4_attn_paged_workspace_bytes, (out is None,))

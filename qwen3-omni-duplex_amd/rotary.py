@@ -81,9 +81,16 @@ class Rotary:
             factor = 0.1 * math.log(scale) + 1 if factor is None else factor
         return cls(f.float(), factor=1.0 if factor is None else factor, **kw)
 
+    def __reduce__(self):
+        return _rebuilt, (self.inv_freq, self.layout, self.factor, self.axes)
+
     def __repr__(self) -> str:
         return (f"Rotary(dims={self.dims}, layout={self.layout!r}, factor={self.factor}"
                 + (f", axes={self.axes}" if self.axes else "") + ")")
+
+
+def _rebuilt(inv_freq, layout, factor, axes) -> Rotary:
+    return Rotary(inv_freq, layout=layout, factor=factor, axes=axes)
 
 
 def interleaved_axes(sections: Sequence[int]) -> tuple[int, ...]:
@@ -115,9 +122,41 @@ def _turn_c(turn: torch.Tensor, rotary: Rotary, batched: bool, B: int, T: int,
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
-    """The first and last byte that a tensor covers."""
+    """The first byte that a tensor covers, and the one behind its last."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() - 1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def overlaps(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether elements of x may be elements of y (of as many dimensions): their memory meets, and
+    they are not separate parts of one strided tensor, as q and k of a fused projection are."""
+    (a, b), (c, d) = _span(x), _span(y)
+    if b <= c or d <= a:
+        return False
+    if a > c:
+        x, y, a, c = y, x, c, a
+    if x.element_size() != y.element_size() or (c - a) % x.element_size():
+        return True
+    dims = []  # (stride, x's size, y's size) where one of them has several
+    for n, s, m, t in zip(x.shape, x.stride(), y.shape, y.stride()):
+        if n > 1 and m > 1 and s != t:
+            return True
+        if n > 1 or m > 1:
+            dims.append((s if n > 1 else t, n, m))
+    # where y begins in x's steps, from the largest; x lies at [0, n) and y at [q, q + m) of each
+    off, apart, inner = (c - a) // x.element_size(), False, []
+    for s, n, m in sorted(dims, reverse=True):
+        q = off // s if s else 0
+        off -= q * s
+        apart |= q >= n
+        inner.append((s, max(n, q + m)))
+    # what the smaller steps reach must stay below a step, or places are not unique
+    reach = off
+    for s, n in reversed(inner):
+        if reach >= s:
+            return True
+        reach += (n - 1) * s
+    return not apart and off == 0
 
 
 def _apart(shape: tuple[int, ...], stride: tuple[int, ...]) -> bool:
@@ -150,19 +189,18 @@ def _into(xs: list[torch.Tensor], out: tuple[torch.Tensor | None, ...],
     if len(outs) != len(xs) or any(t is None for t in outs):
         raise RuntimeError("out holds a tensor for each input")
     _lib.require_device(*xs, *outs)
-    cs = []
-    for t, x in zip(outs, xs):
-        y = _batched(t, 4, "out")
+    cs, ys = [], [_batched(t, 4, "out") for t in outs]
+    if len(ys) > 1 and (overlaps(ys[0], ys[1]) or overlaps(ys[0], xs[1])
+                        or overlaps(ys[1], xs[0])):
+        raise RuntimeError("an output overlaps the other one or the other input")
+    for y, x in zip(ys, xs):
         if y.shape != x.shape or y.dtype != x.dtype:
             raise RuntimeError(f"out must be a {tuple(x.shape)} tensor of {x.dtype}")
         if not _apart(y.shape, y.stride()):
             raise RuntimeError("out's rows must be dense and lie apart")
         if y.data_ptr() != x.data_ptr() or y.stride() != x.stride():  # not in place
-            lo, hi = _span(y)
-            for z in xs:
-                a, b = _span(z)
-                if lo <= b and a <= hi:
-                    raise RuntimeError("out is its input itself or does not overlap the inputs")
+            if overlaps(y, x):
+                raise RuntimeError("out is its input itself or does not overlap it")
             if not _apart(x.shape, x.stride()):
                 x = x.contiguous()
                 held.append(x)
@@ -185,7 +223,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
     back: rope(rope(x, p), -p) is x to rounding, and the gradient of rope(x, p) is that of its
     output turned by -p.  A position at or behind +-2^24 gives NaN, an int is refused.  q and k
     may have any strides above a dense last dimension, and so may out, a pair of tensors that
-    are q and k themselves (in place) or do not overlap them.  Padding (counts,
+    are q and k themselves (in place) or do not overlap them or each other.  Padding (counts,
     int32 [B] on the device) is zeros in new outputs and left as it is in given ones."""
     dev = _lib.require_device(q, k, counts)
     code = _lib.half_code(q.dtype)

@@ -200,6 +200,8 @@ def test_python_refuses(pkg, monkeypatch):
                         (k.float(), k.float(), "float16")):
         with pytest.raises(RuntimeError, match=match):
             pkg.PagedCache(a, b)
+    with pytest.raises(RuntimeError, match="their own"):
+        pkg.PagedCache(k, k)
     c = pkg.PagedCache(k, k.clone())
     q = torch.zeros(2, 3, 4, 128, dtype=bf)
     t = torch.zeros(2, 2, dtype=torch.int32)
@@ -240,8 +242,65 @@ def test_python_refuses(pkg, monkeypatch):
     for x, y in ((room[:, :3], room[:, 1:]), (room[:, 1:], room[:, :3])):
         with pytest.raises(RuntimeError, match="overlap"):
             pkg.rope(x, None, 0, r, out=(y, None))
+    f = torch.zeros(2, 3, 8 * 128, dtype=bf).unflatten(2, (8, 128))
+    for a, b, out in ((f[:, :, :4], f[:, :, 3:], (f[:, :, :4], f[:, :, 3:])),
+                      (f[:, :, :4], f[:, :, :4], (f[:, :, :4], q)),
+                      (f[:, :, :4], f[:, :, 4:], (q, q)),
+                      (f[:, :, :4], f[:, :, 4:], (f[:, :, 4:], f[:, :, :4])),
+                      (f[:, :, :4], f[:, :, 4:], (f[:, :, :4], f[:, :, 3:7]))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            pkg.rope(a, b, 0, r, out=out)
+    with pytest.raises(RuntimeError, match="overlap"):
+        pkg.attn_paged(q, c, t, 0, out=q)
+    rows = torch.zeros(2 * 3 * 8 * 128, dtype=bf)
+    with pytest.raises(RuntimeError, match="overlap"):
+        pkg.paged_append(rows.view(2, 3, -1), 4, w, w, 1e-6, r, 0, c, t,
+                         out=rows[:2 * 3 * 4 * 128].view(2, 3, 4, 128))
     with pytest.raises(RuntimeError, match="apart"):
         pkg.rope(q, None, 0, r, out=(q[:1].expand(2, 3, 4, 128), None))
+
+
+def test_overlap_of_views(pkg):
+    from qwen3_omni_duplex_amd.rotary import overlaps
+
+    f = torch.zeros(3, 5, 10 * 16).unflatten(2, (10, 16))
+    q, k, v = f[:, :, :4], f[:, :, 4:6], f[:, :, 6:]
+    assert not any(overlaps(a, b) for a, b in ((q, k), (k, q), (k, v), (q, v), (v, k)))
+    assert overlaps(q, q) and overlaps(f[:, :, :5], k) and overlaps(k, f[:, :, 5:])
+    assert not overlaps(f[:, :2], f[:, 2:4].clone()) and overlaps(f[:, 1:3], f[:, 2:4])
+    assert not overlaps(f[:1], f[1:2]) and not overlaps(f[:, :1, :4], f[:, :1, 4:])
+    assert not overlaps(f[:, :1, :4], f[:, 1:2, :4])
+    h = f.transpose(1, 2)  # heads before tokens
+    assert not overlaps(h[:, :, :2], h[:, :, 2:]) and overlaps(h[:, :, :3], h[:, :, 2:])
+    assert overlaps(f, f[:, :, :, ::2].expand(3, 5, 10, 8)) and overlaps(f[0:1].expand(3, 5, 10, 16), f)
+    w = torch.zeros(4096)
+    for i in range(300):  # against the elements themselves
+        g = torch.Generator().manual_seed(i)
+        n = torch.randint(1, 4, (2, 3), generator=g).tolist()
+        s = torch.randint(1, 30, (3,), generator=g).tolist()
+        o = torch.randint(0, 60, (2,), generator=g).tolist()
+        x, y = (w.as_strided(n[k], s, o[k]) for k in (0, 1))
+        ids = [set(torch.arange(4096).as_strided(n[k], s, o[k]).flatten().tolist()) for k in (0, 1)]
+        assert overlaps(x, y) or not ids[0] & ids[1]  # it may refuse what is apart, never the reverse
+    one = torch.zeros(64).view(1, 1, 4, 16)
+    assert not overlaps(one[:, :, :2], one[:, :, 2:]) and overlaps(one[:, :, :3], one[:, :, 2:])
+
+
+def test_copies(pkg, monkeypatch):
+    """A copied handle holds its own tensors' addresses."""
+    import copy
+    import pickle
+
+    from qwen3_omni_duplex_amd import _lib
+
+    monkeypatch.setattr(_lib, "require_device", lambda *ts: torch.device("cpu"))
+    c = pkg.PagedCache(*(torch.zeros(4, 2, 16, 128, dtype=torch.bfloat16) for _ in range(2)))
+    d = copy.deepcopy(c)
+    assert d.k.data_ptr() != c.k.data_ptr() and d._c[4] == d.k.data_ptr() and d.pages == 4
+    r = pkg.Rotary.plain(32, 1e4, axes=[0, 1] * 8, factor=1.5, layout="interleaved")
+    for s in (copy.deepcopy(r), pickle.loads(pickle.dumps(r))):
+        assert torch.equal(s.inv_freq, r.inv_freq) and repr(s) == repr(r)
+        assert s._c.inv_freq == s.inv_freq.data_ptr() != r.inv_freq.data_ptr()
 
 
 def test_cpu_tensors_are_refused(pkg):
