@@ -15,6 +15,7 @@ import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libi4moe.so"
 ABI_VERSION = 9
+ERR_WORKSPACE = -7  # I4_ERR_WORKSPACE
 ERR_HANDOFF = -10  # I4_ERR_HANDOFF: the one code a kernel stores in a status word
 
 # element types and layouts (include/i4moe.h)
@@ -92,6 +93,9 @@ class KV8CacheC(ctypes.Structure):
                 ("n_kv_heads", c_int32), ("blocks", c_int32), ("head_dim", c_int32),
                 ("dtype", c_int32), ("format", c_int32)]
 
+
+# The structs of the paged entries come as their bytes (struct.pack: 0.2 us; a Structure's
+# instance and its conversion: 0.8), of a handle's as its address.
 
 class RotaryC(ctypes.Structure):
     """struct i4_rotary"""
@@ -226,15 +230,13 @@ SIGNATURES = {
     "i4_attn_kv8": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
                             POINTER(KV8CacheC), c_void_p, c_int, c_void_p, c_int, c_int,
                             ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
-    "i4_rope": (c_int, [POINTER(HeadsC), POINTER(HeadsC), c_int, c_int, c_int, c_int,
-                        POINTER(RotaryC), c_void_p, c_int, POINTER(TurnC), c_void_p, c_int,
-                        c_void_p]),
+    "i4_rope": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
+                        c_void_p, c_void_p, c_int, c_void_p]),
     "i4_paged_append": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int, c_void_p,
-                                c_void_p, ctypes.c_float, POINTER(RotaryC), c_void_p, c_int,
-                                POINTER(TurnC), c_void_p, c_int, c_void_p,
-                                POINTER(PagedCacheC), c_void_p]),
+                                c_void_p, ctypes.c_float, c_void_p, c_void_p, c_int, c_void_p,
+                                c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "i4_attn_paged": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
-                              POINTER(PagedCacheC), c_void_p, c_int, c_void_p, c_int, c_int,
+                              c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
                               c_int, ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "i4_attn_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int,
                                                  c_int]),

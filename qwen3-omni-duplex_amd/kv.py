@@ -179,40 +179,56 @@ def rope_append(qkv: torch.Tensor, n_heads: int, n_kv_heads: int, q_norm_w: torc
     return q
 
 
+def _held(workspace: Workspace | None, dev: torch.device,
+          stream: int) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """The scratch and the counters that are there already where _scratch would look; nothing
+    under capture, where their owner has to know.  Held by the caller as _scratch's are."""
+    ws = _STREAM_WS.get((dev.index, stream)) if workspace is None else workspace
+    if ws is None:
+        return None, None
+    buf, counters = ws.buf, ws._counters
+    if buf is None or counters is None or buf.device != dev or counters.device != dev \
+            or torch.cuda.is_current_stream_capturing():
+        return None, None
+    return buf, counters
+
+
+def _bounds(window: int | None, sinks: int) -> tuple[int, int]:
+    """The window (0: none) and the first tokens beside it, as the entries take them."""
+    if window is None:
+        if sinks:
+            raise RuntimeError("sinks are the first tokens outside a window: give the window too")
+        return 0, 0
+    if window < 1:
+        raise RuntimeError("window must be at least 1 (None: no bound)")
+    return min(window, 2**31 - 1), min(sinks, 2**31 - 1)
+
+
 def _attend(entry, cc, keys: int, q: torch.Tensor, dev: torch.device,
             pos: int | torch.Tensor, window: int | None, sinks: int, scale: float | None,
             counts: torch.Tensor | None, out: torch.Tensor | None,
-            workspace: Workspace | None, sizes=None, zero: tuple[bool, ...] = ()) -> torch.Tensor:
-    """The call that attn_window, attn_kv8 and attn_paged share; keys: the positions of the
-    cache; sizes: what names the workspace's; zero: (whether the entry is to set the padding's
-    rows to zero,) of an entry that can."""
+            workspace: Workspace | None) -> torch.Tensor:
+    """The call that attn_window and attn_kv8 share; keys: the positions of the cache."""
     x = _batched(q, 4, "q")
     B, T, nh, hd = x.shape
     if B != cc.batch or hd != cc.head_dim:
         raise RuntimeError(f"q {tuple(q.shape)} does not match the cache's batch {cc.batch} and "
                            f"head_dim {cc.head_dim}")
-    if window is not None and window < 1:
-        raise RuntimeError("window must be at least 1 (None: no bound)")
-    sinks = min(sinks, 2**31 - 1)
-    if window is None and sinks:
-        raise RuntimeError("sinks are the first tokens outside a window: give the window too")
+    w, sinks = _bounds(window, sinks)
     if x.stride(3) != 1:
         x = x.contiguous()
-    y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd),
-             counts is not None and not zero)
+    y = _out(out, x, (B, T, nh, hd) if q.dim() == 4 else (T, nh, hd), counts is not None)
     on_dev = isinstance(pos, torch.Tensor)
     pd, ph = (_int32(pos, B, dev, "pos"), 0) if on_dev else (None, _host_pos(pos, T, keys))
-    w = 0 if window is None else min(window, 2**31 - 1)
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
-            return _attend(entry, cc, keys, q, dev, pos, window, sinks, scale, counts, y,
-                           workspace, sizes, zero)
-    need = (sizes or _lib.lib().i4_attn_window_workspace_bytes)(
+            return _attend(entry, cc, keys, q, dev, pos, window, sinks, scale, counts, y, workspace)
+    need = _lib.lib().i4_attn_window_workspace_bytes(
         B, T, nh, cc.n_kv_heads, keys if on_dev else ph + T, w, sinks)
     ws, counters = _scratch(workspace, need, dev, True) if need else (None, None)
     s0, s1, s2, _ = x.stride()
     rc = entry(x.data_ptr(), _lib.half_code(x.dtype), T, s0, s1, s2, nh, ctypes.byref(cc),
-               pd, ph, _int32(counts, B, dev, "counts"), *zero, w, sinks,
+               pd, ph, _int32(counts, B, dev, "counts"), w, sinks,
                hd ** -0.5 if scale is None else scale, y.data_ptr(), _lib.ptr(ws), need,
                _lib.ptr(counters), _lib.stream(dev))
     if rc:

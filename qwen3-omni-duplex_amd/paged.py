@@ -19,14 +19,16 @@ Every op enqueues on torch's current stream of the tensors' device and does not 
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 
 import torch
 
-from . import _lib
-from .kv import _attend, _batched, _call, _host_pos, _int32, _out
+from . import _lib, kv
+from .kv import _batched, _call, _host_pos, _int32, _out
 from .ops import Workspace
 from .rotary import Rotary, _turn_c, overlaps
+
+_paged = struct.Struct("<3Q3q7i4x").pack  # struct i4_pagedcache
 
 
 class PagedCache:
@@ -69,17 +71,22 @@ class PagedCache:
     n_kv_heads = property(lambda self: self._c[2])
     head_dim = property(lambda self: self._c[3])
 
-    def _with(self, table: torch.Tensor, B: int, dev: torch.device) -> _lib.PagedCacheC:
-        """struct i4_pagedcache of this pool under a call's table."""
+    def _with(self, table: torch.Tensor, B: int) -> tuple[bytes, int]:
+        """struct i4_pagedcache of this pool under a call's table, and its positions."""
         shape, stride = table.shape, table.stride()
-        if len(shape) not in (1, 2) or (shape[0] if len(shape) == 2 else 1) != B \
-                or table.dtype != torch.int32 or table.device != dev or shape[-1] < 1 \
-                or stride[-1] != 1 and shape[-1] > 1:
+        if len(shape) == 2 and shape[0] == B:
+            step, n, last = stride[0], shape[1], stride[1]
+        elif len(shape) == 1 and B == 1:
+            step, n, last = 0, shape[0], stride[0]
+        else:
+            n = 0
+        if n < 1 or last != 1 and n > 1 or table.dtype != torch.int32 \
+                or table.get_device() != self.k.get_device():
             raise RuntimeError(f"the table is int32 [{B}, n] on the tensors' device, a sequence's "
                                f"entries adjacent")
-        pages, page, n, hd, k, v, ps, hs, dt = self._c
-        return _lib.PagedCacheC(k, v, table.data_ptr(), ps, hs, stride[0] if B > 1 else 0, B, n,
-                                pages, page, shape[-1], hd, dt)
+        pages, page, heads, hd, k, v, ps, hs, dt = self._c
+        return _paged(k, v, table.data_ptr(), ps, hs, step, B, heads, pages, page, n, hd,
+                      dt), n * page
 
 
 def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
@@ -98,11 +105,11 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
     dev = _lib.require_device(qkv, q_norm_w, k_norm_w, cache.k, turn, counts, out)
     x = _batched(qkv, 3, "qkv")
     B, T, width = x.shape
-    cc = cache._with(table, B, dev)
-    hd = cc.head_dim
-    if cc.dtype != _lib.half_code(x.dtype):
+    cc, keys = cache._with(table, B)
+    _, _, n_kv, hd, _, _, _, _, dtype = cache._c
+    if x.dtype != cache.k.dtype:
         raise RuntimeError("the pages must have the activation dtype")
-    if width != (n_heads + 2 * cc.n_kv_heads) * hd:
+    if width != (n_heads + 2 * n_kv) * hd:
         raise RuntimeError("qkv's width does not match the head counts")
     for w in (q_norm_w, k_norm_w):
         if w is not None and (w.dtype != x.dtype or w.shape != (hd,) or w.stride(0) != 1):
@@ -118,11 +125,11 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
         raise RuntimeError("out must not overlap qkv")
     on_dev = isinstance(pos, torch.Tensor)
     tc = None if turn is None else _turn_c(turn, rotary, qkv.dim() == 3, B, T, dev)
-    _call(dev, _lib.lib().i4_paged_append, x.data_ptr(), cc.dtype, T, x.stride(0), x.stride(1),
-          n_heads, _lib.ptr(q_norm_w), _lib.ptr(k_norm_w), eps, rotary._c,
+    _call(dev, _lib.lib().i4_paged_append, x.data_ptr(), dtype, T, x.stride(0), x.stride(1),
+          n_heads, _lib.ptr(q_norm_w), _lib.ptr(k_norm_w), eps, rotary._at,
           _int32(pos, B, dev, "pos") if on_dev else None,
-          0 if on_dev else _host_pos(pos, T, cc.table_len * cc.page), tc,
-          _int32(counts, B, dev, "counts"), out is None, q.data_ptr(), ctypes.byref(cc))
+          0 if on_dev else _host_pos(pos, T, keys), tc, _int32(counts, B, dev, "counts"),
+          out is None, q.data_ptr(), cc)
     return q
 
 
@@ -136,10 +143,37 @@ def attn_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor,
     (paged_append), and with a window those j > p - window or j < sinks.  The same roundings
     as attn_window (i4_attn_paged)."""
     dev = _lib.require_device(q, cache.k, counts, out)
-    cc = cache._with(table, q.shape[0] if q.dim() == 4 else 1, dev)
-    if out is not None and out.dim() == q.dim() and overlaps(
-            *(_batched(t, 4, "q") for t in (out, q))):
+    x = q if q.dim() == 4 else _batched(q, 4, "q")
+    B, T, nh, hd = shape = x.shape
+    cc, keys = cache._with(table, B)
+    _, _, n_kv, head_dim, _, _, _, _, dtype = cache._c
+    if hd != head_dim:
+        raise RuntimeError(f"q {tuple(q.shape)} does not match the cache's head_dim {head_dim}")
+    w, sinks = kv._bounds(window, sinks)
+    if x.stride(3) != 1:
+        x = x.contiguous()
+    y = _out(out, x, shape if q.dim() == 4 else shape[1:], False)
+    if out is not None and overlaps(out, q):
         raise RuntimeError("out must not overlap q")
-    lib = _lib.lib()
-    return _attend(lib.i4_attn_paged, cc, cc.table_len * cc.page, q, dev, pos, window, sinks, scale,
-                   counts, out, workspace, lib.i4_attn_paged_workspace_bytes, (out is None,))
+    pd, ph = (_int32(pos, B, dev, "pos"), 0) if isinstance(pos, torch.Tensor) \
+        else (None, _host_pos(pos, T, keys))
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return attn_paged(q, cache, table, pos, window=window, sinks=sinks, scale=scale,
+                              counts=counts, out=out, workspace=workspace)
+    lib, s = _lib.lib(), x.stride()
+    args = (x.data_ptr(), _lib.half_code(x.dtype), T, s[0], s[1], s[2], nh, cc, pd, ph,
+            None if counts is None else _int32(counts, B, dev, "counts"), out is None, w, sinks,
+            hd ** -0.5 if scale is None else scale, y.data_ptr())
+    # the workspace that is there, and only if it does not do what the call needs
+    stream = _lib.stream(dev)
+    ws, counters = kv._held(workspace, dev, stream)
+    rc = lib.i4_attn_paged(*args, None, 0, None, stream) if ws is None else lib.i4_attn_paged(
+        *args, ws.data_ptr(), ws.numel(), counters.data_ptr(), stream)
+    if rc == _lib.ERR_WORKSPACE:
+        need = lib.i4_attn_paged_workspace_bytes(B, T, nh, n_kv, keys if pd else ph + T, w, sinks)
+        ws, counters = kv._scratch(workspace, need, dev, True)
+        rc = lib.i4_attn_paged(*args, ws.data_ptr(), need, _lib.ptr(counters), stream)
+    if rc:
+        _lib.check(rc)
+    return y

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Sequence
 
 import torch
@@ -19,7 +20,9 @@ import torch
 from . import _lib
 from .kv import _batched, _call, _int32
 
-_HeadsC, _empty = _lib.HeadsC, torch.empty_like
+_heads = struct.Struct("<2Q6qi4x").pack  # struct i4_heads
+_turn = struct.Struct("<Q2qi4x").pack    # struct i4_turn
+_empty = torch.empty_like
 _DENSE = torch.contiguous_format
 LAYOUTS = {"half": 0, "interleaved": 1}
 MAX_PAIRS = 128
@@ -32,7 +35,7 @@ class Rotary:
     multiplies cos and sin (the attention factor of a scaled table).  axes: for tokens that are
     given several positions, which of them each pair turns by.  The table is copied to the host."""
 
-    __slots__ = ("inv_freq", "layout", "factor", "axes", "dims", "_bytes", "_c")
+    __slots__ = ("inv_freq", "layout", "factor", "axes", "dims", "_bytes", "_c", "_at")
 
     def __init__(self, inv_freq: torch.Tensor, *, layout: str = "half", factor: float = 1.0,
                  axes: Sequence[int] | None = None):
@@ -54,6 +57,7 @@ class Rotary:
         self._bytes = None if axes is None else (ctypes.c_uint8 * n)(*self.axes)
         self._c = _lib.RotaryC(f.data_ptr(), None if axes is None else
                                ctypes.addressof(self._bytes), self.factor, n, LAYOUTS[layout])
+        self._at = ctypes.addressof(self._c)
 
     @classmethod
     def plain(cls, dims: int, theta: float, **kw) -> "Rotary":
@@ -104,7 +108,7 @@ def interleaved_axes(sections: Sequence[int]) -> tuple[int, ...]:
 
 
 def _turn_c(turn: torch.Tensor, rotary: Rotary, batched: bool, B: int, T: int,
-            dev: torch.device) -> _lib.TurnC:
+            dev: torch.device) -> bytes:
     """struct i4_turn of given positions [B, T] or [axes, B, T] ([T] or [axes, T] for tokens
     without a batch)."""
     t = turn if batched else turn.unsqueeze(-2) if turn.dim() else turn
@@ -117,8 +121,8 @@ def _turn_c(turn: torch.Tensor, rotary: Rotary, batched: bool, B: int, T: int,
                            f"{'none' if rotary.axes is None else max(rotary.axes) + 1}")
     if turn.dtype != torch.int32 or turn.device != dev or (T > 1 and t.stride(-1) != 1):
         raise RuntimeError("given positions are int32 on the tensors' device, tokens adjacent")
-    return _lib.TurnC(turn.data_ptr(), t.stride(0) if axes > 1 else 0,
-                      t.stride(-2) if B > 1 else 0, axes)
+    return _turn(turn.data_ptr(), t.stride(0) if axes > 1 else 0, t.stride(-2) if B > 1 else 0,
+                 axes)
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -166,7 +170,7 @@ def _apart(shape: tuple[int, ...], stride: tuple[int, ...]) -> bool:
         shape[1] == 1 or stride[1] >= hd) and (shape[0] == 1 or stride[0] >= hd)
 
 
-def _new(x: torch.Tensor, T: int, hd: int, held: list[torch.Tensor]) -> _lib.HeadsC:
+def _new(x: torch.Tensor, T: int, hd: int, held: list[torch.Tensor]) -> bytes:
     """A dense output for x [B, T, heads, hd], appended to held, and struct i4_heads of both.
     What the struct points at is held until the call is queued."""
     B, _, n, _ = x.shape
@@ -177,11 +181,11 @@ def _new(x: torch.Tensor, T: int, hd: int, held: list[torch.Tensor]) -> _lib.Hea
         held.insert(0, x)
     y = _empty(x, memory_format=_DENSE)
     held.append(y)
-    return _HeadsC(x.data_ptr(), y.data_ptr(), a, b, c, T * n * hd, n * hd, hd, n)
+    return _heads(x.data_ptr(), y.data_ptr(), a, b, c, T * n * hd, n * hd, hd, n)
 
 
 def _into(xs: list[torch.Tensor], out: tuple[torch.Tensor | None, ...],
-          held: list[torch.Tensor]) -> list[_lib.HeadsC | None]:
+          held: list[torch.Tensor]) -> list[bytes | None]:
     """struct i4_heads of the inputs and the given outputs, checked."""
     outs = list(out)
     if len(outs) == 2 and len(xs) == 1 and outs[1] is None:
@@ -204,8 +208,8 @@ def _into(xs: list[torch.Tensor], out: tuple[torch.Tensor | None, ...],
             if not _apart(x.shape, x.stride()):
                 x = x.contiguous()
                 held.append(x)
-        cs.append(_lib.HeadsC(x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3],
-                              x.shape[2]))
+        cs.append(_heads(x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3],
+                         x.shape[2]))
     return cs if len(cs) > 1 else [cs[0], None]
 
 
@@ -256,7 +260,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
         kc = None if k is None else _new(xs[1], T, hd, held)
     else:
         qc, kc = _into(xs, out, held)
-    _call(dev, _lib.lib().i4_rope, qc, kc, code, B, T, hd, rotary._c, pd, ph, turn,
+    _call(dev, _lib.lib().i4_rope, qc, kc, code, B, T, hd, rotary._at, pd, ph, turn,
           None if counts is None else _int32(counts, B, dev, "counts"), out is None)
     if out is not None:
         return out[0] if k is None else (out[0], out[1])

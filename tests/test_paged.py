@@ -49,18 +49,22 @@ def heads(lb, **kw):
     return lb.HeadsC(**{**base, **kw})
 
 
+def at(c):
+    return None if c is None else ctypes.byref(c)
+
+
 def call_rope(lb, lib, q=None, k=None, r=None, turn=None, **kw):
     a = {**dict(xt=2, B=2, T=4, hd=128, pos_dev=None, pos=0, counts=None), **kw}
-    return lib.i4_rope(q or heads(lb), k, a["xt"], a["B"], a["T"], a["hd"], r or rotary(lb),
-                       a["pos_dev"], a["pos"], turn, a["counts"], 0, None)
+    return lib.i4_rope(at(q or heads(lb)), at(k), a["xt"], a["B"], a["T"], a["hd"],
+                       at(r or rotary(lb)), a["pos_dev"], a["pos"], at(turn), a["counts"], 0, None)
 
 
 def call_append(lb, lib, c=None, r=None, turn=None, **kw):
     a = {**dict(qkv=P, xt=2, T=1, bs=16 * 128, ts=16 * 128, nh=8, qw=P, kw=P, pos_dev=None, pos=0,
                 counts=None, out=P), **kw}
     return lib.i4_paged_append(a["qkv"], a["xt"], a["T"], a["bs"], a["ts"], a["nh"], a["qw"],
-                               a["kw"], 1e-6, r or rotary(lb), a["pos_dev"], a["pos"], turn,
-                               a["counts"], 0, a["out"], c or cache(lb), None)
+                               a["kw"], 1e-6, at(r or rotary(lb)), a["pos_dev"], a["pos"], at(turn),
+                               a["counts"], 0, a["out"], at(c or cache(lb)), None)
 
 
 def call_attn(lb, lib, c=None, **kw):
@@ -68,7 +72,7 @@ def call_attn(lb, lib, c=None, **kw):
                 counts=None, window=0, sinks=0, scale=0.1, out=P, ws=P, wsb=1 << 40,
                 counters=None), **kw}
     return lib.i4_attn_paged(a["q"], a["xt"], a["T"], a["bs"], a["ts"], a["hs"], a["nh"],
-                             c or cache(lb), a["pos_dev"], a["pos"], a["counts"], 0, a["window"],
+                             at(c or cache(lb)), a["pos_dev"], a["pos"], a["counts"], 0, a["window"],
                              a["sinks"], a["scale"], a["out"], a["ws"], a["wsb"], a["counters"],
                              None)
 
@@ -258,6 +262,24 @@ def test_python_refuses(pkg, monkeypatch):
                          out=rows[:2 * 3 * 4 * 128].view(2, 3, 4, 128))
     with pytest.raises(RuntimeError, match="apart"):
         pkg.rope(q, None, 0, r, out=(q[:1].expand(2, 3, 4, 128), None))
+
+
+def test_structs_are_packed_as_declared(pkg, monkeypatch):
+    """The bytes that the wrappers pass are the structs' own."""
+    from qwen3_omni_duplex_amd import _lib, paged, rotary
+
+    monkeypatch.setattr(_lib, "require_device", lambda *ts: torch.device("cpu"))
+    assert rotary._heads(1, 2, 3, 4, 5, 6, 7, -8, 9) == bytes(_lib.HeadsC(1, 2, 3, 4, 5, 6, 7, -8, 9))
+    assert rotary._turn(1, 2, 3, 4) == bytes(_lib.TurnC(1, 2, 3, 4))
+    assert paged._paged(*range(1, 14)) == bytes(_lib.PagedCacheC(*range(1, 14)))
+    c = pkg.PagedCache(*(torch.zeros(4, 2, 16, 128, dtype=torch.float16) for _ in range(2)))
+    t = torch.zeros(3, 9, dtype=torch.int32)[:, :5]
+    got, keys = c._with(t, 3)
+    s = _lib.PagedCacheC.from_buffer_copy(got)
+    assert keys == 80 and (s.k, s.v, s.table) == (c.k.data_ptr(), c.v.data_ptr(), t.data_ptr())
+    assert (s.page_stride, s.head_stride, s.table_stride) == (2 * 16 * 128, 16 * 128, 9)
+    assert (s.batch, s.n_kv_heads, s.pages, s.page, s.table_len, s.head_dim, s.dtype) == \
+        (3, 2, 4, 16, 5, 128, 1)
 
 
 def test_overlap_of_views(pkg):
