@@ -456,7 +456,8 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
       const int32_t* table = a.pg.table + b * a.pg.ts;
       Half16 h;
       // halves of 32 positions as below; the pages of the half after the next are looked up
-      // while the next one's rows are loaded
+      // while the next one's rows are loaded (32 sessions over up to 32000 positions in pages of
+      // 16: 232 us, 6.1 TB/s)
       const int e = 2 * i1;
       int x = 2 * i0 + __builtin_amdgcn_readfirstlane(wave);
       auto pos0 = [&](int y) { return 64 * ct.at(y >> 1) + 32 * (y & 1); };

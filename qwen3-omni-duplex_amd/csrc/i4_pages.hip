@@ -1,6 +1,7 @@
 // Rows of the fused q|k|v projection into a cache in pages: RMSNorm of the queries and keys (if
 // the model has it), rotary embedding, and keys and values to the rows of their positions'
-// pages.  fp32 inside, rounded once.  Bound by the rows' bytes.  A workgroup takes one token
+// pages.  fp32 inside, rounded once.  Bound by the rows' bytes: 5001 tokens of 40 heads take
+// 19.2 us (5.3 TB/s), those of 24 sessions 3.9, which is latency.  A workgroup takes one token
 // (several share its heads where tokens are few): its angles are computed once; a head is 16
 // lanes of 8 dims, so that a half pair's other dim is in a lane pairs / 8 away (8 for a whole
 // head: half a DPP row), and a neighbour's is in the same lane.

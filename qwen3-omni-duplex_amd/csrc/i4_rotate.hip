@@ -1,7 +1,8 @@
 // Rotary embedding of rows of heads: pair (a, b) of a head's dims, turned by the angle
 // p inv_freq,
 //   a' = (a cos - b sin) factor,  b' = (b cos + a sin) factor,
-// with the pair's dims half of the turned part apart, or neighbours.  Bound by the rows' bytes.
+// with the pair's dims half of the turned part apart, or neighbours.  Bound by the rows' bytes:
+// 6001 tokens of 36 heads of 128 dims take 19.6 us (5.6 TB/s), a token 3.1, which is a launch.
 //
 // A workgroup takes some tokens and all of their heads, so that a token's angles are computed
 // once.  An item is two vectors of V elements, V pairs of them (or dims behind the turned ones,
@@ -159,6 +160,81 @@ __global__ __launch_bounds__(256) void k_rope(RopeCall a, RotaryTable<kPairs> rt
   }
 }
 
+// Halves whose number of pairs is not a multiple of 4, in rows that allow 16 bytes: an item is one
+// such vector of a head, and its dims' partners, at any distance, come through LDS.
+template <int XT>
+__global__ __launch_bounds__(256) void k_rope_odd(RopeCall a, RotaryTable<kPairs> rt) {
+  constexpr int kPad = 2 * kPairs / 8 * 9;  // dims d at d + d / 8: lanes are 8 dims apart
+  __shared__ __align__(16) uint16_t s_x[256 * 8];
+  __shared__ float s_c[kTokens * kPad], s_s[kTokens * kPad];
+  __shared__ int s_state[kTokens];
+  enum { kPadding, kGood, kOutside };
+  const int n = rt.n, heads = a.q.heads + a.k.heads, row0 = blockIdx.x * a.each;
+  const int rows = min(a.each, a.rows - row0), total = rows * heads;  // heads of all its tokens
+  const int b0 = row0 / a.tk.T, t0 = row0 - b0 * a.tk.T;
+  const int round = 256 / a.items;  // heads at a time
+  const int mine = quotient(threadIdx.x, a.items), d0 = 8 * (threadIdx.x - mine * a.items);
+  struct Item {
+    u32x4 x;
+    uint16_t* y;
+    int r;
+  };
+  auto load = [&](int rh) {
+    Item m{};
+    if (mine >= round || rh >= total) return m;
+    const int r = quotient(rh, heads), h = rh - r * heads;
+    const int over = quotient(t0 + r, a.tk.T), b = b0 + over, t = t0 + r - over * a.tk.T;
+    const bool key = h >= a.q.heads;
+    const Heads& g = key ? a.k : a.q;
+    const int hh = key ? h - a.q.heads : h;
+    m.y = g.y + b * g.yb + t * g.yt + hh * g.yh + d0;
+    m.r = r;
+    if (t < count_of(a.tk, b)) m.x = ldg16(g.x + b * g.xb + t * g.xt + hh * g.xh + d0);
+    return m;
+  };
+  int base = blockIdx.y * round;
+  Item m = load(base + mine);  // on its way while the angles are computed
+  for (int j = threadIdx.x; j < rows * n; j += 256) {
+    const int r = quotient(j, n), e = j - r * n;
+    const int over = quotient(t0 + r, a.tk.T), b = b0 + over, t = t0 + r - over * a.tk.T;
+    const int p = (int)((u32)first_pos(a.tk, b) + (u32)t);  // as in k_rope
+    if (e == 0)
+      s_state[r] = t >= count_of(a.tk, b) ? kPadding : turns(a.turn, b, t, p) ? kGood : kOutside;
+    float c, s;
+    angle_of(turn_pos(a.turn, rt.axis[e], b, t, p), rt.f[e], c, s);
+    const int lo = r * kPad + e + (e >> 3), f = e + n, hi = r * kPad + f + (f >> 3);
+    s_c[lo] = s_c[hi] = c * rt.factor;
+    s_s[hi] = s * rt.factor;
+    s_s[lo] = -s_s[hi];
+  }
+  for (; base < total; base += round * gridDim.y) {
+    __syncthreads();  // the round before has read s_x
+    *(u32x4*)(s_x + 8 * threadIdx.x) = m.x;
+    __syncthreads();
+    const Item next = load(base + round * gridDim.y + mine);
+    if (m.y) {
+      const int state = s_state[m.r];
+      const uint16_t* x = s_x + 8 * (threadIdx.x - d0 / 8);  // the head's row
+      u32x4 out = m.x;
+      if (state != kGood) {
+        out = u32x4{} + (state == kPadding ? 0u : (u32)Half<XT>::QNAN * 0x10001u);
+      } else if (d0 < 2 * n) {
+        uint16_t e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int d = min(d0 + i, 2 * n - 1), at = m.r * kPad + d + (d >> 3);
+          const float u = Half<XT>::to_f32(x[d]), o = Half<XT>::to_f32(x[d < n ? d + n : d - n]);
+          e[i] = d0 + i < 2 * n ? Half<XT>::from_f32(fmaf(u, s_c[at], o * s_s[at])) : x[d0 + i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = e[2 * i] | (u32)e[2 * i + 1] << 16;
+      }
+      if (state != kPadding || a.zero) *(u32x4*)m.y = out;
+    }
+    m = next;
+  }
+}
+
 template <int V>
 static void rope_go(const RopeCall& a, const RotaryTable<kPairs>& rt, int layout, bool f16,
                     hipStream_t s) {
@@ -242,16 +318,22 @@ extern "C" int i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B,
   if (k) a.k = heads_of(*k, B, T);
   // the widest vector that a head's parts and all rows allow
   const int n = rotary->pairs;
+  const bool half = rotary->layout == I4_ROPE_HALF;
   int v = vector_of(a.q, 8);
   if (k) v = vector_of(a.k, v);
-  while (v > 1 && (head_dim % v || (rotary->layout == I4_ROPE_HALF && n % v))) v /= 2;
+  while (v > 1 && head_dim % v) v /= 2;
+  // Through LDS where vectors of 2 or 4 bytes would be left and rows are many: 3000 tokens of 36
+  // heads of 72 dims 11.8 us against 21.2 (9 pairs), 11.4 against 13.3 (18), but 12.0 against 9.9
+  // (36: 8 bytes), and 1000 of 16 heads of 64 dims (30 pairs) 4.5 against 4.1.
+  const bool odd = half && v == 8 && n % 4 && (int64_t)B * T * (q->heads + a.k.heads) >= 1 << 15;
+  while (v > 1 && !odd && half && n % v) v /= 2;
   a.tk = Tokens{pos_dev, counts, pos, T};
   a.turn = turn_of(turn);
   a.rows = B * T;
   a.hd = head_dim;
   a.zero = zero_padding;
-  a.items = rotary->layout == I4_ROPE_HALF ? n / v + (head_dim - 2 * n + 2 * v - 1) / (2 * v)
-                                           : (head_dim + 2 * v - 1) / (2 * v);
+  a.items = odd ? head_dim / 8 : half ? n / v + (head_dim - 2 * n + 2 * v - 1) / (2 * v)
+                                      : (head_dim + 2 * v - 1) / (2 * v);
   // A token a workgroup, or the heads of one shared out where the chip has room: 24 tokens of 72
   // heads of 256 dims 6.7 us with one workgroup a token, 3.3 with five.  Two tokens where there
   // are many (3000 of 36 heads of 128: 12.1, 10.7, 11.3 us with one, two, four), four where a token
@@ -263,7 +345,11 @@ extern "C" int i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B,
   while (a.shares * 256 < items && (int64_t)a.rows * (a.shares + 1) <= 512) ++a.shares;
   const RotaryTable<kPairs> rt = rotary_table<kPairs>(rotary);
   const bool f16 = x_dtype == I4_F16;
-  if (v == 8) rope_go<8>(a, rt, rotary->layout, f16, stream);
+  if (odd) {
+    const dim3 grid((unsigned)((a.rows + a.each - 1) / a.each), (unsigned)a.shares);
+    if (f16) k_rope_odd<I4_F16><<<grid, 256, 0, stream>>>(a, rt);
+    else k_rope_odd<I4_BF16><<<grid, 256, 0, stream>>>(a, rt);
+  } else if (v == 8) rope_go<8>(a, rt, rotary->layout, f16, stream);
   else if (v == 4) rope_go<4>(a, rt, rotary->layout, f16, stream);
   else if (v == 2) rope_go<2>(a, rt, rotary->layout, f16, stream);
   else rope_go<1>(a, rt, rotary->layout, f16, stream);

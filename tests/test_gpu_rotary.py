@@ -44,7 +44,11 @@ def given(dev, B, T, pos, form, seed=7):
     (1, 4, 3, 1, 64, 62, 2**24 - 50, "start", 1.0),  # positions at the end of the range
     (1, 300, 2, 1, 70, 70, -150, "int", 1.0),       # from negative ones to positive ones
     (4, 1100, 1, 1, 64, 32, 5, "start", 2.0),       # more tokens than one a workgroup
-    (1, 2100, 2, 1, 128, 128, 40000, "int", 1.0)])
+    (1, 2100, 2, 1, 128, 128, 40000, "int", 1.0),
+    (1, 4200, 5, 3, 72, 18, 100, "tokens", 1.25),   # pairs through LDS: 9 of them,
+    (3, 1100, 10, 2, 80, 20, 7, "axes", 1.0),       # 10, positions on axes,
+    (1, 2050, 16, 0, 256, 250, 2**20, "int", 1.0),  # 125 of a wide head,
+    (33, 1, 1000, 24, 64, 62, 9, "start", 0.5)])    # 31, and a token's heads shared out
 def test_rope_matches_64_bits(pkg, dev, dtype, layout, B, T, nh, nkv, hd, dims, pos, form, factor):
     q, k = rand(dev, B, T, nh, hd, seed=1, dtype=dtype), rand(dev, B, T, nkv, hd, seed=2,
                                                               dtype=dtype)
@@ -98,6 +102,46 @@ def test_views_and_in_place(pkg, dev, layout, hd, dims, shift):
     k.copy_(before[shift:shift + B * T * width].view(B, T, width)[..., nh * hd:(nh + nkv) * hd]
             .unflatten(-1, (nkv, hd)))
     assert same(flat, before)
+
+
+@pytest.mark.parametrize("dtype", DTS)
+def test_pairs_through_lds(pkg, dev, dtype):
+    """In place in the fused rows, padding, positions outside and values that are not finite,
+    where the number of pairs is odd and rows are many: as rows of few tokens."""
+    B, T, nh, nkv, hd, dims = 3, 1500, 6, 2, 72, 18
+    r = pkg.Rotary.plain(dims, 1e4)
+    rows = rand(dev, B, T, (nh + 2 * nkv) * hd, seed=1, dtype=dtype)
+    rows[0, 3, 5], rows[1, 7, 30], rows[1, 7, hd - 1] = float("inf"), float("-inf"), float("nan")
+    x = rows.unflatten(-1, (-1, hd))
+    counts, pos = i32(dev, [T, 0, T - 9]), i32(dev, [2**24 - 700, 5, 0])
+
+    def turned(x, b, lo, hi):
+        q, k = x[b:b + 1, lo:hi, :nh], x[b:b + 1, lo:hi, nh:nh + nkv]
+        return pkg.rope(q, k, int(pos[b]) + lo, r)
+
+    torch.full_like(x[:, :, :nh], 5.0)  # leaves memory that is not zeros
+    got = pkg.rope(x[:, :, :nh], x[:, :, nh:nh + nkv], pos, r, counts=counts)
+    for y in got:
+        assert torch.isnan(y[0, 700:]).all() and not y[1].any() and not y[2, T - 9:].any()
+    for b, n in ((0, 700), (2, T - 9)):
+        for lo in range(0, n, 100):
+            for a, w in zip(got, turned(x, b, lo, min(lo + 100, n))):
+                a, w = a[b, lo:min(lo + 100, n)], w[0]
+                assert torch.equal(torch.isfinite(a), torch.isfinite(w))
+                a, w = (z.double().nan_to_num(0, 0, 0) for z in (a, w))
+                # the same products, summed in either order: one more rounding of each, and
+                # then half a step apart at most, or one where that tips
+                assert ((a - w).abs() <= 2.01 * kvref.half_step(dtype) * w.abs() + 1e-6).all()
+    want = [g.clone() for g in got]
+    keep = rows.clone()
+    pkg.rope(x[:, :, :nh], x[:, :, nh:nh + nkv], pos, r, counts=counts,
+             out=(x[:, :, :nh], x[:, :, nh:nh + nkv]))
+    for y, w, lo, n in ((x, want[0], 0, nh), (x, want[1], nh, nkv)):
+        for b, c in ((0, T), (2, T - 9)):
+            assert same(y[b, :c, lo:lo + n].contiguous(), w[b, :c].contiguous())
+    y = keep.unflatten(-1, (-1, hd))
+    assert same(x[:, :, nh + nkv:].contiguous(), y[:, :, nh + nkv:].contiguous())
+    assert same(x[1], y[1]) and same(x[2, T - 9:], y[2, T - 9:])
 
 
 def test_one_sequence_without_a_batch(pkg, dev):
