@@ -186,8 +186,8 @@ def _held(workspace: Workspace | None, dev: torch.device,
     ws = _STREAM_WS.get((dev.index, stream)) if workspace is None else workspace
     if ws is None:
         return None, None
-    buf, counters = ws.buf, ws._counters
-    if buf is None or counters is None or buf.device != dev or counters.device != dev \
+    buf, counters, i = ws.buf, ws._counters, dev.index
+    if buf is None or counters is None or buf.get_device() != i or counters.get_device() != i \
             or torch.cuda.is_current_stream_capturing():
         return None, None
     return buf, counters

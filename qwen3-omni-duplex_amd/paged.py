@@ -37,10 +37,10 @@ class PagedCache:
     write the tensors in place and the object holds their addresses, so they cannot be
     replaced."""
 
-    __slots__ = ("k", "v", "_c")
+    __slots__ = ("k", "v", "device", "dtype", "_c", "_index")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
-        _lib.require_device(k, v)
+        self.device = _lib.require_device(k, v)
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
             raise RuntimeError("k and v are [pages, n_kv_heads, page, head_dim] and agree in "
                                "shape, strides and dtype")
@@ -51,7 +51,8 @@ class PagedCache:
             raise RuntimeError("k and v must be pools of their own")
         if page < 16 or page > 1024 or page & (page - 1):
             raise RuntimeError(f"a page holds 16 to 1024 positions, a power of two, got {page}")
-        self.k, self.v = k, v
+        self.k, self.v, self.dtype = k, v, k.dtype
+        self._index = k.get_device()
         self._c = (pages, page, n, hd, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1),
                    _lib.half_code(k.dtype))
 
@@ -71,6 +72,13 @@ class PagedCache:
     n_kv_heads = property(lambda self: self._c[2])
     head_dim = property(lambda self: self._c[3])
 
+    def _beside(self, *ts: torch.Tensor | None) -> torch.device:
+        """The device of the pool and of the given tensors."""
+        for t in ts:
+            if t is not None and t.get_device() != self._index:
+                _lib.require_device(self.k, t)  # which says what is wrong
+        return self.device
+
     def _with(self, table: torch.Tensor, B: int) -> tuple[bytes, int]:
         """struct i4_pagedcache of this pool under a call's table, and its positions."""
         shape, stride = table.shape, table.stride()
@@ -81,7 +89,7 @@ class PagedCache:
         else:
             n = 0
         if n < 1 or last != 1 and n > 1 or table.dtype != torch.int32 \
-                or table.get_device() != self.k.get_device():
+                or table.get_device() != self._index:
             raise RuntimeError(f"the table is int32 [{B}, n] on the tensors' device, a sequence's "
                                f"entries adjacent")
         pages, page, heads, hd, k, v, ps, hs, dt = self._c
@@ -102,12 +110,13 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
     turn: the positions that the angles take where they are not the tokens' own, as rope takes
     them ([B, T] or [axes, B, T]).  "half" embeddings turn a multiple of 16 dims here.  fp32
     inside, rounded once (i4_paged_append)."""
-    dev = _lib.require_device(qkv, q_norm_w, k_norm_w, cache.k, turn, counts, out)
-    x = _batched(qkv, 3, "qkv")
+    dev = cache._beside(qkv, q_norm_w, k_norm_w, turn, counts, out)
+    batched = qkv.dim() == 3
+    x = qkv if batched else _batched(qkv, 3, "qkv")
     B, T, width = x.shape
     cc, keys = cache._with(table, B)
     _, _, n_kv, hd, _, _, _, _, dtype = cache._c
-    if x.dtype != cache.k.dtype:
+    if x.dtype != cache.dtype:
         raise RuntimeError("the pages must have the activation dtype")
     if width != (n_heads + 2 * n_kv) * hd:
         raise RuntimeError("qkv's width does not match the head counts")
@@ -117,19 +126,25 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
     if rotary.dims > hd or rotary.layout == "half" and rotary.dims % 16:
         raise RuntimeError(f"{rotary.dims} of {hd} dims turn: at most all, and with the layout "
                            "'half' a multiple of 16")
-    if x.stride(2) != 1:
+    b, t, e = x.stride()
+    if e != 1:
         x = x.contiguous()
-    shape = (B, T, n_heads, hd)
-    q = _out(out, x, shape if qkv.dim() == 3 else shape[1:], False)
-    if out is not None and overlaps(q.view(B, T, n_heads, hd), x.unflatten(2, (-1, hd))):
-        raise RuntimeError("out must not overlap qkv")
-    on_dev = isinstance(pos, torch.Tensor)
-    tc = None if turn is None else _turn_c(turn, rotary, qkv.dim() == 3, B, T, dev)
-    _call(dev, _lib.lib().i4_paged_append, x.data_ptr(), dtype, T, x.stride(0), x.stride(1),
-          n_heads, _lib.ptr(q_norm_w), _lib.ptr(k_norm_w), eps, rotary._at,
-          _int32(pos, B, dev, "pos") if on_dev else None,
-          0 if on_dev else _host_pos(pos, T, keys), tc, _int32(counts, B, dev, "counts"),
-          out is None, q.data_ptr(), cc)
+        b, t, _ = x.stride()
+    shape = (B, T, n_heads, hd) if batched else (T, n_heads, hd)
+    if out is None:
+        q = x.new_empty(shape)
+    else:
+        q = _out(out, x, shape, False)
+        if overlaps(q.view(B, T, n_heads, hd), x.unflatten(2, (-1, hd))):
+            raise RuntimeError("out must not overlap qkv")
+    pd, ph = (_int32(pos, B, dev, "pos"), 0) if isinstance(pos, torch.Tensor) \
+        else (None, _host_pos(pos, T, keys))
+    tc = None if turn is None else _turn_c(turn, rotary, batched, B, T, dev)
+    _call(dev, _lib.lib().i4_paged_append, x.data_ptr(), dtype, T, b, t, n_heads,
+          None if q_norm_w is None else q_norm_w.data_ptr(),
+          None if k_norm_w is None else k_norm_w.data_ptr(), eps, rotary._at, pd, ph, tc,
+          None if counts is None else _int32(counts, B, dev, "counts"), out is None,
+          q.data_ptr(), cc)
     return q
 
 
@@ -142,27 +157,34 @@ def attn_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor,
     pos + t, over the positions of their sequence's table up to and including theirs
     (paged_append), and with a window those j > p - window or j < sinks.  The same roundings
     as attn_window (i4_attn_paged)."""
-    dev = _lib.require_device(q, cache.k, counts, out)
+    dev = cache._beside(q, counts, out)
     x = q if q.dim() == 4 else _batched(q, 4, "q")
-    B, T, nh, hd = shape = x.shape
+    B, T, nh, hd = x.shape
     cc, keys = cache._with(table, B)
     _, _, n_kv, head_dim, _, _, _, _, dtype = cache._c
     if hd != head_dim:
         raise RuntimeError(f"q {tuple(q.shape)} does not match the cache's head_dim {head_dim}")
+    if q.dtype != cache.dtype:
+        raise RuntimeError("the pages must have the activation dtype")
     w, sinks = kv._bounds(window, sinks)
-    if x.stride(3) != 1:
+    b, t, h, e = x.stride()
+    if e != 1:
         x = x.contiguous()
-    y = _out(out, x, shape if q.dim() == 4 else shape[1:], False)
-    if out is not None and overlaps(out, q):
-        raise RuntimeError("out must not overlap q")
+        b, t, h, _ = x.stride()
+    if out is None:
+        y = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+    else:
+        y = _out(out, x, tuple(q.shape), False)
+        if overlaps(out, q):
+            raise RuntimeError("out must not overlap q")
     pd, ph = (_int32(pos, B, dev, "pos"), 0) if isinstance(pos, torch.Tensor) \
         else (None, _host_pos(pos, T, keys))
     if torch.cuda.current_device() != dev.index:
         with torch.cuda.device(dev):
             return attn_paged(q, cache, table, pos, window=window, sinks=sinks, scale=scale,
                               counts=counts, out=out, workspace=workspace)
-    lib, s = _lib.lib(), x.stride()
-    args = (x.data_ptr(), _lib.half_code(x.dtype), T, s[0], s[1], s[2], nh, cc, pd, ph,
+    lib = _lib.lib()
+    args = (x.data_ptr(), dtype, T, b, t, h, nh, cc, pd, ph,
             None if counts is None else _int32(counts, B, dev, "counts"), out is None, w, sinks,
             hd ** -0.5 if scale is None else scale, y.data_ptr())
     # the workspace that is there, and only if it does not do what the call needs
