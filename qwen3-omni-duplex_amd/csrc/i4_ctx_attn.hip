@@ -35,9 +35,9 @@ struct CtxSplit {
     return (size_t)parts * ((KHD + 2) * 4) + ((size_t)plan * 4 + 255) / 256 * 256;
   }
 };
-// share: whether the tiles may be shared out
+// pages: of a call over pages; share: whether many rows' tiles may be shared out there
 static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, int sinks,
-                          bool share) {
+                          bool pages, bool share) {
   const int R = T * (nq / nkv);
   const bool few = R <= kFewRows;
   // the context tiles of 64 that one row tile sees at most
@@ -52,12 +52,24 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
     // as many workgroups as the chip holds at once (two a CU), or two or four times that
     // where the heads are too many to share that evenly; at least a tile for each wave
     int64_t w = heads <= 128 ? 512 : heads <= 256 ? 1024 : 2048;
+    // Over pages, where heads are few, one workgroup a CU and fewer parts: a kv head's last
+    // workgroup reads 32 parts in one round of loads, and another round costs more than it saves
+    // in the tiles until they are many.  4 kv heads of one sequence over 30000 positions 20.8 us
+    // with 32 parts each, 22.9 with 64, 36.1 with 118, over 60000 30.6 with 32 and 64; one over
+    // 30000 20.0, 18.8 and 24.1; 2 sequences of 4 over up to 16000 18.4 with 24 on average, 22.4
+    // with 32, 22.1 with 64; 8 over 4000 16.6 with 256 workgroups, 19.5 with 512, 8 over 30000 77
+    // and 79; but 16 of 8 kv heads over 16000 135 and 108.  (Over one run of rows the splits are
+    // what they were: they decide a row's bits.)
+    if (pages && heads <= 32) {
+      const int parts = B > 1 ? 24 : tiles > (heads <= 2 ? 250 : 600) ? 64 : 32;
+      w = tiles <= 128 || heads * parts > 256 ? 256 : heads * parts;
+    }
     if (w > heads * ((tiles + 3) / 4)) w = heads * ((tiles + 3) / 4);
     if (w <= heads || heads > kShared) w = heads;
     return {1, (int)w, w > heads ? w * kFewRows : 0, 0};
   }
   const int64_t tiled = (R + kTileRows - 1) / kTileRows;
-  if (share && B > 1 && B * tiled <= kPlanned && heads * tiled <= kSharedTiles &&
+  if (pages && share && B > 1 && B * tiled <= kPlanned && heads * tiled <= kSharedTiles &&
       tiles >= kSharedSpan) {
     const int64_t w = runs_of(heads * tiled * (tiles + kRowTile));
     return {1, (int)w, 2 * w * kTileRows, (int)(B * tiled) + 2};
@@ -79,7 +91,7 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
 
 static int launch(CtxArgs& a, int xt, int fmt, int keys, const i4_span& w, hipStream_t stream) {
   const CtxSplit sp = ctx_split(a.B, a.tk.T, a.nq, a.nkv, keys, w.window, w.sinks,
-                                fmt == kPaged && (a.tk.pos_dev || a.tk.counts));
+                                fmt == kPaged, a.tk.pos_dev || a.tk.counts);
   a.S = sp.S;
   a.wgs = sp.wgs;
   a.part = (float*)w.workspace;
@@ -97,24 +109,24 @@ static int launch(CtxArgs& a, int xt, int fmt, int keys, const i4_span& w, hipSt
 }  // namespace i4
 
 static size_t ctx_bytes(int B, int T, int n_heads, int n_kv_heads, int keys, int window, int sinks,
-                        bool share) {
+                        bool pages, bool share) {
   if (B < 1 || T < 1 || T > i4::KV_MAX_LEN || n_kv_heads < 1 || n_heads < n_kv_heads ||
       n_heads > 1024 || n_heads % n_kv_heads || keys < 1 || window < 0 || sinks < 0)
     return 0;
   if (n_kv_heads > 1024 || B > 65535) return 0;
-  return i4::ctx_split(B, T, n_heads, n_kv_heads, keys, window, sinks, share).bytes();
+  return i4::ctx_split(B, T, n_heads, n_kv_heads, keys, window, sinks, pages, share).bytes();
 }
 
 extern "C" {
 
 size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                       int window, int sinks) {
-  return ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, false);
+  return ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, false, false);
 }
 size_t i4_attn_paged_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                      int window, int sinks) {
-  const size_t split = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, false);
-  const size_t shared = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true);
+  const size_t split = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true, false);
+  const size_t shared = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true, true);
   return split > shared ? split : shared;
 }
 

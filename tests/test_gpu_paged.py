@@ -128,6 +128,30 @@ def test_attention_is_that_over_rows(pkg, dev, dtype, page, B, T, nh, nkv, pos, 
                 pkg.attn_window(q, rows[0], rows[1], pos, **bounds))
 
 
+@pytest.mark.parametrize("dtype", DTS)
+@pytest.mark.parametrize("B,T,nh,nkv,pos,window,sinks", [
+    (1, 1, 32, 4, 8192, None, 0),     # one context tile more than 128
+    (1, 1, 32, 4, 20011, None, 0),    # 32 parts a kv head
+    (1, 2, 8, 1, 20011, None, 0),     # 64
+    (1, 3, 4, 2, 33000, 17000, 70),
+    (2, 1, 32, 4, 17000, None, 0),    # ages apart: most of the parts are the older's
+    (4, 4, 12, 3, 9999, 9000, 1),
+    (3, 1, 11, 11, 8500, None, 0)])   # one head too many for few
+def test_long_contexts_of_few_rows(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
+    """Contexts so long that the splits differ from those over rows, against 64 bits: ages that
+    the host knows and the device's, the first sequence the oldest, the last one young."""
+    q, rows = case(dev, B, T, nh, nkv, pos + T, dtype)
+    at = [pos // (5 * b + 1) for b in range(B)]
+    cache, table = pool_of(pkg, dev, rows, [p + T for p in at], 64, width=-(-(pos + T) // 64))
+    bounds = dict(window=window, sinks=sinks)
+    want, tol = kvref.attention(q, rows[0], rows[1], at, [T] * B, window, sinks)
+    got = pkg.attn_paged(q, cache, table, i32(dev, at), **bounds)
+    check(got, want, tol)
+    assert same(pkg.attn_paged(q, cache, table, i32(dev, at), **bounds), got)
+    if B == 1:
+        check(pkg.attn_paged(q, cache, table, pos, **bounds), want, tol)
+
+
 @pytest.mark.parametrize("T", [1, 3, 40])
 def test_padding_and_positions_outside(pkg, dev, T):
     """Counts, a given output whose padding stays, and device positions outside the table."""
