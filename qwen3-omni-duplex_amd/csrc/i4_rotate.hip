@@ -335,14 +335,16 @@ extern "C" int i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B,
   a.items = odd ? head_dim / 8 : half ? n / v + (head_dim - 2 * n + 2 * v - 1) / (2 * v)
                                       : (head_dim + 2 * v - 1) / (2 * v);
   // A token a workgroup, or the heads of one shared out where the chip has room: 24 tokens of 72
-  // heads of 256 dims 6.7 us with one workgroup a token, 3.3 with five.  Two tokens where there
-  // are many (3000 of 36 heads of 128: 12.1, 10.7, 11.3 us with one, two, four), four where a token
-  // is less than half a workgroup's items (3000 of 2 heads: 5.5, 4.2, 3.7), one again where it
-  // is several rounds of them (3000 of 72 heads of 256: 44.1, 46.6, 48.9).
+  // heads of 256 dims 6.7 us with one workgroup a token, 3.3 with five; 400 of them 8.3 with room
+  // for 1024 workgroups, 9.5 for 512 and 8.2 for 2048, but 1000 of 36 heads of 128 6.4, 6.4 and
+  // 6.9.  Two tokens where there are many (3000 of 36 heads of 128: 12.1, 10.7, 11.3 us with one,
+  // two, four), four where a token is less than half a workgroup's items (3000 of 2 heads: 5.5,
+  // 4.2, 3.7), one again where it is several rounds of them (3000 of 72 heads of 256: 44.1, 46.6,
+  // 48.9).
   const int items = (a.q.heads + a.k.heads) * a.items;
   a.each = a.rows < 1536 || items > 512 ? 1 : items < 128 ? 4 : 2;
   a.shares = 1;
-  while (a.shares * 256 < items && (int64_t)a.rows * (a.shares + 1) <= 512) ++a.shares;
+  while (a.shares * 256 < items && (int64_t)a.rows * (a.shares + 1) <= 1024) ++a.shares;
   const RotaryTable<kPairs> rt = rotary_table<kPairs>(rotary);
   const bool f16 = x_dtype == I4_F16;
   if (odd) {
