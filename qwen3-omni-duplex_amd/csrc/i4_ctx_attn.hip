@@ -56,12 +56,15 @@ static CtxSplit ctx_split(int B, int T, int nq, int nkv, int keys, int window, i
     // workgroup reads 32 parts in one round of loads, and another round costs more than it saves
     // in the tiles until they are many.  4 kv heads of one sequence over 30000 positions 20.8 us
     // with 32 parts each, 22.9 with 64, 36.1 with 118, over 60000 30.6 with 32 and 64; one over
-    // 30000 20.0, 18.8 and 24.1; 2 sequences of 4 over up to 16000 18.4 with 24 on average, 22.4
-    // with 32, 22.1 with 64; 8 over 4000 16.6 with 256 workgroups, 19.5 with 512, 8 over 30000 77
-    // and 79; but 16 of 8 kv heads over 16000 135 and 108.  (Over one run of rows the splits are
-    // what they were: they decide a row's bits.)
+    // 30000 20.0, 18.8 and 24.1.  Of several sequences, with 24 parts on average, 48 and (of 4 kv
+    // heads 32, all that there are) 64: 2 of 4 over up to 16000 18.4, 22.1, 22.2, up to 100000
+    // 71, 77, 77; 2 of one over up to 16000 15.8, 16.8, 16.8, up to 100000 52, 36, 34; 4 of one
+    // over up to 100000 56, 43, 45.  8 of 4 over up to 4000 16.6 with 256 workgroups, 19.5 with
+    // 512, up to 30000 77 and 79; but 16 of 8 over up to 16000 135 and 108.  (Over one run of rows
+    // the splits are what they were: they decide a row's bits.)
     if (pages && heads <= 32) {
-      const int parts = B > 1 ? 24 : tiles > (heads <= 2 ? 250 : 600) ? 64 : 32;
+      const int parts = B > 1 ? (heads <= 6 && tiles > 400 ? 48 : 24)
+                              : (tiles > (heads <= 2 ? 250 : 600) ? 64 : 32);
       w = tiles <= 128 || heads * parts > 256 ? 256 : heads * parts;
     }
     if (w > heads * ((tiles + 3) / 4)) w = heads * ((tiles + 3) / 4);

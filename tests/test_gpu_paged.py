@@ -136,6 +136,7 @@ def test_attention_is_that_over_rows(pkg, dev, dtype, page, B, T, nh, nkv, pos, 
     (1, 3, 4, 2, 33000, 17000, 70),
     (2, 1, 32, 4, 17000, None, 0),    # ages apart: most of the parts are the older's
     (4, 4, 12, 3, 9999, 9000, 1),
+    (3, 2, 4, 2, 26000, None, 0),     # more parts of few heads
     (3, 1, 11, 11, 8500, None, 0)])   # one head too many for few
 def test_long_contexts_of_few_rows(pkg, dev, dtype, B, T, nh, nkv, pos, window, sinks):
     """Contexts so long that the splits differ from those over rows, against 64 bits: ages that
