@@ -47,7 +47,7 @@ class PagedCache:
         pages, n, page, hd = k.shape
         if k.stride(3) != 1 or k.stride(2) != hd:
             raise RuntimeError("the rows of a head's page must be dense")
-        if k.data_ptr() == v.data_ptr():
+        if k.numel() and overlaps(k, v):
             raise RuntimeError("k and v must be pools of their own")
         if page < 16 or page > 1024 or page & (page - 1):
             raise RuntimeError(f"a page holds 16 to 1024 positions, a power of two, got {page}")

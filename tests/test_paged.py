@@ -308,6 +308,20 @@ def test_overlap_of_views(pkg):
     assert not overlaps(one[:, :, :2], one[:, :, 2:]) and overlaps(one[:, :, :3], one[:, :, 2:])
 
 
+def test_pools_that_overlap(pkg, monkeypatch):
+    """k and v share no element: not one tensor, not pages or heads apart of one; beside each
+    other in one allocation in any way they may lie."""
+    monkeypatch.setattr(pkg.paged._lib, "require_device", lambda *ts: torch.device("cuda", 0))
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda self: 0)
+    x = torch.zeros(7, 4, 16, 128, dtype=torch.bfloat16)
+    for k, v in ((x, x), (x[:6], x[1:]), (x[1:], x[:6]), (x[:, :3], x[:, 1:])):
+        with pytest.raises(RuntimeError, match="pools of their own"):
+            pkg.PagedCache(k, v)
+    for k, v in ((x[:3], x[3:6]), (x[:, :2], x[:, 2:]), (x[::2][:3], x[1::2]), (x[:, ::2], x[:, 1::2]),
+                 (x.transpose(0, 1)[:2], x.transpose(0, 1)[2:])):
+        assert pkg.PagedCache(k, v).page == 16
+
+
 def test_copies(pkg, monkeypatch):
     """A copied handle holds its own tensors' addresses."""
     import copy
