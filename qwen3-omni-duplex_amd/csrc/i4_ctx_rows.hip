@@ -157,6 +157,18 @@ __device__ inline void scores16(const Half16& h, const u32x4 (&q)[4], f32x4 (&s)
   }
 }
 
+// A key's values in a cache's rows, for clean16.  It is passed by value: a lambda that refers to
+// the caller's variables changed the code of the masks around it, 77 instructions more with 8-bit
+// blocks (a token over 8191 of them 12.8 -> 13.3 us).
+struct BufferRows {
+  rsrc_t r;
+  int row0;
+  u32 stride;
+  __device__ inline u32x4 operator()(int j, u32 at) const {
+    return __builtin_amdgcn_raw_buffer_load_b128(r, (u32)(row0 + j) * stride + at, 0, 0);
+  }
+};
+
 // Values that a row does not see must not reach it (0 times an infinity is NaN): before the
 // product of a tile that is not seen in full, the values of keys that no row sees are
 // cleared; where rows differ, infinities and NaN are taken out and added to the rows that
@@ -512,9 +524,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
         if (x + 4 < e) load_k16(h, kr, jn, stride, m, qd);
         weights<XT, 2>(acc, s, a.c2, partial, j0 + 8 * qd, p, a.w);
         if (partial)
-          clean16<XT>(acc, h, [&](int j, u32 at) {
-            return __builtin_amdgcn_raw_buffer_load_b128(vr, (u32)(j0 + j) * stride + at, 0, 0);
-          }, j0, m, qd, plo, phi, p, a.w);
+          clean16<XT>(acc, h, BufferRows{vr, j0, stride}, j0, m, qd, plo, phi, p, a.w);
         values16<XT>(acc, h, s);
         if (x + 4 < e) load_v16(h, vr, jn, stride, m, qd);
       }
@@ -558,9 +568,7 @@ __global__ __launch_bounds__(256, 2) void k_ctx_rows(CtxArgs a) {
           f32x4 s[2];
           scores16<XT>(h, qn, s);
           weights<XT, 2>(acc, s, a.c2, true, j0 + 8 * qd, p, a.w);
-          clean16<XT>(acc, h, [&](int j, u32 at) {
-            return __builtin_amdgcn_raw_buffer_load_b128(vr, (u32)(row0 + j) * stride + at, 0, 0);
-          }, j0, m, qd, plo, phi, p, a.w);
+          clean16<XT>(acc, h, BufferRows{vr, row0, stride}, j0, m, qd, plo, phi, p, a.w);
           values16<XT>(acc, h, s);
         }
       }
