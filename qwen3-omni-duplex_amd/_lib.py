@@ -306,6 +306,23 @@ def stream(device: torch.device) -> int:
     return _raw_stream(device.index)
 
 
+class Handle:
+    """An object that holds addresses for the kernels: its attributes are set once, so that no
+    tensor can be taken from behind its address.  (Properties over other slots would do too, and
+    cost each call their reads.)"""
+
+    __slots__ = ()
+
+    def __setattr__(self, name: str, value) -> None:
+        if hasattr(self, name):
+            raise AttributeError(f"{type(self).__name__}.{name} cannot be replaced: make another "
+                                 f"{type(self).__name__}")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name: str) -> None:
+        raise AttributeError(f"{type(self).__name__}.{name} cannot be taken away")
+
+
 def require_device(*ts: torch.Tensor | None) -> torch.device:
     dev, index = None, -2
     for t in ts:

@@ -31,11 +31,11 @@ from .rotary import Rotary, _turn_c, overlaps
 _paged = struct.Struct("<3Q3q7i4x").pack  # struct i4_pagedcache
 
 
-class PagedCache:
+class PagedCache(_lib.Handle):
     """The pool: k and v [pages, n_kv_heads, page, head_dim] in 16 bits, views of any strides
     whose pages' rows are dense (a head's page is page * head_dim adjacent values).  The kernels
     write the tensors in place and the object holds their addresses, so they cannot be
-    replaced."""
+    replaced (AttributeError)."""
 
     __slots__ = ("k", "v", "device", "dtype", "_c", "_index")
 

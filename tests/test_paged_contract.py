@@ -1,0 +1,40 @@
+"""What the handles and calls of the paged cache and the rotary embeddings promise beyond their
+results: on the host, before any launch."""
+from __future__ import annotations
+
+import copy
+
+import pytest
+import torch
+
+BF = torch.bfloat16
+
+
+@pytest.fixture
+def on_cpu(pkg, monkeypatch):
+    """Tensors of the CPU pass for the device's: checks that come before any address is used."""
+    from qwen3_omni_duplex_amd import _lib
+
+    monkeypatch.setattr(_lib, "require_device", lambda *ts: torch.device("cpu"))
+    return pkg
+
+
+def pool(pkg, shape=(4, 2, 16, 128)):
+    return pkg.PagedCache(torch.zeros(shape, dtype=BF), torch.zeros(shape, dtype=BF))
+
+
+def test_a_pool_keeps_its_tensors(on_cpu):
+    """The kernels hold the tensors' addresses: nothing can be put in their place, and what the
+    object says of itself stays what they read."""
+    c = pool(on_cpu)
+    k, other = c.k, torch.zeros_like(c.k)
+    for name, value in (("k", other), ("v", other), ("device", "cpu"), ("dtype", torch.float16),
+                        ("page", 32), ("pages", 9), ("_c", ()), ("k", c.k)):
+        with pytest.raises(AttributeError):
+            setattr(c, name, value)
+    for name in ("k", "v", "_c"):
+        with pytest.raises(AttributeError):
+            delattr(c, name)
+    assert c.k is k and c._c[4] == k.data_ptr() and c.page == 16
+    d = copy.deepcopy(c)
+    assert d.k.data_ptr() == d._c[4] != c._c[4]
