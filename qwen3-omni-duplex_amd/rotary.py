@@ -29,11 +29,12 @@ MAX_PAIRS = 128
 MAX_POS = 1 << 24
 
 
-class Rotary:
+class Rotary(_lib.Handle):
     """Pair i of a head's first 2 len(inv_freq) dims turns by the angle position * inv_freq[i]:
     dims i and i + len(inv_freq) (layout "half") or 2 i and 2 i + 1 ("interleaved").  factor
     multiplies cos and sin (the attention factor of a scaled table).  axes: for tokens that are
-    given several positions, which of them each pair turns by.  The table is copied to the host."""
+    given several positions, which of them each pair turns by.  The table is copied to the host;
+    the kernels take it from there, so none of this can be replaced (AttributeError)."""
 
     __slots__ = ("inv_freq", "layout", "factor", "axes", "dims", "_bytes", "_c", "_at")
 

@@ -38,3 +38,18 @@ def test_a_pool_keeps_its_tensors(on_cpu):
     assert c.k is k and c._c[4] == k.data_ptr() and c.page == 16
     d = copy.deepcopy(c)
     assert d.k.data_ptr() == d._c[4] != c._c[4]
+
+
+def test_a_rotary_embedding_keeps_its_table(pkg):
+    """The struct that the kernels read holds the table's address, the layout and the factor."""
+    r = pkg.Rotary.plain(32, 1e4, factor=1.5, axes=[0, 1] * 8)
+    f = r.inv_freq
+    for name, value in (("factor", 3.0), ("inv_freq", torch.ones(16)), ("layout", "interleaved"),
+                        ("axes", None), ("dims", 16), ("_c", None), ("_bytes", None), ("_at", 0)):
+        with pytest.raises(AttributeError):
+            setattr(r, name, value)
+    with pytest.raises(AttributeError):
+        del r.inv_freq
+    assert r.inv_freq is f and r._c.inv_freq == f.data_ptr()
+    assert (r.factor, r._c.factor, r.layout, r._c.layout, r.dims) == (1.5, 1.5, "half", 0, 32)
+    assert copy.deepcopy(r).factor == 1.5
