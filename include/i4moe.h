@@ -831,8 +831,8 @@ int    i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B, int T, 
 
 /* A 16-bit cache in pages: position j of sequence b is row j % page of page
  * table[b][j / page], k and v [pages][n_kv_heads][page][head_dim] with strides in elements (the
- * same for k and v, any order; the page head_dim values of a head's page adjacent, 16-byte
- * aligned).  Entries that no visible position needs are not used and may hold anything.  An
+ * same for k and v, in any order that keeps pages and heads apart: the larger steps over all that
+ * the smaller one reaches; the page head_dim values of a head's page adjacent, 16-byte aligned).  Entries that no visible position needs are not used and may hold anything.  An
  * entry outside [0, pages) where one is needed is never followed: the append writes nothing and
  * gives a NaN row, the attention a NaN row to the queries that see such a position.  Several
  * sequences may hold a page; who appends to one holds it alone.  head_dim == 128, page a power

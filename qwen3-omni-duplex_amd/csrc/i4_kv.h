@@ -71,6 +71,13 @@ __device__ inline PageRows page_rows(const Pages& pg, const int32_t* row, int g,
   return page_rows_of(id, pg.pages, pg.ps, pg.hs, pg.shift, KHD * 2, g, j);
 }
 
+// Whether n x m blocks that are distinct along each dimension (strides sn and sm) are so along
+// both: the larger stride steps over all that the smaller one reaches.
+inline bool blocks_apart(int64_t size, int n, int64_t sn, int m, int64_t sm) {
+  if (n < 2 || m < 2) return true;
+  return sn < sm ? sm >= size + (__int128)(n - 1) * sn : sn >= size + (__int128)(m - 1) * sm;
+}
+
 // A block's scale from what is stored: at least the smallest that the append writes, so that
 // nothing is divided by a scale of 0 (an empty cache's, or another quantiser's for a block of
 // zeros); NaN stays.  Taken where the scale is used, not where it is loaded: there it would

@@ -148,6 +148,8 @@ int i4_check_pagedcache(const i4_pagedcache* c) {
   if (((uintptr_t)c->k & 15) || ((uintptr_t)c->v & 15) || ((uintptr_t)c->table & 3) ||
       (c->page_stride & 7) || (c->head_stride & 7))
     return I4_ERR_ALIGN;
+  if (!i4::blocks_apart(rows, c->pages, c->page_stride, c->n_kv_heads, c->head_stride))
+    return I4_ERR_STRIDE;
   return I4_OK;
 }
 

@@ -26,7 +26,7 @@ import torch
 from . import _lib, kv
 from .kv import _batched, _call, _host_pos, _int32, _out
 from .ops import Workspace
-from .rotary import Rotary, _turn_c, overlaps
+from .rotary import Rotary, _turn_c, distinct, overlaps
 
 _paged = struct.Struct("<3Q3q7i4x").pack  # struct i4_pagedcache
 
@@ -47,6 +47,8 @@ class PagedCache(_lib.Handle):
         pages, n, page, hd = k.shape
         if k.stride(3) != 1 or k.stride(2) != hd:
             raise RuntimeError("the rows of a head's page must be dense")
+        if not distinct(page * hd, (pages, k.stride(0)), (n, k.stride(1))):
+            raise RuntimeError("pages or heads of the pool overlap")
         if k.numel() and overlaps(k, v):
             raise RuntimeError("k and v must be pools of their own")
         if page < 16 or page > 1024 or page & (page - 1):

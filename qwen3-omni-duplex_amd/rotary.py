@@ -164,6 +164,17 @@ def overlaps(x: torch.Tensor, y: torch.Tensor) -> bool:
     return not apart and off == 0
 
 
+def distinct(size: int, *dims: tuple[int, int]) -> bool:
+    """Whether blocks of `size` adjacent elements, dims of (count, stride) of them, are distinct:
+    each dimension steps over all that the smaller strides reach."""
+    for n, s in sorted(dims, key=lambda d: d[1]):
+        if n > 1:
+            if s < size:
+                return False
+            size += (n - 1) * s
+    return True
+
+
 def _apart(shape: tuple[int, ...], stride: tuple[int, ...]) -> bool:
     """Whether the rows [B, T, heads, head_dim] are dense and lie apart."""
     hd = shape[3]

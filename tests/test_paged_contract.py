@@ -7,6 +7,9 @@ import copy
 import pytest
 import torch
 
+from tests.test_kv import ALIGN, STRIDE, P
+from tests.test_paged import cache, call_append, call_attn, lb  # noqa: F401 (a fixture)
+
 BF = torch.bfloat16
 
 
@@ -53,3 +56,38 @@ def test_a_rotary_embedding_keeps_its_table(pkg):
     assert r.inv_freq is f and r._c.inv_freq == f.data_ptr()
     assert (r.factor, r._c.factor, r.layout, r._c.layout, r.dims) == (1.5, 1.5, "half", 0, 32)
     assert copy.deepcopy(r).factor == 1.5
+
+
+def distinct_elements(x):
+    """Whether no two places of a view are one element (by counting them)."""
+    at = torch.zeros(1, dtype=torch.long)
+    for n, s in zip(x.shape, x.stride()):
+        at = (at[:, None] + torch.arange(n) * s).flatten()
+    return at.unique().numel() == at.numel()
+
+
+POOLS = [  # pages, heads, strides of pages and heads in pages' rows (16 x 128 values), distinct
+    (4, 4, 1, 1, False), (4, 4, 4, 1, True), (4, 4, 1, 4, True), (4, 4, 3, 1, False),
+    (4, 4, 1, 3, False), (5, 3, 3, 1, True), (5, 3, 1, 5, True), (5, 3, 1, 4, False),
+    (3, 4, 9, 2, True), (3, 4, 2, 6, True), (1, 4, 1, 1, True), (4, 1, 1, 1, True),
+    (1, 4, 0, 1, True), (4, 1, 1, 0, True), (2, 2, 0, 1, False)]
+
+
+@pytest.mark.parametrize("pages,heads,ps,hs,good", POOLS)
+def test_pages_of_a_pool_are_distinct(lb, on_cpu, pages, heads, ps, hs, good):  # noqa: F811
+    """Pages or heads that lie on each other would be written by several sessions or heads."""
+    rows = 16 * 128
+    k, v = (torch.zeros(40 * rows, dtype=BF).as_strided(
+        (pages, heads, 16, 128), (ps * rows, hs * rows, 128, 1)) for _ in range(2))
+    assert distinct_elements(k) == good
+    bad = dict(pages=pages, n_kv_heads=heads, page=16, page_stride=ps * rows, head_stride=hs * rows)
+    if good:
+        assert on_cpu.PagedCache(k, v).pages == pages
+        # the C entries come as far as the checks behind it, and are stopped there
+        assert call_append(lb, on_cpu.lib(), cache(lb, **bad), nh=heads, qkv=P + 2) == ALIGN
+        assert call_attn(lb, on_cpu.lib(), cache(lb, **bad), nh=heads, q=P + 2) == ALIGN
+    else:
+        with pytest.raises(RuntimeError, match="overlap"):
+            on_cpu.PagedCache(k, v)
+        assert call_append(lb, on_cpu.lib(), cache(lb, **bad), nh=heads) == STRIDE
+        assert call_attn(lb, on_cpu.lib(), cache(lb, **bad), nh=heads) == STRIDE
