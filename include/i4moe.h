@@ -813,7 +813,8 @@ typedef struct i4_turn {
 
 /* Rows of heads that a rotation reads and writes: token t, head h of sequence b at
  * x + b xb + t xt + h xh (elements), and y likewise; y is x itself (the same strides: in place)
- * or does not overlap it. */
+ * or does not overlap it.  y's rows do not overlap each other: ordered by size, each of its strides
+ * steps over all that the smaller ones reach. */
 typedef struct i4_heads {
   const void* x;
   void*       y;

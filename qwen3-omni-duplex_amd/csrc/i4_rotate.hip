@@ -272,6 +272,22 @@ static int heads_check(const i4_heads* g, int B, int T, int hd) {
   if (((uintptr_t)g->x & 1) || ((uintptr_t)g->y & 1)) return I4_ERR_ALIGN;
   return I4_OK;
 }
+// Whether the output's rows, which several workgroups write, are distinct: from the smallest
+// stride on, each steps over all that the ones before reach.
+static bool rows_apart(const i4_heads* g, int B, int T, int hd) {
+  int64_t n[3] = {B, T, g->heads}, s[3] = {g->yb, g->yt, g->yh};
+  __int128 reach = hd;
+  for (int i = 0; i < 3; ++i) {
+    int j = -1;
+    for (int k = 0; k < 3; ++k)
+      if (n[k] > 1 && (j < 0 || s[k] < s[j])) j = k;
+    if (j < 0) break;
+    if (s[j] < reach) return false;
+    reach += (__int128)(n[j] - 1) * s[j];
+    n[j] = 1;
+  }
+  return true;
+}
 
 }  // namespace i4
 
@@ -311,6 +327,8 @@ extern "C" int i4_rope(const i4_heads* q, const i4_heads* k, int x_dtype, int B,
   if (!rc && k) rc = heads_check(k, B, T, head_dim);
   if (rc) return rc;
   if ((int64_t)B * T > kMaxGrid) return I4_ERR_SHAPE;
+  if (!rows_apart(q, B, T, head_dim) || (k && !rows_apart(k, B, T, head_dim)))
+    return I4_ERR_STRIDE;
   if (((uintptr_t)pos_dev & 3) || ((uintptr_t)counts & 3)) return I4_ERR_ALIGN;
   if (!turn && !pos_dev && (pos <= -ROPE_MAX_POS || pos > ROPE_MAX_POS - T)) return I4_ERR_SHAPE;
   RopeCall a{};

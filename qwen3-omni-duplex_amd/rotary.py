@@ -175,8 +175,8 @@ def distinct(size: int, *dims: tuple[int, int]) -> bool:
     return True
 
 
-def _apart(shape: tuple[int, ...], stride: tuple[int, ...]) -> bool:
-    """Whether the rows [B, T, heads, head_dim] are dense and lie apart."""
+def _dense(shape: tuple[int, ...], stride: tuple[int, ...]) -> bool:
+    """Whether the rows [B, T, heads, head_dim] are as the entry reads them."""
     hd = shape[3]
     return stride[3] == 1 and (shape[2] == 1 or stride[2] >= hd) and (
         shape[1] == 1 or stride[1] >= hd) and (shape[0] == 1 or stride[0] >= hd)
@@ -212,12 +212,13 @@ def _into(xs: list[torch.Tensor], out: tuple[torch.Tensor | None, ...],
     for y, x in zip(ys, xs):
         if y.shape != x.shape or y.dtype != x.dtype:
             raise RuntimeError(f"out must be a {tuple(x.shape)} tensor of {x.dtype}")
-        if not _apart(y.shape, y.stride()):
+        if not _dense(y.shape, y.stride()) \
+                or not distinct(y.shape[3], *zip(y.shape[:3], y.stride()[:3])):
             raise RuntimeError("out's rows must be dense and lie apart")
         if y.data_ptr() != x.data_ptr() or y.stride() != x.stride():  # not in place
             if overlaps(y, x):
                 raise RuntimeError("out is its input itself or does not overlap it")
-            if not _apart(x.shape, x.stride()):
+            if not _dense(x.shape, x.stride()):
                 x = x.contiguous()
                 held.append(x)
         cs.append(_heads(x.data_ptr(), y.data_ptr(), *x.stride()[:3], *y.stride()[:3],
@@ -239,7 +240,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
     back: rope(rope(x, p), -p) is x to rounding, and the gradient of rope(x, p) is that of its
     output turned by -p.  A position at or behind +-2^24 gives NaN, an int is refused.  q and k
     may have any strides above a dense last dimension, and so may out, a pair of tensors that
-    are q and k themselves (in place) or do not overlap them or each other.  Padding (counts,
+    are q and k themselves (in place) or do not overlap them, each other or themselves.  Padding (counts,
     int32 [B] on the device) is zeros in new outputs and left as it is in given ones."""
     dev = _lib.require_device(q, k, counts)
     code = _lib.half_code(q.dtype)

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from tests.test_kv import ALIGN, STRIDE, P
-from tests.test_paged import cache, call_append, call_attn, lb  # noqa: F401 (a fixture)
+from tests.test_paged import cache, call_append, call_attn, call_rope, heads, lb, rotary as rot  # noqa: F401 (a fixture)
 
 BF = torch.bfloat16
 
@@ -91,3 +91,35 @@ def test_pages_of_a_pool_are_distinct(lb, on_cpu, pages, heads, ps, hs, good):  
             on_cpu.PagedCache(k, v)
         assert call_append(lb, on_cpu.lib(), cache(lb, **bad), nh=heads) == STRIDE
         assert call_attn(lb, on_cpu.lib(), cache(lb, **bad), nh=heads) == STRIDE
+
+
+OUTPUTS = [  # strides of sequences, tokens and heads in rows (2 x 3 x 4 of 16 dims), distinct
+    ((12, 4, 1), True), ((12, 1, 3), True), ((4, 8, 1), True), ((1, 8, 2), True),
+    ((40, 9, 2), True), ((12, 1, 1), False), ((12, 4, 4), False), ((12, 3, 1), False),
+    ((12, 1, 2), False), ((9, 4, 1), False), ((1, 1, 1), False), ((4, 4, 1), False)]
+
+
+@pytest.mark.parametrize("strides,good", OUTPUTS)
+def test_rows_of_an_output_are_distinct(lb, on_cpu, strides, good):  # noqa: F811
+    """Rows that lie on each other are written by several workgroups at once."""
+    (b, t, h), hd = strides, 16
+    y = torch.zeros(100 * hd, dtype=BF).as_strided((2, 3, 4, hd), (b * hd, t * hd, h * hd, 1))
+    x = torch.zeros(2, 3, 4, hd, dtype=BF)
+    r = on_cpu.Rotary.plain(hd, 1e4)
+    assert distinct_elements(y) == good
+    c = dict(xb=192, xt=64, xh=16, yb=b * hd, yt=t * hd, yh=h * hd, heads=4)
+    one = dict(pairs=8)
+    if good:  # as far as the next check, in place too
+        assert call_rope(lb, on_cpu.lib(), heads(lb, **c), r=rot(lb, **one), hd=hd, T=3,
+                         pos_dev=P + 2) == ALIGN
+    else:
+        for out in ((y, None), (x, y)):
+            with pytest.raises(RuntimeError, match="apart"):
+                on_cpu.rope(x, None if out[1] is None else x.clone(), 0, r, out=out)
+        with pytest.raises(RuntimeError, match="apart"):
+            on_cpu.rope(y, None, 0, r, out=(y, None))
+        for q, k in ((c, None), ({}, c)):
+            base = dict(xb=192, xt=64, xh=16, yb=192, yt=64, yh=16, heads=4)
+            assert call_rope(lb, on_cpu.lib(), heads(lb, **{**base, **q}),
+                             k and heads(lb, **k), r=rot(lb, **one), hd=hd, T=3,
+                             pos_dev=P + 2) == STRIDE
