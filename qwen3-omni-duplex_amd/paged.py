@@ -81,6 +81,12 @@ class PagedCache(_lib.Handle):
                 _lib.require_device(self.k, t)  # which says what is wrong
         return self.device
 
+    def _beyond(self, out: torch.Tensor) -> None:
+        """A given output lies outside the pool, which a call reads or writes as it writes it."""
+        rows = out.view(1, 1, -1, out.shape[-1])
+        if overlaps(rows, self.k) or overlaps(rows, self.v):
+            raise RuntimeError("out must not overlap the pool")
+
     def _with(self, table: torch.Tensor, B: int) -> tuple[bytes, int]:
         """struct i4_pagedcache of this pool under a call's table, and its positions."""
         shape, stride = table.shape, table.stride()
@@ -137,8 +143,10 @@ def paged_append(qkv: torch.Tensor, n_heads: int, q_norm_w: torch.Tensor | None,
         q = x.new_empty(shape)
     else:
         q = _out(out, x, shape, False)
-        if overlaps(q.view(B, T, n_heads, hd), x.unflatten(2, (-1, hd))):
+        y = q.view(B, T, n_heads, hd)
+        if overlaps(y, x.unflatten(2, (-1, hd))):
             raise RuntimeError("out must not overlap qkv")
+        cache._beyond(y)
     pd, ph = (_int32(pos, B, dev, "pos"), 0) if isinstance(pos, torch.Tensor) \
         else (None, _host_pos(pos, T, keys))
     tc = None if turn is None else _turn_c(turn, rotary, batched, B, T, dev)
@@ -179,6 +187,7 @@ def attn_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor,
         y = _out(out, x, tuple(q.shape), False)
         if overlaps(out, q):
             raise RuntimeError("out must not overlap q")
+        cache._beyond(out)
     pd, ph = (_int32(pos, B, dev, "pos"), 0) if isinstance(pos, torch.Tensor) \
         else (None, _host_pos(pos, T, keys))
     if torch.cuda.current_device() != dev.index:

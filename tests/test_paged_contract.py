@@ -123,3 +123,27 @@ def test_rows_of_an_output_are_distinct(lb, on_cpu, strides, good):  # noqa: F81
             assert call_rope(lb, on_cpu.lib(), heads(lb, **{**base, **q}),
                              k and heads(lb, **k), r=rot(lb, **one), hd=hd, T=3,
                              pos_dev=P + 2) == STRIDE
+
+
+def test_outputs_lie_outside_the_pool(on_cpu, monkeypatch):
+    """A call reads or writes the pool while it writes its output."""
+    room = torch.zeros(3, 4, 2, 16, 128, dtype=BF)  # two pools, and rows behind them
+    c = on_cpu.PagedCache(room[0], room[1])
+    t = torch.zeros(1, 2, dtype=torch.int32)
+    q, x = torch.zeros(1, 3, 4, 128, dtype=BF), torch.zeros(1, 3, 8 * 128, dtype=BF)
+    r = on_cpu.Rotary.plain(128, 1e4)
+    flat = room.view(-1, 128)
+    edge = 2 * 4 * 2 * 16  # the first row behind the pools
+    for row in (0, 100, 128, edge - 12, edge - 1):
+        out = flat[row:row + 12].view(1, 3, 4, 128)
+        with pytest.raises(RuntimeError, match="overlap the pool"):
+            on_cpu.attn_paged(q, c, t, 0, out=out)
+        with pytest.raises(RuntimeError, match="overlap the pool"):
+            on_cpu.paged_append(x, 4, None, None, 1e-6, r, 0, c, t, out=out)
+        with pytest.raises(RuntimeError, match="overlap the pool"):
+            on_cpu.attn_paged(q[0], c, t[0], 0, out=out[0])
+    behind = flat[edge:edge + 12].view(1, 3, 4, 128)
+    for call in (lambda: on_cpu.attn_paged(q, c, t, 40, out=behind),
+                 lambda: on_cpu.paged_append(x, 4, None, None, 1e-6, r, 40, c, t, out=behind)):
+        with pytest.raises(RuntimeError, match="outside"):  # the check behind this one
+            call()
