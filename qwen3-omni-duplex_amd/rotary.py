@@ -67,21 +67,43 @@ class Rotary(_lib.Handle):
 
     @classmethod
     def scaled(cls, dims: int, theta: float, scale: float, trained: int | None = None, *,
-               slow: float = 1.0, fast: float = 32.0, factor: float | None = None,
-               **kw) -> "Rotary":
+               slow: float = 1.0, fast: float = 32.0, blend: str = "turns", whole: bool = True,
+               factor: float | None = None, **kw) -> "Rotary":
         """A table for contexts `scale` times as long as the model was trained for.
 
         trained None: every position is divided by scale.  Else by parts (arXiv 2309.00071): a
         pair that turns more than `fast` times within `trained` positions keeps its frequency,
         one that turns less than `slow` times has it divided by scale, and those between are
-        blended by their number of turns; factor defaults to 0.1 ln(scale) + 1."""
-        if scale < 1 or not fast > slow:
-            raise RuntimeError("scale is at least 1, and fast above slow")
-        f = theta ** (-torch.arange(0, dims, 2, dtype=torch.double) / dims)
+        blended; factor defaults to 0.1 ln(scale) + 1.  blend says by what:
+
+        "turns"  by their number of turns, as that paper's text has it
+        "pairs"  by their number, linearly between the two bounds, each a pair's number (whole:
+                 the next whole one outwards).  That is the table of published checkpoints whose
+                 config says "yarn"; the frequencies in between differ from the other rule's by
+                 up to half."""
+        if not scale >= 1 or not fast > slow or not slow > 0:
+            raise RuntimeError("scale is at least 1, and fast above slow above 0")
+        if blend not in ("turns", "pairs"):
+            raise RuntimeError(f"blend is 'turns' or 'pairs', got {blend!r}")
+        i = torch.arange(0, dims, 2, dtype=torch.double)
+        f = theta ** (-i / dims)
         if trained is None:
             f = f / scale
         else:
-            keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+            if blend == "turns":
+                keep = ((trained * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+            else:
+                # pair n turns trained theta ** (-2 n / dims) / (2 pi) times
+                lo, hi = (dims * math.log(trained / (2 * math.pi * n)) / (2 * math.log(theta))
+                          for n in (fast, slow))
+                if whole:
+                    lo, hi = math.floor(lo), math.ceil(hi)
+                lo, hi = max(lo, 0), min(hi, dims - 1)
+                if lo > hi:
+                    raise RuntimeError(f"no pair turns between {slow} and {fast} times within "
+                                       f"{trained} positions")
+                # (bounds at one pair: a step behind it)
+                keep = 1 - ((i / 2 - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
             f = f * keep + f / scale * (1 - keep)
             factor = 0.1 * math.log(scale) + 1 if factor is None else factor
         return cls(f.float(), factor=1.0 if factor is None else factor, **kw)

@@ -1,0 +1,65 @@
+"""Rotary tables and the loader's reading of a config against transformers' own module (the
+installed transformers, fp32 on the CPU)."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+M = pytest.importorskip("transformers.models.qwen3_omni_moe.modeling_qwen3_omni_moe")
+
+# What fp32 costs the module's table, relative: the exponent's rounding (2^-25 ln theta, at most
+# 2^-21), the power and quotients (2^-22), and the blend's share, off by 2^-22, of up to
+# scale - 1 <= 31 times the slowed frequency (2^-17).  Another rule is off by 2^-7 and more.
+FP32 = 2.0 ** -16
+
+
+def theirs(rope, head_dim=128, theta=1e6, **kw):
+    """The module for a config with these rope parameters."""
+    from transformers.models.qwen3_omni_moe.configuration_qwen3_omni_moe import (
+        Qwen3OmniMoeTextConfig,
+    )
+
+    return M.Qwen3OmniMoeThinkerTextRotaryEmbedding(Qwen3OmniMoeTextConfig(
+        hidden_size=128, num_attention_heads=2, num_key_value_heads=1, head_dim=head_dim,
+        rope_scaling=dict(rope), rope_theta=theta, num_hidden_layers=1, num_experts=4,
+        num_experts_per_tok=2, moe_intermediate_size=32, intermediate_size=64, **kw))
+
+
+def close(ours, module):
+    torch.testing.assert_close(ours.inv_freq.double(), module.inv_freq.double(), rtol=FP32, atol=0)
+    assert math.isclose(ours.factor, module.attention_scaling, rel_tol=2.0 ** -22)
+
+
+@pytest.mark.parametrize("dims,theta,scale,trained,kw", [
+    (128, 1e6, 4.0, 32768, {}), (128, 1e4, 8.0, 4096, {}), (64, 1e4, 16.0, 2048, {}),
+    (128, 1e6, 1.0, 32768, {}), (128, 1e6, 2.0, 262144, {"slow": 2.0, "fast": 16.0}),
+    (128, 1e6, 4.0, 32768, {"whole": False}), (32, 500.0, 32.0, 100, {}),
+    (128, 100.0, 4.0, 1000000, {}), (256, 1e6, 4.0, 20, {}), (128, 1e6, 4.0, 32768,
+                                                             {"factor": 1.25})])
+def test_scaled_tables_are_those_of_checkpoints(pkg, dims, theta, scale, trained, kw):
+    rope = {"rope_type": "yarn", "factor": scale, "original_max_position_embeddings": trained}
+    for ours, name in (("slow", "beta_slow"), ("fast", "beta_fast"), ("whole", "truncate"),
+                       ("factor", "attention_factor")):
+        if ours in kw:
+            rope[name] = kw[ours]
+    close(pkg.Rotary.scaled(dims, theta, scale, trained, blend="pairs", **kw),
+          theirs(rope, dims, theta))
+    if scale > 1 and (dims, theta) == (128, 1e6):  # the paper's text is another table
+        other = pkg.Rotary.scaled(dims, theta, scale, trained, **{**kw, "whole": True})
+        want = theirs(rope, dims, theta).inv_freq
+        assert ((other.inv_freq - want).abs() > 2.0 ** -7 * want).any()
+
+
+def test_divided_positions(pkg):
+    close(pkg.Rotary.scaled(128, 1e6, 4.0), theirs({"rope_type": "linear", "factor": 4.0}))
+
+
+def test_scaled_refuses(pkg):
+    for kw, match in ((dict(blend="both"), "blend"), (dict(slow=0.0), "slow"),
+                      (dict(scale=math.nan), "scale"),
+                      (dict(blend="pairs", trained=2), "no pair")):
+        a = {**dict(scale=4.0, trained=4096), **kw}
+        with pytest.raises(RuntimeError, match=match):
+            pkg.Rotary.scaled(64, 1e4, a.pop("scale"), a.pop("trained"), **a)
