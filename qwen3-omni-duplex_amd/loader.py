@@ -28,6 +28,7 @@ Checkpoint tensor names (Qwen3-Omni, transformers 4.57 layout):
 from __future__ import annotations
 
 import json
+import math
 from pathlib import Path
 
 import torch
@@ -224,24 +225,53 @@ def rope_theta(tc: dict) -> float:
     return 10000.0
 
 
+def _rope_config(tc: dict) -> tuple[dict, str]:
+    """What a text config says of its rotary embedding, and the embedding's type."""
+    rope = {**(tc.get("rope_parameters") or {}), **(tc.get("rope_scaling") or {})}
+    return rope, str(rope.get("rope_type") or rope.get("type") or "default")
+
+
 def thinker_rotary(tc: dict, head_dim: int) -> Rotary:
-    """The rotary embedding of a text config: the default table, and where it has interleaved
-    sections (mrope_section) the axes of the tokens of images, video and audio."""
-    sections, interleaved = None, False
-    for src in (tc.get("rope_parameters") or {}, tc.get("rope_scaling") or {}):
-        sections = src.get("mrope_section", sections)
-        interleaved |= bool(src.get("mrope_interleaved") or src.get("interleaved"))
-    table = rope_inv_freq(head_dim, rope_theta(tc))
-    if not interleaved or not sections or sum(sections) != table.numel():
-        return Rotary(table)
-    return Rotary(table, axes=interleaved_axes(sections))
+    """The rotary embedding of a text config (Qwen3OmniMoeThinkerTextRotaryEmbedding,
+    transformers 5.15): the default table, one of divided positions ("linear") or one scaled by
+    parts ("yarn"), other types are refused; and where it has interleaved sections
+    (mrope_section) the axes of the tokens of images, video and audio."""
+    rope, kind = _rope_config(tc)
+    sections = rope.get("mrope_section")
+    interleaved = bool(rope.get("mrope_interleaved") or rope.get("interleaved"))
+    axes = interleaved_axes(sections) if interleaved and sections \
+        and 2 * sum(sections) == head_dim else None
+    theta = rope_theta(tc)
+    if kind == "default":
+        return Rotary(rope_inv_freq(head_dim, theta), axes=axes)
+    if kind not in ("linear", "yarn"):
+        raise NotImplementedError(f"rotary embeddings of type {kind!r} are not read")
+    if rope.get("factor") is None:
+        raise ValueError(f"a rotary embedding of type {kind!r} without its factor")
+    if rope.get("partial_rotary_factor") not in (None, 1, 1.0):
+        raise NotImplementedError("scaled rotary embeddings of part of a head are not read")
+    scale = float(rope["factor"])
+    if kind == "linear":
+        return Rotary.scaled(head_dim, theta, scale, axes=axes)
+    trained = rope.get("original_max_position_embeddings") or tc.get("max_position_embeddings")
+    if not trained:
+        raise ValueError("a rotary embedding of type 'yarn' without the length that the model "
+                         "was trained for")
+    factor = rope.get("attention_factor")
+    if factor is None and rope.get("mscale") and rope.get("mscale_all_dim"):
+        factor = (0.1 * rope["mscale"] * math.log(scale) + 1) / (
+            0.1 * rope["mscale_all_dim"] * math.log(scale) + 1)
+    return Rotary.scaled(head_dim, theta, scale, trained, blend="pairs",
+                         slow=rope.get("beta_slow") or 1.0, fast=rope.get("beta_fast") or 32.0,
+                         whole=rope.get("truncate", True), factor=factor, axes=axes)
 
 
 def load_thinker_layer(ckpt: Checkpoint, layer: int, device="cuda", dtype=torch.bfloat16,
                        max_len: int = 4096, layouts: str = "both",
                        **context) -> ThinkerDecoderLayer:
     """One Thinker decoder layer for decode (context: ThinkerAttention's window, sinks,
-    kv_dtype, pages, page and rotary, with pages by default the config's with its axes):
+    kv_dtype, pages, page and rotary, with pages by default the config's with its axes;
+    without pages a config's table has to be the default one):
     attention (input_layernorm, q|k|v in one
     launch, q_norm / k_norm, rotary, KV cache of max_len positions, o_proj) and the MoE
     block with its post_attention_layernorm (clock.py:45-103 loads the same tensors)."""
@@ -251,6 +281,9 @@ def load_thinker_layer(ckpt: Checkpoint, layer: int, device="cuda", dtype=torch.
     hd = int(tc.get("head_dim") or tc["hidden_size"] // nh)
     if context.get("pages") is not None and context.get("rotary") is None:
         context = {**context, "rotary": thinker_rotary(tc, hd)}
+    elif context.get("pages") is None and _rope_config(tc)[1] != "default":
+        raise NotImplementedError(f"rotary embeddings of type {_rope_config(tc)[1]!r} need a "
+                                  "cache in pages")
     proj = load_attention(ckpt, layer, device, fuse_qkv=True)
     attn = ThinkerAttention(
         proj["qkv"], proj["o"],

@@ -63,3 +63,64 @@ def test_scaled_refuses(pkg):
         a = {**dict(scale=4.0, trained=4096), **kw}
         with pytest.raises(RuntimeError, match=match):
             pkg.Rotary.scaled(64, 1e4, a.pop("scale"), a.pop("trained"), **a)
+
+
+CONFIGS = [
+    {"rope_type": "default"}, {"type": "default"}, {"rope_type": "linear", "factor": 4.0},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768},
+    {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 8192},
+    {"rope_type": "yarn", "factor": 2.0},  # trained for max_position_embeddings
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768,
+     "attention_factor": 1.5, "beta_fast": 16.0, "beta_slow": 2.0},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768,
+     "mscale": 0.7, "mscale_all_dim": 1.0, "truncate": False},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768,
+     "mscale": 0.7, "attention_factor": None, "beta_fast": None}]
+
+
+@pytest.mark.parametrize("rope", CONFIGS)
+@pytest.mark.parametrize("where", ["rope_scaling", "rope_parameters"])
+def test_loader_builds_the_config_s_table(pkg, rope, where):
+    from qwen3_omni_duplex_amd.loader import thinker_rotary
+
+    tc = {"rope_theta": 1e6, "max_position_embeddings": 65536, where: rope}
+    close(thinker_rotary(tc, 128), theirs(rope, max_position_embeddings=65536))
+    axes = {"mrope_section": [24, 20, 20], "mrope_interleaved": True}
+    with_axes = thinker_rotary({**tc, where: {**rope, **axes}}, 128)
+    assert with_axes.axes == pkg.interleaved_axes([24, 20, 20])
+    close(with_axes, theirs(rope, max_position_embeddings=65536))
+
+
+@pytest.mark.parametrize("rope", [
+    {"rope_type": "dynamic", "factor": 4.0}, {"rope_type": "llama3", "factor": 8.0},
+    {"type": "longrope", "factor": 4.0}, {"rope_type": "linear"}, {"rope_type": "yarn"},
+    {"rope_type": "yarn", "factor": 4.0}, {"rope_type": "linear", "factor": 2.0,
+                                           "partial_rotary_factor": 0.5}])
+def test_loader_refuses_other_tables(pkg, rope):
+    """A rotation that is not built is refused, not replaced by the plain one."""
+    from qwen3_omni_duplex_amd.loader import thinker_rotary
+
+    with pytest.raises((NotImplementedError, ValueError), match="rotary"):
+        thinker_rotary({"rope_theta": 1e6, "rope_scaling": rope}, 128)
+
+
+@pytest.mark.parametrize("context", [{}, {"window": 64}, {"kv_dtype": torch.int8}])
+def test_a_scaled_table_needs_pages(pkg, tmp_path, context):
+    """The other caches' entries turn by the plain table: a config with another one is refused
+    before a weight is read, a default one is not."""
+    import json
+
+    from qwen3_omni_duplex_amd import loader
+
+    def layer(rope):
+        tc = {"num_attention_heads": 8, "num_key_value_heads": 2, "hidden_size": 1024,
+              "head_dim": 128, "rope_theta": 1e6, "rope_scaling": rope}
+        (tmp_path / "config.json").write_text(json.dumps({"text_config": tc}))
+        (tmp_path / "model.safetensors.index.json").write_text('{"weight_map": {}}')
+        return loader.load_thinker_layer(loader.Checkpoint(tmp_path), 0, "cpu", **context)
+
+    with pytest.raises(NotImplementedError, match="pages"):
+        layer({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768})
+    for rope in ({"rope_type": "default"}, None):
+        with pytest.raises(KeyError):  # the first weight
+            layer(rope)
