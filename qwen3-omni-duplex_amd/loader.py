@@ -30,6 +30,7 @@ from __future__ import annotations
 import json
 import math
 from pathlib import Path
+from typing import Sequence
 
 import torch
 
@@ -231,16 +232,19 @@ def _rope_config(tc: dict) -> tuple[dict, str]:
     return rope, str(rope.get("rope_type") or rope.get("type") or "default")
 
 
-def thinker_rotary(tc: dict, head_dim: int) -> Rotary:
+# the sections of a Thinker whose config names none
+SECTIONS = (24, 20, 20)
+
+
+def thinker_rotary(tc: dict, head_dim: int, sections: Sequence[int] | None = None) -> Rotary:
     """The rotary embedding of a text config (Qwen3OmniMoeThinkerTextRotaryEmbedding,
     transformers 5.15): the default table, one of divided positions ("linear") or one scaled by
-    parts ("yarn"), other types are refused; and where it has interleaved sections
-    (mrope_section) the axes of the tokens of images, video and audio."""
+    parts ("yarn"), other types are refused; and the axes of the tokens of images, video and
+    audio, interleaved in its sections (mrope_section, else the ones given).  Sections that are
+    not as many as the pairs give no axes: positions on several are then refused by the call."""
     rope, kind = _rope_config(tc)
-    sections = rope.get("mrope_section")
-    interleaved = bool(rope.get("mrope_interleaved") or rope.get("interleaved"))
-    axes = interleaved_axes(sections) if interleaved and sections \
-        and 2 * sum(sections) == head_dim else None
+    sections = rope.get("mrope_section") or sections
+    axes = interleaved_axes(sections) if sections and 2 * sum(sections) == head_dim else None
     theta = rope_theta(tc)
     if kind == "default":
         return Rotary(rope_inv_freq(head_dim, theta), axes=axes)
@@ -280,7 +284,7 @@ def load_thinker_layer(ckpt: Checkpoint, layer: int, device="cuda", dtype=torch.
     nh, nkv = int(tc["num_attention_heads"]), int(tc["num_key_value_heads"])
     hd = int(tc.get("head_dim") or tc["hidden_size"] // nh)
     if context.get("pages") is not None and context.get("rotary") is None:
-        context = {**context, "rotary": thinker_rotary(tc, hd)}
+        context = {**context, "rotary": thinker_rotary(tc, hd, SECTIONS)}
     elif context.get("pages") is None and _rope_config(tc)[1] != "default":
         raise NotImplementedError(f"rotary embeddings of type {_rope_config(tc)[1]!r} need a "
                                   "cache in pages")

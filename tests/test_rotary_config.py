@@ -124,3 +124,47 @@ def test_a_scaled_table_needs_pages(pkg, tmp_path, context):
     for rope in ({"rope_type": "default"}, None):
         with pytest.raises(KeyError):  # the first weight
             layer(rope)
+
+
+def angles(module, p):
+    """The angle of each pair that the module turns tokens at p [3, T] by, modulo a turn."""
+    cos, sin = module(torch.zeros(1, p.shape[1], 128), p[:, None])
+    return torch.atan2(sin[0], cos[0])[:, :cos.shape[-1] // 2]
+
+
+@pytest.mark.parametrize("rope", [
+    {"rope_type": "default", "mrope_section": [24, 20, 20], "mrope_interleaved": True},
+    {"rope_type": "default", "mrope_section": [24, 20, 20]},
+    {"rope_type": "default", "mrope_section": [32, 16, 16], "mrope_interleaved": False},
+    {"rope_type": "default"}, {}])
+def test_axes_of_a_config(pkg, rope, monkeypatch):
+    """Which position each pair turns by, found from the module's angles: with a flag or without,
+    and by the default sections where there are none.  The loader's path gives these axes."""
+    from qwen3_omni_duplex_amd import loader
+
+    module = theirs(rope or {"rope_type": "default"})
+    far = torch.tensor([[0], [0], [0]])
+    axes = [None] * 64
+    for a in range(3):
+        p = far.clone()
+        p[a] = 1
+        for i in (angles(module, p)[0] != 0).nonzero()[:, 0].tolist():
+            assert axes[i] is None
+            axes[i] = a
+    tc = {"num_attention_heads": 8, "num_key_value_heads": 2, "head_dim": 128, "rope_theta": 1e6,
+          "rope_scaling": rope}
+
+    class Config:
+        def text_config(self):
+            return tc
+
+        def tensor(self, name):
+            return torch.zeros(1)
+
+    seen = {}
+    monkeypatch.setattr(loader, "load_attention", lambda *a, **kw: {"qkv": None, "o": None})
+    monkeypatch.setattr(loader, "ThinkerAttention", lambda *a, **kw: seen.update(kw))
+    monkeypatch.setattr(loader, "load_moe_layer", lambda *a, **kw: None)
+    monkeypatch.setattr(loader, "ThinkerDecoderLayer", lambda *a: None)
+    loader.load_thinker_layer(Config(), 0, "cpu", pages=4)
+    assert seen["rotary"].axes == tuple(axes)
