@@ -804,7 +804,8 @@ typedef struct i4_rotary {
 
 /* Positions given for each token: int32 [axes][B][T] on the device (strides in elements, tokens
  * adjacent), for angles alone; several axes need rotary->axes.  |position| < 2^24; one outside
- * makes the token's rows NaN.  Negative ones turn back. */
+ * makes the token's rows NaN.  The negated ones turn back (times factor^2; a negated start does not:
+ * its token t turns by -pos + t). */
 typedef struct i4_turn {
   const int32_t* pos;
   int64_t axis_stride, batch_stride;

@@ -258,12 +258,18 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, pos: int | torch.Tensor, rotar
     pos: an int or int32 [B] on the device, the position of each sequence's first token; or the
     positions of the tokens themselves, int32 [B, T] on the device, or [axes, B, T] for a rotary
     embedding with axes ([T] or [axes, T] for tokens without a batch); with one position a token
-    every pair turns by it, as text tokens do.  Negative positions turn
-    back: rope(rope(x, p), -p) is x to rounding, and the gradient of rope(x, p) is that of its
-    output turned by -p.  A position at or behind +-2^24 gives NaN, an int is refused.  q and k
-    may have any strides above a dense last dimension, and so may out, a pair of tensors that
-    are q and k themselves (in place) or do not overlap them, each other or themselves.  Padding (counts,
-    int32 [B] on the device) is zeros in new outputs and left as it is in given ones."""
+    every pair turns by it, as text tokens do.  A position at or behind +-2^24 gives NaN, an int
+    is refused.
+
+    Negative positions turn back: with p the tokens' own positions ([B, T] or [axes, B, T]; T
+    tokens behind a start take theirs, since -start is a start again) rope(rope(x, p), -p) is
+    factor ** 2 x to rounding, and rope(dy, -p) the gradient of rope(x, p).  No autograd graph is
+    recorded.
+
+    q and k may have any strides above a dense last dimension, and so may out, a pair of tensors
+    that are q and k themselves (in place) or do not overlap them, each other or themselves.
+    Padding (counts, int32 [B] on the device) is zeros in new outputs and left as it is in given
+    ones."""
     dev = _lib.require_device(q, k, counts)
     code = _lib.half_code(q.dtype)
     batched = q.dim() == 4
