@@ -861,14 +861,17 @@ int    i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batch_stride
                        const int32_t* counts, int zero_padding, void* q_out,
                        const i4_pagedcache* cache, hipStream_t stream);
 
-/* i4_attn_window over pages.  Workspace: i4_attn_paged_workspace_bytes, keys = pos + T, or
- * table_len page for a device position. */
+/* i4_attn_window over pages.  Workspace: i4_attn_paged_call_bytes, keys = pos + T, or table_len
+ * page for a device position; on_device: whether pos_dev or counts are given (such calls of many
+ * rows may be split in another way).  i4_attn_paged_workspace_bytes holds either. */
 int    i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
                      int64_t q_token_stride, int64_t q_head_stride, int n_heads,
                      const i4_pagedcache* cache, const int32_t* pos_dev, int pos,
                      const int32_t* counts, int zero_padding, int window, int sinks, float scale,
                      void* out, void* workspace, size_t workspace_bytes, int32_t* counters,
                      hipStream_t stream);
+size_t i4_attn_paged_call_bytes(int B, int T, int n_heads, int n_kv_heads, int keys, int window,
+                                int sinks, int on_device);
 size_t i4_attn_paged_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                      int window, int sinks);
 

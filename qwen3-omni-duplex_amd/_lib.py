@@ -238,6 +238,8 @@ SIGNATURES = {
     "i4_attn_paged": (c_int, [c_void_p, c_int, c_int, c_int64, c_int64, c_int64, c_int,
                               c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
                               c_int, ctypes.c_float, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "i4_attn_paged_call_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                            c_int]),
     "i4_attn_paged_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int,
                                                  c_int]),
     "i4_dmoe_forward": (c_int, [c_void_p, c_int, c_int, POINTER(DmoeWeightsC), c_int, c_int,

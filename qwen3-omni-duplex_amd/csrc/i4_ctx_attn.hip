@@ -126,10 +126,16 @@ size_t i4_attn_window_workspace_bytes(int B, int T, int n_heads, int n_kv_heads,
                                       int window, int sinks) {
   return ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, false, false);
 }
+size_t i4_attn_paged_call_bytes(int B, int T, int n_heads, int n_kv_heads, int keys, int window,
+                                int sinks, int on_device) {
+  return ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true, on_device != 0);
+}
 size_t i4_attn_paged_workspace_bytes(int B, int T, int n_heads, int n_kv_heads, int keys,
                                      int window, int sinks) {
-  const size_t split = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true, false);
-  const size_t shared = ctx_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, true, true);
+  const size_t split =
+      i4_attn_paged_call_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, 0);
+  const size_t shared =
+      i4_attn_paged_call_bytes(B, T, n_heads, n_kv_heads, keys, window, sinks, 1);
   return split > shared ? split : shared;
 }
 
@@ -243,7 +249,8 @@ int i4_attn_paged(const void* q, int x_dtype, int T, int64_t q_batch_stride,
   rc = query_check(q, x_dtype, cache->dtype, B, T, q_batch_stride, q_token_stride, q_head_stride,
                    n_heads, nkv, pos_dev, pos, counts, len, window, sinks, scale, out, workspace,
                    workspace_bytes,
-                   i4_attn_paged_workspace_bytes(B, T, n_heads, nkv, keys, window, sinks),
+                   i4_attn_paged_call_bytes(B, T, n_heads, nkv, keys, window, sinks,
+                                            pos_dev || counts),
                    counters);
   if (rc) return rc;
   CtxArgs a = ctx_args(q, B, T, q_batch_stride, q_token_stride, q_head_stride, n_heads, nkv, pos_dev,

@@ -204,7 +204,8 @@ def attn_paged(q: torch.Tensor, cache: PagedCache, table: torch.Tensor,
     rc = lib.i4_attn_paged(*args, None, 0, None, stream) if ws is None else lib.i4_attn_paged(
         *args, ws.data_ptr(), ws.numel(), counters.data_ptr(), stream)
     if rc == _lib.ERR_WORKSPACE:
-        need = lib.i4_attn_paged_workspace_bytes(B, T, nh, n_kv, keys if pd else ph + T, w, sinks)
+        need = lib.i4_attn_paged_call_bytes(B, T, nh, n_kv, keys if pd else ph + T, w, sinks,
+                                            pd is not None or counts is not None)
         ws, counters = kv._scratch(workspace, need, dev, True)
         rc = lib.i4_attn_paged(*args, ws.data_ptr(), need, _lib.ptr(counters), stream)
     if rc:

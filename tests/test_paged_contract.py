@@ -7,7 +7,7 @@ import copy
 import pytest
 import torch
 
-from tests.test_kv import ALIGN, STRIDE, P
+from tests.test_kv import ALIGN, STRIDE, WORKSPACE, P
 from tests.test_paged import cache, call_append, call_attn, call_rope, heads, lb, rotary as rot  # noqa: F401 (a fixture)
 
 BF = torch.bfloat16
@@ -147,3 +147,29 @@ def test_outputs_lie_outside_the_pool(on_cpu, monkeypatch):
                  lambda: on_cpu.paged_append(x, 4, None, None, 1e-6, r, 40, c, t, out=behind)):
         with pytest.raises(RuntimeError, match="outside"):  # the check behind this one
             call()
+
+
+@pytest.mark.parametrize("B,T,nh,nkv,pos,window", [
+    (2, 100, 32, 4, 8000, 0), (4, 400, 32, 4, 9000, 0), (2, 100, 32, 4, 8000, 3000),
+    (1, 64, 32, 4, 30000, 0), (3, 17, 8, 1, 16000, 0), (24, 1, 32, 4, 20000, 0),
+    (1, 1, 8, 2, 5000, 0), (2, 300, 8, 2, 100, 0)])
+@pytest.mark.parametrize("form", ["host", "counts", "device"])
+def test_a_call_needs_the_scratch_that_it_uses(lb, pkg, B, T, nh, nkv, pos, window, form):  # noqa: F811
+    """One byte less than i4_attn_paged_call_bytes is refused, that many are not.  A call whose
+    lengths the host knows is split as attn_window's of many rows are, and needs no more."""
+    lib = pkg.lib()
+    n = -(-(pos + T) // 64)
+    keys = n * 64 if form == "device" else pos + T
+    size = (B, T, nh, nkv, keys, window, 0)
+    need = lib.i4_attn_paged_call_bytes(*size, form != "host")
+    assert need <= lib.i4_attn_paged_workspace_bytes(*size) \
+        == max(lib.i4_attn_paged_call_bytes(*size, d) for d in (0, 1))
+    if form == "host" and T * nh // nkv > 16:
+        assert need == lib.i4_attn_window_workspace_bytes(*size)
+    c = cache(lb, batch=B, n_kv_heads=nkv, table_len=n, table_stride=n, pages=5)
+    a = dict(T=T, nh=nh, ts=nh * 128, bs=T * nh * 128, window=window,
+             pos=0 if form == "device" else pos, pos_dev=P if form == "device" else None,
+             counts=P if form == "counts" else None)
+    if need:
+        assert call_attn(lb, lib, c, **a, wsb=need - 1) == WORKSPACE
+        assert call_attn(lb, lib, c, **a, wsb=need, ws=P + 128) == ALIGN  # the check behind it
