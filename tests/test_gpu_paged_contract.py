@@ -7,6 +7,7 @@ import torch
 from tests import _kv_ref as kvref
 from tests import _paged_ref as ref
 from tests.test_gpu_kv import i32, rand, same
+from tests.test_gpu_kv_module import build, near, tokens
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
@@ -60,3 +61,43 @@ def test_scratch_of_a_call_with_host_positions(pkg, dev):
     most = 4 * h * (cache.v.double().abs().max() + top) + 2.1 * h * top
     assert (a.double() - b.double()).abs().max() <= most
     assert same(pkg.attn_paged(q, cache, table, pos, workspace=ws), a)
+
+
+@pytest.mark.parametrize("T", [1, 4, 30])
+def test_a_session_without_its_page_stays_alone(pkg, dev, T):
+    """Sessions that lack a page, are past their table's end or padded with NaN give NaN rows of
+    their own; the others' rows and pages are what they are without them."""
+    page, layers, H = 16, 2, 1024
+    dec, twin = (build(pkg, dev, layers=layers, pages=40, page=page) for _ in range(2))
+    table = torch.arange(30, dtype=torch.int32, device=dev).view(5, 6)
+    h = torch.stack([tokens(dev, 80, seed=s) for s in range(5)])
+    for d in (dec, twin):
+        d.step(h[:, :40], 0, table=table)
+    pools = [c for l in dec.layers for c in (l.attn.paged.k, l.attn.paged.v)]
+    before = [c.clone() for c in pools]
+    x, tab = h[:, 40:40 + T].clone(), table.clone()
+    tab[1, 0] = -1           # lacks a page of its past
+    tab[2, 40 // page:] = 99  # and one of its own tokens': not a page of the pool
+    pos = i32(dev, [40, 40, 40, 6 * page, 40])
+    counts = i32(dev, [T, T, T, T, T - 1])
+    if T > 1:
+        x[4, T - 1:] = float("nan")
+    got = dec.step(x, pos, table=tab, counts=counts)
+    good = [0, 4]
+    want = twin.step(x[good], 40, table=table[good], counts=counts[good])
+    assert torch.isnan(got[1:4]).all()
+    for i, b in enumerate(good):
+        n = int(counts[b])
+        if n:
+            assert near(got[b, :n], want[i, :n])
+    other = [c for l in twin.layers for c in (l.attn.paged.k, l.attn.paged.v)]
+    for c, old, o in zip(pools, before, other):
+        assert near(c[table[good].long()], o[table[good].long()])
+        # of the others, the first layer's own rows are finite and in their pages alone; nothing
+        # of a session without its page or place is written
+        assert same(c[table[2].long()], old[table[2].long()])
+        assert same(c[table[3].long()], old[table[3].long()])
+        assert same(c[30:], old[30:]) and same(c[table[1, :2].long()], old[table[1, :2].long()])
+    again = dec.step(x, i32(dev, [40] * 5), table=table, counts=counts)  # all of them well again
+    assert torch.isfinite(again[:4]).all()
+    assert near(again[0], twin.step(x[:1], 40, table=table[:1])[0])
