@@ -29,10 +29,11 @@ from .ops import Workspace
 from .rotary import Rotary, _turn_c, distinct, overlaps
 
 _paged = struct.Struct("<3Q3q7i4x").pack  # struct i4_pagedcache
+HEAD_DIM = 128
 
 
 class PagedCache(_lib.Handle):
-    """The pool: k and v [pages, n_kv_heads, page, head_dim] in 16 bits, views of any strides
+    """The pool: k and v [pages, n_kv_heads, page, 128] in 16 bits, views of any strides
     whose pages' rows are dense (a head's page is page * head_dim adjacent values).  The kernels
     write the tensors in place and the object holds their addresses, so they cannot be
     replaced (AttributeError)."""
@@ -45,6 +46,8 @@ class PagedCache(_lib.Handle):
             raise RuntimeError("k and v are [pages, n_kv_heads, page, head_dim] and agree in "
                                "shape, strides and dtype")
         pages, n, page, hd = k.shape
+        if hd != HEAD_DIM:
+            raise RuntimeError(f"the kernels take heads of {HEAD_DIM} dims, got {hd}")
         if k.stride(3) != 1 or k.stride(2) != hd:
             raise RuntimeError("the rows of a head's page must be dense")
         if not distinct(page * hd, (pages, k.stride(0)), (n, k.stride(1))):
@@ -59,7 +62,7 @@ class PagedCache(_lib.Handle):
                    _lib.half_code(k.dtype))
 
     @classmethod
-    def empty(cls, n_kv_heads: int, pages: int, page: int = 64, head_dim: int = 128, *,
+    def empty(cls, n_kv_heads: int, pages: int, page: int = 64, head_dim: int = HEAD_DIM, *,
               dtype: torch.dtype = torch.bfloat16,
               device: torch.device | str = "cuda") -> "PagedCache":
         """A pool of zeros."""

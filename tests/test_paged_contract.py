@@ -173,3 +173,12 @@ def test_a_call_needs_the_scratch_that_it_uses(lb, pkg, B, T, nh, nkv, pos, wind
     if need:
         assert call_attn(lb, lib, c, **a, wsb=need - 1) == WORKSPACE
         assert call_attn(lb, lib, c, **a, wsb=need, ws=P + 128) == ALIGN  # the check behind it
+
+
+@pytest.mark.parametrize("hd", [64, 96, 256])
+def test_a_pool_of_other_heads_is_refused(on_cpu, hd):
+    """No call takes it."""
+    with pytest.raises(RuntimeError, match="128 dims"):
+        pool(on_cpu, (4, 2, 16, hd))
+    with pytest.raises(RuntimeError, match="128 dims"):
+        on_cpu.PagedCache.empty(2, 4, 16, hd, device="cpu")
