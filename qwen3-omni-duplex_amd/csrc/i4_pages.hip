@@ -187,9 +187,10 @@ extern "C" int i4_paged_append(const void* qkv, int x_dtype, int T, int64_t batc
                 Tokens{pos_dev, counts, pos, T}, turn_of(turn), n_heads, nkv, zero_padding, eps};
   const RotaryTable<KHD / 2> rt = rotary_table<KHD / 2>(rotary);
   // The heads of few tokens are shared out, 16 a workgroup at least, while the chip has room for
-  // all workgroups at once (8 a CU): 24 tokens of 40 heads 3.0 us against 4.0 with one workgroup a
-  // token; 400 of 40 and 500 of 80 heads 4.3 and 6.5 us against 4.9 and 8.2 with room for 512
-  // workgroups, 1000 of 40 6.4 against 7.4 and 7.5 with room for 512 and 4096.
+  // all workgroups at once (8 a CU).  Traced, over four sets of rows and pages: 24 tokens of 40
+  // heads 3.9 us against 4.7 with one workgroup a token; 400 of 40 and 500 of 80 heads 4.9 and
+  // 6.6 us against 5.5 and 8.1 with room for 512 workgroups, 1000 of 40 6.4 against 7.2 and 7.5
+  // with room for 512 and 4096.
   const int heads = n_heads + 2 * nkv;
   int shares = 1;
   while (shares * 16 < heads && (int64_t)B * T * (shares + 1) <= 2048) ++shares;

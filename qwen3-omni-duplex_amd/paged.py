@@ -33,10 +33,10 @@ HEAD_DIM = 128
 
 
 class PagedCache(_lib.Handle):
-    """The pool: k and v [pages, n_kv_heads, page, 128] in 16 bits, views of any strides
-    whose pages' rows are dense (a head's page is page * head_dim adjacent values).  The kernels
-    write the tensors in place and the object holds their addresses, so they cannot be
-    replaced (AttributeError)."""
+    """The pool: k and v [pages, n_kv_heads, page, 128] in 16 bits, views of any strides that
+    keep pages and heads apart and whose pages' rows are dense (a head's page is page * 128
+    adjacent values).  The kernels write the tensors in place and the object holds their
+    addresses, so they cannot be replaced (AttributeError)."""
 
     __slots__ = ("k", "v", "device", "dtype", "_c", "_index")
 
