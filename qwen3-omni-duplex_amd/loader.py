@@ -227,9 +227,11 @@ def rope_theta(tc: dict) -> float:
 
 
 def _rope_config(tc: dict) -> tuple[dict, str]:
-    """What a text config says of its rotary embedding, and the embedding's type."""
+    """What a text config says of its rotary embedding, and the type of its table ("mrope" says
+    that there are sections: the table is the default one)."""
     rope = {**(tc.get("rope_parameters") or {}), **(tc.get("rope_scaling") or {})}
-    return rope, str(rope.get("rope_type") or rope.get("type") or "default")
+    kind = str(rope.get("rope_type") or rope.get("type") or "default")
+    return rope, "default" if kind == "mrope" else kind
 
 
 # the sections of a Thinker whose config names none

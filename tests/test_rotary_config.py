@@ -121,7 +121,7 @@ def test_a_scaled_table_needs_pages(pkg, tmp_path, context):
 
     with pytest.raises(NotImplementedError, match="pages"):
         layer({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768})
-    for rope in ({"rope_type": "default"}, None):
+    for rope in ({"rope_type": "default"}, {"type": "mrope", "mrope_section": [24, 20, 20]}, None):
         with pytest.raises(KeyError):  # the first weight
             layer(rope)
 
@@ -168,3 +168,12 @@ def test_axes_of_a_config(pkg, rope, monkeypatch):
     monkeypatch.setattr(loader, "ThinkerDecoderLayer", lambda *a: None)
     loader.load_thinker_layer(Config(), 0, "cpu", pages=4)
     assert seen["rotary"].axes == tuple(axes)
+
+
+def test_mrope_is_the_default_table(pkg):
+    from qwen3_omni_duplex_amd.loader import thinker_rotary
+
+    r = thinker_rotary({"rope_theta": 1e6, "rope_scaling": {"type": "mrope",
+                                                            "mrope_section": [24, 20, 20]}}, 128)
+    close(r, theirs({"rope_type": "default"}))
+    assert r.axes == pkg.interleaved_axes([24, 20, 20])
