@@ -8,7 +8,9 @@ import pytest
 import torch
 
 from tests.test_kv import ALIGN, STRIDE, WORKSPACE, P
-from tests.test_paged import cache, call_append, call_attn, call_rope, heads, lb, rotary as rot  # noqa: F401 (a fixture)
+from tests.test_paged import cache, call_append, call_attn, call_rope, heads
+from tests.test_paged import lb  # noqa: F401 (a fixture)
+from tests.test_paged import rotary as rot
 
 BF = torch.bfloat16
 
@@ -89,8 +91,8 @@ def test_pages_of_a_pool_are_distinct(lb, on_cpu, pages, heads, ps, hs, good):  
     else:
         with pytest.raises(RuntimeError, match="overlap"):
             on_cpu.PagedCache(k, v)
-        assert call_append(lb, on_cpu.lib(), cache(lb, **bad), nh=heads) == STRIDE
-        assert call_attn(lb, on_cpu.lib(), cache(lb, **bad), nh=heads) == STRIDE
+        assert call_append(lb, on_cpu.lib(), cache(lb, **bad), nh=heads, qkv=P + 2) == STRIDE
+        assert call_attn(lb, on_cpu.lib(), cache(lb, **bad), nh=heads, q=P + 2) == STRIDE
 
 
 OUTPUTS = [  # strides of sequences, tokens and heads in rows (2 x 3 x 4 of 16 dims), distinct
@@ -154,7 +156,8 @@ def test_outputs_lie_outside_the_pool(on_cpu, monkeypatch):
     (1, 64, 32, 4, 30000, 0), (3, 17, 8, 1, 16000, 0), (24, 1, 32, 4, 20000, 0),
     (1, 1, 8, 2, 5000, 0), (2, 300, 8, 2, 100, 0)])
 @pytest.mark.parametrize("form", ["host", "counts", "device"])
-def test_a_call_needs_the_scratch_that_it_uses(lb, pkg, B, T, nh, nkv, pos, window, form):  # noqa: F811
+def test_a_call_needs_the_scratch_that_it_uses(lb, pkg, B, T, nh, nkv, pos, window,  # noqa: F811
+                                               form):
     """One byte less than i4_attn_paged_call_bytes is refused, that many are not.  A call whose
     lengths the host knows is split as attn_window's of many rows are, and needs no more."""
     lib = pkg.lib()
